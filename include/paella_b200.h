@@ -210,6 +210,79 @@ PB_API int pb_conv2d_umma_noalloc(const pb_op_params* p, void* stream, uint32_t 
 PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
 
 /* ------------------------------------------------------------------------ *
+ * Operators of language models: what one attention layer does to serve the next tokens.  No counterpart in the
+ * reference, whose adapters serve image models.  In the manner of the operators above: a params structure filled by the
+ * caller, `_info` for the geometry a job stage declares, `_launch` to enqueue on `stream` (a cudaStream_t of the current
+ * device, where all buffers live).
+ *  - Each launcher enqueues one kernel, whose every block reports start/end on `notifier` (may be NULL) for `job_id`.
+ *  - Strides are in elements.  Buffers may lie anywhere inside larger ones; outputs do not overlap inputs unless a text says so.
+ *  - Launches allocate nothing and may be captured into a CUDA graph, the first one included.  The pointers and sizes of the
+ *    params are read at the launch, what they point to when the kernels run.
+ *  - What the host can see to be wrong is refused with PB_ERR_INVALID before anything is enqueued.  What only the device can
+ *    see (a page, position, slot or length out of range) raises the flag that pb_device_error_flag reads; what such a value
+ *    says below is done, and nothing outside the buffers is touched.
+ * ------------------------------------------------------------------------ */
+typedef enum pb_dtype {
+    PB_F32 = 0,
+    PB_BF16 = 1,
+    PB_F16 = 2               /* language-model operators only */
+} pb_dtype;
+
+/* Norms of queries and keys for each head, and their rotation by position, in one pass.
+ * z = x * weight / sqrt(mean(x^2) + eps) over a head's head_dim values (weight NULL: z = x), then for each pair (a, b) of
+ * the first rot_dim values of z, with c and s of the pair at the token's position: (a c - b s, b c + a s).  Pairs are
+ * (i, i + rot_dim / 2), or (2 i, 2 i + 1) with `interleaved`.  In fp32, rounded once.
+ * A token whose position lies outside of [0, max_position) is left out: its outputs stay as they were. */
+typedef struct pb_qk_rope_params {
+    int32_t dtype;               /* PB_F32, PB_BF16 or PB_F16: q, k and their outputs */
+    int32_t tokens;              /* 0 = nothing to do */
+    int32_t q_heads, kv_heads;   /* either may be 0 */
+    int32_t head_dim;            /* 1 to 256 */
+    int32_t rot_dim;             /* even, 0 (no rotation) to head_dim */
+    int32_t interleaved;
+    int32_t max_position;        /* rows of cos_sin */
+    float eps;
+    int32_t reserved;            /* 0 */
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride;                       /* from token to token, head to head */
+    int64_t q_out_stride, q_out_head_stride, k_out_stride, k_out_head_stride;
+    const void *q, *k;
+    void *q_out, *k_out;         /* may be q and k, with their strides */
+    const float *q_weight, *k_weight;   /* [head_dim], or NULL for no norm */
+    const float* cos_sin;        /* [max_position][rot_dim]: rot_dim / 2 cosines, then as many sines */
+    const int32_t* positions;    /* [tokens] */
+} pb_qk_rope_params;
+PB_API int pb_qk_rope_info(const pb_qk_rope_params* p, pb_launch_info* out);
+PB_API int pb_qk_rope_launch(const pb_qk_rope_params* p, void* stream, uint32_t job_id, void* notifier);
+
+/* Appends the tokens' keys and values to a paged cache, the keys normed and rotated on the way as above (k_weight NULL: no
+ * norm; rot_dim 0: no rotation), the values as they are; and, with q_heads > 0, norms and rotates the tokens' queries in the
+ * same launch, so that a decode step's preparation is one kernel.
+ * Token t goes to row slots[t] % page_size of page slots[t] / page_size.  A negative slot marks a padded row: nothing is
+ * stored for it (its query is still computed if its position is a valid one).  Slots of one launch are distinct. */
+typedef struct pb_kv_append_params {
+    int32_t dtype;               /* PB_F32, PB_BF16 or PB_F16: k, v, q and the cache */
+    int32_t tokens;              /* 0 = nothing to do */
+    int32_t q_heads, kv_heads, head_dim, rot_dim, interleaved, max_position;   /* as above; kv_heads >= 1 */
+    float eps;
+    int32_t page_size;           /* >= 1 */
+    int64_t n_pages;
+    int64_t k_stride, k_head_stride, v_stride, v_head_stride;
+    int64_t page_stride, token_stride, head_stride;      /* of k_cache and v_cache */
+    int64_t q_stride, q_head_stride, q_out_stride, q_out_head_stride;
+    const void *k, *v;
+    const float* k_weight;
+    const float* cos_sin;
+    const int32_t* positions;    /* [tokens]; NULL when rot_dim is 0 */
+    const int64_t* slots;        /* [tokens] */
+    void *k_cache, *v_cache;
+    const void* q;
+    void* q_out;                 /* may be q, with its strides */
+    const float* q_weight;
+} pb_kv_append_params;
+PB_API int pb_kv_append_info(const pb_kv_append_params* p, pb_launch_info* out);
+PB_API int pb_kv_append_launch(const pb_kv_append_params* p, void* stream, uint32_t job_id, void* notifier);
+
+/* ------------------------------------------------------------------------ *
  * Model packs and instances: the graph executor behind the model job adapters
  * (replaces tvm::runtime::Module::LoadFromFile + "run"/"get_input"/"get_output",
  * jobs/tvm_mnist/tvm_mnist.cpp:24-33).

@@ -17,6 +17,10 @@ STAGE_NAMES = ["input", "conv_simt", "conv_umma", "dwconv", "dense", "maxpool", 
                "mnist_fused", "affine", "detect"]
 
 
+# element types (pb_dtype)
+F32, BF16, F16 = 0, 1, 2
+
+
 class PbError(RuntimeError):
     pass
 
@@ -33,6 +37,22 @@ class OpParams(C.Structure):
                [("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
                 ("scratch", C.c_void_p), ("scratch_bytes", C.c_uint64),
                 ("batch", C.c_int32), ("dil_h", C.c_int32), ("dil_w", C.c_int32), ("reserved", C.c_int32)]
+
+
+class QkRopeParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rot_dim", "interleaved", "max_position")] + \
+               [("eps", C.c_float), ("reserved", C.c_int32)] + \
+               [(n, C.c_int64) for n in ("q_stride", "q_head_stride", "k_stride", "k_head_stride", "q_out_stride", "q_out_head_stride",
+                                         "k_out_stride", "k_out_head_stride")] + \
+               [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "cos_sin", "positions")]
+
+
+class KvAppendParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rot_dim", "interleaved", "max_position")] + \
+               [("eps", C.c_float), ("page_size", C.c_int32)] + \
+               [(n, C.c_int64) for n in ("n_pages", "k_stride", "k_head_stride", "v_stride", "v_head_stride", "page_stride", "token_stride",
+                                         "head_stride", "q_stride", "q_head_stride", "q_out_stride", "q_out_head_stride")] + \
+               [(n, C.c_void_p) for n in ("k", "v", "k_weight", "cos_sin", "positions", "slots", "k_cache", "v_cache", "q", "q_out", "q_weight")]
 
 
 class ServerConfig(C.Structure):
@@ -135,6 +155,10 @@ SIGNATURES = {
     "pb_op_pack_weights": (C.c_int64, [_I, C.POINTER(OpParams), _VP, _VP]),
     "pb_conv_umma_supported": (_I, [C.POINTER(OpParams)]),
     "pb_conv2d_umma_noalloc": (_I, [C.POINTER(OpParams), _VP, _U32, _VP]),
+    "pb_qk_rope_info": (_I, [C.POINTER(QkRopeParams), C.POINTER(LaunchInfo)]),
+    "pb_qk_rope_launch": (_I, [C.POINTER(QkRopeParams), _VP, _U32, _VP]),
+    "pb_kv_append_info": (_I, [C.POINTER(KvAppendParams), C.POINTER(LaunchInfo)]),
+    "pb_kv_append_launch": (_I, [C.POINTER(KvAppendParams), _VP, _U32, _VP]),
     "pb_device_error_flag": (_I, [_I, C.POINTER(_U32), _I]),
     "pb_set_conv_split_gain_us": (None, [C.c_double]),
     "pb_conv_umma_time": (_I, [C.POINTER(OpParams), _I, _I, _SZ, C.POINTER(C.c_double)]),

@@ -1,0 +1,362 @@
+// Norms of queries and keys for each head with the rotation by position, and the same on the way into a paged cache.
+//
+//   z = x * w / sqrt(mean(x^2) + eps);   (a, b) -> (a c - b s, b c + a s) for the pairs of the first rot_dim values
+//
+// Both are bound by memory: every head is read once and written once, 4 operations a byte.  A group of lanes takes a head, each
+// lane both halves of its pairs, so that the rotation needs no exchange and only the norm's sum does (three shuffles for a head
+// of 128 values in 16 bits, whose group is eight lanes).  A group takes up to four heads of one token: the loads of all of them
+// are in flight before the first is used, and the rotation's row is loaded once.
+#include <cuda.h>
+
+#include "lm.cuh"
+
+namespace pb {
+namespace {
+
+__device__ uint32_t g_rope_flag;
+
+// One class of heads: queries, keys or values.  dst is found from the slot for keys and values of an append.
+struct HeadSet {
+    const void* src;
+    void* dst;
+    const float* weight;
+    int64_t src_token, src_head, dst_token, dst_head;
+};
+
+struct RopeArgs {
+    HeadSet set[3];            // queries, keys, values
+    int first[3];              // heads before the end of each set: queries, then keys, then values
+    int tokens, head_dim, rot_dim, interleaved, max_position, lanes;   // lanes: of a group, a power of two
+    int slices;                // groups that share a token's heads out
+    float eps;
+    const float* cos_sin;
+    const int32_t* positions;
+    // an append: keys and values go to pages
+    const int64_t* slots;      // NULL otherwise
+    int64_t n_slots, page_stride, row_stride;
+    int page_size;
+};
+
+// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS heads of a token.
+template <typename T, int V, int CH, int HEADS>
+__global__ void __launch_bounds__(256) rope_kernel(RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    griddep_wait();
+    if (nf) nf->start(job_id);
+    griddep_launch();
+    using Vt = LmVec<T, V>;
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / a.lanes;
+    const int64_t token = group >> 32 ? group / a.slices : (uint32_t)group / (uint32_t)a.slices;    // (a 64-bit quotient takes some 70 instructions)
+    const int slice = (int)(group - token * a.slices);
+    bool live = token < a.tokens;
+    int64_t slot = 0, page = 0;
+    bool store = true;                                   // keys and values of this token are stored
+    int pos = 0;
+    if (live) {
+        if (a.slots) {
+            slot = a.slots[token];
+            store = slot >= 0;
+            if (slot >= a.n_slots) {
+                if (lane == 0) atomicExch(&g_rope_flag, kFlagLmSlot);
+                live = false;
+            }
+            page = slot >> 32 ? slot / a.page_size : (uint32_t)slot / (uint32_t)a.page_size;
+            slot -= page * a.page_size;
+        }
+        if (a.rot_dim) {
+            pos = a.positions[token];
+            if (pos < 0 || pos >= a.max_position) {
+                if (lane == 0 && store && live) atomicExch(&g_rope_flag, kFlagLmPosition);
+                live = false;
+            }
+        }
+    }
+    // where this lane's chunks lie: `lo` and `hi`, V values each
+    const int half = a.rot_dim / 2, turned = half / V;
+    int lo[CH], hi[CH];                                  // -1 = none
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = lane + c * a.lanes;
+        if (i < turned) {
+            lo[c] = a.interleaved ? 2 * V * i : V * i;
+            hi[c] = a.interleaved ? lo[c] + V : lo[c] + half;
+        } else {
+            lo[c] = a.rot_dim + 2 * V * (i - turned);
+            hi[c] = lo[c] + V;
+        }
+        if (lo[c] >= a.head_dim) lo[c] = -1;
+        if (hi[c] >= a.head_dim) hi[c] = -1;
+    }
+    Vt x[HEADS][CH][2];
+    int which[HEADS];
+    T* dst[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        const int head = slice + h * a.slices;
+        which[h] = head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2;
+        if (!live || head >= a.first[2] || (which[h] && !store)) which[h] = -1;
+        if (which[h] < 0) continue;
+        const HeadSet& s = a.set[which[h]];
+        const int within = head - (which[h] ? a.first[which[h] - 1] : 0);
+        const T* src = static_cast<const T*>(s.src) + token * s.src_token + within * s.src_head;
+        dst[h] = static_cast<T*>(s.dst) + within * s.dst_head +
+                 (which[h] && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (lo[c] >= 0) x[h][c][0] = *reinterpret_cast<const Vt*>(src + lo[c]);
+            if (hi[c] >= 0) x[h][c][1] = *reinterpret_cast<const Vt*>(src + hi[c]);
+        }
+    }
+    float co[CH][V], si[CH][V];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i = lane + c * a.lanes;
+        if (live && i < turned) {
+            const float* row = a.cos_sin + (int64_t)pos * a.rot_dim + V * i;
+            constexpr int W = V < 4 ? V : 4;
+#pragma unroll
+            for (int j = 0; j < V; j += W) {
+                const LmVec<float, W> cv = *reinterpret_cast<const LmVec<float, W>*>(row + j);
+                const LmVec<float, W> sv = *reinterpret_cast<const LmVec<float, W>*>(row + half + j);
+#pragma unroll
+                for (int k = 0; k < W; ++k) { co[c][j + k] = cv.v[k]; si[c][j + k] = sv.v[k]; }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) { co[c][j] = 1.f; si[c][j] = 0.f; }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        const int w = which[h];
+        if (__all_sync(0xffffffffu, w < 0)) continue;
+        const float* weight = w < 0 ? nullptr : a.set[w].weight;
+        float z[CH][2][V];
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const bool there = (p ? hi[c] : lo[c]) >= 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    z[c][p][j] = w >= 0 && there ? lm_to_f<T>(x[h][c][p].v[j]) : 0.f;
+                    sum += z[c][p][j] * z[c][p][j];
+                }
+            }
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (w < 0) continue;
+        if (weight) {
+            const float r = rsqrtf(sum / (float)a.head_dim + a.eps);
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int at = p ? hi[c] : lo[c];
+                    if (at < 0) continue;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) z[c][p][j] *= r * __ldg(weight + at + j);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            Vt out[2];
+            const int i = lane + c * a.lanes;
+            const bool turn = w < 2 && i < turned;
+            if (turn && a.interleaved) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {            // pair j of the chunk: values 2 j and 2 j + 1
+                    const float A = 2 * j < V ? z[c][0][(2 * j) % V] : z[c][1][(2 * j) % V];
+                    const float B = 2 * j + 1 < V ? z[c][0][(2 * j + 1) % V] : z[c][1][(2 * j + 1) % V];
+                    out[(2 * j) / V].v[(2 * j) % V] = lm_from_f<T>(A * co[c][j] - B * si[c][j]);
+                    out[(2 * j + 1) / V].v[(2 * j + 1) % V] = lm_from_f<T>(B * co[c][j] + A * si[c][j]);
+                }
+            } else if (turn) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    out[0].v[j] = lm_from_f<T>(z[c][0][j] * co[c][j] - z[c][1][j] * si[c][j]);
+                    out[1].v[j] = lm_from_f<T>(z[c][1][j] * co[c][j] + z[c][0][j] * si[c][j]);
+                }
+            } else if (weight) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    out[0].v[j] = lm_from_f<T>(z[c][0][j]);
+                    out[1].v[j] = lm_from_f<T>(z[c][1][j]);
+                }
+            } else {                                     // as it was, a NaN's bits too
+                out[0] = x[h][c][0];
+                out[1] = x[h][c][1];
+            }
+            if (lo[c] >= 0) *reinterpret_cast<Vt*>(dst[h] + lo[c]) = out[0];
+            if (hi[c] >= 0) *reinterpret_cast<Vt*>(dst[h] + hi[c]) = out[1];
+        }
+    }
+    if (nf) nf->end(job_id);
+}
+
+typedef void (*RopeFn)(RopeArgs, uint32_t, FinishedBlockNotifier*);
+
+struct RopePlan {
+    RopeArgs a;
+    RopeFn fn;
+    unsigned blocks;
+};
+
+// All accesses of V values of `es` bytes of this set are aligned to their size.
+bool vectors_fit(const HeadSet& s, int heads, int V, size_t es) {
+    if (!heads) return true;
+    return aligned(s.src, V * es) && aligned(s.dst, V * es) && s.src_token % V == 0 && s.src_head % V == 0 && s.dst_token % V == 0 && s.dst_head % V == 0;
+}
+
+template <typename T>
+RopeFn pick(int V, int heads) {
+    constexpr int VN = 16 / (int)sizeof(T);
+    if (V == VN) return heads == 4 ? rope_kernel<T, VN, 1, 4> : heads == 2 ? rope_kernel<T, VN, 1, 2> : rope_kernel<T, VN, 1, 1>;
+    return rope_kernel<T, 1, 4, 1>;
+}
+
+int plan_rope(const char* who, int dtype, RopePlan& pl) {
+    RopeArgs& a = pl.a;
+    const size_t es = dtype_bytes(dtype);
+    const int VN = (int)(16 / es);
+    // 16 bytes an access where every pair's halves, every head and every row of the table allow it, single values otherwise
+    bool wide = (a.rot_dim / 2) % VN == 0 && a.head_dim % VN == 0 && (a.rot_dim == 0 || aligned(a.cos_sin, 16));
+    int before = 0;
+    for (int i = 0; i < 3; ++i) {
+        wide = wide && vectors_fit(a.set[i], a.first[i] - before, VN, es);
+        before = a.first[i];
+    }
+    if (a.slots) wide = wide && a.page_stride % VN == 0 && a.row_stride % VN == 0;
+    const int V = wide ? VN : 1;
+    const int chunks = a.rot_dim / 2 / V + ceil_div(a.head_dim - a.rot_dim, 2 * V), per_lane = wide ? 1 : 4;
+    a.lanes = 1;
+    while (a.lanes * per_lane < chunks) a.lanes *= 2;
+    const int heads = a.first[2];
+    // Heads of a group: as many as leave the GPU two waves of threads.
+    int each = 1;
+    if (wide)
+        for (int e = 4; e > 1; e /= 2)
+            if (heads >= e && (int64_t)a.tokens * ceil_div(heads, e) * a.lanes >= 2 * 148 * 2048) { each = e; break; }
+    a.slices = ceil_div(heads, each);
+    const int64_t blocks = ceil_div<int64_t>((int64_t)a.tokens * a.slices * a.lanes, 256);
+    PB_REQUIRE(blocks <= 0x7fffffff, "%s: %d tokens of %d heads are too many for one launch", who, a.tokens, heads);
+    pl.blocks = blocks > 0 ? (unsigned)blocks : 1u;
+    pl.fn = dtype == PB_F32 ? pick<float>(V, each) : dtype == PB_BF16 ? pick<__nv_bfloat16>(V, each) : pick<__half>(V, each);
+    return PB_OK;
+}
+
+int check_heads(const char* who, int dtype, int tokens, int q_heads, int kv_heads, int head_dim, int rot_dim, int max_position, const float* cos_sin, const int32_t* positions) {
+    PB_REQUIRE(is_float_dtype(dtype), "%s: dtype %d (PB_F32, PB_BF16 or PB_F16)", who, dtype);
+    PB_REQUIRE(tokens >= 0, "%s: %d tokens", who, tokens);
+    PB_REQUIRE(q_heads >= 0 && kv_heads >= 0 && q_heads <= 65536 && kv_heads <= 65536, "%s: %d query heads, %d key heads", who, q_heads, kv_heads);
+    PB_REQUIRE(head_dim >= 1 && head_dim <= 256, "%s: head_dim %d (1 to 256)", who, head_dim);
+    PB_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, "%s: rot_dim %d (even, 0 to head_dim %d)", who, rot_dim, head_dim);
+    PB_REQUIRE(rot_dim == 0 || tokens == 0 || (max_position > 0 && cos_sin && positions && aligned(cos_sin, 4) && aligned(positions, 4)), "%s: a rotation needs cos_sin, positions and max_position", who);
+    return PB_OK;
+}
+
+int rope_plan(const pb_qk_rope_params* p, RopePlan& pl) {
+    const char* who = "pb_qk_rope";
+    PB_REQUIRE(p != nullptr, "%s: NULL params", who);
+    const int rc = check_heads(who, p->dtype, p->tokens, p->q_heads, p->kv_heads, p->head_dim, p->rot_dim, p->max_position, p->cos_sin, p->positions);
+    if (rc != PB_OK) return rc;
+    PB_REQUIRE(p->q_heads + p->kv_heads > 0, "%s: no heads", who);
+    const size_t es = dtype_bytes(p->dtype);
+    if (p->tokens > 0) {
+        PB_REQUIRE(p->q_heads == 0 || (p->q && p->q_out), "%s: NULL q or q_out", who);
+        PB_REQUIRE(p->kv_heads == 0 || (p->k && p->k_out), "%s: NULL k or k_out", who);
+        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->k_out, es), "%s: a buffer is not aligned to its elements", who);
+    }
+    RopeArgs& a = pl.a;
+    memset(&a, 0, sizeof(a));
+    a.set[0] = {p->q, p->q_out, p->q_weight, p->q_stride, p->q_head_stride, p->q_out_stride, p->q_out_head_stride};
+    a.set[1] = {p->k, p->k_out, p->k_weight, p->k_stride, p->k_head_stride, p->k_out_stride, p->k_out_head_stride};
+    a.first[0] = p->q_heads;
+    a.first[1] = a.first[2] = p->q_heads + p->kv_heads;
+    a.tokens = p->tokens; a.head_dim = p->head_dim; a.rot_dim = p->rot_dim; a.interleaved = p->interleaved != 0; a.max_position = p->max_position;
+    a.eps = p->eps; a.cos_sin = p->cos_sin; a.positions = p->positions;
+    return plan_rope(who, p->dtype, pl);
+}
+
+int append_plan(const pb_kv_append_params* p, RopePlan& pl) {
+    const char* who = "pb_kv_append";
+    PB_REQUIRE(p != nullptr, "%s: NULL params", who);
+    const int rc = check_heads(who, p->dtype, p->tokens, p->q_heads, p->kv_heads, p->head_dim, p->rot_dim, p->max_position, p->cos_sin, p->positions);
+    if (rc != PB_OK) return rc;
+    PB_REQUIRE(p->kv_heads > 0, "%s: no key heads", who);
+    PB_REQUIRE(p->page_size >= 1 && p->n_pages >= 0 && p->n_pages <= INT64_MAX / p->page_size, "%s: %lld pages of %d rows", who, (long long)p->n_pages, p->page_size);
+    const size_t es = dtype_bytes(p->dtype);
+    if (p->tokens > 0) {
+        PB_REQUIRE(p->k && p->v && p->k_cache && p->v_cache && p->slots && aligned(p->slots, 8), "%s: NULL k, v, cache or slots", who);
+        PB_REQUIRE(p->q_heads == 0 || (p->q && p->q_out), "%s: NULL q or q_out", who);
+        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->v, es) && aligned(p->k_cache, es) && aligned(p->v_cache, es), "%s: a buffer is not aligned to its elements", who);
+    }
+    RopeArgs& a = pl.a;
+    memset(&a, 0, sizeof(a));
+    a.set[0] = {p->q, p->q_out, p->q_weight, p->q_stride, p->q_head_stride, p->q_out_stride, p->q_out_head_stride};
+    a.set[1] = {p->k, p->k_cache, p->k_weight, p->k_stride, p->k_head_stride, 0, p->head_stride};
+    a.set[2] = {p->v, p->v_cache, nullptr, p->v_stride, p->v_head_stride, 0, p->head_stride};
+    a.first[0] = p->q_heads;
+    a.first[1] = p->q_heads + p->kv_heads;
+    a.first[2] = p->q_heads + 2 * p->kv_heads;
+    a.tokens = p->tokens; a.head_dim = p->head_dim; a.rot_dim = p->rot_dim; a.interleaved = p->interleaved != 0; a.max_position = p->max_position;
+    a.eps = p->eps; a.cos_sin = p->cos_sin; a.positions = p->positions;
+    a.slots = p->slots; a.n_slots = p->n_pages * p->page_size; a.page_size = p->page_size; a.page_stride = p->page_stride; a.row_stride = p->token_stride;
+    return plan_rope(who, p->dtype, pl);
+}
+
+int rope_info(const RopePlan& pl, int dtype, pb_launch_info* out) {
+    memset(out, 0, sizeof(*out));
+    const RopeArgs& a = pl.a;
+    const uint64_t t = (uint64_t)a.tokens, es = dtype_bytes(dtype);
+    out->num_blocks = pl.blocks;
+    out->threads_per_block = 256;
+    out->regs_per_thread = lm_regs(pl.fn);
+    out->flops = t * ((uint64_t)a.first[1] * 3 * a.rot_dim + 4ull * a.head_dim * ((a.set[0].weight ? a.first[0] : 0) + (a.set[1].weight ? a.first[1] - a.first[0] : 0)));
+    out->bytes = t * (2 * es * a.head_dim * a.first[2] + (a.rot_dim ? 4ull * a.rot_dim + 4 : 0) + (a.slots ? 8 : 0));
+    return PB_OK;
+}
+
+}  // namespace
+
+uint32_t* lm_rope_error_flag_ptr() {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_rope_flag) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+    return (uint32_t*)p;
+}
+
+}  // namespace pb
+
+extern "C" {
+
+int pb_qk_rope_info(const pb_qk_rope_params* p, pb_launch_info* out) {
+    pb::RopePlan pl;
+    const int rc = pb::rope_plan(p, pl);
+    if (rc != PB_OK) return rc;
+    PB_REQUIRE(out != nullptr, "pb_qk_rope_info: NULL out");
+    return pb::rope_info(pl, p->dtype, out);
+}
+
+int pb_qk_rope_launch(const pb_qk_rope_params* p, void* stream, uint32_t job_id, void* notifier) {
+    pb::RopePlan pl;
+    const int rc = pb::rope_plan(p, pl);
+    if (rc != PB_OK) return rc;
+    return pb::lm_launch("pb_qk_rope", pl.fn, dim3(pl.blocks), dim3(256), 0, (cudaStream_t)stream, 1, pl.a, job_id, (pb::FinishedBlockNotifier*)notifier);
+}
+
+int pb_kv_append_info(const pb_kv_append_params* p, pb_launch_info* out) {
+    pb::RopePlan pl;
+    const int rc = pb::append_plan(p, pl);
+    if (rc != PB_OK) return rc;
+    PB_REQUIRE(out != nullptr, "pb_kv_append_info: NULL out");
+    return pb::rope_info(pl, p->dtype, out);
+}
+
+int pb_kv_append_launch(const pb_kv_append_params* p, void* stream, uint32_t job_id, void* notifier) {
+    pb::RopePlan pl;
+    const int rc = pb::append_plan(p, pl);
+    if (rc != PB_OK) return rc;
+    return pb::lm_launch("pb_kv_append", pl.fn, dim3(pl.blocks), dim3(256), 0, (cudaStream_t)stream, 1, pl.a, job_id, (pb::FinishedBlockNotifier*)notifier);
+}
+
+}  // extern "C"

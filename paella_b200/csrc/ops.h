@@ -116,6 +116,9 @@ int conv_umma_multi_launch(const ConvUmmaMulti* m, cudaStream_t st, uint32_t job
 int conv_umma_time(const pb_op_params* p, int mode, int iters, size_t flush_bytes, double* us_out);
 void conv_umma_set_split_gain_us(double us);   // < 0: back to PB_CONV_SPLIT_GAIN_US / the default
 int conv_umma_launch_noalloc(const pb_op_params* p, cudaStream_t st, uint32_t job_id, void* notifier);
+// The error flag words of the language-model operators' kernels on the current device (file-scope device words: nothing is
+// allocated, so a first launch may be captured).
+uint32_t* lm_rope_error_flag_ptr();
 uint32_t* noalloc_error_flag_ptr(int device);   // NULL until the no-allocation path ran on the device
 
 }  // namespace pb

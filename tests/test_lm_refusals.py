@@ -1,0 +1,57 @@
+"""What the language-model operators refuse before anything is enqueued, and what they declare; no GPU is used."""
+import ctypes as C
+
+import pytest
+
+from paella_b200 import capi
+from tests import lm_util as lu
+
+A = 1 << 20      # an address that stands for a buffer: nothing reads it
+
+
+def rope(**over):
+    f = dict(dtype=capi.BF16, tokens=4, q_heads=4, kv_heads=2, head_dim=64, rot_dim=64, max_position=16, eps=1e-6, q_stride=256, q_head_stride=64, k_stride=128,
+             k_head_stride=64, q_out_stride=256, q_out_head_stride=64, k_out_stride=128, k_out_head_stride=64, q=A, k=A, q_out=A, k_out=A, cos_sin=A, positions=A)
+    return capi.QkRopeParams(**{**f, **over})
+
+
+def append(**over):
+    f = dict(dtype=capi.BF16, tokens=4, q_heads=4, kv_heads=2, head_dim=64, rot_dim=64, max_position=16, eps=1e-6, page_size=16, n_pages=4, k_stride=128,
+             k_head_stride=64, v_stride=128, v_head_stride=64, page_stride=2048, token_stride=128, head_stride=64, q_stride=256, q_head_stride=64,
+             q_out_stride=256, q_out_head_stride=64, k=A, v=A, cos_sin=A, positions=A, slots=A, k_cache=A, v_cache=A, q=A, q_out=A)
+    return capi.KvAppendParams(**{**f, **over})
+
+
+BAD_HEADS = [dict(dtype=3), dict(dtype=-1), dict(tokens=-1), dict(q_heads=-1), dict(kv_heads=-1), dict(kv_heads=70000), dict(head_dim=0), dict(head_dim=257), dict(rot_dim=63),
+             dict(rot_dim=66), dict(rot_dim=-2), dict(max_position=0), dict(cos_sin=None), dict(positions=None), dict(q=None), dict(q_out=None), dict(k=None),
+             dict(q=A + 1), dict(k=A + 1), dict(cos_sin=A + 2), dict(positions=A + 2)]
+
+
+@pytest.mark.parametrize("over", BAD_HEADS + [dict(q_heads=0, kv_heads=0), dict(k_out=None), dict(tokens=2 ** 31 - 1, q_heads=65536, kv_heads=65536)])
+def test_rope_refusals(over):
+    assert lu.refused("qk_rope", rope(**over)).startswith("pb_qk_rope")
+
+
+@pytest.mark.parametrize("over", BAD_HEADS + [dict(kv_heads=0), dict(page_size=0), dict(n_pages=-1), dict(n_pages=2 ** 62), dict(v=None), dict(slots=None), dict(slots=A + 4),
+                                              dict(k_cache=None), dict(v_cache=None), dict(v_cache=A + 1)])
+def test_append_refusals(over):
+    assert lu.refused("kv_append", append(**over)).startswith("pb_kv_append")
+
+
+def test_null_params_are_refused():
+    L, li = capi.load(), capi.LaunchInfo()
+    for name, kind in (("qk_rope", capi.QkRopeParams), ("kv_append", capi.KvAppendParams)):
+        assert getattr(L, f"pb_{name}_info")(None, C.byref(li)) == -2
+        assert getattr(L, f"pb_{name}_launch")(None, None, 0, None) == -2
+
+
+def test_struct_sizes_match_the_header():
+    assert C.sizeof(capi.QkRopeParams) == 10 * 4 + 8 * 8 + 8 * 8
+    assert C.sizeof(capi.KvAppendParams) == 10 * 4 + 12 * 8 + 11 * 8
+
+
+def test_declared_work():
+    li = lu.info("qk_rope", rope())
+    assert li.bytes == 4 * (2 * 2 * 64 * 6 + 4 * 64 + 4) and li.threads_per_block == 256 and li.num_blocks >= 1
+    li = lu.info("kv_append", append(tokens=0))
+    assert li.bytes == 0 and li.num_blocks == 1
