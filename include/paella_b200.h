@@ -228,6 +228,41 @@ typedef enum pb_dtype {
     PB_F16 = 2               /* language-model operators only */
 } pb_dtype;
 
+/* 8-bit integers and a scale for each token: q[t][k] = rint(x[t][k] * (127 * (1 / max_t))), halves to even, with max_t the
+ * largest magnitude of row t, and scale[t] = max_t / 127; every operation is rounded to fp32.  A row whose max_t is below 2^-119 (all
+ * zeros among them) becomes zeros with scale 0; one that holds a NaN or an infinity becomes zeros with scale NaN, which
+ * makes its results NaN. */
+typedef struct pb_int8_quantize_params {
+    int32_t tokens, channels;    /* rows (0 = nothing to do) and their length (>= 1) */
+    int32_t x_dtype;             /* PB_F32, PB_BF16 or PB_F16 */
+    int32_t reserved;            /* 0 */
+    int64_t x_stride, q_stride;  /* from row to row */
+    const void* x;
+    int8_t* q;
+    float* scale;                /* [tokens] */
+} pb_int8_quantize_params;
+PB_API int pb_int8_quantize_info(const pb_int8_quantize_params* p, pb_launch_info* out);
+PB_API int pb_int8_quantize_launch(const pb_int8_quantize_params* p, void* stream, uint32_t job_id, void* notifier);
+
+/* A dense layer in 8-bit integers: y[t][n] = act(x_scale[t] * w_scale[n] * sum_k x[t][k] * w[n][k] + bias[n]).
+ * The sum is exact (32-bit integers, hence in_channels <= 131071). */
+typedef struct pb_int8_dense_params {
+    int32_t tokens, in_channels, out_channels;   /* tokens 0 = nothing to do */
+    int32_t y_dtype;             /* PB_F32, PB_BF16 or PB_F16 */
+    int32_t act;                 /* 0 none, 1 relu, 2 relu6 */
+    int32_t reserved;            /* 0 */
+    int64_t x_stride, w_stride;  /* multiples of 16 (rows start on 16 bytes; what lies behind in_channels is not read) */
+    int64_t y_stride;
+    const int8_t* x;             /* [tokens][in_channels], 16-byte aligned */
+    const float* x_scale;        /* [tokens] */
+    const int8_t* w;             /* [out_channels][in_channels], 16-byte aligned */
+    const float* w_scale;        /* [out_channels] */
+    const float* bias;           /* [out_channels] or NULL */
+    void* y;                     /* [tokens][out_channels] */
+} pb_int8_dense_params;
+PB_API int pb_int8_dense_info(const pb_int8_dense_params* p, pb_launch_info* out);
+PB_API int pb_int8_dense_launch(const pb_int8_dense_params* p, void* stream, uint32_t job_id, void* notifier);
+
 /* Norms of queries and keys for each head, and their rotation by position, in one pass.
  * z = x * weight / sqrt(mean(x^2) + eps) over a head's head_dim values (weight NULL: z = x), then for each pair (a, b) of
  * the first rot_dim values of z, with c and s of the pair at the token's position: (a c - b s, b c + a s).  Pairs are

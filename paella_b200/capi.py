@@ -39,6 +39,17 @@ class OpParams(C.Structure):
                 ("batch", C.c_int32), ("dil_h", C.c_int32), ("dil_w", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Int8QuantizeParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "channels", "x_dtype", "reserved")] + [(n, C.c_int64) for n in ("x_stride", "q_stride")] + \
+               [(n, C.c_void_p) for n in ("x", "q", "scale")]
+
+
+class Int8DenseParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "in_channels", "out_channels", "y_dtype", "act", "reserved")] + \
+               [(n, C.c_int64) for n in ("x_stride", "w_stride", "y_stride")] + \
+               [(n, C.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "y")]
+
+
 class QkRopeParams(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("dtype", "tokens", "q_heads", "kv_heads", "head_dim", "rot_dim", "interleaved", "max_position")] + \
                [("eps", C.c_float), ("reserved", C.c_int32)] + \
@@ -155,6 +166,10 @@ SIGNATURES = {
     "pb_op_pack_weights": (C.c_int64, [_I, C.POINTER(OpParams), _VP, _VP]),
     "pb_conv_umma_supported": (_I, [C.POINTER(OpParams)]),
     "pb_conv2d_umma_noalloc": (_I, [C.POINTER(OpParams), _VP, _U32, _VP]),
+    "pb_int8_quantize_info": (_I, [C.POINTER(Int8QuantizeParams), C.POINTER(LaunchInfo)]),
+    "pb_int8_quantize_launch": (_I, [C.POINTER(Int8QuantizeParams), _VP, _U32, _VP]),
+    "pb_int8_dense_info": (_I, [C.POINTER(Int8DenseParams), C.POINTER(LaunchInfo)]),
+    "pb_int8_dense_launch": (_I, [C.POINTER(Int8DenseParams), _VP, _U32, _VP]),
     "pb_qk_rope_info": (_I, [C.POINTER(QkRopeParams), C.POINTER(LaunchInfo)]),
     "pb_qk_rope_launch": (_I, [C.POINTER(QkRopeParams), _VP, _U32, _VP]),
     "pb_kv_append_info": (_I, [C.POINTER(KvAppendParams), C.POINTER(LaunchInfo)]),

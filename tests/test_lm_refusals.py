@@ -55,3 +55,36 @@ def test_declared_work():
     assert li.bytes == 4 * (2 * 2 * 64 * 6 + 4 * 64 + 4) and li.threads_per_block == 256 and li.num_blocks >= 1
     li = lu.info("kv_append", append(tokens=0))
     assert li.bytes == 0 and li.num_blocks == 1
+
+
+def quantize(**over):
+    return capi.Int8QuantizeParams(**{**dict(tokens=4, channels=64, x_dtype=capi.BF16, x_stride=64, q_stride=64, x=A, q=A, scale=A), **over})
+
+
+def dense(**over):
+    return capi.Int8DenseParams(**{**dict(tokens=4, in_channels=64, out_channels=32, y_dtype=capi.BF16, x_stride=64, w_stride=64, y_stride=32, x=A, x_scale=A, w=A, w_scale=A, y=A), **over})
+
+
+@pytest.mark.parametrize("over", [dict(tokens=-1), dict(channels=0), dict(x_dtype=3), dict(x=None), dict(q=None), dict(scale=None), dict(x=A + 1), dict(scale=A + 2)])
+def test_quantize_refusals(over):
+    assert lu.refused("int8_quantize", quantize(**over)).startswith("pb_int8_quantize")
+
+
+@pytest.mark.parametrize("over", [dict(tokens=-1), dict(in_channels=0), dict(out_channels=0), dict(in_channels=131072, x_stride=131072, w_stride=131072), dict(y_dtype=3), dict(act=3), dict(act=-1),
+                                  dict(x_stride=72), dict(w_stride=8), dict(x_stride=48), dict(w_stride=48), dict(x=A + 8), dict(w=A + 4), dict(x=None), dict(x_scale=None), dict(w=None),
+                                  dict(w_scale=None), dict(y=None), dict(y=A + 1), dict(bias=A + 2), dict(x_scale=A + 1)])
+def test_dense_refusals(over):
+    assert lu.refused("int8_dense", dense(**over)).startswith("pb_int8_dense")
+
+
+def test_int8_struct_sizes_and_null_params():
+    assert C.sizeof(capi.Int8QuantizeParams) == 4 * 4 + 2 * 8 + 3 * 8 and C.sizeof(capi.Int8DenseParams) == 6 * 4 + 3 * 8 + 6 * 8
+    L, li = capi.load(), capi.LaunchInfo()
+    for name in ("int8_quantize", "int8_dense"):
+        assert getattr(L, f"pb_{name}_info")(None, C.byref(li)) == -2
+        assert getattr(L, f"pb_{name}_launch")(None, None, 0, None) == -2
+
+
+def test_declared_work_of_a_dense_layer():
+    li = lu.info("int8_dense", dense(bias=A))
+    assert li.flops == 2 * 4 * 64 * 32 and li.bytes == 4 * 64 + 32 * 64 + 4 * 4 + 8 * 32 + 2 * 4 * 32
