@@ -317,6 +317,40 @@ typedef struct pb_kv_append_params {
 PB_API int pb_kv_append_info(const pb_kv_append_params* p, pb_launch_info* out);
 PB_API int pb_kv_append_launch(const pb_kv_append_params* p, void* stream, uint32_t job_id, void* notifier);
 
+/* Attention of one new token for every sequence of a batch whose sequences share a prefix, over a paged cache.  Sequence b
+ * sees the prefix's prefix_len tokens (pages prefix_pages[0 ..], read once for the whole batch) and then its own
+ * own_lens[b] tokens (pages block_table[b][0 ..]): out = softmax(scale * q K^T) V, query head h over key head
+ * h / (q_heads / kv_heads).  Products of bf16 / fp16 operands in fp32; softmax in fp32, its values rounded to the
+ * cache's type before they meet V.  A sequence that sees no token at all gets zeros.  What lies in a page behind the
+ * last token is not used, whatever it holds.
+ * A length outside of [0, max_own_len] counts as the nearer end, a page number outside of [0, n_pages) as a page of
+ * zeros. */
+typedef struct pb_prefix_attn_params {
+    int32_t dtype;               /* PB_BF16 or PB_F16 */
+    int32_t batch;               /* 0 = nothing to do */
+    int32_t q_heads, kv_heads;   /* q_heads a multiple of kv_heads */
+    int32_t head_dim;            /* a multiple of 8, 8 to 128 */
+    int32_t page_size;           /* a multiple of 8 */
+    int32_t max_blocks;          /* entries of a row of block_table that may be read */
+    int32_t prefix_len;          /* tokens, >= 0; ends anywhere in its last page */
+    int32_t max_own_len;         /* the most that own_lens holds; <= max_blocks * page_size */
+    float scale;
+    int64_t n_pages;
+    int64_t q_stride, q_head_stride, out_stride, out_head_stride;    /* of q and out */
+    int64_t page_stride, token_stride, head_stride;                  /* of k_cache and v_cache: multiples of 8 */
+    int64_t table_stride;        /* of block_table, from sequence to sequence */
+    const void* q;               /* [batch][q_heads][head_dim], 16-byte aligned rows */
+    void* out;
+    const void *k_cache, *v_cache;   /* 16-byte aligned */
+    const int32_t* prefix_pages; /* [ceil(prefix_len / page_size)] */
+    const int32_t* block_table;  /* [batch][max_blocks]; NULL when max_own_len is 0 */
+    const int32_t* own_lens;     /* [batch]; NULL when max_own_len is 0 */
+    void* scratch;               /* pb_launch_info.scratch_bytes of device memory, 16-byte aligned, for one launch in flight at */
+    uint64_t scratch_bytes;      /* a time; written before it is read, so it needs no initialisation */
+} pb_prefix_attn_params;
+PB_API int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out);
+PB_API int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t job_id, void* notifier);
+
 /* ------------------------------------------------------------------------ *
  * Model packs and instances: the graph executor behind the model job adapters
  * (replaces tvm::runtime::Module::LoadFromFile + "run"/"get_input"/"get_output",

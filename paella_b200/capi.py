@@ -66,6 +66,15 @@ class KvAppendParams(C.Structure):
                [(n, C.c_void_p) for n in ("k", "v", "k_weight", "cos_sin", "positions", "slots", "k_cache", "v_cache", "q", "q_out", "q_weight")]
 
 
+class PrefixAttnParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "page_size", "max_blocks", "prefix_len", "max_own_len")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_int64) for n in ("n_pages", "q_stride", "q_head_stride", "out_stride", "out_head_stride", "page_stride", "token_stride", "head_stride",
+                                         "table_stride")] + \
+               [(n, C.c_void_p) for n in ("q", "out", "k_cache", "v_cache", "prefix_pages", "block_table", "own_lens", "scratch")] + \
+               [("scratch_bytes", C.c_uint64)]
+
+
 class ServerConfig(C.Structure):
     _fields_ = [("device", C.c_int32), ("num_streams", C.c_uint32), ("extra_kernels", C.c_uint32),
                 ("unfairness_threshold", C.c_float), ("sched_sleep", C.c_uint32), ("ring_capacity", C.c_uint64),
@@ -174,6 +183,8 @@ SIGNATURES = {
     "pb_qk_rope_launch": (_I, [C.POINTER(QkRopeParams), _VP, _U32, _VP]),
     "pb_kv_append_info": (_I, [C.POINTER(KvAppendParams), C.POINTER(LaunchInfo)]),
     "pb_kv_append_launch": (_I, [C.POINTER(KvAppendParams), _VP, _U32, _VP]),
+    "pb_prefix_attn_info": (_I, [C.POINTER(PrefixAttnParams), C.POINTER(LaunchInfo)]),
+    "pb_prefix_attn_launch": (_I, [C.POINTER(PrefixAttnParams), _VP, _U32, _VP]),
     "pb_device_error_flag": (_I, [_I, C.POINTER(_U32), _I]),
     "pb_set_conv_split_gain_us": (None, [C.c_double]),
     "pb_conv_umma_time": (_I, [C.POINTER(OpParams), _I, _I, _SZ, C.POINTER(C.c_double)]),

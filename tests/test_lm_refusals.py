@@ -88,3 +88,29 @@ def test_int8_struct_sizes_and_null_params():
 def test_declared_work_of_a_dense_layer():
     li = lu.info("int8_dense", dense(bias=A))
     assert li.flops == 2 * 4 * 64 * 32 and li.bytes == 4 * 64 + 32 * 64 + 4 * 4 + 8 * 32 + 2 * 4 * 32
+
+
+def attn(**over):
+    f = dict(dtype=capi.BF16, batch=4, q_heads=8, kv_heads=2, head_dim=64, page_size=16, max_blocks=4, prefix_len=100, max_own_len=64, scale=0.125, n_pages=40, q_stride=512,
+             q_head_stride=64, out_stride=512, out_head_stride=64, page_stride=2048, token_stride=128, head_stride=64, table_stride=4, q=A, out=A, k_cache=A, v_cache=A,
+             prefix_pages=A, block_table=A, own_lens=A, scratch=A, scratch_bytes=1 << 40)
+    return capi.PrefixAttnParams(**{**f, **over})
+
+
+@pytest.mark.parametrize("over", [dict(dtype=capi.F32), dict(dtype=3), dict(batch=-1), dict(q_heads=0), dict(kv_heads=0), dict(q_heads=7), dict(head_dim=136), dict(head_dim=12), dict(head_dim=0),
+                                  dict(page_size=0), dict(page_size=12), dict(max_blocks=-1), dict(max_own_len=65), dict(max_own_len=-1), dict(prefix_len=-1), dict(scale=float("nan")),
+                                  dict(scale=float("inf")), dict(n_pages=-1), dict(n_pages=2 ** 31), dict(page_stride=2050), dict(token_stride=4), dict(head_stride=63), dict(q_stride=12), dict(q_head_stride=4),
+                                  dict(q=A + 8), dict(k_cache=A + 2), dict(v_cache=A + 8), dict(out=A + 1), dict(q=None), dict(out=None), dict(k_cache=None), dict(v_cache=None),
+                                  dict(prefix_pages=None), dict(block_table=None), dict(own_lens=None), dict(own_lens=A + 2)])
+def test_attention_refusals(over):
+    assert lu.refused("prefix_attn", attn(**over)).startswith("pb_prefix_attn")
+
+
+def test_attention_struct_size_and_declared_work():
+    assert C.sizeof(capi.PrefixAttnParams) == 10 * 4 + 9 * 8 + 9 * 8
+    li = lu.info("prefix_attn", attn())
+    assert li.flops == 4 * 64 * 8 * 4 * 164 and li.num_blocks >= 1
+    assert lu.info("prefix_attn", attn(prefix_len=0, prefix_pages=None)).num_blocks >= 1
+    assert lu.info("prefix_attn", attn(max_own_len=0, block_table=None, own_lens=None, max_blocks=0)).num_blocks >= 1
+    L = capi.load()
+    assert L.pb_prefix_attn_info(None, C.byref(li)) == -2 and L.pb_prefix_attn_launch(None, None, 0, None) == -2
