@@ -2409,6 +2409,19 @@ int encode_tiled_bf16(const void* base, int rank, const uint64_t* dims, const ui
     return PB_OK;
 }
 
+int encode_tiled_sw128(CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMap* out) {
+    EncodeTiledFn enc = encode_fn();
+    PB_REQUIRE(enc != nullptr, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(out, type, (cuuint32_t)rank, const_cast<void*>(base), (const cuuint64_t*)dims, (const cuuint64_t*)strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with CUresult %d (rank %d, box %u x %u)", (int)r, rank, box[0], box[1]);
+        return PB_ERR_INVALID;
+    }
+    return PB_OK;
+}
+
 int encode_pixels_f32(const void* base, int channels, int stride, int W, int H, int batch, int pad_w, int pad_h, int reach_w, int reach_h, int stride_w,
                       int stride_h, bool tiled, int box_channels, int box_pixels, CUtensorMap* out) {
     CUresult r;

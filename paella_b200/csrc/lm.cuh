@@ -6,6 +6,7 @@
 #include <llis/job/finished_block_notifier.h>
 
 #include <cstring>
+#include <type_traits>
 
 #include "launch_slot.cuh"
 #include "ops.h"
@@ -16,7 +17,7 @@ namespace pb {
 using llis::job::FinishedBlockNotifier;
 
 // Codes of the error flag.
-constexpr uint32_t kFlagLmPosition = 0x301, kFlagLmSlot = 0x302, kFlagLmLength = 0x303, kFlagLmPage = 0x304;
+constexpr uint32_t kFlagLmPosition = 0x301, kFlagLmSlot = 0x302, kFlagLmLength = 0x303, kFlagLmPage = 0x304, kFlagLmWait = 0x310;
 
 inline size_t dtype_bytes(int dtype) { return dtype == PB_F32 ? 4 : 2; }
 inline bool is_float_dtype(int dtype) { return dtype == PB_F32 || dtype == PB_BF16 || dtype == PB_F16; }

@@ -46,6 +46,10 @@ double conv_split_gain_us();      // see pb_set_conv_split_gain_us
 // Tensor map of a bf16 tensor without swizzle; elements outside read as zeros, or as NaN.
 int encode_tiled_bf16(const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, bool nan_fill, CUtensorMap* out);
 
+// Tensor map whose boxes arrive with the 128-byte swizzle of the tensor cores' operands; elements outside read as zeros.  strides: bytes, of
+// dimensions 1 and up.  PB_ERR_INVALID where the driver does not take the sizes or strides.
+int encode_tiled_sw128(CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMap* out);
+
 // conv_umma.cu: tcgen05 implicit-GEMM convolution (bf16 operands, fp32 accumulation in TMEM)
 bool conv_umma_supported(const pb_op_params* p);
 // How a launch is cut.  It travels beside pb_op_params: a launch that is given none (NULL below) has the GPU to itself and
