@@ -4,108 +4,472 @@
 //   q[t][k] = rint(x[t][k] * (127 * (1 / max_t))), s[t] = max_t / 127;   y[t][n] = act(s[t] * ws[n] * sum_k q[t][k] w[n][k] + b[n])
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "lm.cuh"
+#include "umma.cuh"
 
 namespace pb {
 namespace {
 
+__device__ uint32_t g_int8_flag;
+
 // ---- activations to 8 bits ---------------------------------------------------------------
-// A block takes a row: the largest magnitude first, then the row again (from the caches) for the integers.
-template <typename T>
-__global__ void __launch_bounds__(256) int8_quantize_kernel(const T* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int tokens, int channels,
-                                                            uint32_t job_id, FinishedBlockNotifier* nf) {
+// Bound by memory: a row is read once, stays in registers, and leaves as a quarter or half of its bytes.  `Row` threads take a row (a warp a
+// short one, the block a long one) in vectors of 16 bytes; what does not fit the registers is read a second time, from the caches.
+struct QuantizeArgs {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    int64_t x_stride, q_stride;
+    int tokens, channels;
+};
+
+__device__ __forceinline__ int8_t to_int8(float v, float inv) { return (int8_t)__float2int_rn(v * inv); }
+
+template <typename T, bool WIDE, int ROW>
+__global__ void __launch_bounds__(256) int8_quantize_kernel(const __grid_constant__ QuantizeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1, HELD = WIDE ? 4 : 8;
+    using In = LmVec<T, V>;
+    using Out = LmVec<int8_t, V>;
     __shared__ float red[8];
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
-    const int64_t t = blockIdx.x;
-    if (t < tokens) {
-        const T* row = x + t * x_stride;
-        float most = 0.f;
-        bool odd = false;                              // a NaN or an infinity
-        for (int k = threadIdx.x; k < channels; k += 256) {
-            const float v = fabsf(lm_to_f<T>(row[k]));
-            odd |= !(v <= 3.402823466e38f);
-            most = fmaxf(most, v);
-        }
-        if (odd) most = INFINITY;
+    const int me = threadIdx.x % ROW, vectors = a.channels / V, tail = vectors * V + me;
+    const int64_t t = (int64_t)blockIdx.x * (256 / ROW) + threadIdx.x / ROW;
+    const bool live = t < a.tokens;
+    const T* row = static_cast<const T*>(a.x) + (live ? t : 0) * a.x_stride;
+    const int mine = live ? vectors : 0;
+    In held[HELD];
+    float most = 0.f;
+    bool odd = false;                                  // a NaN or an infinity
+    const auto look = [&](float v) {
+        v = fabsf(v);
+        odd |= !(v <= 3.402823466e38f);
+        most = fmaxf(most, v);
+    };
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int i = 0; i < HELD; ++i)
+        if (me + i * ROW < mine) held[i] = *reinterpret_cast<const In*>(row + (int64_t)(me + i * ROW) * V);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (me + i * ROW < mine) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) look(lm_to_f<T>(held[i].v[j]));
+        }
+    for (int i = me + HELD * ROW; i < mine; i += ROW) {
+        const In x = *reinterpret_cast<const In*>(row + (int64_t)i * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) look(lm_to_f<T>(x.v[j]));
+    }
+    const bool has_tail = live && tail < a.channels;   // (fewer than V values)
+    const float last = has_tail ? lm_to_f<T>(row[tail]) : 0.f;
+    look(last);
+    if (odd) most = INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (ROW > 32) {
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
         __syncthreads();
         most = red[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, red[i]);
-        const bool zero = !(most >= 0x1p-119f) || most == INFINITY;
-        const float inv = zero ? 0.f : 127.f * __fdiv_rn(1.f, most);
-        if (threadIdx.x == 0) scale[t] = most == INFINITY ? NAN : zero ? 0.f : __fdiv_rn(most, 127.f);
-        for (int k = threadIdx.x; k < channels; k += 256) q[t * q_stride + k] = zero ? (int8_t)0 : (int8_t)__float2int_rn(lm_to_f<T>(row[k]) * inv);
     }
+    const bool zero = !(most >= 0x1p-119f) || most == INFINITY;
+    const float inv = zero ? 0.f : 127.f * __fdiv_rn(1.f, most);
+    if (live && me == 0) a.scale[t] = most == INFINITY ? NAN : zero ? 0.f : __fdiv_rn(most, 127.f);
+    int8_t* dst = a.q + (live ? t : 0) * a.q_stride;
+    const auto put = [&](int i, const In& x) {
+        Out q;
+#pragma unroll
+        for (int j = 0; j < V; ++j) q.v[j] = zero ? (int8_t)0 : to_int8(lm_to_f<T>(x.v[j]), inv);
+        *reinterpret_cast<Out*>(dst + (int64_t)i * V) = q;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (me + i * ROW < mine) put(me + i * ROW, held[i]);
+    for (int i = me + HELD * ROW; i < mine; i += ROW) put(i, *reinterpret_cast<const In*>(row + (int64_t)i * V));
+    if (has_tail) dst[tail] = zero ? (int8_t)0 : to_int8(last, inv);
     if (nf) nf->end(job_id);
+}
+
+typedef void (*QuantizeFn)(QuantizeArgs, uint32_t, FinishedBlockNotifier*);
+struct QuantizePlan {
+    QuantizeFn fn;
+    unsigned blocks;
+};
+template <typename T> QuantizeFn quantize_fn(bool wide, bool warp) {
+    if (wide) return warp ? int8_quantize_kernel<T, true, 32> : int8_quantize_kernel<T, true, 256>;
+    return warp ? int8_quantize_kernel<T, false, 32> : int8_quantize_kernel<T, false, 256>;
 }
 
 // ---- the product ---------------------------------------------------------------------------
+// Y^T = W X^T on the tensor cores: operand A is 128 output channels, operand B up to 256 tokens, both as they lie in memory (rows
+// of in_channels, 128 bytes a k-block, the 128-byte swizzle), the sums 32-bit integers in tensor memory, a lane for each channel.
+// So a weight row's scale and bias are a thread's own, few tokens make a narrow tile instead of an empty one, and neighbouring
+// lanes hold neighbouring values of y.
+//
+// Few tokens are bound by reading the weights, many by the tensor cores.  int8_few_kernel: a tile of 128 channels for each block, its
+// reduction shared by the blocks of a cluster where the tiles alone leave SMs idle; the sums meet in shared memory (whole numbers:
+// their order changes nothing).  int8_many_kernel: a pair of SMs on a tile of 256 channels, each block with its own half of the
+// channels and half of the tokens: 32 KB a k-block and SM for 512 clocks of products, which the path from the L2 cache into an SM (some 60 bytes a
+// clock) feeds; a lone SM on 128 x 256 would need 48 KB.
 struct DenseArgs {
-    const int8_t *x, *w;
     const float *x_scale, *w_scale, *bias;
     void* y;
-    int64_t x_stride, w_stride, y_stride;
+    int64_t y_stride;
     int T, K, N, act;
+    int kblocks, BN, stages, splits;       // BN: tokens of a tile
+    int channel_tiles, token_tiles;
+    int y_vec;                             // rows of y take 16-byte stores
 };
 
-__device__ __forceinline__ float int8_result(const DenseArgs& a, int acc, float xs, float ws, float b) {
-    float v = fmaf((float)acc, xs * ws, b);
-    if (a.act >= 1) v = v < 0.f ? 0.f : v;             // (a NaN stays one)
-    if (a.act == 2) v = v > 6.f ? 6.f : v;
+constexpr uint32_t kABytes = 128 * 128;
+constexpr int kMaxInt8Stages = 16;
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Signed 8-bit operands, both along k, 32-bit integer sums.
+__device__ __forceinline__ uint32_t i8_idesc(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+__device__ __forceinline__ float int8_result(int act, int acc, float s, float b) {
+    float v = fmaf((float)acc, s, b);
+    if (act >= 1) v = v < 0.f ? 0.f : v;               // (a NaN stays one)
+    if (act == 2) v = v > 6.f ? 6.f : v;
     return v;
 }
 
-// 64 x 64 results of a block, four by four a thread; four products an instruction.
+__device__ __forceinline__ void wait_for_copies() {    // an aborted block's copies end before their shared memory does
+    const unsigned long long t0 = globaltimer_ns();
+    for (int i = 0; i < 100000 && globaltimer_ns() - t0 < 50000; ++i) __nanosleep(500);
+}
+
 template <typename Y>
-__global__ void __launch_bounds__(256) int8_dense_kernel(DenseArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
-    __shared__ int sx[16][65], sw[16][65];             // 64 bytes of each row, word by word
+__global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                                                       uint32_t job_id, FinishedBlockNotifier* nf) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_full[kMaxInt8Stages], s_empty[kMaxInt8Stages], s_sums;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile uint32_t s_abort;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 128u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
+    const int n0 = tile % a.channel_tiles * 128, t0 = tile / a.channel_tiles * a.BN;
+    const int kb0 = a.kblocks * rank / a.splits, nkb = a.kblocks * (rank + 1) / a.splits - kb0;
+    uint32_t cols = 32;
+    while ((int)cols < a.BN) cols *= 2;
+    if (warp == 5) {
+        tcgen05_alloc(smem_u32(&s_tmem), cols);
+        tcgen05_relinquish();
+    }
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int i = 0; i < a.stages; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&s_sums), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (warp == 4 && elect_one()) {
+        // the weights come into the L2 cache while the launch that makes the activations still runs
+        for (int i = 0; i < nkb && i < a.stages; ++i)
+            asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&wmap), "r"((kb0 + i) * 128), "r"(n0) : "memory");
+    }
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, row = threadIdx.x >> 2, part = threadIdx.x & 3;
-    const int tiles = (a.N + 63) / 64, t0 = (int)(blockIdx.x / tiles) * 64, n0 = (int)(blockIdx.x % tiles) * 64;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += 64) {
-        const int k = k0 + 16 * part;
+    bool ok = true;
+    if (warp == 4) {
+        for (int i = 0; i < nkb; ++i) {
+            const int st = i % a.stages, use = i / a.stages;
+            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), (use - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) break;
+            if (elect_one()) {
+                const uint32_t bar = smem_u32(&s_full[st]), at = ring + st * stage_bytes;
+                mbar_arrive_expect_tx(bar, stage_bytes);
+                tma_load_2d(at, &wmap, (kb0 + i) * 128, n0, bar);
+                tma_load_2d(at + kABytes, &xmap, (kb0 + i) * 128, t0, bar);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 5) {
+        const uint32_t idesc = i8_idesc(128, a.BN);
+        for (int i = 0; i < nkb; ++i) {
+            const int st = i % a.stages;
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), (i / a.stages) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
+            if (!ok) break;
+            tcgen05_fence_after();
+            const uint64_t da = umma_desc_sw128(ring + st * stage_bytes), db = umma_desc_sw128(ring + st * stage_bytes + kABytes);
+            if (elect_one()) {
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const int r = (which ? n0 : t0) + row;
-            const int8_t* src = which ? a.w + r * a.w_stride : a.x + r * a.x_stride;
-            int v[4] = {0, 0, 0, 0};
-            if (r < (which ? a.N : a.T) && k < a.K) {
-                if (k + 16 <= a.K) {
-                    *reinterpret_cast<int4*>(v) = *reinterpret_cast<const int4*>(src + k);
-                } else {
-                    for (int j = 0; j < a.K - k; ++j) v[j / 4] |= (int)(uint8_t)src[k + j] << (8 * (j % 4));
+                for (int k = 0; k < 4; ++k) mma_i8<false>(tmem, da + 2 * k, db + 2 * k, idesc, i > 0 || k > 0);
+                tcgen05_commit(smem_u32(&s_empty[st]));
+            }
+            __syncwarp();
+        }
+        if (ok && elect_one()) tcgen05_commit(smem_u32(&s_sums));
+        __syncwarp();
+    }
+    const int n = n0 + 32 * (warp & 3) + lane, tokens = min(a.BN, a.T - t0);
+    const bool mine = warp < 4 && n < a.N;
+    const float ws = mine ? __ldg(a.w_scale + n) : 0.f, bias = mine && a.bias ? __ldg(a.bias + n) : 0.f;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    if (warp < 4) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_sums), 0, &s_abort, &g_int8_flag, kFlagLmWait));
+        tcgen05_fence_after();
+        if (ok) {
+            for (int j0 = 0; j0 < tokens; j0 += 16) {
+                uint32_t v[16];
+                tcgen05_ld16(lanes + j0, v);
+                tcgen05_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (a.splits > 1) {                // [token][channel] of this block's sums, over the operands that made them
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + (uint32_t)((j0 + j) * 128 + 32 * warp + lane) * 4u), "r"(v[j]) : "memory");
+                    } else if (mine && j0 + j < tokens) {
+                        static_cast<Y*>(a.y)[(int64_t)(t0 + j0 + j) * a.y_stride + n] = lm_from_f<Y>(int8_result(a.act, (int)v[j], __ldcg(a.x_scale + t0 + j0 + j) * ws, bias));
+                    }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) (which ? sw : sx)[4 * part + j][row] = v[j];
         }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int l = 0; l < 4; ++l) acc[i][l] = __dp4a(sx[j][ty * 4 + i], sw[j][tx * 4 + l], acc[i][l]);
-        __syncthreads();
     }
-    for (int i = 0; i < 4; ++i)
-        for (int l = 0; l < 4; ++l) {
-            const int t = t0 + ty * 4 + i, n = n0 + tx * 4 + l;
-            if (t >= a.T || n >= a.N) continue;
-            static_cast<Y*>(a.y)[t * a.y_stride + n] = lm_from_f<Y>(int8_result(a, acc[i][l], a.x_scale[t], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+    if (a.splits > 1) {
+        cluster_arrive();
+        cluster_wait();
+        if (warp < 4 && ok && mine) {
+            for (int j = rank; j < tokens; j += a.splits) {
+                int sum = 0;
+                for (int r = 0; r < a.splits; ++r) {
+                    int v;
+                    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(ring + (uint32_t)(j * 128 + 32 * warp + lane) * 4u, (uint32_t)r)) : "memory");
+                    sum += v;
+                }
+                static_cast<Y*>(a.y)[(int64_t)(t0 + j) * a.y_stride + n] = lm_from_f<Y>(int8_result(a.act, sum, __ldcg(a.x_scale + t0 + j) * ws, bias));
+            }
         }
+        cluster_arrive();                              // nobody's sums go before everybody has read them
+        cluster_wait();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (s_abort) wait_for_copies();
+    if (warp == 5) {
+        tcgen05_fence_after();
+        tcgen05_dealloc(tmem, cols);
+    }
     if (nf) nf->end(job_id);
 }
+
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar) : "memory");
+}
+// Arrives on the barrier at this offset in both blocks once the pair's products so far are complete.
+__device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+__device__ __forceinline__ bool all_of_128(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
+}
+
+constexpr uint32_t kOutBytes = 32 * 128 * 4;           // 32 tokens of 128 channels on their way out
+
+// A pair of blocks walks its share of the tiles.  Warps 0-3: results, a lane a channel; warp 4: copies of this block's operands; warp 5 of the first
+// block: the products of both.  Two accumulators: the results of a tile leave under the products of the next.
+template <typename Y>
+__global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                                                           uint32_t job_id, FinishedBlockNotifier* nf) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_full[kMaxInt8Stages], s_empty[kMaxInt8Stages], s_sums[2], s_read[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile uint32_t s_abort;
+    __shared__ float s_xs[256];
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 64u, out = ring + a.stages * stage_bytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x & 1, pairs = gridDim.x / 2, tiles = a.channel_tiles * a.token_tiles;
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int i = 0; i < a.stages; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s_sums[i]), 1);
+            mbar_init(smem_u32(&s_read[i]), 2);        // the results warps of both blocks
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();                                    // both blocks' barriers and tensor memory are set up
+    tcgen05_fence_after();
+    const uint32_t tmem = s_tmem;
+    griddep_wait();
+    if (nf) nf->start(job_id);
+    griddep_launch();
+
+    // Neighbouring pairs take the tokens of the same channels, then the next channels: all of them together read few rows of both operands.
+    if (warp == 4) {
+        int it = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+            const int n0 = tile / a.token_tiles * 256 + 128 * rank, t0 = tile % a.token_tiles * a.BN + (a.BN / 2) * rank;
+            for (int i = 0; i < a.kblocks; ++i, ++it) {
+                const int st = it % a.stages, use = it / a.stages;
+                if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), (use - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&s_full[st]), first = cluster_addr(bar, 0u), at = ring + st * stage_bytes;
+                    if (rank == 0) mbar_arrive_expect_tx(bar, 2 * stage_bytes);      // both blocks' copies
+                    tma_load_2d_pair(at, &wmap, i * 128, n0, first);
+                    tma_load_2d_pair(at + kABytes, &xmap, i * 128, t0, first);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 5) {
+        if (rank == 0) {
+            const uint32_t idesc = i8_idesc(256, a.BN);
+            int it = 0, turn = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs, ++turn) {
+                const int acc = turn & 1;
+                if (turn >= 2) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_read[acc]), (turn / 2 - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
+                if (!ok) break;
+                tcgen05_fence_after();
+                for (int i = 0; i < a.kblocks; ++i, ++it) {
+                    const int st = it % a.stages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), (it / a.stages) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint64_t da = umma_desc_sw128(ring + st * stage_bytes), db = umma_desc_sw128(ring + st * stage_bytes + kABytes);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_i8<true>(tmem + 256 * acc, da + 2 * k, db + 2 * k, idesc, i > 0 || k > 0);
+                        tcgen05_commit_pair(smem_u32(&s_empty[st]));
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one()) tcgen05_commit_pair(smem_u32(&s_sums[acc]));
+                __syncwarp();
+            }
+        }
+    } else {
+        int turn = 0;
+        for (int tile = blockIdx.x >> 1; tile < tiles; tile += pairs, ++turn) {
+            const int acc = turn & 1, n0 = tile / a.token_tiles * 256 + 128 * rank, t0 = tile % a.token_tiles * a.BN, tokens = min(a.BN, a.T - t0);
+            const int n = n0 + 32 * warp + lane;
+            const float ws = n < a.N ? __ldg(a.w_scale + n) : 0.f, bias = n < a.N && a.bias ? __ldg(a.bias + n) : 0.f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");                         // the last tile's scales and values have been read
+            for (int j = threadIdx.x; j < a.BN; j += 128) s_xs[j] = j < tokens ? __ldcg(a.x_scale + t0 + j) : 0.f;
+            // (the four warps go on together or not at all: they meet at barriers)
+            if (!all_of_128(mbar_wait(smem_u32(&s_sums[acc]), (turn / 2) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) break;
+            tcgen05_fence_after();
+            for (int j0 = 0; j0 < a.BN; j0 += 32) {
+                if (j0 >= tokens) break;
+                uint32_t v[32];
+                tcgen05_ld32(tmem + ((uint32_t)warp << 21) + 256 * acc + j0, v);
+                tcgen05_wait_ld();
+                if (j0 + 32 >= tokens) {                                            // the accumulator's last columns: it may be written again
+                    tcgen05_fence_before();
+                    __syncwarp();
+                }
+                const uint32_t me = out + (uint32_t)(32 * warp + lane) * 4u;
+                if constexpr (sizeof(Y) == 4) {        // [token][channel]
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(me + j * 512), "f"(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias)) : "memory");
+                } else {                               // two tokens a word: [token / 2][channel]
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(me + j * 256),
+                                     "r"(lm_pack2<Y>(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias), int8_result(a.act, (int)v[j + 1], s_xs[j0 + j + 1] * ws, bias))) : "memory");
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                // out: 16 bytes of a row for each thread where y's rows allow it, and the lanes side by side in any case
+                const int left = min(32, tokens - j0), width = min(128, a.N - n0);
+                Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + j0) * a.y_stride + n0;
+                if constexpr (sizeof(Y) == 4) {
+                    if (a.y_vec && width == 128) {
+                        for (int i = threadIdx.x; i < left * 32; i += 128) *reinterpret_cast<uint4*>(dst + (i >> 5) * a.y_stride + (i & 31) * 4) = ld_shared_v4(out + i * 16);
+                    } else {
+                        for (int j = 0; j < left; ++j)
+                            if ((int)threadIdx.x < width) {
+                                float f;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(out + j * 512 + threadIdx.x * 4) : "memory");
+                                dst[j * a.y_stride + threadIdx.x] = f;
+                            }
+                    }
+                } else {
+                    if (a.y_vec && width == 128) {
+                        for (int i = threadIdx.x; i < 16 * 16; i += 128) {         // tokens 2 (i / 16) and + 1, channels 8 (i % 16) and up
+                            const uint4 p = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32), q = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32 + 16);
+                            Y* at = dst + (i >> 4) * 2 * a.y_stride + (i & 15) * 8;
+                            if ((i >> 4) * 2 < left)
+                                *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(p.x, p.y, 0x5410), __byte_perm(p.z, p.w, 0x5410), __byte_perm(q.x, q.y, 0x5410), __byte_perm(q.z, q.w, 0x5410));
+                            if ((i >> 4) * 2 + 1 < left)
+                                *reinterpret_cast<uint4*>(at + a.y_stride) = make_uint4(__byte_perm(p.x, p.y, 0x7632), __byte_perm(p.z, p.w, 0x7632), __byte_perm(q.x, q.y, 0x7632), __byte_perm(q.z, q.w, 0x7632));
+                        }
+                    } else {
+                        for (int j = 0; j < left; ++j)
+                            if ((int)threadIdx.x < width) {
+                                uint32_t f;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(f) : "r"(out + (j >> 1) * 512 + threadIdx.x * 4) : "memory");
+                                const uint16_t h = (uint16_t)(j & 1 ? f >> 16 : f);
+                                dst[j * a.y_stride + threadIdx.x] = *reinterpret_cast<const Y*>(&h);
+                            }
+                    }
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            if (threadIdx.x == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_u32(&s_read[acc]), 0u)) : "memory");
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (s_abort) wait_for_copies();
+    cluster_arrive();
+    cluster_wait();                                    // neither block's memory goes before both have finished
+    if (warp == 5) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (nf) nf->end(job_id);
+}
+
+// No tokens: the records alone.
+__global__ void int8_nothing_kernel(uint32_t job_id, FinishedBlockNotifier* nf) {
+    griddep_wait();
+    if (nf) nf->start(job_id);
+    if (nf) nf->end(job_id);
+}
+
+typedef void (*DenseFn)(DenseArgs, CUtensorMap, CUtensorMap, uint32_t, FinishedBlockNotifier*);
+struct DensePlan {
+    DenseArgs a;
+    bool many;
+    DenseFn fn;
+    unsigned blocks;
+    uint32_t smem, tmem_cols;
+};
 
 int check_quantize(const pb_int8_quantize_params* p) {
     const char* who = "pb_int8_quantize";
@@ -134,7 +498,85 @@ int check_dense(const pb_int8_dense_params* p) {
     return PB_OK;
 }
 
+int plan_quantize(const pb_int8_quantize_params* p, QuantizePlan& pl) {
+    const int rc = check_quantize(p);
+    if (rc != PB_OK) return rc;
+    const size_t es = dtype_bytes(p->x_dtype);
+    const int V = (int)(16 / es);
+    const bool wide = aligned(p->x, 16) && p->x_stride % V == 0 && aligned(p->q, V) && p->q_stride % V == 0;
+    // a warp holds 128 vectors of a row; longer rows take a block
+    const bool warp = p->channels <= 128 * (wide ? V : 2);
+    pl.fn = p->x_dtype == PB_F32 ? quantize_fn<float>(wide, warp) : p->x_dtype == PB_BF16 ? quantize_fn<__nv_bfloat16>(wide, warp) : quantize_fn<__half>(wide, warp);
+    pl.blocks = p->tokens > 0 ? (unsigned)(warp ? ceil_div(p->tokens, 8) : p->tokens) : 1u;
+    return PB_OK;
+}
+
+// Clocks of a launch, from what an SM does in one: products of BN tokens with 128 channels (four instructions a k-block, BN / 2 clocks each, but no fewer
+// than shared memory needs for both operands at 128 bytes a clock), copies at 60 bytes a clock.
+double kblock_clocks(int BN, int b_rows) {
+    const double mma = 4 * std::max(BN / 2.0, 32 + b_rows / 4.0), copy = (128 + b_rows) * 128 / 60.0;
+    return std::max(mma, copy);
+}
+
+int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
+    const int rc = check_dense(p);
+    if (rc != PB_OK) return rc;
+    DenseArgs& a = pl.a;
+    a = {p->x_scale, p->w_scale, p->bias, p->y, p->y_stride, p->tokens, p->in_channels, p->out_channels, p->act};
+    a.kblocks = ceil_div(a.K, 128);
+    const int T = a.T > 0 ? a.T : 1;
+    double best = 1e300;
+    // one block a tile, up to 8 blocks on its reduction
+    for (int tt = ceil_div(T, 128); tt <= ceil_div(T, 128) + 1; ++tt) {
+        const int BN = round_up(ceil_div(T, tt), 16), tiles = ceil_div(T, BN);
+        for (int S = 1; S <= 8 && S <= a.kblocks; S *= 2) {
+            const double blocks = (double)ceil_div(a.N, 128) * tiles * S;
+            const double clocks = std::ceil(blocks / 148) * ceil_div(a.kblocks, S) * kblock_clocks(BN, BN) + (S > 1 ? 1500 + 8.0 * BN : 0) + 10.0 * BN;
+            if (clocks < best) { best = clocks; pl.many = false; a.BN = BN; a.token_tiles = tiles; a.splits = S; }
+        }
+    }
+    // pairs of SMs on 256 channels
+    if (T > 64)
+        for (int BN = 64; BN <= 256; BN += 32) {
+            const int tiles = ceil_div(T, BN);
+            const double clocks = std::ceil((double)ceil_div(a.N, 256) * tiles / 74) * a.kblocks * kblock_clocks(BN, BN / 2) + 2000 + 10.0 * BN;
+            if (clocks < best) { best = clocks; pl.many = true; a.BN = BN; a.token_tiles = tiles; a.splits = 1; }
+        }
+    a.channel_tiles = ceil_div(a.N, pl.many ? 256 : 128);
+    const uint32_t stage = kABytes + (uint32_t)a.BN * (pl.many ? 64 : 128);
+    if (pl.many) {
+        a.stages = (int)std::min<uint32_t>(kMaxInt8Stages, (227 * 1024 - 4096 - kOutBytes) / stage);
+        pl.smem = 1024 + a.stages * stage + kOutBytes;
+        const int64_t tiles = (int64_t)a.channel_tiles * a.token_tiles;
+        PB_REQUIRE(tiles <= 0x3fffffff, "pb_int8_dense: too many results for one launch");
+        pl.blocks = 2 * (unsigned)std::min<int64_t>(tiles, 74);
+        pl.tmem_cols = 512;
+        a.splits = 2;          // blocks of a cluster
+        pl.fn = p->y_dtype == PB_F32 ? int8_many_kernel<float> : p->y_dtype == PB_BF16 ? int8_many_kernel<__nv_bfloat16> : int8_many_kernel<__half>;
+    } else {
+        // two blocks an SM: what they have in flight covers the memory's latency
+        a.stages = (int)std::min<uint32_t>(std::min<uint32_t>(kMaxInt8Stages, ceil_div(a.kblocks, a.splits)), (110 * 1024) / stage);
+        pl.smem = 1024 + std::max<uint32_t>(a.stages * stage, a.splits > 1 ? a.BN * 512 : 0);
+        const int64_t blocks = (int64_t)a.channel_tiles * a.token_tiles * a.splits;
+        PB_REQUIRE(blocks <= 0x7fffffff, "pb_int8_dense: too many results for one launch");
+        pl.blocks = (unsigned)blocks;
+        pl.tmem_cols = 32;
+        while ((int)pl.tmem_cols < a.BN) pl.tmem_cols *= 2;
+        pl.fn = p->y_dtype == PB_F32 ? int8_few_kernel<float> : p->y_dtype == PB_BF16 ? int8_few_kernel<__nv_bfloat16> : int8_few_kernel<__half>;
+    }
+    const int V = (int)(16 / dtype_bytes(p->y_dtype));
+    a.y_vec = aligned(p->y, 16) && p->y_stride % V == 0;
+    return PB_OK;
+}
+
 }  // namespace
+
+uint32_t* lm_int8_error_flag_ptr() {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_int8_flag) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+    return (uint32_t*)p;
+}
+
 }  // namespace pb
 
 using namespace pb;
@@ -142,59 +584,59 @@ using namespace pb;
 extern "C" {
 
 int pb_int8_quantize_info(const pb_int8_quantize_params* p, pb_launch_info* out) {
-    const int rc = check_quantize(p);
+    QuantizePlan pl;
+    const int rc = plan_quantize(p, pl);
     if (rc != PB_OK) return rc;
     PB_REQUIRE(out != nullptr, "pb_int8_quantize_info: NULL out");
     memset(out, 0, sizeof(*out));
-    out->num_blocks = p->tokens > 0 ? (uint32_t)p->tokens : 1u;
+    out->num_blocks = pl.blocks;
     out->threads_per_block = 256;
     out->smem_per_block = 32;
-    out->regs_per_thread = p->x_dtype == PB_F32 ? lm_regs(int8_quantize_kernel<float>) : p->x_dtype == PB_BF16 ? lm_regs(int8_quantize_kernel<__nv_bfloat16>) : lm_regs(int8_quantize_kernel<__half>);
+    out->regs_per_thread = lm_regs(pl.fn);
     out->bytes = (uint64_t)p->tokens * ((dtype_bytes(p->x_dtype) + 1) * p->channels + 4);
     return PB_OK;
 }
 
 int pb_int8_quantize_launch(const pb_int8_quantize_params* p, void* stream, uint32_t job_id, void* notifier) {
-    const int rc = check_quantize(p);
+    QuantizePlan pl;
+    const int rc = plan_quantize(p, pl);
     if (rc != PB_OK) return rc;
-    const dim3 grid(p->tokens > 0 ? (unsigned)p->tokens : 1u);
-    FinishedBlockNotifier* nf = (FinishedBlockNotifier*)notifier;
-    const char* who = "pb_int8_quantize";
-#define PB_QUANTIZE(T) lm_launch(who, int8_quantize_kernel<T>, grid, dim3(256), 0, (cudaStream_t)stream, 1, (const T*)p->x, p->x_stride, p->q, p->q_stride, p->scale, p->tokens, p->channels, job_id, nf)
-    if (p->x_dtype == PB_F32) return PB_QUANTIZE(float);
-    if (p->x_dtype == PB_BF16) return PB_QUANTIZE(__nv_bfloat16);
-    return PB_QUANTIZE(__half);
-#undef PB_QUANTIZE
+    const QuantizeArgs a = {p->x, p->q, p->scale, p->x_stride, p->q_stride, p->tokens, p->channels};
+    return lm_launch("pb_int8_quantize", pl.fn, dim3(pl.blocks), dim3(256), 0, (cudaStream_t)stream, 1, a, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 int pb_int8_dense_info(const pb_int8_dense_params* p, pb_launch_info* out) {
-    const int rc = check_dense(p);
+    DensePlan pl;
+    const int rc = plan_dense(p, pl);
     if (rc != PB_OK) return rc;
     PB_REQUIRE(out != nullptr, "pb_int8_dense_info: NULL out");
     memset(out, 0, sizeof(*out));
     const uint64_t t = (uint64_t)p->tokens, k = (uint64_t)p->in_channels, n = (uint64_t)p->out_channels;
-    const uint64_t blocks = ceil_div<uint64_t>(t, 64) * ceil_div<uint64_t>(n, 64);
-    PB_REQUIRE(blocks <= 0x7fffffff, "pb_int8_dense: too many results for one launch");
-    out->num_blocks = blocks > 0 ? (uint32_t)blocks : 1u;
-    out->threads_per_block = 256;
-    out->smem_per_block = 2 * 16 * 65 * 4;
-    out->regs_per_thread = p->y_dtype == PB_F32 ? lm_regs(int8_dense_kernel<float>) : p->y_dtype == PB_BF16 ? lm_regs(int8_dense_kernel<__nv_bfloat16>) : lm_regs(int8_dense_kernel<__half>);
+    out->num_blocks = p->tokens > 0 ? pl.blocks : 1;
+    out->threads_per_block = 192;
+    out->smem_per_block = pl.smem;
+    out->regs_per_thread = lm_regs(pl.fn);
+    out->tmem_cols_per_block = pl.tmem_cols;
     out->flops = 2 * t * k * n;
     out->bytes = t * k + n * k + 4 * t + (p->bias ? 8 : 4) * n + t * n * dtype_bytes(p->y_dtype);
     return PB_OK;
 }
 
 int pb_int8_dense_launch(const pb_int8_dense_params* p, void* stream, uint32_t job_id, void* notifier) {
-    pb_launch_info li;
-    const int rc = pb_int8_dense_info(p, &li);
+    DensePlan pl;
+    const int rc = plan_dense(p, pl);
     if (rc != PB_OK) return rc;
-    const DenseArgs a = {p->x, p->w, p->x_scale, p->w_scale, p->bias, p->y, p->x_stride, p->w_stride, p->y_stride, p->tokens, p->in_channels, p->out_channels, p->act};
-    FinishedBlockNotifier* nf = (FinishedBlockNotifier*)notifier;
-    const char* who = "pb_int8_dense";
-    const dim3 grid(li.num_blocks);
-    if (p->y_dtype == PB_F32) return lm_launch(who, int8_dense_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, 1, a, job_id, nf);
-    if (p->y_dtype == PB_BF16) return lm_launch(who, int8_dense_kernel<__nv_bfloat16>, grid, dim3(256), 0, (cudaStream_t)stream, 1, a, job_id, nf);
-    return lm_launch(who, int8_dense_kernel<__half>, grid, dim3(256), 0, (cudaStream_t)stream, 1, a, job_id, nf);
+    if (p->tokens == 0) return lm_launch("pb_int8_dense", int8_nothing_kernel, dim3(1), dim3(192), 0, (cudaStream_t)stream, 1, job_id, (FinishedBlockNotifier*)notifier);
+    const uint64_t wdims[2] = {(uint64_t)p->in_channels, (uint64_t)p->out_channels}, xdims[2] = {(uint64_t)p->in_channels, (uint64_t)p->tokens};
+    // (the stride of a lone row is never used)
+    const uint64_t wstride = p->out_channels > 1 ? (uint64_t)p->w_stride : round_up<uint64_t>(p->in_channels, 16), xstride = p->tokens > 1 ? (uint64_t)p->x_stride : round_up<uint64_t>(p->in_channels, 16);
+    const uint32_t wbox[2] = {128, 128}, xbox[2] = {128, (uint32_t)(pl.many ? pl.a.BN / 2 : pl.a.BN)};
+    CUtensorMap wmap, xmap;
+    int e = encode_tiled_sw128(CU_TENSOR_MAP_DATA_TYPE_UINT8, p->w, 2, wdims, &wstride, wbox, &wmap);
+    if (e == PB_OK) e = encode_tiled_sw128(CU_TENSOR_MAP_DATA_TYPE_UINT8, p->x, 2, xdims, &xstride, xbox, &xmap);
+    if (e != PB_OK) return e;
+    PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem));
+    return lm_launch("pb_int8_dense", pl.fn, dim3(pl.blocks), dim3(192), pl.smem, (cudaStream_t)stream, pl.a.splits, pl.a, wmap, xmap, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 }  // extern "C"

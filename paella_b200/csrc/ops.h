@@ -123,6 +123,7 @@ int conv_umma_launch_noalloc(const pb_op_params* p, cudaStream_t st, uint32_t jo
 // The error flag words of the language-model operators' kernels on the current device (file-scope device words: nothing is
 // allocated, so a first launch may be captured).
 uint32_t* lm_rope_error_flag_ptr();
+uint32_t* lm_int8_error_flag_ptr();
 uint32_t* lm_attn_error_flag_ptr();
 uint32_t* noalloc_error_flag_ptr(int device);   // NULL until the no-allocation path ran on the device
 
