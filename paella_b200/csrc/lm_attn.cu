@@ -28,7 +28,7 @@ struct AttnArgs {
     float scale;
     // the prefix's split
     int row_tiles, pairs, splits, key_tiles, box_rows;
-    float* part_o;             // [kv_heads][pairs][splits][2][128][DP]
+    float* part_o;             // [row_tiles][kv_heads][splits][128][DP], a row's 16-byte piece i at i ^ (row % 32)
     float2* part_ml;           // the same without DP: (m, l)
     // own tokens
     int kv_heads, row_groups, ranks, early, out_vec;
@@ -38,6 +38,18 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+// Whether it holds for all of the 256 threads of the softmax warps, which meet here.
+__device__ __forceinline__ bool all_of_256(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -67,12 +79,13 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + 2 * kTile;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     const int pair = blockIdx.x % a.pairs, split = (blockIdx.x / a.pairs) % a.splits, kvh = blockIdx.x / (a.pairs * a.splits);
     const int kt0 = (int)((int64_t)a.key_tiles * split / a.splits), n = (int)((int64_t)a.key_tiles * (split + 1) / a.splits) - kt0;
     const bool two = 2 * pair + 1 < a.row_tiles;      // two row tiles; otherwise one, its key tiles dealt to both softmax groups
     const int jobs = two ? 2 * n : n;                 // job i: softmax group i & 1, key tile i / 2 or i
+    const int tail = min(128, a.prefix_len - (kt0 + n - 1) * 128);       // keys of the last tile
 
     if (warp == 9) {
         tcgen05_alloc(smem_u32(&s_tmem), 512);
@@ -95,12 +108,14 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = uniform(s_tmem);
     griddep_wait();
     griddep_launch();          // own_kernel, which reads nothing that precedes this launch in the stream but what has ended here
 
     if (warp == 8) {
         // Keys and values in the order in which the products ask for them.
+        int st = 0;
+        uint32_t parity = 1;
         for (int pos = 0; pos < 2 * n; ++pos) {
             bool values;
             int t;
@@ -109,7 +124,6 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
             else if (pos == 2 * n - 1) { values = true; t = n - 1; }
             else if (pos & 1) { values = false; t = (pos + 1) >> 1; }
             else { values = true; t = (pos - 2) >> 1; }
-            const int st = pos % kStages, use = pos / kStages;
             const int key0 = (kt0 + t) * 128, left = min(128, a.prefix_len - key0), boxes = (left + a.box_rows - 1) / a.box_rows;
             const bool mine = lane < boxes * kBlocks;
             const int box = lane / kBlocks, blk = lane % kBlocks, key = key0 + box * a.box_rows;
@@ -121,65 +135,79 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                     page = a.n_pages;                 // outside of the map: zeros
                 }
             }
-            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), (use - 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait))) break;
+            if (pos >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_attn_flag, kFlagLmWait))) break;
             const uint32_t bar = smem_u32(&s_full[st]);
             if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
             __syncwarp();
             if (mine) tma_load_4d(ring + st * kTile + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, key % a.page, kvh, page, bar);
+            if (++st == kStages) { st = 0; parity ^= 1; }
         }
     } else if (warp == 9) {
         constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t idesc_s = (1u << 4) | kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+        // The places of the next key and value tiles in the ring: job i's keys are entry 2 t of it with two row tiles, else 0, 1, 3, 5 ...; its values
+        // 2 t + 1, else 2, 4, 6 ... and the last entry.
+        struct Place {
+            int st;
+            uint32_t parity;
+            __device__ __forceinline__ void on(int by) {
+                st += by;
+                if (st >= kStages) { st -= kStages; parity ^= 1; }
+            }
+        } keys = {0, 0}, values = {two || n == 1 ? 1 : 2, 0};
         bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_q), 0, &s_abort, &g_attn_flag, kFlagLmWait));
-        const auto stage_ready = [&](int pos) {
-            return __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[pos % kStages]), (pos / kStages) & 1, &s_abort, &g_attn_flag, kFlagLmWait));
-        };
+        const uint64_t desc_q = umma_desc_sw128(q_smem), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
         const auto scores = [&](int i) {
-            const int g = i & 1, t = two ? i >> 1 : i, pos = two ? 2 * t : t == 0 ? 0 : 2 * t - 1;
-            if (!stage_ready(pos)) return false;
+            const int g = i & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[keys.st]), keys.parity, &s_abort, &g_attn_flag, kFlagLmWait))) return false;
             tcgen05_fence_after();
-            const uint64_t dq = umma_desc_sw128(q_smem + (two ? g * kTile : 0)), dk = umma_desc_sw128(ring + (pos % kStages) * kTile);
+            const uint64_t dq = desc_q + (uint64_t)(two && g ? kTile >> 4 : 0), dk = desc_k + (uint64_t)(keys.st * (int)(kTile >> 4));
+            const uint32_t d = tmem + g * 128;
+            const bool last = !two || g == 1;
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     const uint64_t at = (uint64_t)((k >> 2) * (kBlock >> 4) + (k & 3) * 2);
-                    tcgen05_mma_bf16(tmem + g * 128, dq + at, dk + at, idesc_s, k > 0);
+                    tcgen05_mma_bf16(d, dq + at, dk + at, idesc_s, k > 0);
                 }
                 tcgen05_commit(smem_u32(&s_scores[g]));
-                if (!two || g == 1) tcgen05_commit(smem_u32(&s_empty[pos % kStages]));
+                if (last) tcgen05_commit(smem_u32(&s_empty[keys.st]));
             }
             __syncwarp();
+            if (last) keys.on(!two && i == 0 ? 1 : 2);
             return true;
         };
-        for (int i = 0; i < 2 && ok; ++i)
-            if (i < jobs) ok = scores(i);
+        if (ok) ok = scores(0);
+        if (ok && jobs > 1) ok = scores(1);
         for (int i = 0; i < jobs && ok; ++i) {
-            const int g = i & 1, t = two ? i >> 1 : i, pos = two ? 2 * t + 1 : t == n - 1 ? 2 * n - 1 : 2 * t + 2;
-            ok = stage_ready(pos);
+            const int g = i & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[values.st]), values.parity, &s_abort, &g_attn_flag, kFlagLmWait));
             if (!ok) break;
-            const uint32_t v_smem = ring + (pos % kStages) * kTile;
-            const int left = a.prefix_len - (kt0 + t) * 128;
-            if (left < 128 && (!two || g == 0)) {
-                // Rows behind the last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.
-                for (int c = lane; c < (128 - left) * 8 * kBlocks; c += 32) {
-                    const int blk = c / ((128 - left) * 8), at = c % ((128 - left) * 8);
-                    st_shared_v4(v_smem + blk * kBlock + left * 128 + at * 16, 0, 0, 0, 0);
+            const bool last = !two || g == 1;
+            if (i + 2 >= jobs && tail < 128 && (!two || g == 0) && i / (two ? 2 : 1) == n - 1) {
+                // Rows behind the prefix's last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.
+                const uint32_t v_smem = ring + values.st * kTile;
+                for (int c = lane; c < (128 - tail) * 8 * kBlocks; c += 32) {
+                    const int blk = c / ((128 - tail) * 8), at = c % ((128 - tail) * 8);
+                    st_shared_v4(v_smem + blk * kBlock + tail * 128 + at * 16, 0, 0, 0, 0);
                 }
                 fence_proxy_async();
                 __syncwarp();
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_probs[g]), (i >> 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait));
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_probs[g]), (uint32_t)(i >> 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait));
             if (!ok) break;
             tcgen05_fence_after();
-            const uint64_t dv = umma_desc_sw128_mn(v_smem, kBlock);
+            const uint64_t dv = desc_v + (uint64_t)(values.st * (int)(kTile >> 4));
+            const uint32_t d = tmem + 256 + g * DP, p = tmem + g * 128, more = i > 1;
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) tcgen05_mma_f16_ts(tmem + 256 + g * DP, tmem + g * 128 + k * 8, dv + (uint64_t)(k * (2048 >> 4)), idesc_o, i > 1 || k > 0);
-                if (!two || g == 1) tcgen05_commit(smem_u32(&s_empty[pos % kStages]));
+                for (int k = 0; k < 8; ++k) tcgen05_mma_f16_ts(d, p + k * 8, dv + (uint64_t)(k * (2048 >> 4)), idesc_o, more | (uint32_t)(k > 0));
+                if (last) tcgen05_commit(smem_u32(&s_empty[values.st]));
                 if (i + 2 >= jobs) tcgen05_commit(smem_u32(&s_done[g]));
             }
             __syncwarp();
+            if (last) values.on(!two && i == n - 2 ? 1 : 2);
             if (i + 2 < jobs) ok = scores(i + 2);
         }
     } else {
@@ -188,42 +216,50 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
         const int row = (2 * pair + (two ? g : 0)) * 128 + in_tile;
         const bool live_warp = row - lane < rows;
         if (two || g == 0) {
-            const T* src = nullptr;
-            if (row < rows) src = static_cast<const T*>(a.q) + (int64_t)(row / a.group) * a.q_stride + (int64_t)(kvh * a.group + row % a.group) * a.q_head;
-            const uint32_t dst = q_smem + g * kTile + in_tile * 128, flip = a.scale < 0.f ? 0x80008000u : 0u;      // |scale| from here on
+            // 16 bytes at a time, neighbouring lanes on neighbouring bytes of a row; |scale| from here on
+            constexpr int kPerRow = DP / 8, kMine = kPerRow;
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            const int row0 = row - in_tile, thread = threadIdx.x & 127;
+            uint4 v[kMine];
 #pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < rows && 8 * c < a.D) v = __ldcg(reinterpret_cast<const uint4*>(src + 8 * c));
-                st_shared_v4(dst + (c >> 3) * kBlock + (((c & 7) ^ (in_tile & 7)) << 4), v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            for (int i = 0; i < kMine; ++i) {
+                const int r = row0 + (i * 128 + thread) / kPerRow, c = thread % kPerRow;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (r < rows && 8 * c < a.D)
+                    v[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(r / a.group) * a.q_stride + (int64_t)(kvh * a.group + r % a.group) * a.q_head + 8 * c));
+            }
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int r = (i * 128 + thread) / kPerRow, c = thread % kPerRow;
+                st_shared_v4(q_smem + g * kTile + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
             }
         }
         fence_proxy_async();
         mbar_arrive(smem_u32(&s_q));
 
         const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-38f);                  // (a scale of 0 must not meet the infinities of masked keys)
+        const uint64_t c2 = pack_f32x2(__float_as_uint(c), __float_as_uint(c));
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         int done = 0;
         for (int i = g; i < jobs; i += 2, ++done) {
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_scores[g]), done & 1, &s_abort, &g_attn_flag, kFlagLmWait));
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_scores[g]), (uint32_t)done & 1, &s_abort, &g_attn_flag, kFlagLmWait));
             if (!ok) break;
             if (live_warp) {
                 tcgen05_fence_after();
-                const int left = a.prefix_len - (kt0 + (two ? i >> 1 : i)) * 128;
                 const uint32_t ts = tmem + lanes + g * 128;
                 uint32_t s[128];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) tcgen05_ld32(ts + 32 * j, s + 32 * j);
                 tcgen05_wait_ld();
-                if (left < 128) {
+                if ((two ? i >> 1 : i) == n - 1 && tail < 128) {
 #pragma unroll
                     for (int j = 0; j < 128; ++j)
-                        if (j >= left) s[j] = 0xff800000u;
+                        if (j >= tail) s[j] = 0xff800000u;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(s[j]));
+                for (int j = 0; j < 128; j += 2) top[(j >> 1) & 3] = fmaxf(top[(j >> 1) & 3], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
                 const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                 if (done == 0) {
                     m = next;
@@ -242,45 +278,109 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                     l *= keep;
                     m = next;
                 }
-                const float base = m == -INFINITY ? 0.f : m * c - p_shift<T>();
-                float sum[4] = {};
+                const float base = m == -INFINITY ? 0.f : p_shift<T>() - m * c;
+                const uint64_t base2 = pack_f32x2(__float_as_uint(base), __float_as_uint(base));
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t p[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        const float x = ex2(fmaf(__uint_as_float(s[64 * h + 2 * j]), c, -base)), y = ex2(fmaf(__uint_as_float(s[64 * h + 2 * j + 1]), c, -base));
-                        sum[j & 3] += x + y;
+                        float x, y;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(s[64 * h + 2 * j], s[64 * h + 2 * j + 1]), c2, base2), x, y);
+                        x = ex2(x);
+                        y = ex2(y);
+                        sum[j & 1] = add_f32x2(sum[j & 1], pack_f32x2(__float_as_uint(x), __float_as_uint(y)));
                         p[j] = lm_pack2<T>(x, y);
                     }
                     tcgen05_st32(ts + 32 * h, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float x, y;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), x, y);
+                l += x + y;
                 tcgen05_wait_st();
                 tcgen05_fence_before();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_probs[g]));
         }
-        // this block's part of the row
-        const int64_t part = ((int64_t)((int64_t)kvh * a.pairs + pair) * a.splits + split) * 2 + g;
         if (ok && done > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_done[g]), 0, &s_abort, &g_attn_flag, kFlagLmWait));
-        if (ok && live_warp) {
-            tcgen05_fence_after();
-            if (row < rows) a.part_ml[part * 128 + in_tile] = make_float2(m == -INFINITY ? m : m * c, l);
-            if (done > 0) {
-                float* dst = a.part_o + (part * 128 + in_tile) * DP;
+        // This block's part of the rows.  A lone row tile's two accumulators become one first: the groups exchange halves of the values through the
+        // shared memory that all products have left.  A row lies as DP / 4 pieces of 16 bytes, piece i at i ^ (row % 32): 32 rows are written without
+        // bank conflicts and leave as one copy.
+        constexpr int kPieces = DP / 4;
+        const uint32_t my_row = q_smem + (uint32_t)in_tile * (DP * 4);
+        const auto piece = [&](uint32_t at, int i) { return at + (uint32_t)((i ^ (in_tile & 31 & (kPieces - 1))) * 16); };
+        m = m == -INFINITY ? m : m * c;
+        if (!two) {
+            const uint32_t swap = q_smem + 128 * DP * 4;                        // (m, l) of both groups behind the rows
+            ok = all_of_256(ok);                       // both groups' products have ended
+            if (ok) {
+                tcgen05_fence_after();
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(swap + (g * 128 + in_tile) * 8), "f"(m), "f"(l) : "memory");
+                // the half that the other group finishes
+#pragma unroll 1
+                for (int j = (g ^ 1) * (DP / 2); j < (g ^ 1) * (DP / 2) + DP / 2; j += 32) {
+                    uint32_t o[32];
+                    tcgen05_ld32(tmem + lanes + 256 + g * DP + j, o);
+                    tcgen05_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) st_shared_v4(piece(my_row, j / 4 + e), o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+            }
+            ok = all_of_256(ok);
+            if (ok) {
+                float m1, l1;
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(m1), "=f"(l1) : "r"(swap + ((g ^ 1) * 128 + in_tile) * 8) : "memory");
+                const float both = fmaxf(m, m1), f = m == -INFINITY ? 0.f : ex2(m - both), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - both);
+                const bool alone = n < 2;              // the second group had no key tile: its accumulator holds nothing
+#pragma unroll 1
+                for (int j = g * (DP / 2); j < g * (DP / 2) + DP / 2; j += 32) {
+                    uint32_t o[32];
+                    tcgen05_ld32(tmem + lanes + 256 + g * DP + j, o);
+                    tcgen05_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint4 x = ld_shared_v4(piece(my_row, j / 4 + e));
+                        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                        uint32_t r[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float mine = __uint_as_float(o[4 * e + k]), other = __uint_as_float(w[k]);
+                            r[k] = __float_as_uint(alone ? (g ? other : mine) : mine * f + other * f1);
+                        }
+                        st_shared_v4(piece(my_row, j / 4 + e), r[0], r[1], r[2], r[3]);
+                    }
+                }
+                l = alone ? (g ? l1 : l) : l * f + l1 * f1;
+                m = both;
+            }
+            fence_proxy_async();
+            ok = all_of_256(ok);
+        } else if (ok) {
+            // the other group's products may still read queries and tiles: each group waits for both
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_done[g ^ 1]), 0, &s_abort, &g_attn_flag, kFlagLmWait));
+            if (ok && live_warp) {
+                tcgen05_fence_after();
 #pragma unroll 1
                 for (int j = 0; j < DP; j += 32) {
                     uint32_t o[32];
                     tcgen05_ld32(tmem + lanes + 256 + g * DP + j, o);
                     tcgen05_wait_ld();
-                    if (row < rows) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4*>(dst + j + e) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-                    }
+                    for (int e = 0; e < 8; ++e) st_shared_v4(piece(my_row + g * (128 * DP * 4), j / 4 + e), o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
+                fence_proxy_async();
+            }
+            __syncwarp();
+        }
+        if (ok && live_warp && (two || g == 0)) {
+            const int64_t part = ((int64_t)(2 * pair + (two ? g : 0)) * a.kv_heads + kvh) * a.splits + split;
+            if (row < rows) a.part_ml[part * 128 + in_tile] = make_float2(m, l);
+            if (lane == 0) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + (part * 128 + in_tile) * DP), "r"(my_row + (two ? g * (128 * DP * 4) : 0)), "n"(32 * DP * 4) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
         }
     }
@@ -295,6 +395,9 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
         tcgen05_dealloc(tmem, 512);
     }
 }
+
+constexpr int kMaxSplits = 148, kMaxRanks = 8, kMaxParts = 192;
+static_assert(kMaxSplits + 4 * kMaxRanks <= kMaxParts && kMaxParts % 32 == 0, "a row's parts");
 
 // ---- own tokens, and the parts together ------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -333,9 +436,10 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64;
     __shared__ __align__(16) float s_o[4][R][DP];
     __shared__ __align__(8) float2 s_ml[4][R];
+    __shared__ float s_w[R][kMaxParts];
     if (!a.early) griddep_wait();
     if (nf) nf->start(job_id);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = blockIdx.x % a.ranks;
     int unit = blockIdx.x / a.ranks;
     const int zg = unit % a.row_groups;
@@ -365,18 +469,26 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                 if (t * 8 + g < rows && 32 * i + 8 * c < a.D)
                     q[t][i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)(kvh * a.group + row0 + t * 8 + g) * a.q_head + 32 * i + 8 * c));
             }
-        const int32_t* table = a.block_table + b * a.table_stride;
-        const int64_t head = (int64_t)kvh * a.head_stride;
-        // where the 8 tokens at 16 chunk + 8 half lie (a page holds a multiple of 8), or -1: zeros
-        const auto where = [&](int chunk, int half) -> int64_t {
-            const int token = 16 * chunk + 8 * half;
+        // Where this warp's chunks lie, two halves of 8 tokens each (a page holds a multiple of 8), or -1: zeros.  A lane looks a chunk's pages up, for 32
+        // chunks at a time: their latency is paid once.
+        int64_t at_lo = -1, at_hi = -1;
+        const auto look_up = [&](int token) -> int64_t {
             if (token >= own) return -1;
-            const int at = token / a.page, page = __ldcg(table + at);
+            const int at = token / a.page, page = __ldcg(a.block_table + b * a.table_stride + at);
             if (page < 0 || page >= a.n_pages) {
-                if (lane == 0) atomicExch(&g_attn_flag, kFlagLmPage);
+                atomicExch(&g_attn_flag, kFlagLmPage);
                 return -1;
             }
-            return page * a.page_stride + (token - at * a.page) * a.token_stride + head;
+            return page * a.page_stride + (token - at * a.page) * a.token_stride + (int64_t)kvh * a.head_stride;
+        };
+        const auto where = [&](int turn, int64_t& lo, int64_t& hi) {           // of chunk first + 4 turn, turns in order
+            if ((turn & 31) == 0) {
+                const int chunk = first + 4 * (turn + lane);
+                at_lo = chunk < last ? look_up(16 * chunk) : -1;
+                at_hi = chunk < last ? look_up(16 * chunk + 8) : -1;
+            }
+            lo = __shfl_sync(0xffffffffu, at_lo, turn & 31);
+            hi = __shfl_sync(0xffffffffu, at_hi, turn & 31);
         };
         uint4 k[KB][2], v[VB][4];
         const auto load_k = [&](int chunk, int64_t lo, int64_t hi) {
@@ -408,13 +520,13 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             }
         };
         const float scale = a.scale * kLog2e;
-        int64_t lo = where(first, 0), hi = where(first, 1);
+        int64_t lo, hi;
+        where(0, lo, hi);
         load_k(first, lo, hi);
         load_v(first, lo, hi);
-        for (int chunk = first; chunk < last; chunk += 4) {
+        for (int chunk = first, turn = 1; chunk < last; chunk += 4, ++turn) {
             const int next = chunk + 4;
-            int64_t nlo = -1, nhi = -1;
-            if (next < last) { nlo = where(next, 0); nhi = where(next, 1); }
+            if (next < last) where(turn, lo, hi);
             float s[NT][4] = {};
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
@@ -425,7 +537,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                     mma_16x8x16<T>(s[t], a1, q[t][i].z, q[t][i].w);
                 }
             }
-            if (next < last) load_k(next, nlo, nhi);
+            if (next < last) load_k(next, lo, hi);
             const bool in0 = 16 * chunk + g < own, in1 = 16 * chunk + g + 8 < own;
             float up[NT][2];
             bool grown = false;
@@ -476,7 +588,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                     for (int t = 0; t < NT; ++t) mma_16x8x16<T>(o[i][e][t], av, p0[t], p1[t]);
                 }
             }
-            if (next < last) load_v(next, nlo, nhi);
+            if (next < last) load_v(next, lo, hi);
         }
     }
     // this warp's part: (m, l) and O of its rows, values 64 i + 8 g + 2 e and + 1
@@ -500,53 +612,79 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     if (a.ranks > 1) { cluster_arrive(); cluster_wait(); }
     else __syncthreads();
 
-    // The parts joined: a float4 of a row for `lanes` neighbouring threads, which deal the parts out among themselves.
-    const int items = rows * (DP / 4);
+    // The parts joined.  First the weights 2^(m_i - M) / sum 2^(m_i - M) l_i of each row's parts, a row a warp, a part a lane; then a float4 of a row for
+    // `lanes` neighbouring threads, which deal the parts out among themselves.
+    const int ahead = a.prefix_len > 0 ? a.splits : 0, parts = ahead + (own > 0 ? 4 * a.ranks : 0);
+    const auto first_part = [&](int row) {             // of the prefix for this row, as a row of part_ml
+        const int flat = b * a.group + row0 + row;
+        return (((int64_t)(flat >> 7) * a.kv_heads + kvh) * a.splits << 7) + (flat & 127);
+    };
+    for (int row = warp; row < rows; row += 4) {
+        const float2* ml = a.part_ml + first_part(row);
+        float2 x[kMaxParts / 32];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 32; ++k) {
+            const int i = lane + 32 * k, w = i - ahead;
+            x[k] = make_float2(-INFINITY, 0.f);
+            if (i < ahead) x[k] = __ldcg(ml + (int64_t)i * 128);
+            else if (i < parts) x[k] = ld_cluster_f2(cluster_addr(smem_u32(&s_ml[w & 3][row]), (uint32_t)w >> 2));
+        }
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 32; ++k) top = fmaxf(top, x[k].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 32; ++k) {
+            x[k].x = x[k].x == -INFINITY ? 0.f : ex2(x[k].x - top);
+            sum = fmaf(x[k].x, x[k].y, sum);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = 1.f / sum;
+#pragma unroll
+        for (int k = 0; k < kMaxParts / 32; ++k)
+            if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;
+    }
+    __syncthreads();
+    constexpr int kPieces = DP / 4;
+    const int items = rows * kPieces;
     int lanes = 1;
     while (lanes < 32 && items * lanes * 2 <= 128 * a.ranks) lanes *= 2;
     const int sub = threadIdx.x & (lanes - 1);
     for (int base = 0; base < items; base += 128 * a.ranks / lanes) {
         const int item = base + (rank * 128 + threadIdx.x) / lanes;
         const bool real = item < items;
-        const int row = real ? item / (DP / 4) : 0, col = real ? item % (DP / 4) * 4 : 0;
-        // the prefix's parts of this row
-        const int flat = b * a.group + row0 + row, tile = flat >> 7, pair = tile >> 1, in_tile = flat & 127;
-        const bool two = 2 * pair + 1 < a.row_tiles;
-        const int64_t part0 = ((int64_t)kvh * a.pairs + pair) * a.splits * 2 + (two ? tile & 1 : 0);
-        const int step = two ? 2 : 1, ahead = a.prefix_len > 0 ? (two ? a.splits : 2 * a.splits) : 0, mine = own > 0 ? 4 * a.ranks : 0;
-        float top = -INFINITY;
-        for (int i = sub; real && i < ahead + mine; i += lanes) {
-            const int w = i - ahead;
-            const float2 ml = i < ahead ? __ldcg(a.part_ml + (part0 + (int64_t)i * step) * 128 + in_tile) : ld_cluster_f2(cluster_addr(smem_u32(&s_ml[w & 3][row]), w >> 2));
-            top = fmaxf(top, ml.x);
-        }
-        for (int k = lanes >> 1; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const int row = real ? item / kPieces : 0, i4 = item % kPieces;
+        const int64_t at = first_part(row);
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + at * DP) + (i4 ^ ((int)at & 31 & (kPieces - 1)));
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-#pragma unroll 4
-        for (int i = sub; real && i < ahead + mine; i += lanes) {
-            const int w = i - ahead;
-            const int64_t part = (part0 + (int64_t)i * step) * 128 + in_tile;
-            const float2 ml = i < ahead ? __ldcg(a.part_ml + part) : ld_cluster_f2(cluster_addr(smem_u32(&s_ml[w & 3][row]), w >> 2));
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;               // no token, or none with a finite score: O may not have been written
-            const float4 x = i < ahead ? __ldcg(reinterpret_cast<const float4*>(a.part_o + part * DP + col)) : ld_cluster_f4(cluster_addr(smem_u32(&s_o[w & 3][row][col]), w >> 2));
-            const float f = ex2(ml.x - top);
-            sum = fmaf(f, ml.y, sum);
-            acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+        const auto add = [&](float w, float4 x) {
+            acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y); acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
+        };
+        if (real) {
+            int i = sub;
+            for (; i + 7 * lanes < ahead; i += 8 * lanes) {
+                float4 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = __ldcg(src + (int64_t)(i + k * lanes) * 128 * kPieces);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) add(s_w[row][i + k * lanes], x[k]);
+            }
+            for (; i < ahead; i += lanes) add(s_w[row][i], __ldcg(src + (int64_t)i * 128 * kPieces));
+            for (i = sub; i < parts - ahead; i += lanes)
+                add(s_w[row][ahead + i], ld_cluster_f4(cluster_addr(smem_u32(&s_o[i & 3][row][4 * i4]), (uint32_t)i >> 2)));
         }
         for (int k = lanes >> 1; k > 0; k >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, k);
             acc.x += __shfl_xor_sync(0xffffffffu, acc.x, k); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, k);
             acc.z += __shfl_xor_sync(0xffffffffu, acc.z, k); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, k);
         }
-        if (!real || sub != 0 || col >= a.D) continue;
-        if (a.prefix_len + own == 0) acc = make_float4(0.f, 0.f, 0.f, 0.f), sum = 1.f;
-        T* dst = static_cast<T*>(a.out) + b * a.out_stride + (int64_t)(kvh * a.group + row0 + row) * a.out_head + col;
-        const float inv = 1.f / sum;
+        if (!real || sub != 0 || 4 * i4 >= a.D) continue;
+        T* dst = static_cast<T*>(a.out) + b * a.out_stride + (int64_t)(kvh * a.group + row0 + row) * a.out_head + 4 * i4;
         if (a.out_vec) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(lm_pack2<T>(acc.x * inv, acc.y * inv), lm_pack2<T>(acc.z * inv, acc.w * inv));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(lm_pack2<T>(acc.x, acc.y), lm_pack2<T>(acc.z, acc.w));
         } else {
-            dst[0] = lm_from_f<T>(acc.x * inv); dst[1] = lm_from_f<T>(acc.y * inv); dst[2] = lm_from_f<T>(acc.z * inv); dst[3] = lm_from_f<T>(acc.w * inv);
+            dst[0] = lm_from_f<T>(acc.x); dst[1] = lm_from_f<T>(acc.y); dst[2] = lm_from_f<T>(acc.z); dst[3] = lm_from_f<T>(acc.w);
         }
     }
     if (a.ranks > 1) { cluster_arrive_relaxed(); cluster_wait(); }        // the others have read this block's part
@@ -610,10 +748,10 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     while (a.box_rows < 128 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
     const int64_t units = (int64_t)a.pairs * a.kv_heads;
     a.splits = 1;
-    if (units > 0 && units < 148) a.splits = (int)(148 / units);
+    if (units > 0 && units < kMaxSplits) a.splits = (int)(kMaxSplits / units);
     if (a.splits > a.key_tiles) a.splits = a.key_tiles > 0 ? a.key_tiles : 1;
     pl.prefix_blocks = a.prefix_len > 0 ? units * a.splits : 0;
-    const uint64_t parts = (uint64_t)pl.prefix_blocks * 2 * 128;
+    const uint64_t parts = pl.prefix_blocks > 0 ? (uint64_t)a.row_tiles * a.kv_heads * a.splits * 128 : 0;
     pl.scratch = parts * ((uint64_t)pl.DP * 4 + 8);
     a.part_o = (float*)p->scratch;
     a.part_ml = (float2*)((char*)p->scratch + parts * pl.DP * 4);
@@ -621,7 +759,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     a.row_groups = ceil_div(a.group, 8 * pl.NT);
     const int64_t own_units = (int64_t)a.batch * a.kv_heads * a.row_groups;
     a.ranks = 1;
-    while (a.ranks < 8 && own_units * a.ranks < 2 * 148 && a.max_own / (2 * a.ranks) >= 128) a.ranks *= 2;
+    while (a.ranks < kMaxRanks && own_units * a.ranks < 2 * 148 && a.max_own / (2 * a.ranks) >= 128) a.ranks *= 2;
     pl.own_blocks = own_units > 0 ? own_units * a.ranks : 1;
     PB_REQUIRE(pl.prefix_blocks <= 0x7fffffff && pl.own_blocks <= 0x7fffffff, "%s: too many blocks for one launch", who);
     a.early = pl.prefix_blocks > 0;

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ D
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 128u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
     const int n0 = tile % a.channel_tiles * 128, t0 = tile / a.channel_tiles * a.BN;
     const int kb0 = a.kblocks * rank / a.splits, nkb = a.kblocks * (rank + 1) / a.splits - kb0;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ D
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = uniform(s_tmem);
     if (warp == 4 && elect_one()) {
         // the weights come into the L2 cache while the launch that makes the activations still runs
         for (int i = 0; i < nkb && i < a.stages; ++i)
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
     __shared__ volatile uint32_t s_abort;
     __shared__ float s_xs[256];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 64u, out = ring + a.stages * stage_bytes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pairs = gridDim.x / 2, tiles = a.channel_tiles * a.token_tiles;
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
     cluster_arrive();
     cluster_wait();                                    // both blocks' barriers and tensor memory are set up
     tcgen05_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = uniform(s_tmem);
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();

@@ -226,6 +226,11 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t x, uint64_t y) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
 __device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
     uint32_t l, h;
     asm("mov.b64 {%0, %1}, %2;" : "=r"(l), "=r"(h) : "l"(v));
