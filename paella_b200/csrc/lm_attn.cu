@@ -52,6 +52,26 @@ __device__ __forceinline__ bool all_of_256(bool ok) {
     return all != 0;
 }
 
+// 2^x of a pair on the multipliers, beside ex2 on the special-function unit, which alone would take as long as the products: x = i + f with |f| <= 1/2
+// (the sum with 1.5 x 2^23 rounds to a whole number), 2^f as the polynomial of degree 5 with the least largest relative error (Remez's exchange;
+// 2^-23.7, 2^-22.2 with fp32's roundings), i added to its exponent.  Below 2^-126: nothing.  For x < 127; a NaN stays one.
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+    const auto both = [](float v) { return pack_f32x2(__float_as_uint(v), __float_as_uint(v)); };
+    float lo, hi;
+    unpack_f32x2(x, lo, hi);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
+    x = pack_f32x2(__float_as_uint(lo), __float_as_uint(hi));
+    const uint64_t t = add_f32x2(x, both(12582912.f)), f = fma_f32x2(add_f32x2(t, both(-12582912.f)), both(-1.f), x);
+    uint64_t r = fma_f32x2(both(0.0013276472454890609f), f, both(0.009675540961325169f));
+    r = fma_f32x2(r, f, both(0.05550713092088699f));
+    r = fma_f32x2(r, f, both(0.24022120237350464f));
+    r = fma_f32x2(r, f, both(0.6931469440460205f));
+    r = fma_f32x2(r, f, both(1.0000001192092896f));
+    r = pack_f32x2((uint32_t)r + ((uint32_t)t << 23), (uint32_t)(r >> 32) + ((uint32_t)(t >> 32) << 23));
+    return add_f32x2(r, both(-0x1p-126f));
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's maximum is followed only once it has grown by 2^8: until then the values are up to 2^8 times too large, which fp32 sums and the
 // 16-bit values' exponents hold, and the accumulator need not be rescaled.
@@ -59,11 +79,36 @@ constexpr float kSlack = 8.f;
 // fp16 has few exponents below 1: its values are scaled up by 2^5 (2^13 with the slack; the sums with them).
 template <typename T> __device__ __forceinline__ constexpr float p_shift() { return sizeof(T) == 2 && std::is_same<T, __half>::value ? 5.f : 0.f; }
 
+// 64 keys: 2^(s c + base) from their scores, rounded to pairs, and the sum of what they were.  One pair in four on the multipliers.
+template <typename T>
+__device__ __forceinline__ float values_of(const uint32_t* s, float c, float base, uint32_t (&p)[32]) {
+    const uint64_t c2 = pack_f32x2(__float_as_uint(c), __float_as_uint(c)), base2 = pack_f32x2(__float_as_uint(base), __float_as_uint(base));
+    uint64_t sum[2] = {0, 0};
+    float x, y;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        uint64_t e = fma_f32x2(pack_f32x2(s[2 * j], s[2 * j + 1]), c2, base2);
+        if (j % 4 == 3) {
+            e = ex2_pair(e);
+            unpack_f32x2(e, x, y);
+        } else {
+            unpack_f32x2(e, x, y);
+            x = ex2(x);
+            y = ex2(y);
+            e = pack_f32x2(__float_as_uint(x), __float_as_uint(y));
+        }
+        sum[j & 1] = add_f32x2(sum[j & 1], e);
+        p[j] = lm_pack2<T>(x, y);
+    }
+    unpack_f32x2(add_f32x2(sum[0], sum[1]), x, y);
+    return x + y;
+}
+
 // ---- the prefix ----------------------------------------------------------------------------------------------
 // A block takes a range of the prefix's keys for one key head and a pair of row tiles, or, where the last row tile is alone, that tile with its
-// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warp 8 loads keys and values, warp 9 issues the
-// products: S = Q K^T of the one tile runs while the other's softmax does.  S (128 columns) becomes P in place (64 columns of 16-bit pairs), the A
-// operand of O += P V.  Tensor memory: S0 S1 O0 O1.
+// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warp 8 loads keys and values, warps 9 and 10
+// issue the products of one of the pair each: S = Q K^T of the one tile runs while the other's softmax does.  S (128 columns) becomes P in place (64 columns of 16-bit pairs), the A
+// operand of O += P V, whose first half starts when half of P is there.  Tensor memory: S0 S1 O0 O1.
 template <int DP> struct PrefixShape {
     static constexpr uint32_t tile = 128 * DP * 2;                   // bytes of 128 rows
     static constexpr int stages = DP == 128 ? 5 : 10;                // tiles of keys or values in flight
@@ -71,11 +116,11 @@ template <int DP> struct PrefixShape {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages;
     constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2], s_probs[2], s_done[2], s_q;
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_done[2], s_q;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + 2 * kTile;
@@ -84,7 +129,6 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
     const int pair = blockIdx.x % a.pairs, split = (blockIdx.x / a.pairs) % a.splits, kvh = blockIdx.x / (a.pairs * a.splits);
     const int kt0 = (int)((int64_t)a.key_tiles * split / a.splits), n = (int)((int64_t)a.key_tiles * (split + 1) / a.splits) - kt0;
     const bool two = 2 * pair + 1 < a.row_tiles;      // two row tiles; otherwise one, its key tiles dealt to both softmax groups
-    const int jobs = two ? 2 * n : n;                 // job i: softmax group i & 1, key tile i / 2 or i
     const int tail = min(128, a.prefix_len - (kt0 + n - 1) * 128);       // keys of the last tile
 
     if (warp == 9) {
@@ -95,11 +139,14 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
         s_abort = 0;
         for (int i = 0; i < kStages; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&s_empty[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), two ? 2 : 1);       // groups that use a tile
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&s_scores[i]), 1);
-            mbar_init(smem_u32(&s_probs[i]), 4);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(smem_u32(&s_scores[i][h]), 1);
+                mbar_init(smem_u32(&s_probs[i][h]), 4);
+            }
+            mbar_init(smem_u32(&s_half[i]), 1);
             mbar_init(smem_u32(&s_done[i]), 1);
         }
         mbar_init(smem_u32(&s_q), 256);
@@ -142,51 +189,53 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
             if (mine) tma_load_4d(ring + st * kTile + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, key % a.page, kvh, page, bar);
             if (++st == kStages) { st = 0; parity ^= 1; }
         }
-    } else if (warp == 9) {
+    } else if (warp == 9 || warp == 10) {
+        // The products of one softmax group: two warps, so that the waits of one lie under the products of the other.
         constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-        constexpr uint32_t idesc_s = (1u << 4) | kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t idesc_s = (1u << 4) | kType | ((64u >> 3) << 17) | ((128u >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
-        // The places of the next key and value tiles in the ring: job i's keys are entry 2 t of it with two row tiles, else 0, 1, 3, 5 ...; its values
-        // 2 t + 1, else 2, 4, 6 ... and the last entry.
+        // The ring's entries of key tile t and its values: 2 t and 2 t + 1 with two row tiles; otherwise keys are entries 0, 1, 3, 5 ..., values 2, 4, 6
+        // ... and the last one.
         struct Place {
-            int st;
-            uint32_t parity;
-            __device__ __forceinline__ void on(int by) {
+            uint32_t st, parity;
+            __device__ __forceinline__ void on(uint32_t by) {
                 st += by;
                 if (st >= kStages) { st -= kStages; parity ^= 1; }
             }
-        } keys = {0, 0}, values = {two || n == 1 ? 1 : 2, 0};
-        bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_q), 0, &s_abort, &g_attn_flag, kFlagLmWait));
-        const uint64_t desc_q = umma_desc_sw128(q_smem), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
-        const auto scores = [&](int i) {
-            const int g = i & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[keys.st]), keys.parity, &s_abort, &g_attn_flag, kFlagLmWait))) return false;
+        };
+        const int g = warp - 9, mine = two ? n : (n - g + 1) / 2;      // key tiles of this group: g, g + 2 ... or all
+        Place keys = {two ? 0u : (uint32_t)g, 0}, values = {two ? 1u : g == n - 1 ? 2u * n - 1u : 2u * g + 2u, 0};
+        const uint32_t d_s = tmem + g * 128, d_o = tmem + 256 + g * DP;
+        const uint64_t desc_q = umma_desc_sw128(q_smem + (two ? g * kTile : 0)), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
+        const uint32_t high_k = (uint32_t)(desc_k >> 32), high_v = (uint32_t)(desc_v >> 32), low_q = (uint32_t)desc_q;
+        const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &s_abort, &g_attn_flag, kFlagLmWait)); };
+        // Scores of 64 keys, the first or second half of a tile, into their own 64 columns.
+        const auto scores = [&](int u, uint32_t h) {
+            if (h == 0 && !wait(&s_full[keys.st], keys.parity)) return false;
             tcgen05_fence_after();
-            const uint64_t dq = desc_q + (uint64_t)(two && g ? kTile >> 4 : 0), dk = desc_k + (uint64_t)(keys.st * (int)(kTile >> 4));
-            const uint32_t d = tmem + g * 128;
-            const bool last = !two || g == 1;
+            const uint32_t low = (uint32_t)desc_k + keys.st * (kTile >> 4) + h * (8192 >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
-                    const uint64_t at = (uint64_t)((k >> 2) * (kBlock >> 4) + (k & 3) * 2);
-                    tcgen05_mma_bf16(d, dq + at, dk + at, idesc_s, k > 0);
+                    const uint32_t at = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
+                    tcgen05_mma_bf16(d_s + h * 64, pack_f32x2(low_q + at, high_k), pack_f32x2(low + at, high_k), idesc_s, k > 0);
                 }
-                tcgen05_commit(smem_u32(&s_scores[g]));
-                if (last) tcgen05_commit(smem_u32(&s_empty[keys.st]));
+                tcgen05_commit(smem_u32(&s_scores[g][h]));
+                if (h == 1) tcgen05_commit(smem_u32(&s_empty[keys.st]));
             }
             __syncwarp();
-            if (last) keys.on(!two && i == 0 ? 1 : 2);
+            if (h == 1) keys.on(two ? 2 : u == 0 && g == 0 ? 3 : 4);
             return true;
         };
-        if (ok) ok = scores(0);
-        if (ok && jobs > 1) ok = scores(1);
-        for (int i = 0; i < jobs && ok; ++i) {
-            const int g = i & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[values.st]), values.parity, &s_abort, &g_attn_flag, kFlagLmWait));
+        bool ok = wait(&s_q, 0);
+        if (ok && mine > 0) ok = scores(0, 0) && scores(0, 1);
+        for (int u = 0; ok && u < mine; ++u) {
+            const bool last = u == mine - 1;
+            ok = wait(&s_full[values.st], values.parity);
             if (!ok) break;
-            const bool last = !two || g == 1;
-            if (i + 2 >= jobs && tail < 128 && (!two || g == 0) && i / (two ? 2 : 1) == n - 1) {
-                // Rows behind the prefix's last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.
+            if ((two ? u : g + 2 * u) == n - 1 && tail < 128) {
+                // Rows behind the prefix's last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.  (With two row tiles
+                // both warps write these zeros before they use them.)
                 const uint32_t v_smem = ring + values.st * kTile;
                 for (int c = lane; c < (128 - tail) * 8 * kBlocks; c += 32) {
                     const int blk = c / ((128 - tail) * 8), at = c % ((128 - tail) * 8);
@@ -195,22 +244,26 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                 fence_proxy_async();
                 __syncwarp();
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_probs[g]), (uint32_t)(i >> 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait));
-            if (!ok) break;
-            tcgen05_fence_after();
-            const uint64_t dv = desc_v + (uint64_t)(values.st * (int)(kTile >> 4));
-            const uint32_t d = tmem + 256 + g * DP, p = tmem + g * 128, more = i > 1;
-            if (elect_one()) {
+            const uint32_t low = (uint32_t)desc_v + values.st * (kTile >> 4), more = u > 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) tcgen05_mma_f16_ts(d, p + k * 8, dv + (uint64_t)(k * (2048 >> 4)), idesc_o, more | (uint32_t)(k > 0));
-                if (last) tcgen05_commit(smem_u32(&s_empty[values.st]));
-                if (i + 2 >= jobs) tcgen05_commit(smem_u32(&s_done[g]));
+            for (uint32_t h = 0; h < 2; ++h) {
+                ok = wait(&s_probs[g][h], (uint32_t)u & 1);
+                if (!ok) break;
+                tcgen05_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tcgen05_mma_f16_ts(d_o, d_s + h * 64 + k * 8, pack_f32x2(low + (4 * h + k) * (2048 >> 4), high_v), idesc_o, more | (uint32_t)(h > 0 || k > 0));
+                    if (h == 1) tcgen05_commit(smem_u32(&s_empty[values.st]));
+                    if (last) tcgen05_commit(smem_u32(h == 0 ? &s_half[g] : &s_done[g]));
+                }
+                __syncwarp();
+                if (!last) ok = scores(u + 1, h);
+                if (!ok) break;
             }
-            __syncwarp();
-            if (last) values.on(!two && i == n - 2 ? 1 : 2);
-            if (i + 2 < jobs) ok = scores(i + 2);
+            values.on(two ? 2 : g + (u + 1) * 2 == n - 1 ? 3 : 4);
         }
-    } else {
+    } else if (warp < 8) {
         const int g = warp >> 2, in_tile = (warp & 3) * 32 + lane, rows = a.batch * a.group;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                       // this warp's lanes of tensor memory
         const int row = (2 * pair + (two ? g : 0)) * 128 + in_tile;
@@ -238,32 +291,37 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
         mbar_arrive(smem_u32(&s_q));
 
         const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-38f);                  // (a scale of 0 must not meet the infinities of masked keys)
-        const uint64_t c2 = pack_f32x2(__float_as_uint(c), __float_as_uint(c));
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        int done = 0;
-        for (int i = g; i < jobs; i += 2, ++done) {
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_scores[g]), (uint32_t)done & 1, &s_abort, &g_attn_flag, kFlagLmWait));
+        const int mine = two ? n : (n - g + 1) / 2;
+        for (int i = 0; i < 2 * mine; ++i) {
+            const int h = i & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_scores[g][h]), (uint32_t)(i >> 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait));
             if (!ok) break;
             if (live_warp) {
                 tcgen05_fence_after();
-                const uint32_t ts = tmem + lanes + g * 128;
-                uint32_t s[128];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) tcgen05_ld32(ts + 32 * j, s + 32 * j);
+                const uint32_t ts = tmem + lanes + g * 128 + h * 64;
+                uint32_t s[64], p[32];
+                tcgen05_ld32(ts, s);
+                tcgen05_ld32(ts + 32, s + 32);
                 tcgen05_wait_ld();
-                if ((two ? i >> 1 : i) == n - 1 && tail < 128) {
+                if ((two ? i >> 1 : g + 2 * (i >> 1)) == n - 1 && tail < 128) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (j >= tail) s[j] = 0xff800000u;
+                    for (int j = 0; j < 64; ++j)
+                        if (j >= tail - 64 * h) s[j] = 0xff800000u;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 128; j += 2) top[(j >> 1) & 3] = fmaxf(top[(j >> 1) & 3], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                for (int j = 0; j < 64; j += 2) top[(j >> 1) & 3] = fmaxf(top[(j >> 1) & 3], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
                 const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-                if (done == 0) {
+                if (i == 0) {
                     m = next;
                 } else if (__any_sync(0xffffffffu, (next - m) * c > kSlack)) {   // (a NaN difference, -inf to -inf, is no growth)
+                    // The products of the half before may still be adding to O: the scores behind them tell of their end, or, for the last half, a barrier.
+                    ok = __all_sync(0xffffffffu, i + 1 < 2 * mine ? mbar_wait(smem_u32(&s_scores[g][h ^ 1]), (uint32_t)((i + 1) >> 1) & 1, &s_abort, &g_attn_flag, kFlagLmWait)
+                                                                  : mbar_wait(smem_u32(&s_half[g]), 0, &s_abort, &g_attn_flag, kFlagLmWait));
+                    if (!ok) break;
+                    tcgen05_fence_after();
                     const float keep = next == m ? 1.f : ex2((m - next) * c);
                     const uint32_t to = tmem + lanes + 256 + g * DP;
 #pragma unroll 1
@@ -278,33 +336,15 @@ __global__ void __launch_bounds__(320, 1) prefix_kernel(const __grid_constant__ 
                     l *= keep;
                     m = next;
                 }
-                const float base = m == -INFINITY ? 0.f : p_shift<T>() - m * c;
-                const uint64_t base2 = pack_f32x2(__float_as_uint(base), __float_as_uint(base));
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float x, y;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(s[64 * h + 2 * j], s[64 * h + 2 * j + 1]), c2, base2), x, y);
-                        x = ex2(x);
-                        y = ex2(y);
-                        sum[j & 1] = add_f32x2(sum[j & 1], pack_f32x2(__float_as_uint(x), __float_as_uint(y)));
-                        p[j] = lm_pack2<T>(x, y);
-                    }
-                    tcgen05_st32(ts + 32 * h, p);
-                }
-                float x, y;
-                unpack_f32x2(add_f32x2(sum[0], sum[1]), x, y);
-                l += x + y;
+                l += values_of<T>(s, c, m == -INFINITY ? 0.f : p_shift<T>() - m * c, p);
+                tcgen05_st32(ts, p);
                 tcgen05_wait_st();
                 tcgen05_fence_before();
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_probs[g]));
+            if (lane == 0) mbar_arrive(smem_u32(&s_probs[g][h]));
         }
-        if (ok && done > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_done[g]), 0, &s_abort, &g_attn_flag, kFlagLmWait));
+        if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_done[g]), 0, &s_abort, &g_attn_flag, kFlagLmWait));
         // This block's part of the rows.  A lone row tile's two accumulators become one first: the groups exchange halves of the values through the
         // shared memory that all products have left.  A row lies as DP / 4 pieces of 16 bytes, piece i at i ^ (row % 32): 32 rows are written without
         // bank conflicts and leave as one copy.
@@ -770,7 +810,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
 template <typename T, int DP>
 int launch_prefix(const AttnPlan& pl, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
     PB_CUDA(cudaFuncSetAttribute(prefix_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrefixShape<DP>::smem));
-    return lm_launch("pb_prefix_attn (prefix)", prefix_kernel<T, DP>, dim3((unsigned)pl.prefix_blocks), dim3(320), PrefixShape<DP>::smem, st, 1, pl.a, km, vm);
+    return lm_launch("pb_prefix_attn (prefix)", prefix_kernel<T, DP>, dim3((unsigned)pl.prefix_blocks), dim3(352), PrefixShape<DP>::smem, st, 1, pl.a, km, vm);
 }
 
 }  // namespace
