@@ -72,6 +72,12 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     return add_f32x2(r, both(-0x1p-126f));
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {        // (NaNs lose, as in fmaxf)
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's maximum is followed only once it has grown by 2^8: until then the values are up to 2^8 times too large, which fp32 sums and the
 // 16-bit values' exponents hold, and the accumulator need not be rescaled.
@@ -117,18 +123,19 @@ template <int DP> struct PrefixShape {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages;
+    constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages + 1;
     constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_done[2], s_q;
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_q;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
-    const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + 2 * kTile;
+    const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     const int pair = blockIdx.x % a.pairs, split = (blockIdx.x / a.pairs) % a.splits, kvh = blockIdx.x / (a.pairs * a.splits);
     const int kt0 = (int)((int64_t)a.key_tiles * split / a.splits), n = (int)((int64_t)a.key_tiles * (split + 1) / a.splits) - kt0;
     const bool two = 2 * pair + 1 < a.row_tiles;      // two row tiles; otherwise one, its key tiles dealt to both softmax groups
+    const uint32_t ring = q_smem + (two ? 2 : 1) * kTile, stages = two ? kStages - 1 : kStages;      // a lone tile leaves its partner's place to the ring
     const int tail = min(128, a.prefix_len - (kt0 + n - 1) * 128);       // keys of the last tile
 
     if (warp == 9) {
@@ -147,6 +154,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
                 mbar_init(smem_u32(&s_probs[i][h]), 4);
             }
             mbar_init(smem_u32(&s_half[i]), 1);
+            mbar_init(smem_u32(&s_turn[i]), 1);
             mbar_init(smem_u32(&s_done[i]), 1);
         }
         mbar_init(smem_u32(&s_q), 256);
@@ -160,34 +168,50 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
     griddep_launch();          // own_kernel, which reads nothing that precedes this launch in the stream but what has ended here
 
     if (warp == 8) {
-        // Keys and values in the order in which the products ask for them.
-        int st = 0;
-        uint32_t parity = 1;
-        for (int pos = 0; pos < 2 * n; ++pos) {
+        // Keys and values in the order in which the products ask for them.  A lane copies a box: `box_rows` tokens of a page, 64 values of each.  Its page is
+        // looked up four copies ahead (each on its own took 1500 clocks, which was the time of a tile).
+        const int box = lane / kBlocks, blk = lane % kBlocks;
+        const auto tile_of = [&](int pos, bool& values) {
+            if (two) { values = pos & 1; return pos >> 1; }
+            values = pos == 2 * n - 1 || (pos > 0 && !(pos & 1));
+            return pos == 0 ? 0 : pos == 2 * n - 1 ? n - 1 : values ? (pos - 2) >> 1 : (pos + 1) >> 1;
+        };
+        int page[4], row[4];
+        const auto look_up = [&](int pos, int& page, int& row) {
             bool values;
-            int t;
-            if (two) { values = pos & 1; t = pos >> 1; }
-            else if (pos == 0) { values = false; t = 0; }
-            else if (pos == 2 * n - 1) { values = true; t = n - 1; }
-            else if (pos & 1) { values = false; t = (pos + 1) >> 1; }
-            else { values = true; t = (pos - 2) >> 1; }
-            const int key0 = (kt0 + t) * 128, left = min(128, a.prefix_len - key0), boxes = (left + a.box_rows - 1) / a.box_rows;
-            const bool mine = lane < boxes * kBlocks;
-            const int box = lane / kBlocks, blk = lane % kBlocks, key = key0 + box * a.box_rows;
-            int page = 0;
-            if (mine) {
-                page = __ldcg(a.prefix_pages + key / a.page);
-                if (page < 0 || page >= a.n_pages) {
-                    atomicExch(&g_attn_flag, kFlagLmPage);
-                    page = a.n_pages;                 // outside of the map: zeros
-                }
+            const int key = (kt0 + tile_of(pos, values)) * 128 + box * a.box_rows;
+            if (pos < 2 * n && box * a.box_rows < 128 && key < a.prefix_len) {
+                const int at = key / a.page;
+                page = __ldcg(a.prefix_pages + at);
+                row = key - at * a.page;
             }
-            if (pos >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_attn_flag, kFlagLmWait))) break;
-            const uint32_t bar = smem_u32(&s_full[st]);
-            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
-            __syncwarp();
-            if (mine) tma_load_4d(ring + st * kTile + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, key % a.page, kvh, page, bar);
-            if (++st == kStages) { st = 0; parity ^= 1; }
+        };
+#pragma unroll
+        for (int k = 0; k < 4; ++k) look_up(k, page[k], row[k]);
+        uint32_t st = 0, parity = 1;
+        bool ok = true;
+        for (int pos0 = 0; pos0 < 2 * n && ok; pos0 += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int pos = pos0 + k;
+                if (pos >= 2 * n || !ok) break;
+                bool values;
+                const int left = min(128, a.prefix_len - (kt0 + tile_of(pos, values)) * 128), boxes = (left + a.box_rows - 1) / a.box_rows;
+                if (pos >= (int)stages) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_attn_flag, kFlagLmWait));
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&s_full[st]);
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
+                __syncwarp();
+                if (lane < boxes * kBlocks) {
+                    if (page[k] < 0 || page[k] >= a.n_pages) {
+                        atomicExch(&g_attn_flag, kFlagLmPage);
+                        page[k] = a.n_pages;          // outside of the map: zeros
+                    }
+                    tma_load_4d(ring + st * kTile + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, row[k], kvh, page[k], bar);
+                }
+                look_up(pos + 4, page[k], row[k]);
+                if (++st == stages) { st = 0; parity ^= 1; }
+            }
         }
     } else if (warp == 9 || warp == 10) {
         // The products of one softmax group: two warps, so that the waits of one lie under the products of the other.
@@ -198,9 +222,9 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
         // ... and the last one.
         struct Place {
             uint32_t st, parity;
-            __device__ __forceinline__ void on(uint32_t by) {
+            __device__ __forceinline__ void on(uint32_t by, uint32_t stages) {
                 st += by;
-                if (st >= kStages) { st -= kStages; parity ^= 1; }
+                if (st >= stages) { st -= stages; parity ^= 1; }
             }
         };
         const int g = warp - 9, mine = two ? n : (n - g + 1) / 2;      // key tiles of this group: g, g + 2 ... or all
@@ -209,6 +233,16 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
         const uint64_t desc_q = umma_desc_sw128(q_smem + (two ? g * kTile : 0)), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
         const uint32_t high_k = (uint32_t)(desc_k >> 32), high_v = (uint32_t)(desc_v >> 32), low_q = (uint32_t)desc_q;
         const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &s_abort, &g_attn_flag, kFlagLmWait)); };
+        // With two row tiles the groups take turns at the tensor cores, a half's values and the next scores in its place at a time: one's softmax then lies under
+        // the other's products.  (Left alone they fall into step: products of both mixed, then softmax of both.)  The turn goes on with half of the scores still
+        // to be issued, so that the other warp has seen it when they have been.
+        uint32_t turn = 0;
+        const auto take_turn = [&]() {
+            if (!two) return true;
+            const bool now = wait(&s_turn[g], turn);
+            turn ^= 1;
+            return now;
+        };
         // Scores of 64 keys, the first or second half of a tile, into their own 64 columns.
         const auto scores = [&](int u, uint32_t h) {
             if (h == 0 && !wait(&s_full[keys.st], keys.parity)) return false;
@@ -217,6 +251,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
+                    if (two && k == DP / 32) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
                     const uint32_t at = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
                     tcgen05_mma_bf16(d_s + h * 64, pack_f32x2(low_q + at, high_k), pack_f32x2(low + at, high_k), idesc_s, k > 0);
                 }
@@ -224,11 +259,14 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
                 if (h == 1) tcgen05_commit(smem_u32(&s_empty[keys.st]));
             }
             __syncwarp();
-            if (h == 1) keys.on(two ? 2 : u == 0 && g == 0 ? 3 : 4);
+            if (h == 1) keys.on(two ? 2 : u == 0 && g == 0 ? 3 : 4, stages);
             return true;
         };
         bool ok = wait(&s_q, 0);
-        if (ok && mine > 0) ok = scores(0, 0) && scores(0, 1);
+        if (ok && g == 1) ok = take_turn();
+        if (ok && mine > 0) ok = scores(0, 0);
+        if (ok) ok = take_turn();
+        if (ok && mine > 0) ok = scores(0, 1);
         for (int u = 0; ok && u < mine; ++u) {
             const bool last = u == mine - 1;
             ok = wait(&s_full[values.st], values.parity);
@@ -247,7 +285,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
             const uint32_t low = (uint32_t)desc_v + values.st * (kTile >> 4), more = u > 0;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
-                ok = wait(&s_probs[g][h], (uint32_t)u & 1);
+                ok = wait(&s_probs[g][h], (uint32_t)u & 1) && take_turn();
                 if (!ok) break;
                 tcgen05_fence_after();
                 if (elect_one()) {
@@ -259,9 +297,11 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
                 }
                 __syncwarp();
                 if (!last) ok = scores(u + 1, h);
+                else if (two && elect_one()) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
+                __syncwarp();
                 if (!ok) break;
             }
-            values.on(two ? 2 : g + (u + 1) * 2 == n - 1 ? 3 : 4);
+            values.on(two ? 2 : g + (u + 1) * 2 == n - 1 ? 3 : 4, stages);
         }
     } else if (warp < 8) {
         const int g = warp >> 2, in_tile = (warp & 3) * 32 + lane, rows = a.batch * a.group;
@@ -312,7 +352,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 64; j += 2) top[(j >> 1) & 3] = fmaxf(top[(j >> 1) & 3], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                for (int j = 0; j < 64; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
                 const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                 if (i == 0) {
                     m = next;
