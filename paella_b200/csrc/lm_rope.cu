@@ -4,8 +4,8 @@
 //
 // Both are bound by memory: every head is read once and written once, 4 operations a byte.  A group of lanes takes a head, each
 // lane both halves of its pairs, so that the rotation needs no exchange and only the norm's sum does (three shuffles for a head
-// of 128 values in 16 bits, whose group is eight lanes).  A group takes up to four heads of one token: the loads of all of them
-// are in flight before the first is used, and the rotation's row is loaded once.
+// of 128 values in 16 bits, whose group is eight lanes).  A group takes up to four neighbouring heads of one token: the loads of all
+// of them are in flight before the first is used, and the rotation's row is loaded once.
 #include <cuda.h>
 
 #include "lm.cuh"
@@ -35,42 +35,28 @@ struct RopeArgs {
     const int64_t* slots;      // NULL otherwise
     int64_t n_slots, page_stride, row_stride;
     int page_size;
+    int wide_weights;          // weights are 16-byte aligned
 };
 
-// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS heads of a token.
-template <typename T, int V, int CH, int HEADS>
-__global__ void __launch_bounds__(256) rope_kernel(RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS neighbouring heads of a token.
+// HELD: a lane's values wait in shared memory, in slots of its own, instead of registers: with 128 bytes of each thread on the way four blocks fit an SM, and
+// what they wait for (x, and behind the position the rotation's row) is covered by 128 KB in flight.  16384 tokens of 40 heads of 128 in bf16: TIMES
+template <typename T, int V, int CH, int HEADS, bool HELD>
+__global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    using Vt = LmVec<T, V>;
+    __shared__ __align__(16) Vt s_x[HELD ? HEADS * CH * 2 : 1][HELD ? 256 : 1];
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
-    using Vt = LmVec<T, V>;
     const int lane = threadIdx.x & (a.lanes - 1);
     const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / a.lanes;
     const int64_t token = group >> 32 ? group / a.slices : (uint32_t)group / (uint32_t)a.slices;    // (a 64-bit quotient takes some 70 instructions)
-    const int slice = (int)(group - token * a.slices);
+    const int head0 = (int)(group - token * a.slices) * HEADS;
     bool live = token < a.tokens;
-    int64_t slot = 0, page = 0;
-    bool store = true;                                   // keys and values of this token are stored
     int pos = 0;
-    if (live) {
-        if (a.slots) {
-            slot = a.slots[token];
-            store = slot >= 0;
-            if (slot >= a.n_slots) {
-                if (lane == 0) atomicExch(&g_rope_flag, kFlagLmSlot);
-                live = false;
-            }
-            page = slot >> 32 ? slot / a.page_size : (uint32_t)slot / (uint32_t)a.page_size;
-            slot -= page * a.page_size;
-        }
-        if (a.rot_dim) {
-            pos = a.positions[token];
-            if (pos < 0 || pos >= a.max_position) {
-                if (lane == 0 && store && live) atomicExch(&g_rope_flag, kFlagLmPosition);
-                live = false;
-            }
-        }
-    }
+    int64_t slot = 0;
+    if (live && a.rot_dim) pos = a.positions[token];
+    if (live && a.slots) slot = a.slots[token];
     // where this lane's chunks lie: `lo` and `hi`, V values each
     const int half = a.rot_dim / 2, turned = half / V;
     int lo[CH], hi[CH];                                  // -1 = none
@@ -87,25 +73,41 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a, uint32_t job_id, 
         if (lo[c] >= a.head_dim) lo[c] = -1;
         if (hi[c] >= a.head_dim) hi[c] = -1;
     }
-    Vt x[HEADS][CH][2];
-    int which[HEADS];
-    T* dst[HEADS];
+    Vt x[HELD ? 1 : HEADS][CH][2];
+    const auto set_of = [&](int head) { return head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2; };
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-        const int head = slice + h * a.slices;
-        which[h] = head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2;
-        if (!live || head >= a.first[2] || (which[h] && !store)) which[h] = -1;
-        if (which[h] < 0) continue;
-        const HeadSet& s = a.set[which[h]];
-        const int within = head - (which[h] ? a.first[which[h] - 1] : 0);
-        const T* src = static_cast<const T*>(s.src) + token * s.src_token + within * s.src_head;
-        dst[h] = static_cast<T*>(s.dst) + within * s.dst_head +
-                 (which[h] && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
+        const int head = head0 + h;
+        if (!live || head >= a.first[2]) continue;
+        const int w = set_of(head);
+        const T* src = static_cast<const T*>(a.set[w].src) + token * a.set[w].src_token + (head - (w ? a.first[w - 1] : 0)) * a.set[w].src_head;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if (lo[c] >= 0) x[h][c][0] = *reinterpret_cast<const Vt*>(src + lo[c]);
-            if (hi[c] >= 0) x[h][c][1] = *reinterpret_cast<const Vt*>(src + hi[c]);
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int at = p ? hi[c] : lo[c];
+                if (at < 0) continue;
+                if constexpr (HELD)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&s_x[(h * CH + c) * 2 + p][threadIdx.x])), "l"(src + at) : "memory");
+                else
+                    x[h][c][p] = *reinterpret_cast<const Vt*>(src + at);
+            }
+    }
+    if constexpr (HELD) asm volatile("cp.async.commit_group;" ::: "memory");
+    bool store = true;                                   // keys and values of this token are stored
+    int64_t page = 0;
+    if (live && a.slots) {
+        store = slot >= 0;
+        if (slot >= a.n_slots) {
+            if (lane == 0) atomicExch(&g_rope_flag, kFlagLmSlot);
+            live = false;
         }
+        page = slot >> 32 ? slot / a.page_size : (uint32_t)slot / (uint32_t)a.page_size;
+        slot -= page * a.page_size;
+    }
+    if (live && a.rot_dim && (pos < 0 || pos >= a.max_position)) {
+        if (lane == 0 && store) atomicExch(&g_rope_flag, kFlagLmPosition);
+        live = false;
     }
     float co[CH][V], si[CH][V];
 #pragma unroll
@@ -126,36 +128,60 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a, uint32_t job_id, 
             for (int j = 0; j < V; ++j) { co[c][j] = 1.f; si[c][j] = 0.f; }
         }
     }
-#pragma unroll
+    if constexpr (HELD) asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll(HELD ? 1 : HEADS)
     for (int h = 0; h < HEADS; ++h) {
-        const int w = which[h];
+        const int head = head0 + h;
+        int w = set_of(head);
+        if (!live || head >= a.first[2] || (w && !store)) w = -1;
         if (__all_sync(0xffffffffu, w < 0)) continue;
-        const float* weight = w < 0 ? nullptr : a.set[w].weight;
+        const HeadSet& s = a.set[w < 0 ? 0 : w];
+        const float* weight = w < 0 ? nullptr : s.weight;
+        T* dst = static_cast<T*>(s.dst) + (head - (w > 0 ? a.first[w - 1] : 0)) * s.dst_head +
+                 (w > 0 && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
+        Vt in[CH][2];
         float z[CH][2][V];
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                const bool there = (p ? hi[c] : lo[c]) >= 0;
+                const bool there = w >= 0 && (p ? hi[c] : lo[c]) >= 0;
+                if constexpr (HELD) {
+                    if (there) in[c][p] = s_x[(h * CH + c) * 2 + p][threadIdx.x];
+                } else {
+                    in[c][p] = x[h][c][p];
+                }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    z[c][p][j] = w >= 0 && there ? lm_to_f<T>(x[h][c][p].v[j]) : 0.f;
+                    z[c][p][j] = there ? lm_to_f<T>(in[c][p].v[j]) : 0.f;
                     sum += z[c][p][j] * z[c][p][j];
                 }
             }
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (__any_sync(0xffffffffu, weight != nullptr))
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (w < 0) continue;
         if (weight) {
             const float r = rsqrtf(sum / (float)a.head_dim + a.eps);
+            constexpr int W = V < 4 ? V : 4;             // (weights may lie at any float: wide accesses only where they do not)
+            const bool wide = V >= 4 && a.wide_weights;
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     const int at = p ? hi[c] : lo[c];
                     if (at < 0) continue;
+                    if (wide) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) z[c][p][j] *= r * __ldg(weight + at + j);
+                        for (int j = 0; j < V; j += W) {
+                            const LmVec<float, W> wv = *reinterpret_cast<const LmVec<float, W>*>(weight + at + j);
+#pragma unroll
+                            for (int k = 0; k < W; ++k) z[c][p][j + k] *= r * wv.v[k];
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) z[c][p][j] *= r * weight[at + j];
+                    }
                 }
         }
 #pragma unroll
@@ -184,11 +210,11 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a, uint32_t job_id, 
                     out[1].v[j] = lm_from_f<T>(z[c][1][j]);
                 }
             } else {                                     // as it was, a NaN's bits too
-                out[0] = x[h][c][0];
-                out[1] = x[h][c][1];
+                out[0] = in[c][0];
+                out[1] = in[c][1];
             }
-            if (lo[c] >= 0) *reinterpret_cast<Vt*>(dst[h] + lo[c]) = out[0];
-            if (hi[c] >= 0) *reinterpret_cast<Vt*>(dst[h] + hi[c]) = out[1];
+            if (lo[c] >= 0) *reinterpret_cast<Vt*>(dst + lo[c]) = out[0];
+            if (hi[c] >= 0) *reinterpret_cast<Vt*>(dst + hi[c]) = out[1];
         }
     }
     if (nf) nf->end(job_id);
@@ -211,8 +237,8 @@ bool vectors_fit(const HeadSet& s, int heads, int V, size_t es) {
 template <typename T>
 RopeFn pick(int V, int heads) {
     constexpr int VN = 16 / (int)sizeof(T);
-    if (V == VN) return heads == 4 ? rope_kernel<T, VN, 1, 4> : heads == 2 ? rope_kernel<T, VN, 1, 2> : rope_kernel<T, VN, 1, 1>;
-    return rope_kernel<T, 1, 4, 1>;
+    if (V == VN) return heads == 4 ? rope_kernel<T, VN, 1, 4, true> : heads == 2 ? rope_kernel<T, VN, 1, 2, false> : rope_kernel<T, VN, 1, 1, false>;
+    return rope_kernel<T, 1, 4, 1, false>;
 }
 
 int plan_rope(const char* who, int dtype, RopePlan& pl) {
@@ -227,6 +253,7 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
         before = a.first[i];
     }
     if (a.slots) wide = wide && a.page_stride % VN == 0 && a.row_stride % VN == 0;
+    a.wide_weights = aligned(a.set[0].weight, 16) && aligned(a.set[1].weight, 16);
     const int V = wide ? VN : 1;
     const int chunks = a.rot_dim / 2 / V + ceil_div(a.head_dim - a.rot_dim, 2 * V), per_lane = wide ? 1 : 4;
     a.lanes = 1;
