@@ -9,6 +9,7 @@
 #include <cuda.h>
 
 #include "lm.cuh"
+#include "umma.cuh"
 
 namespace pb {
 namespace {
@@ -28,7 +29,7 @@ struct RopeArgs {
     int first[3];              // heads before the end of each set: queries, then keys, then values
     int tokens, head_dim, rot_dim, interleaved, max_position, lanes;   // lanes: of a group, a power of two
     int slices;                // groups that share a token's heads out
-    float eps;
+    float eps, inv_dim;
     const float* cos_sin;
     const int32_t* positions;
     // an append: keys and values go to pages
@@ -38,13 +39,10 @@ struct RopeArgs {
     int wide_weights;          // weights are 16-byte aligned
 };
 
-// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS neighbouring heads of a token.
-// HELD: a lane's values wait in shared memory, in slots of its own, instead of registers: with 128 bytes of each thread on the way four blocks fit an SM, and
-// what they wait for (x, and behind the position the rotation's row) is covered by 128 KB in flight.  16384 tokens of 40 heads of 128 in bf16: TIMES
-template <typename T, int V, int CH, int HEADS, bool HELD>
-__global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS neighbouring heads of a token, in registers: few heads, or any alignment.
+template <typename T, int V, int CH, int HEADS>
+__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     using Vt = LmVec<T, V>;
-    __shared__ __align__(16) Vt s_x[HELD ? HEADS * CH * 2 : 1][HELD ? 256 : 1];
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
@@ -73,7 +71,7 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
         if (lo[c] >= a.head_dim) lo[c] = -1;
         if (hi[c] >= a.head_dim) hi[c] = -1;
     }
-    Vt x[HELD ? 1 : HEADS][CH][2];
+    Vt x[HEADS][CH][2];
     const auto set_of = [&](int head) { return head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2; };
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
@@ -86,14 +84,9 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int at = p ? hi[c] : lo[c];
-                if (at < 0) continue;
-                if constexpr (HELD)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&s_x[(h * CH + c) * 2 + p][threadIdx.x])), "l"(src + at) : "memory");
-                else
-                    x[h][c][p] = *reinterpret_cast<const Vt*>(src + at);
+                if (at >= 0) x[h][c][p] = *reinterpret_cast<const Vt*>(src + at);
             }
     }
-    if constexpr (HELD) asm volatile("cp.async.commit_group;" ::: "memory");
     bool store = true;                                   // keys and values of this token are stored
     int64_t page = 0;
     if (live && a.slots) {
@@ -128,8 +121,7 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
             for (int j = 0; j < V; ++j) { co[c][j] = 1.f; si[c][j] = 0.f; }
         }
     }
-    if constexpr (HELD) asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll(HELD ? 1 : HEADS)
+#pragma unroll
     for (int h = 0; h < HEADS; ++h) {
         const int head = head0 + h;
         int w = set_of(head);
@@ -139,7 +131,6 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
         const float* weight = w < 0 ? nullptr : s.weight;
         T* dst = static_cast<T*>(s.dst) + (head - (w > 0 ? a.first[w - 1] : 0)) * s.dst_head +
                  (w > 0 && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
-        Vt in[CH][2];
         float z[CH][2][V];
         float sum = 0.f;
 #pragma unroll
@@ -147,14 +138,9 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const bool there = w >= 0 && (p ? hi[c] : lo[c]) >= 0;
-                if constexpr (HELD) {
-                    if (there) in[c][p] = s_x[(h * CH + c) * 2 + p][threadIdx.x];
-                } else {
-                    in[c][p] = x[h][c][p];
-                }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    z[c][p][j] = there ? lm_to_f<T>(in[c][p].v[j]) : 0.f;
+                    z[c][p][j] = there ? lm_to_f<T>(x[h][c][p].v[j]) : 0.f;
                     sum += z[c][p][j] * z[c][p][j];
                 }
             }
@@ -162,7 +148,7 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
             for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (w < 0) continue;
         if (weight) {
-            const float r = rsqrtf(sum / (float)a.head_dim + a.eps);
+            const float r = rsqrtf(sum * a.inv_dim + a.eps);
             constexpr int W = V < 4 ? V : 4;             // (weights may lie at any float: wide accesses only where they do not)
             const bool wide = V >= 4 && a.wide_weights;
 #pragma unroll
@@ -210,11 +196,216 @@ __global__ void __launch_bounds__(256, HELD ? 4 : 1) rope_kernel(const __grid_co
                     out[1].v[j] = lm_from_f<T>(z[c][1][j]);
                 }
             } else {                                     // as it was, a NaN's bits too
-                out[0] = in[c][0];
-                out[1] = in[c][1];
+                out[0] = x[h][c][0];
+                out[1] = x[h][c][1];
             }
             if (lo[c] >= 0) *reinterpret_cast<Vt*>(dst + lo[c]) = out[0];
             if (hi[c] >= 0) *reinterpret_cast<Vt*>(dst + hi[c]) = out[1];
+        }
+    }
+    if (nf) nf->end(job_id);
+}
+
+// The same for many heads, in accesses of 16 bytes: a lane's values wait in shared memory, in slots of its own, so that a thread has 128 or 256 bytes on the way
+// and an SM 96 or 192 KB, which cover the latency of x and, behind the position, of the rotation's row.  What the general kernel spends most on beside the
+// transfers, weights and rotation for each head, is found once here: products of weight and cosine or sine of a lane's pairs, again only where
+// queries end and keys begin.  16384 tokens of 40 heads of 128 in bf16: TIMES
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t two(float x, float y) { return pack_f32x2(__float_as_uint(x), __float_as_uint(y)); }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// 16 bytes of each half of a lane's chunk to pairs of floats, A and B of the pairs (j, j + 1), and back
+template <typename T, bool interleaved>
+__device__ __forceinline__ void spread(uint4 lo, uint4 hi, uint64_t (&A)[8 / sizeof(T)], uint64_t (&B)[8 / sizeof(T)]) {
+    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
+    if constexpr (sizeof(T) == 4) {
+        if (interleaved) {
+            A[0] = pack_f32x2(l[0], l[2]); B[0] = pack_f32x2(l[1], l[3]); A[1] = pack_f32x2(h[0], h[2]); B[1] = pack_f32x2(h[1], h[3]);
+        } else {
+            A[0] = pack_f32x2(l[0], l[1]); A[1] = pack_f32x2(l[2], l[3]); B[0] = pack_f32x2(h[0], h[1]); B[1] = pack_f32x2(h[2], h[3]);
+        }
+    } else {
+        if (interleaved) {
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                const float2 x = unpack2<T>(l[k]), y = unpack2<T>(l[k + 1]), u = unpack2<T>(h[k]), v = unpack2<T>(h[k + 1]);
+                A[k / 2] = two(x.x, y.x); B[k / 2] = two(x.y, y.y);
+                A[2 + k / 2] = two(u.x, v.x); B[2 + k / 2] = two(u.y, v.y);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 x = unpack2<T>(l[k]), u = unpack2<T>(h[k]);
+                A[k] = two(x.x, x.y);
+                B[k] = two(u.x, u.y);
+            }
+        }
+    }
+}
+template <typename T, bool interleaved>
+__device__ __forceinline__ void gather(const uint64_t (&A)[8 / sizeof(T)], const uint64_t (&B)[8 / sizeof(T)], uint4& lo, uint4& hi) {
+    uint32_t l[4], h[4];
+    constexpr int N = 8 / sizeof(T);
+    float a[2 * N], b[2 * N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        unpack_f32x2(A[j], a[2 * j], a[2 * j + 1]);
+        unpack_f32x2(B[j], b[2 * j], b[2 * j + 1]);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            l[k] = __float_as_uint(interleaved ? (k & 1 ? b[k / 2] : a[k / 2]) : a[k]);
+            h[k] = __float_as_uint(interleaved ? (k & 1 ? b[2 + k / 2] : a[2 + k / 2]) : b[k]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            l[k] = interleaved ? lm_pack2<T>(a[k], b[k]) : lm_pack2<T>(a[2 * k], a[2 * k + 1]);
+            h[k] = interleaved ? lm_pack2<T>(a[4 + k], b[4 + k]) : lm_pack2<T>(b[2 * k], b[2 * k + 1]);
+        }
+    }
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+template <typename T, int HEADS, bool interleaved>
+__global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    constexpr int V = 16 / (int)sizeof(T), N = V / 2;
+    extern __shared__ __align__(16) uint4 s_values[];    // [2 HEADS][256]
+    griddep_wait();
+    if (nf) nf->start(job_id);
+    griddep_launch();
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const uint32_t mates = (a.lanes == 32 ? 0xffffffffu : (1u << a.lanes) - 1u) << (threadIdx.x & 31 & ~(a.lanes - 1));     // the group's lanes
+    const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / a.lanes;
+    const int64_t token = group >> 32 ? group / a.slices : (uint32_t)group / (uint32_t)a.slices;
+    const int head0 = (int)(group - token * a.slices) * HEADS;
+    bool live = token < a.tokens;
+    const int count = live ? min(HEADS, a.first[2] - head0) : 0;
+    int pos = 0;
+    int64_t slot = 0;
+    if (live && a.rot_dim) pos = a.positions[token];
+    if (live && a.slots) slot = a.slots[token];
+    const int half = a.rot_dim / 2;
+    const bool turn = V * lane < half;                   // this lane's chunk is rotated
+    const int lo = turn ? (interleaved ? 2 * V * lane : V * lane) : a.rot_dim + 2 * (V * lane - half), hi = turn && !interleaved ? lo + half : lo + V;
+    const bool has_lo = lo < a.head_dim, has_hi = hi < a.head_dim;
+    const auto set_of = [&](int head) { return head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2; };
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&s_values[threadIdx.x]);
+    for (int h = 0; h < count;) {
+        const int w = set_of(head0 + h), end = min(count, a.first[w] - head0);
+        const T* src = static_cast<const T*>(a.set[w].src) + token * a.set[w].src_token + (head0 + h - (w ? a.first[w - 1] : 0)) * a.set[w].src_head;
+        for (; h < end; ++h, src += a.set[w].src_head) {
+            if (has_lo) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + h * 8192), "l"(src + lo) : "memory");
+            if (has_hi) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + h * 8192 + 4096), "l"(src + hi) : "memory");
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    bool store = true;                                   // keys and values of this token are stored
+    int64_t page = 0;
+    if (live && a.slots) {
+        store = slot >= 0;
+        if (slot >= a.n_slots) {
+            if (lane == 0) atomicExch(&g_rope_flag, kFlagLmSlot);
+            live = false;
+        }
+        page = slot >> 32 ? slot / a.page_size : (uint32_t)slot / (uint32_t)a.page_size;
+        slot -= page * a.page_size;
+    }
+    if (live && a.rot_dim && (pos < 0 || pos >= a.max_position)) {
+        if (lane == 0 && store) atomicExch(&g_rope_flag, kFlagLmPosition);
+        live = false;
+    }
+    uint64_t cosines[N], sines[N];
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), n = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live && turn) {
+            const float* row = a.cos_sin + (int64_t)pos * a.rot_dim + V * lane + 2 * j;
+            c = *reinterpret_cast<const float4*>(row);
+            n = *reinterpret_cast<const float4*>(row + half);
+        }
+        cosines[j] = two(c.x, c.y); cosines[j + 1] = two(c.z, c.w);
+        sines[j] = two(n.x, n.y); sines[j + 1] = two(n.z, n.w);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // Heads of one kind after another.  (The lanes of a group go through this together, the groups of a warp need not.)
+    for (int h = 0; h < count && live;) {
+        const int w = set_of(head0 + h), end = min(count, a.first[w] - head0);
+        const HeadSet& s = a.set[w];
+        if (w && !store) { h = end; continue; }
+        T* dst = static_cast<T*>(s.dst) + (head0 + h - (w ? a.first[w - 1] : 0)) * s.dst_head + (w && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
+        const float* weight = s.weight;
+        if (w == 2 || (!weight && !a.rot_dim)) {         // as they are, a NaN's bits too
+            for (; h < end; ++h, dst += s.dst_head) {
+                if (has_lo) *reinterpret_cast<uint4*>(dst + lo) = s_values[2 * h * 256 + threadIdx.x];
+                if (has_hi) *reinterpret_cast<uint4*>(dst + hi) = s_values[(2 * h + 1) * 256 + threadIdx.x];
+            }
+            continue;
+        }
+        // out A = r (A ca + B nb), out B = r (B cb + A sa) with ca = wa cos, nb = -wb sin, cb = wb cos, sa = wa sin
+        uint64_t ca[N], cb[N], sa[N], nb[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float wa[2], wb[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int at_a = interleaved ? lo + 4 * j + 2 * k : lo + 2 * j + k, at_b = interleaved ? at_a + 1 : hi + 2 * j + k;
+                wa[k] = weight && at_a < a.head_dim ? weight[at_a] : 1.f;
+                wb[k] = weight && at_b < a.head_dim ? weight[at_b] : 1.f;
+            }
+            const uint64_t x = two(wa[0], wa[1]), y = two(wb[0], wb[1]);
+            ca[j] = mul_f32x2(x, cosines[j]);
+            cb[j] = mul_f32x2(y, cosines[j]);
+            sa[j] = mul_f32x2(x, sines[j]);
+            nb[j] = mul_f32x2(y, mul_f32x2(sines[j], two(-1.f, -1.f)));
+        }
+        for (; h < end; ++h, dst += s.dst_head) {
+            uint4 lv = make_uint4(0, 0, 0, 0), hv = lv;
+            if (has_lo) lv = s_values[2 * h * 256 + threadIdx.x];
+            if (has_hi) hv = s_values[(2 * h + 1) * 256 + threadIdx.x];
+            uint64_t A[N], B[N];
+            spread<T, interleaved>(lv, hv, A, B);
+            if (weight) {
+                uint64_t sum2 = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum2 = fma_f32x2(B[j], B[j], fma_f32x2(A[j], A[j], sum2));
+                float x, y;
+                unpack_f32x2(sum2, x, y);
+                float sum = x + y;
+                for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
+                const float r = rsqrtf(sum * a.inv_dim + a.eps);
+                const uint64_t r2 = two(r, r);
+#pragma unroll
+                for (int j = 0; j < N; ++j) A[j] = mul_f32x2(A[j], r2), B[j] = mul_f32x2(B[j], r2);
+            }
+            if (weight || turn) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const uint64_t x = A[j], y = B[j];
+                    A[j] = mul_f32x2(x, ca[j]);
+                    B[j] = mul_f32x2(y, cb[j]);
+                    if (turn) {
+                        A[j] = fma_f32x2(y, nb[j], A[j]);
+                        B[j] = fma_f32x2(x, sa[j], B[j]);
+                    }
+                }
+                gather<T, interleaved>(A, B, lv, hv);
+            }
+            if (has_lo) *reinterpret_cast<uint4*>(dst + lo) = lv;
+            if (has_hi) *reinterpret_cast<uint4*>(dst + hi) = hv;
         }
     }
     if (nf) nf->end(job_id);
@@ -226,6 +417,7 @@ struct RopePlan {
     RopeArgs a;
     RopeFn fn;
     unsigned blocks;
+    int smem;
 };
 
 // All accesses of V values of `es` bytes of this set are aligned to their size.
@@ -235,10 +427,12 @@ bool vectors_fit(const HeadSet& s, int heads, int V, size_t es) {
 }
 
 template <typename T>
-RopeFn pick(int V, int heads) {
+RopeFn pick(bool wide, int heads, bool interleaved) {
     constexpr int VN = 16 / (int)sizeof(T);
-    if (V == VN) return heads == 4 ? rope_kernel<T, VN, 1, 4, true> : heads == 2 ? rope_kernel<T, VN, 1, 2, false> : rope_kernel<T, VN, 1, 1, false>;
-    return rope_kernel<T, 1, 4, 1, false>;
+    if (!wide) return rope_kernel<T, 1, 4, 1>;
+    if (heads == 8) return interleaved ? rope_many_kernel<T, 8, true> : rope_many_kernel<T, 8, false>;
+    if (heads == 4) return interleaved ? rope_many_kernel<T, 4, true> : rope_many_kernel<T, 4, false>;
+    return heads == 2 ? rope_kernel<T, VN, 1, 2> : rope_kernel<T, VN, 1, 1>;
 }
 
 int plan_rope(const char* who, int dtype, RopePlan& pl) {
@@ -253,6 +447,7 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
         before = a.first[i];
     }
     if (a.slots) wide = wide && a.page_stride % VN == 0 && a.row_stride % VN == 0;
+    a.inv_dim = 1.f / (float)a.head_dim;
     a.wide_weights = aligned(a.set[0].weight, 16) && aligned(a.set[1].weight, 16);
     const int V = wide ? VN : 1;
     const int chunks = a.rot_dim / 2 / V + ceil_div(a.head_dim - a.rot_dim, 2 * V), per_lane = wide ? 1 : 4;
@@ -262,13 +457,14 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
     // Heads of a group: as many as leave the GPU two waves of threads.
     int each = 1;
     if (wide)
-        for (int e = 4; e > 1; e /= 2)
-            if (heads >= e && (int64_t)a.tokens * ceil_div(heads, e) * a.lanes >= 2 * 148 * 2048) { each = e; break; }
+        for (int e = 8; e > 1; e /= 2)
+            if (heads >= e && (int64_t)a.tokens * ceil_div(heads, e) * a.lanes >= 2 * 148 * 768) { each = e; break; }
     a.slices = ceil_div(heads, each);
     const int64_t blocks = ceil_div<int64_t>((int64_t)a.tokens * a.slices * a.lanes, 256);
     PB_REQUIRE(blocks <= 0x7fffffff, "%s: %d tokens of %d heads are too many for one launch", who, a.tokens, heads);
     pl.blocks = blocks > 0 ? (unsigned)blocks : 1u;
-    pl.fn = dtype == PB_F32 ? pick<float>(V, each) : dtype == PB_BF16 ? pick<__nv_bfloat16>(V, each) : pick<__half>(V, each);
+    pl.fn = dtype == PB_F32 ? pick<float>(wide, each, a.interleaved) : dtype == PB_BF16 ? pick<__nv_bfloat16>(wide, each, a.interleaved) : pick<__half>(wide, each, a.interleaved);
+    pl.smem = each >= 4 ? each * 8192 : 0;
     return PB_OK;
 }
 
@@ -338,10 +534,16 @@ int rope_info(const RopePlan& pl, int dtype, pb_launch_info* out) {
     const uint64_t t = (uint64_t)a.tokens, es = dtype_bytes(dtype);
     out->num_blocks = pl.blocks;
     out->threads_per_block = 256;
+    out->smem_per_block = (uint32_t)pl.smem;
     out->regs_per_thread = lm_regs(pl.fn);
     out->flops = t * ((uint64_t)a.first[1] * 3 * a.rot_dim + 4ull * a.head_dim * ((a.set[0].weight ? a.first[0] : 0) + (a.set[1].weight ? a.first[1] - a.first[0] : 0)));
     out->bytes = t * (2 * es * a.head_dim * a.first[2] + (a.rot_dim ? 4ull * a.rot_dim + 4 : 0) + (a.slots ? 8 : 0));
     return PB_OK;
+}
+
+int launch_rope(const char* who, const RopePlan& pl, void* stream, uint32_t job_id, void* notifier) {
+    if (pl.smem > 48 * 1024) PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+    return lm_launch(who, pl.fn, dim3(pl.blocks), dim3(256), (size_t)pl.smem, (cudaStream_t)stream, 1, pl.a, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 }  // namespace
@@ -368,7 +570,7 @@ int pb_qk_rope_launch(const pb_qk_rope_params* p, void* stream, uint32_t job_id,
     pb::RopePlan pl;
     const int rc = pb::rope_plan(p, pl);
     if (rc != PB_OK) return rc;
-    return pb::lm_launch("pb_qk_rope", pl.fn, dim3(pl.blocks), dim3(256), 0, (cudaStream_t)stream, 1, pl.a, job_id, (pb::FinishedBlockNotifier*)notifier);
+    return pb::launch_rope("pb_qk_rope", pl, stream, job_id, notifier);
 }
 
 int pb_kv_append_info(const pb_kv_append_params* p, pb_launch_info* out) {
@@ -383,7 +585,7 @@ int pb_kv_append_launch(const pb_kv_append_params* p, void* stream, uint32_t job
     pb::RopePlan pl;
     const int rc = pb::append_plan(p, pl);
     if (rc != PB_OK) return rc;
-    return pb::lm_launch("pb_kv_append", pl.fn, dim3(pl.blocks), dim3(256), 0, (cudaStream_t)stream, 1, pl.a, job_id, (pb::FinishedBlockNotifier*)notifier);
+    return pb::launch_rope("pb_kv_append", pl, stream, job_id, notifier);
 }
 
 }  // extern "C"
