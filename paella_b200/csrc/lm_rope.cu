@@ -341,6 +341,32 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
         sines[j] = two(n.x, n.y); sines[j + 1] = two(n.z, n.w);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // The norms of all heads first: eight sums over the lanes side by side, where one after the other each head would wait for three shuffles and a root.
+    float* const norms = reinterpret_cast<float*>(s_values + 2 * HEADS * 256) + threadIdx.x;     // [HEADS][256]
+    if (live && (a.set[0].weight || a.set[1].weight)) {
+        float sum[HEADS];
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            uint64_t sum2 = 0;
+            if (head0 + h < a.first[1]) {
+                uint64_t A[N], B[N];
+                uint4 lv = make_uint4(0, 0, 0, 0), hv = lv;
+                if (has_lo) lv = s_values[2 * h * 256 + threadIdx.x];
+                if (has_hi) hv = s_values[(2 * h + 1) * 256 + threadIdx.x];
+                spread<T, interleaved>(lv, hv, A, B);
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum2 = fma_f32x2(B[j], B[j], fma_f32x2(A[j], A[j], sum2));
+            }
+            float x, y;
+            unpack_f32x2(sum2, x, y);
+            sum[h] = x + y;
+        }
+        for (int o = a.lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) sum[h] += __shfl_xor_sync(mates, sum[h], o);
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) norms[h * 256] = rsqrtf(sum[h] * a.inv_dim + a.eps);
+    }
     // Heads of one kind after another.  (The lanes of a group go through this together, the groups of a warp need not.)
     for (int h = 0; h < count && live;) {
         const int w = set_of(head0 + h), end = min(count, a.first[w] - head0);
@@ -357,16 +383,20 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
         }
         // out A = r (A ca + B nb), out B = r (B cb + A sa) with ca = wa cos, nb = -wb sin, cb = wb cos, sa = wa sin
         uint64_t ca[N], cb[N], sa[N], nb[N];
+        float w_lo[V], w_hi[V];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            float4 x = make_float4(1.f, 1.f, 1.f, 1.f), y = x;
+            if (weight && has_lo) x = a.wide_weights ? *reinterpret_cast<const float4*>(weight + lo + j) : make_float4(weight[lo + j], weight[lo + j + 1], weight[lo + j + 2], weight[lo + j + 3]);
+            if (weight && has_hi) y = a.wide_weights ? *reinterpret_cast<const float4*>(weight + hi + j) : make_float4(weight[hi + j], weight[hi + j + 1], weight[hi + j + 2], weight[hi + j + 3]);
+            w_lo[j] = x.x; w_lo[j + 1] = x.y; w_lo[j + 2] = x.z; w_lo[j + 3] = x.w;
+            w_hi[j] = y.x; w_hi[j + 1] = y.y; w_hi[j + 2] = y.z; w_hi[j + 3] = y.w;
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            float wa[2], wb[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int at_a = interleaved ? lo + 4 * j + 2 * k : lo + 2 * j + k, at_b = interleaved ? at_a + 1 : hi + 2 * j + k;
-                wa[k] = weight && at_a < a.head_dim ? weight[at_a] : 1.f;
-                wb[k] = weight && at_b < a.head_dim ? weight[at_b] : 1.f;
-            }
-            const uint64_t x = two(wa[0], wa[1]), y = two(wb[0], wb[1]);
+            // (interleaved: pairs 2 j and 2 j + 1 are values 4 j to 4 j + 3 of the lane's 2 V)
+            const float* w4 = 4 * j < V ? w_lo + 4 * j : w_hi + (4 * j - V);
+            const uint64_t x = interleaved ? two(w4[0], w4[2]) : two(w_lo[2 * j], w_lo[2 * j + 1]), y = interleaved ? two(w4[1], w4[3]) : two(w_hi[2 * j], w_hi[2 * j + 1]);
             ca[j] = mul_f32x2(x, cosines[j]);
             cb[j] = mul_f32x2(y, cosines[j]);
             sa[j] = mul_f32x2(x, sines[j]);
@@ -379,14 +409,7 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
             uint64_t A[N], B[N];
             spread<T, interleaved>(lv, hv, A, B);
             if (weight) {
-                uint64_t sum2 = 0;
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum2 = fma_f32x2(B[j], B[j], fma_f32x2(A[j], A[j], sum2));
-                float x, y;
-                unpack_f32x2(sum2, x, y);
-                float sum = x + y;
-                for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
-                const float r = rsqrtf(sum * a.inv_dim + a.eps);
+                const float r = norms[h * 256];
                 const uint64_t r2 = two(r, r);
 #pragma unroll
                 for (int j = 0; j < N; ++j) A[j] = mul_f32x2(A[j], r2), B[j] = mul_f32x2(B[j], r2);
@@ -464,7 +487,7 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
     PB_REQUIRE(blocks <= 0x7fffffff, "%s: %d tokens of %d heads are too many for one launch", who, a.tokens, heads);
     pl.blocks = blocks > 0 ? (unsigned)blocks : 1u;
     pl.fn = dtype == PB_F32 ? pick<float>(wide, each, a.interleaved) : dtype == PB_BF16 ? pick<__nv_bfloat16>(wide, each, a.interleaved) : pick<__half>(wide, each, a.interleaved);
-    pl.smem = each >= 4 ? each * 8192 : 0;
+    pl.smem = each >= 4 ? each * (8192 + 1024) : 0;
     return PB_OK;
 }
 
