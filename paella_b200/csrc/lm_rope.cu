@@ -298,9 +298,13 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
     int64_t slot = 0;
     if (live && a.rot_dim) pos = a.positions[token];
     if (live && a.slots) slot = a.slots[token];
-    const int half = a.rot_dim / 2;
-    const bool turn = V * lane < half;                   // this lane's chunk is rotated
-    const int lo = turn ? (interleaved ? 2 * V * lane : V * lane) : a.rot_dim + 2 * (V * lane - half), hi = turn && !interleaved ? lo + half : lo + V;
+    // This lane's two vectors of V values.  In halves: V values of the first half and their partners.  Pairs side by side: vectors `lane` and `lane` + half
+    // their number, so that neighbouring lanes have neighbouring bytes; what is not rotated in the same way.
+    const int half = a.rot_dim / 2, turned = half / V, rest = interleaved ? a.head_dim / V : (a.head_dim - a.rot_dim) / V, first = interleaved ? lane : lane - turned;
+    const int from = interleaved ? 0 : a.rot_dim, second = first + (rest + 1) / 2;
+    const bool in_halves = !interleaved && lane < turned;
+    const int lo = in_halves ? V * lane : first < (rest + 1) / 2 ? from + V * first : a.head_dim, hi = in_halves ? V * lane + half : second < rest ? from + V * second : a.head_dim;
+    const bool turn_lo = lo < a.rot_dim, turn_hi = hi < a.rot_dim;
     const bool has_lo = lo < a.head_dim, has_hi = hi < a.head_dim;
     const auto set_of = [&](int head) { return head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2; };
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&s_values[threadIdx.x]);
@@ -328,17 +332,21 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
         if (lane == 0 && store) atomicExch(&g_rope_flag, kFlagLmPosition);
         live = false;
     }
-    uint64_t cosines[N], sines[N];
+    float cosines[V], sines[V];                          // of pairs j
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), n = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (live && turn) {
-            const float* row = a.cos_sin + (int64_t)pos * a.rot_dim + V * lane + 2 * j;
-            c = *reinterpret_cast<const float4*>(row);
-            n = *reinterpret_cast<const float4*>(row + half);
+    for (int p = 0; p < 2; ++p) {
+        constexpr int W = V / 2;
+        const int pair = interleaved ? (p ? hi : lo) / 2 : lo + p * W;
+        LmVec<float, W> c, n;
+#pragma unroll
+        for (int k = 0; k < W; ++k) c.v[k] = 1.f, n.v[k] = 0.f;
+        if (live && (interleaved && p ? turn_hi : turn_lo)) {
+            const float* row = a.cos_sin + (int64_t)pos * a.rot_dim + pair;
+            c = *reinterpret_cast<const LmVec<float, W>*>(row);
+            n = *reinterpret_cast<const LmVec<float, W>*>(row + half);
         }
-        cosines[j] = two(c.x, c.y); cosines[j + 1] = two(c.z, c.w);
-        sines[j] = two(n.x, n.y); sines[j + 1] = two(n.z, n.w);
+#pragma unroll
+        for (int k = 0; k < W; ++k) cosines[p * W + k] = c.v[k], sines[p * W + k] = n.v[k];
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     // The norms of all heads first: eight sums over the lanes side by side, where one after the other each head would wait for three shuffles and a root.
@@ -397,10 +405,10 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
             // (interleaved: pairs 2 j and 2 j + 1 are values 4 j to 4 j + 3 of the lane's 2 V)
             const float* w4 = 4 * j < V ? w_lo + 4 * j : w_hi + (4 * j - V);
             const uint64_t x = interleaved ? two(w4[0], w4[2]) : two(w_lo[2 * j], w_lo[2 * j + 1]), y = interleaved ? two(w4[1], w4[3]) : two(w_hi[2 * j], w_hi[2 * j + 1]);
-            ca[j] = mul_f32x2(x, cosines[j]);
-            cb[j] = mul_f32x2(y, cosines[j]);
-            sa[j] = mul_f32x2(x, sines[j]);
-            nb[j] = mul_f32x2(y, mul_f32x2(sines[j], two(-1.f, -1.f)));
+            ca[j] = mul_f32x2(x, two(cosines[2 * j], cosines[2 * j + 1]));
+            cb[j] = mul_f32x2(y, two(cosines[2 * j], cosines[2 * j + 1]));
+            sa[j] = mul_f32x2(x, two(sines[2 * j], sines[2 * j + 1]));
+            nb[j] = mul_f32x2(y, two(-sines[2 * j], -sines[2 * j + 1]));
         }
         for (; h < end; ++h, dst += s.dst_head) {
             uint4 lv = make_uint4(0, 0, 0, 0), hv = lv;
@@ -414,13 +422,13 @@ __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant
 #pragma unroll
                 for (int j = 0; j < N; ++j) A[j] = mul_f32x2(A[j], r2), B[j] = mul_f32x2(B[j], r2);
             }
-            if (weight || turn) {
+            if (weight || turn_lo) {                     // (a lane whose second vector alone turned does not exist)
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     const uint64_t x = A[j], y = B[j];
                     A[j] = mul_f32x2(x, ca[j]);
                     B[j] = mul_f32x2(y, cb[j]);
-                    if (turn) {
+                    if (interleaved && 2 * j >= N ? turn_hi : turn_lo) {
                         A[j] = fma_f32x2(y, nb[j], A[j]);
                         B[j] = fma_f32x2(x, sa[j], B[j]);
                     }
@@ -473,7 +481,8 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
     a.inv_dim = 1.f / (float)a.head_dim;
     a.wide_weights = aligned(a.set[0].weight, 16) && aligned(a.set[1].weight, 16);
     const int V = wide ? VN : 1;
-    const int chunks = a.rot_dim / 2 / V + ceil_div(a.head_dim - a.rot_dim, 2 * V), per_lane = wide ? 1 : 4;
+    int chunks = a.rot_dim / 2 / V + ceil_div(a.head_dim - a.rot_dim, 2 * V);
+    const int per_lane = wide ? 1 : 4;
     a.lanes = 1;
     while (a.lanes * per_lane < chunks) a.lanes *= 2;
     const int heads = a.first[2];

@@ -101,6 +101,45 @@ def test_rope_counts(ty, t, hq, hk):
     assert bool((o[t:] == 9.0).all())
 
 
+# so many tokens that a group takes four and eight heads; vectors in odd number, part rotated, kinds of head that change within a group
+@pytest.mark.parametrize("t,hq,hk,d,rot", [(20000, 7, 2, 128, 128), (30011, 3, 5, 64, 32), (26003, 9, 1, 72, 48), (40000, 5, 2, 104, 32), (60000, 4, 4, 8, 0), (9001, 33, 4, 256, 256), (24000, 8, 3, 96, 96)])
+@pytest.mark.parametrize("ty,interleaved,norm", [("f32", 0, True), ("f32", 1, False), ("bf16", 1, True), ("f16", 0, False), ("bf16", 0, True)])
+def test_many_tokens(ty, interleaved, norm, t, hq, hk, d, rot):
+    g = lu.gen(t + d)
+    x = heads(g, t, hq + 2 * hk, d, ty)
+    q, k, v = x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:]
+    qw, kw = (1 + 0.3 * lu.randn(g, d), 1 + 0.3 * lu.randn(g, d)) if norm else (None, None)
+    tab = table(777, rot)
+    pos = torch.randint(0, 777, (t,), generator=g, device="cuda", dtype=torch.int32)
+    qo, ko = torch.full((t, hq, d), 9.0, device="cuda", dtype=x.dtype), torch.full((t + 1, hk, d), 9.0, device="cuda", dtype=x.dtype)
+    lu.launch("qk_rope", rope_params(ty, q, k, qo, ko, qw, kw, tab, pos, rot, interleaved))
+    gu.sync()
+    check(qo, *ref_heads(q, qw, tab, pos, rot, interleaved), ty)
+    check(ko[:t], *ref_heads(k, kw, tab, pos, rot, interleaved), ty)
+    assert bool((ko[t] == 9.0).all())
+    page, pages = 32, t // 32 + 3
+    kc, vc = (cache(pages, page, hk, d, ty, True) for _ in range(2))
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:t].contiguous()
+    slots[t // 3:t // 3 + 100] = -2
+    qo.fill_(9.0)
+    lu.launch("kv_append", append_params(ty, k, v, kc, vc, slots, page, tab, pos, rot, interleaved, kw, True, q=q, qo=qo, qw=qw))
+    gu.sync()
+    real = slots >= 0
+    ref, mag = ref_heads(k, kw, tab, pos, rot, interleaved)
+    check(rows(kc, slots[real], page, True), ref[real], mag[real], ty)
+    assert torch.equal(rows(vc, slots[real], page, True), v[real])
+    for c in (kc, vc):
+        assert int((c != 9.0).any(-1).sum()) == int(real.sum()) * hk
+    check(qo, *ref_heads(q, qw, tab, pos, rot, interleaved), ty)
+    pos[5], slots[7] = 777, pages * page                         # and what is out of range is left out
+    qo.fill_(9.0)
+    lu.launch("kv_append", append_params(ty, k, v, kc, vc, slots, page, tab, pos, rot, interleaved, kw, True, q=q, qo=qo, qw=qw))
+    gu.sync()
+    assert gu.error_flag() != 0
+    left = [5, 7] if rot else [7]
+    assert bool((qo[left] == 9.0).all()) and bool((qo[[4, 6, 8]] != 9.0).any(-1).all())
+
+
 @pytest.mark.parametrize("shift", [0, 1, 3])
 @pytest.mark.parametrize("interleaved", [0, 1])
 def test_rope_in_place_at_any_element(shift, interleaved):
