@@ -129,6 +129,7 @@ struct DenseArgs {
 constexpr uint32_t kABytes = 128 * 128;
 constexpr int kMaxInt8Stages = 16;
 
+
 template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     if constexpr (PAIR)
@@ -141,8 +142,9 @@ __device__ __forceinline__ uint32_t i8_idesc(int m, int n) { return (2u << 4) | 
 
 __device__ __forceinline__ float int8_result(int act, int acc, float s, float b) {
     float v = fmaf((float)acc, s, b);
-    if (act >= 1) v = v < 0.f ? 0.f : v;               // (a NaN stays one)
-    if (act == 2) v = v > 6.f ? 6.f : v;
+    // (no branches; a NaN stays one)
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(act >= 1 ? 0.f : -INFINITY));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(act == 2 ? 6.f : INFINITY));
     return v;
 }
 
@@ -151,18 +153,22 @@ __device__ __forceinline__ void wait_for_copies() {    // an aborted block's cop
     for (int i = 0; i < 100000 && globaltimer_ns() - t0 < 50000; ++i) __nanosleep(500);
 }
 
-template <typename Y>
+template <typename Y, int HALVES>
 __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                                                        uint32_t job_id, FinishedBlockNotifier* nf) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kMaxInt8Stages], s_empty[kMaxInt8Stages], s_sums;
+    __shared__ uint64_t s_full[kMaxInt8Stages], s_empty[kMaxInt8Stages], s_sums, s_parts;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 128u;
+    __shared__ float s_xs[128];
+    __shared__ volatile uint32_t s_never;              // an abort flag that another wait of this block does not raise
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, half_bytes = kABytes + (uint32_t)a.BN * 128u, stage_bytes = half_bytes * HALVES;
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
     const int n0 = tile % a.channel_tiles * 128, t0 = tile / a.channel_tiles * a.BN;
     const int kb0 = a.kblocks * rank / a.splits, nkb = a.kblocks * (rank + 1) / a.splits - kb0;
+    const int tokens = min(a.BN, a.T - t0), owned = (tokens - rank + a.splits - 1) / a.splits;      // of a split reduction: tokens rank, rank + splits ...
+    const uint32_t parts = ring + a.stages * stage_bytes;                                           // [rank][owned token][channel]: what the cluster's blocks send
     uint32_t cols = 32;
     while ((int)cols < a.BN) cols *= 2;
     if (warp == 5) {
@@ -171,94 +177,134 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ D
     }
     if (threadIdx.x == 0) {
         s_abort = 0;
+        s_never = 0;
         for (int i = 0; i < a.stages; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_empty[i]), 1);
         }
         mbar_init(smem_u32(&s_sums), 1);
+        mbar_init(smem_u32(&s_parts), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (a.splits > 1) mbar_arrive_expect_tx(smem_u32(&s_parts), (uint32_t)(a.splits * owned) * 512u);
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
+    if (a.splits > 1) cluster_arrive();
     const uint32_t tmem = uniform(s_tmem);
     if (warp == 4 && elect_one()) {
         // the weights come into the L2 cache while the launch that makes the activations still runs
-        for (int i = 0; i < nkb && i < a.stages; ++i)
-            asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&wmap), "r"((kb0 + i) * 128), "r"(n0) : "memory");
+        for (int i = 0; i < nkb * HALVES && i < 8; ++i)
+            asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&wmap), "r"((kb0 * HALVES + i) * 128), "r"(n0) : "memory");
     }
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
     bool ok = true;
     if (warp == 4) {
-        for (int i = 0; i < nkb; ++i) {
-            const int st = i % a.stages, use = i / a.stages;
-            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), (use - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) break;
-            if (elect_one()) {
+        if (elect_one()) {
+            uint32_t st = 0, parity = 1;
+            for (int i = 0, x = kb0 * HALVES * 128; i < nkb; ++i) {
+                if (i >= a.stages && !mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_int8_flag, kFlagLmWait)) break;
                 const uint32_t bar = smem_u32(&s_full[st]), at = ring + st * stage_bytes;
                 mbar_arrive_expect_tx(bar, stage_bytes);
-                tma_load_2d(at, &wmap, (kb0 + i) * 128, n0, bar);
-                tma_load_2d(at + kABytes, &xmap, (kb0 + i) * 128, t0, bar);
-            }
-            __syncwarp();
-        }
-    } else if (warp == 5) {
-        const uint32_t idesc = i8_idesc(128, a.BN);
-        for (int i = 0; i < nkb; ++i) {
-            const int st = i % a.stages;
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), (i / a.stages) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
-            if (!ok) break;
-            tcgen05_fence_after();
-            const uint64_t da = umma_desc_sw128(ring + st * stage_bytes), db = umma_desc_sw128(ring + st * stage_bytes + kABytes);
-            if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_i8<false>(tmem, da + 2 * k, db + 2 * k, idesc, i > 0 || k > 0);
-                tcgen05_commit(smem_u32(&s_empty[st]));
+                for (uint32_t h = 0; h < HALVES; ++h, x += 128) {
+                    tma_load_2d(at + h * half_bytes, &wmap, x, n0, bar);
+                    tma_load_2d(at + h * half_bytes + kABytes, &xmap, x, t0, bar);
+                }
+                if (++st == (uint32_t)a.stages) { st = 0; parity ^= 1; }
             }
-            __syncwarp();
         }
-        if (ok && elect_one()) tcgen05_commit(smem_u32(&s_sums));
+        __syncwarp();
+    } else if (warp == 5) {
+        if (elect_one()) {
+            const uint32_t idesc = i8_idesc(128, a.BN), step = stage_bytes >> 4;
+            const uint64_t desc = umma_desc_sw128(ring);
+            const uint32_t high = (uint32_t)(desc >> 32);
+            uint32_t st = 0, parity = 0, low = (uint32_t)desc;
+            for (int i = 0; i < nkb; ++i) {
+                ok = mbar_wait(smem_u32(&s_full[st]), parity, &s_abort, &g_int8_flag, kFlagLmWait);
+                if (!ok) break;
+                tcgen05_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < 4 * HALVES; ++k) {
+                    const uint32_t at = low + (k >> 2) * (half_bytes >> 4) + 2 * (k & 3);
+                    mma_i8<false>(tmem, pack_f32x2(at, high), pack_f32x2(at + (kABytes >> 4), high), idesc, (uint32_t)(i > 0) | (uint32_t)(k > 0));
+                }
+                tcgen05_commit(smem_u32(&s_empty[st]));
+                low += step;
+                if (++st == (uint32_t)a.stages) { st = 0; parity ^= 1; low = (uint32_t)desc; }
+            }
+            if (ok) tcgen05_commit(smem_u32(&s_sums));
+        }
         __syncwarp();
     }
-    const int n = n0 + 32 * (warp & 3) + lane, tokens = min(a.BN, a.T - t0);
+    const int n = n0 + 32 * (warp & 3) + lane;
     const bool mine = warp < 4 && n < a.N;
     const float ws = mine ? __ldg(a.w_scale + n) : 0.f, bias = mine && a.bias ? __ldg(a.bias + n) : 0.f;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     if (warp < 4) {
+        if ((int)threadIdx.x < tokens) s_xs[threadIdx.x] = __ldcg(a.x_scale + t0 + threadIdx.x);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_sums), 0, &s_abort, &g_int8_flag, kFlagLmWait));
         tcgen05_fence_after();
         if (ok) {
-            for (int j0 = 0; j0 < tokens; j0 += 16) {
-                uint32_t v[16];
-                tcgen05_ld16(lanes + j0, v);
-                tcgen05_wait_ld();
+            // (short loops: code that a block runs once comes from the L2 cache, line by line)
+            if (a.splits == 1) {
+                Y* dst = static_cast<Y*>(a.y) + (int64_t)t0 * a.y_stride + n;
+#pragma unroll 1
+                for (int j0 = 0; j0 < tokens; j0 += 8) {
+                    uint32_t v[8];
+                    tcgen05_ld8(lanes + j0, v);
+                    tcgen05_wait_ld();
+                    Y r[8];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (a.splits > 1) {                // [token][channel] of this block's sums, over the operands that made them
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + (uint32_t)((j0 + j) * 128 + 32 * warp + lane) * 4u), "r"(v[j]) : "memory");
-                    } else if (mine && j0 + j < tokens) {
-                        static_cast<Y*>(a.y)[(int64_t)(t0 + j0 + j) * a.y_stride + n] = lm_from_f<Y>(int8_result(a.act, (int)v[j], __ldcg(a.x_scale + t0 + j0 + j) * ws, bias));
+                    for (int j = 0; j < 8; ++j) r[j] = lm_from_f<Y>(int8_result(a.act, (int)v[j], s_xs[(j0 + j) & 127] * ws, bias));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j, dst += a.y_stride)
+                        if (mine && j0 + j < tokens) *dst = r[j];
+                }
+            } else {
+                cluster_wait();                        // the others' barriers are set up
+                const int shift = __ffs(a.splits) - 1; // (blocks of a cluster: a power of two)
+#pragma unroll 1
+                for (int j0 = 0; j0 < tokens; j0 += 8) {
+                    uint32_t v[8];
+                    tcgen05_ld8(lanes + j0, v);
+                    tcgen05_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j0 + j < tokens) {
+                            const uint32_t to = (uint32_t)(j0 + j) & (a.splits - 1), at = (uint32_t)(j0 + j) >> shift, theirs = (tokens - to + a.splits - 1) >> shift;
+                            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                                         ::"r"(cluster_addr(parts + ((rank * theirs + at) * 128 + 32 * warp + lane) * 4u, to)), "r"(v[j]), "r"(cluster_addr(smem_u32(&s_parts), to)) : "memory");
+                        }
+                }
+            }
+        } else if (a.splits > 1) {
+            cluster_wait();
+        }
+        if (a.splits > 1) {
+            // (also a block that has given up waits for what the others send into its memory)
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_parts), 0, &s_never, &g_int8_flag, kFlagLmWait)) && ok;
+            if (ok && mine) {
+                Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + rank) * a.y_stride + n;
+                uint32_t from = parts + (32 * warp + lane) * 4u;
+#pragma unroll 1
+                for (int i = 0; i < owned; ++i, dst += a.splits * a.y_stride, from += 512) {
+                    int sum = 0;
+#pragma unroll 4
+                    for (int r = 0; r < a.splits; ++r) {
+                        int v;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from + r * owned * 512) : "memory");
+                        sum += v;
                     }
+                    *dst = lm_from_f<Y>(int8_result(a.act, sum, s_xs[rank + i * a.splits] * ws, bias));
                 }
             }
         }
-    }
-    if (a.splits > 1) {
-        cluster_arrive();
-        cluster_wait();
-        if (warp < 4 && ok && mine) {
-            for (int j = rank; j < tokens; j += a.splits) {
-                int sum = 0;
-                for (int r = 0; r < a.splits; ++r) {
-                    int v;
-                    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(ring + (uint32_t)(j * 128 + 32 * warp + lane) * 4u, (uint32_t)r)) : "memory");
-                    sum += v;
-                }
-                static_cast<Y*>(a.y)[(int64_t)(t0 + j) * a.y_stride + n] = lm_from_f<Y>(int8_result(a.act, sum, __ldcg(a.x_scale + t0 + j) * ws, bias));
-            }
-        }
-        cluster_arrive();                              // nobody's sums go before everybody has read them
+    } else if (a.splits > 1) {
         cluster_wait();
     }
     tcgen05_fence_before();
@@ -285,7 +331,7 @@ __device__ __forceinline__ bool all_of_128(bool ok) {
     return all != 0;
 }
 
-constexpr uint32_t kOutBytes = 32 * 128 * 4;           // 32 tokens of 128 channels on their way out
+constexpr uint32_t kOutBytes = 16 * 128 * 4;           // 32 tokens of 128 channels in 16 bits on their way out
 
 // A pair of blocks walks its share of the tiles.  Warps 0-3: results, a lane a channel; warp 4: copies of this block's operands; warp 5 of the first
 // block: the products of both.  Two accumulators: the results of a tile leave under the products of the next.
@@ -328,13 +374,18 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
 
     // Neighbouring pairs take the tokens of the same channels, then the next channels: all of them together read few rows of both operands.
     if (warp == 4) {
-        int it = 0;
+        uint32_t st = 0, parity = 1;
+        int filled = 0;
         bool ok = true;
         for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
             const int n0 = tile / a.token_tiles * 256 + 128 * rank, t0 = tile % a.token_tiles * a.BN + (a.BN / 2) * rank;
-            for (int i = 0; i < a.kblocks; ++i, ++it) {
-                const int st = it % a.stages, use = it / a.stages;
-                if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), (use - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) { ok = false; break; }
+            for (int i = 0; i < a.kblocks; ++i) {
+                if (filled == a.stages) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_int8_flag, kFlagLmWait));
+                    if (!ok) break;
+                } else {
+                    ++filled;
+                }
                 if (elect_one()) {
                     const uint32_t bar = smem_u32(&s_full[st]), first = cluster_addr(bar, 0u), at = ring + st * stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(bar, 2 * stage_bytes);      // both blocks' copies
@@ -342,30 +393,34 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
                     tma_load_2d_pair(at + kABytes, &xmap, i * 128, t0, first);
                 }
                 __syncwarp();
+                if (++st == (uint32_t)a.stages) { st = 0; parity ^= 1; }
             }
         }
     } else if (warp == 5) {
         if (rank == 0) {
-            const uint32_t idesc = i8_idesc(256, a.BN);
-            int it = 0, turn = 0;
+            const uint32_t idesc = uniform(i8_idesc(256, a.BN)), step = uniform(stage_bytes >> 4), stages = uniform((uint32_t)a.stages);
+            const uint64_t desc = umma_desc_sw128(uniform(ring));
+            const uint32_t high = (uint32_t)(desc >> 32);
+            uint32_t st = 0, parity = 0, low = (uint32_t)desc;
+            int turn = 0;
             bool ok = true;
             for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs, ++turn) {
-                const int acc = turn & 1;
-                if (turn >= 2) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_read[acc]), (turn / 2 - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
+                const uint32_t acc = turn & 1, sums = tmem + 256 * acc;
+                if (turn >= 2) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_read[acc]), (uint32_t)(turn / 2 - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
                 if (!ok) break;
                 tcgen05_fence_after();
-                for (int i = 0; i < a.kblocks; ++i, ++it) {
-                    const int st = it % a.stages;
-                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), (it / a.stages) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
+                for (int i = 0; i < a.kblocks; ++i) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[st]), parity, &s_abort, &g_int8_flag, kFlagLmWait));
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const uint64_t da = umma_desc_sw128(ring + st * stage_bytes), db = umma_desc_sw128(ring + st * stage_bytes + kABytes);
                     if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) mma_i8<true>(tmem + 256 * acc, da + 2 * k, db + 2 * k, idesc, i > 0 || k > 0);
+                        for (uint32_t k = 0; k < 4; ++k) mma_i8<true>(sums, pack_f32x2(low + 2 * k, high), pack_f32x2(low + (kABytes >> 4) + 2 * k, high), idesc, (uint32_t)(i > 0) | (uint32_t)(k > 0));
                         tcgen05_commit_pair(smem_u32(&s_empty[st]));
                     }
                     __syncwarp();
+                    low += step;
+                    if (++st == stages) { st = 0; parity ^= 1; low = (uint32_t)desc; }
                 }
                 if (ok && elect_one()) tcgen05_commit_pair(smem_u32(&s_sums[acc]));
                 __syncwarp();
@@ -387,58 +442,44 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
                 uint32_t v[32];
                 tcgen05_ld32(tmem + ((uint32_t)warp << 21) + 256 * acc + j0, v);
                 tcgen05_wait_ld();
-                if (j0 + 32 >= tokens) {                                            // the accumulator's last columns: it may be written again
-                    tcgen05_fence_before();
-                    __syncwarp();
-                }
-                const uint32_t me = out + (uint32_t)(32 * warp + lane) * 4u;
-                if constexpr (sizeof(Y) == 4) {        // [token][channel]
+                if (j0 + 32 >= tokens) tcgen05_fence_before();                      // the accumulator's last columns: it may be written again
+                const int left = min(32, tokens - j0);
+                if (sizeof(Y) == 4 || !a.y_vec || n0 + 128 > a.N) {
+                    // a warp's 32 channels of a token are 128 (64) bytes of a row, wherever it starts
+                    Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + j0) * a.y_stride + n;
+                    Y r[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(me + j * 512), "f"(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias)) : "memory");
-                } else {                               // two tokens a word: [token / 2][channel]
+                    for (int j = 0; j < 32; ++j) r[j] = lm_from_f<Y>(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias));
+                    if (left == 32 && n < a.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j, dst += a.y_stride) *dst = r[j];
+                    } else if (n < a.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j, dst += a.y_stride)
+                            if (j < left) *dst = r[j];
+                    }
+                    continue;
+                }
+                if constexpr (sizeof(Y) == 2) {        // two tokens a word in shared memory, [token / 2][channel], and out 16 bytes a thread
+                    const uint32_t me = out + (uint32_t)(32 * warp + lane) * 4u;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2)
                         asm volatile("st.shared.b32 [%0], %1;" ::"r"(me + j * 256),
                                      "r"(lm_pack2<Y>(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias), int8_result(a.act, (int)v[j + 1], s_xs[j0 + j + 1] * ws, bias))) : "memory");
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                // out: 16 bytes of a row for each thread where y's rows allow it, and the lanes side by side in any case
-                const int left = min(32, tokens - j0), width = min(128, a.N - n0);
-                Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + j0) * a.y_stride + n0;
-                if constexpr (sizeof(Y) == 4) {
-                    if (a.y_vec && width == 128) {
-                        for (int i = threadIdx.x; i < left * 32; i += 128) *reinterpret_cast<uint4*>(dst + (i >> 5) * a.y_stride + (i & 31) * 4) = ld_shared_v4(out + i * 16);
-                    } else {
-                        for (int j = 0; j < left; ++j)
-                            if ((int)threadIdx.x < width) {
-                                float f;
-                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(out + j * 512 + threadIdx.x * 4) : "memory");
-                                dst[j * a.y_stride + threadIdx.x] = f;
-                            }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + j0) * a.y_stride + n0;
+                    for (int i = threadIdx.x; i < 16 * 16; i += 128) {             // tokens 2 (i / 16) and + 1, channels 8 (i % 16) and up
+                        const uint4 p = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32), q = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32 + 16);
+                        Y* at = dst + (i >> 4) * 2 * a.y_stride + (i & 15) * 8;
+                        if ((i >> 4) * 2 < left)
+                            *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(p.x, p.y, 0x5410), __byte_perm(p.z, p.w, 0x5410), __byte_perm(q.x, q.y, 0x5410), __byte_perm(q.z, q.w, 0x5410));
+                        if ((i >> 4) * 2 + 1 < left)
+                            *reinterpret_cast<uint4*>(at + a.y_stride) = make_uint4(__byte_perm(p.x, p.y, 0x7632), __byte_perm(p.z, p.w, 0x7632), __byte_perm(q.x, q.y, 0x7632), __byte_perm(q.z, q.w, 0x7632));
                     }
-                } else {
-                    if (a.y_vec && width == 128) {
-                        for (int i = threadIdx.x; i < 16 * 16; i += 128) {         // tokens 2 (i / 16) and + 1, channels 8 (i % 16) and up
-                            const uint4 p = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32), q = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32 + 16);
-                            Y* at = dst + (i >> 4) * 2 * a.y_stride + (i & 15) * 8;
-                            if ((i >> 4) * 2 < left)
-                                *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(p.x, p.y, 0x5410), __byte_perm(p.z, p.w, 0x5410), __byte_perm(q.x, q.y, 0x5410), __byte_perm(q.z, q.w, 0x5410));
-                            if ((i >> 4) * 2 + 1 < left)
-                                *reinterpret_cast<uint4*>(at + a.y_stride) = make_uint4(__byte_perm(p.x, p.y, 0x7632), __byte_perm(p.z, p.w, 0x7632), __byte_perm(q.x, q.y, 0x7632), __byte_perm(q.z, q.w, 0x7632));
-                        }
-                    } else {
-                        for (int j = 0; j < left; ++j)
-                            if ((int)threadIdx.x < width) {
-                                uint32_t f;
-                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(f) : "r"(out + (j >> 1) * 512 + threadIdx.x * 4) : "memory");
-                                const uint16_t h = (uint16_t)(j & 1 ? f >> 16 : f);
-                                dst[j * a.y_stride + threadIdx.x] = *reinterpret_cast<const Y*>(&h);
-                            }
-                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
             }
+            asm volatile("bar.sync 1, 128;" ::: "memory");                         // all four warps have read the accumulator
             if (threadIdx.x == 0)
                 asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_u32(&s_read[acc]), 0u)) : "memory");
         }
@@ -463,6 +504,7 @@ __global__ void int8_nothing_kernel(uint32_t job_id, FinishedBlockNotifier* nf) 
 }
 
 typedef void (*DenseFn)(DenseArgs, CUtensorMap, CUtensorMap, uint32_t, FinishedBlockNotifier*);
+template <typename Y> DenseFn few_fn(int halves) { return halves == 2 ? int8_few_kernel<Y, 2> : int8_few_kernel<Y, 1>; }
 struct DensePlan {
     DenseArgs a;
     bool many;
@@ -526,13 +568,17 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
     a.kblocks = ceil_div(a.K, 128);
     const int T = a.T > 0 ? a.T : 1;
     double best = 1e300;
-    // one block a tile, up to 8 blocks on its reduction
+    int halves = 1;            // of 128 bytes of a row in a stage of int8_few_kernel
+    // One block a tile, up to 8 blocks on its reduction.  Beside what an SM does: the weights from memory, at 3050 bytes a clock where every SM asks for them
+    // and 2700 otherwise, and 2600 clocks for parts that meet.  (24 tokens, 16384 -> 14336: 112 blocks 52 us, 224 that share 42; 4096 -> 14336: 13.7
+    // against 17.7; one token, 4096 -> 4096: 128 blocks that share 6.2 us, 64 6.7.)
     for (int tt = ceil_div(T, 128); tt <= ceil_div(T, 128) + 1; ++tt) {
-        const int BN = round_up(ceil_div(T, tt), 16), tiles = ceil_div(T, BN);
-        for (int S = 1; S <= 8 && S <= a.kblocks; S *= 2) {
+        const int BN = round_up(ceil_div(T, tt), 16), tiles = ceil_div(T, BN), pieces = BN <= 32 ? 2 : 1, few = ceil_div(a.K, 128 * pieces);
+        for (int S = 1; S <= 8 && S <= few; S *= 2) {
             const double blocks = (double)ceil_div(a.N, 128) * tiles * S;
-            const double clocks = std::ceil(blocks / 148) * ceil_div(a.kblocks, S) * kblock_clocks(BN, BN) + (S > 1 ? 1500 + 8.0 * BN : 0) + 10.0 * BN;
-            if (clocks < best) { best = clocks; pl.many = false; a.BN = BN; a.token_tiles = tiles; a.splits = S; }
+            const double work = std::ceil(blocks / 148) * ceil_div(few, S) * pieces * kblock_clocks(BN, BN), memory = (double)a.N * a.K / (blocks >= 148 ? 3050 : 2700);
+            const double clocks = std::max(work, memory) + (S > 1 ? 2600 + 8.0 * BN : 0) + 10.0 * BN;
+            if (clocks < best) { best = clocks; pl.many = false; a.BN = BN; a.token_tiles = tiles; a.splits = S; halves = pieces; }
         }
     }
     // pairs of SMs on 256 channels
@@ -543,7 +589,9 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
             if (clocks < best) { best = clocks; pl.many = true; a.BN = BN; a.token_tiles = tiles; a.splits = 1; }
         }
     a.channel_tiles = ceil_div(a.N, pl.many ? 256 : 128);
-    const uint32_t stage = kABytes + (uint32_t)a.BN * (pl.many ? 64 : 128);
+    // Narrow tiles take 256 bytes of a row a stage: what a stage costs beside its copies and products, 230 clocks, comes half as often.
+    if (!pl.many) a.kblocks = ceil_div(a.K, 128 * halves);
+    const uint32_t stage = pl.many ? kABytes + (uint32_t)a.BN * 64 : (kABytes + (uint32_t)a.BN * 128) * halves;
     if (pl.many) {
         a.stages = (int)std::min<uint32_t>(kMaxInt8Stages, (227 * 1024 - 4096 - kOutBytes) / stage);
         pl.smem = 1024 + a.stages * stage + kOutBytes;
@@ -554,15 +602,21 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
         a.splits = 2;          // blocks of a cluster
         pl.fn = p->y_dtype == PB_F32 ? int8_many_kernel<float> : p->y_dtype == PB_BF16 ? int8_many_kernel<__nv_bfloat16> : int8_many_kernel<__half>;
     } else {
-        // two blocks an SM: what they have in flight covers the memory's latency
-        a.stages = (int)std::min<uint32_t>(std::min<uint32_t>(kMaxInt8Stages, ceil_div(a.kblocks, a.splits)), (110 * 1024) / stage);
-        pl.smem = 1024 + std::max<uint32_t>(a.stages * stage, a.splits > 1 ? a.BN * 512 : 0);
+        // What an SM has in flight covers the memory's latency: up to 200 KB of one block, or 100 KB each of two.  Blocks that have an SM each also keep it to
+        // themselves: two of the next launch, set up beside this one's on an idle SM, would share its path to memory while others have one block.
+        const uint32_t sent = a.splits > 1 ? (uint32_t)a.splits * ceil_div(a.BN, a.splits) * 512 : 0;
+        const bool lone = (int64_t)a.channel_tiles * a.token_tiles * a.splits <= 148;
+        uint32_t room = (lone ? 216 * 1024 : 111 * 1024) - sent;
+        if (room < 2 * stage) room = 216 * 1024 - sent;
+        a.stages = (int)std::min<uint32_t>(std::min<uint32_t>(kMaxInt8Stages, ceil_div(a.kblocks, a.splits)), room / stage);
+        pl.smem = 1024 + a.stages * stage + sent;
+        if (lone && pl.smem < 116 * 1024) pl.smem = 116 * 1024;
         const int64_t blocks = (int64_t)a.channel_tiles * a.token_tiles * a.splits;
         PB_REQUIRE(blocks <= 0x7fffffff, "pb_int8_dense: too many results for one launch");
         pl.blocks = (unsigned)blocks;
         pl.tmem_cols = 32;
         while ((int)pl.tmem_cols < a.BN) pl.tmem_cols *= 2;
-        pl.fn = p->y_dtype == PB_F32 ? int8_few_kernel<float> : p->y_dtype == PB_BF16 ? int8_few_kernel<__nv_bfloat16> : int8_few_kernel<__half>;
+        pl.fn = p->y_dtype == PB_F32 ? few_fn<float>(halves) : p->y_dtype == PB_BF16 ? few_fn<__nv_bfloat16>(halves) : few_fn<__half>(halves);
     }
     const int V = (int)(16 / dtype_bytes(p->y_dtype));
     a.y_vec = aligned(p->y, 16) && p->y_stride % V == 0;
