@@ -506,15 +506,25 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
 }
 
 // A block (or a cluster of `ranks` blocks, each a range of the tokens) takes 8 NT query rows of one sequence and key head.  A warp takes 16 tokens at a
-// time, straight from global memory into the registers that the products read: the order of a head's values within a product's 16 is free as
-// long as both operands have the same, and so is the order of O's rows, hence each lane's 16 bytes are as they lie.
+// time, copied into a ring of its own two to four chunks ahead: 12 warps of an SM have 96 to 192 KB on the way.  (In registers, a chunk ahead, it was 60: 1024
+// sequences' worth of 16 tokens a head came at 3.9 TB/s.)  The order of a head's values within a product's 16 is free as long as both operands have the
+// same, and so is the order of O's rows, hence each lane reads 16 bytes as they lie:
 //   S^T[token][row] = K Q^T:  lane (g, c) = (lane / 4, lane % 4) holds 8 values at 8 c of every 32 of tokens g and g + 8
 //   O^T[value][row] = V^T P^T: 8 values at 8 g of every 64 of tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-// P^T comes out of S^T with a transposition of 8 x 8 in the warp.
+// Piece i of a row lies at i ^ 4 (row % 2) for keys, at i ^ (row & 6) for values: no bank conflicts.  P^T comes out of S^T with a transposition of 8 x 8 in
+// the warp.
+template <int DP> struct OwnShape {
+    static constexpr uint32_t half = 16 * DP * 2;                    // bytes of 16 tokens' keys or values
+    static constexpr int stages = DP == 128 ? 2 : 4;
+    static constexpr uint32_t smem = 4 * stages * 2 * half;
+};
 template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
-    constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64;
-    __shared__ __align__(16) float s_o[4][R][DP];
+    constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64, kStages = OwnShape<DP>::stages;
+    constexpr uint32_t kHalf = OwnShape<DP>::half;
+    static_assert(4 * R * DP * 4 <= OwnShape<DP>::smem, "the warps' parts fit where their rings were");
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    float (*s_o)[R][DP] = reinterpret_cast<float (*)[R][DP]>(smem_raw);
     __shared__ __align__(8) float2 s_ml[4][R];
     __shared__ float s_w[R][kMaxParts];
     if (!a.early) griddep_wait();
@@ -570,54 +580,49 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             lo = __shfl_sync(0xffffffffu, at_lo, turn & 31);
             hi = __shfl_sync(0xffffffffu, at_hi, turn & 31);
         };
-        uint4 k[KB][2], v[VB][4];
-        const auto load_k = [&](int chunk, int64_t lo, int64_t hi) {
-            const int token = 16 * chunk + g;
+        const uint32_t ring = smem_u32(smem_raw) + warp * (kStages * 2 * kHalf);
+        // 16 tokens' keys and values into a stage, neighbouring lanes on neighbouring 16 bytes of a row; what is not there comes as zeros
+        constexpr int kPer = DP / 8, kRows = 32 / kPer;                          // pieces of a row, rows of a turn
+        const int piece = lane % kPer, row0 = lane / kPer;
+        const auto load = [&](int turn) {
+            const int chunk = first + 4 * turn;
+            if (chunk < last) {
+                int64_t lo, hi;
+                where(turn, lo, hi);
+                const uint32_t to = ring + (turn % kStages) * (2 * kHalf);
+                const bool col = 8 * piece < a.D;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t base = h ? hi : lo;
-                const bool there = base >= 0 && token + 8 * h < own;
-                const T* src = static_cast<const T*>(a.k) + base + g * a.token_stride + 8 * c;
-#pragma unroll
-                for (int i = 0; i < KB; ++i) {
-                    k[i][h] = make_uint4(0, 0, 0, 0);
-                    if (there && 32 * i + 8 * c < a.D) k[i][h] = __ldcg(reinterpret_cast<const uint4*>(src + 32 * i));
+                for (int i = 0; i < 16 / kRows; ++i) {
+                    const int row = i * kRows + row0;
+                    const int64_t base = row < 8 ? lo : hi;
+                    const bool there = col && base >= 0 && 16 * chunk + row < own;
+                    const int64_t at = there ? base + (row & 7) * a.token_stride + 8 * piece : 0;
+                    const uint32_t bytes = there ? 16 : 0, dst = to + row * (DP * 2);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + ((piece ^ ((row & 1) << 2)) << 4)), "l"(static_cast<const T*>(a.k) + at), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + kHalf + ((piece ^ (row & 6)) << 4)), "l"(static_cast<const T*>(a.v) + at), "r"(bytes) : "memory");
                 }
             }
-        };
-        const auto load_v = [&](int chunk, int64_t lo, int64_t hi) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int within = 2 * c + (e & 1);
-                const int64_t base = e >> 1 ? hi : lo;
-                const bool there = base >= 0 && 16 * chunk + 8 * (e >> 1) + within < own;
-                const T* src = static_cast<const T*>(a.v) + base + within * a.token_stride + 8 * g;
-#pragma unroll
-                for (int i = 0; i < VB; ++i) {
-                    v[i][e] = make_uint4(0, 0, 0, 0);
-                    if (there && 64 * i + 8 * g < a.D) v[i][e] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * i));
-                }
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         const float scale = a.scale * kLog2e;
-        int64_t lo, hi;
-        where(0, lo, hi);
-        load_k(first, lo, hi);
-        load_v(first, lo, hi);
-        for (int chunk = first, turn = 1; chunk < last; chunk += 4, ++turn) {
-            const int next = chunk + 4;
-            if (next < last) where(turn, lo, hi);
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) load(i);
+#pragma unroll 1
+        for (int chunk = first, turn = 0; chunk < last; chunk += 4, ++turn) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            __syncwarp();
+            const uint32_t keys = ring + (turn % kStages) * (2 * kHalf), values = keys + kHalf;
             float s[NT][4] = {};
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
-                const uint32_t a0[4] = {k[i][0].x, k[i][1].x, k[i][0].y, k[i][1].y}, a1[4] = {k[i][0].z, k[i][1].z, k[i][0].w, k[i][1].w};
+                const uint4 k0 = ld_shared_v4(keys + g * (DP * 2) + (((4 * i + c) ^ ((g & 1) << 2)) << 4)), k1 = ld_shared_v4(keys + (g + 8) * (DP * 2) + (((4 * i + c) ^ ((g & 1) << 2)) << 4));
+                const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     mma_16x8x16<T>(s[t], a0, q[t][i].x, q[t][i].y);
                     mma_16x8x16<T>(s[t], a1, q[t][i].z, q[t][i].w);
                 }
             }
-            if (next < last) load_k(next, lo, hi);
             const bool in0 = 16 * chunk + g < own, in1 = 16 * chunk + g + 8 < own;
             float up[NT][2];
             bool grown = false;
@@ -660,7 +665,10 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             }
 #pragma unroll
             for (int i = 0; i < VB; ++i) {
-                const uint32_t* w0 = &v[i][0].x; const uint32_t* w1 = &v[i][1].x; const uint32_t* w2 = &v[i][2].x; const uint32_t* w3 = &v[i][3].x;
+                uint4 v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ld_shared_v4(values + (2 * c + (e & 1) + 8 * (e >> 1)) * (DP * 2) + (((8 * i + g) ^ (2 * c)) << 4));
+                const uint32_t* w0 = &v[0].x; const uint32_t* w1 = &v[1].x; const uint32_t* w2 = &v[2].x; const uint32_t* w3 = &v[3].x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t av[4] = {__byte_perm(w0[e], w1[e], 0x5410), __byte_perm(w0[e], w1[e], 0x7632), __byte_perm(w2[e], w3[e], 0x5410), __byte_perm(w2[e], w3[e], 0x7632)};
@@ -668,9 +676,12 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                     for (int t = 0; t < NT; ++t) mma_16x8x16<T>(o[i][e][t], av, p0[t], p1[t]);
                 }
             }
-            if (next < last) load_v(next, lo, hi);
+            __syncwarp();
+            load(turn + kStages);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
+    __syncthreads();                                                      // the rings become the warps' parts
     // this warp's part: (m, l) and O of its rows, values 64 i + 8 g + 2 e and + 1
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -785,6 +796,7 @@ struct AttnPlan {
     int64_t prefix_blocks, own_blocks;
     uint64_t scratch;
     OwnFn own;
+    uint32_t own_smem;
 };
 
 int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
@@ -817,6 +829,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     pl.DP = p->head_dim <= 64 ? 64 : 128;
     pl.NT = a.group <= 8 ? 1 : 2;
     pl.half = p->dtype == PB_F16;
+    pl.own_smem = pl.DP == 64 ? OwnShape<64>::smem : OwnShape<128>::smem;
     pl.own = pl.half ? own_fn<__half>(pl.DP, pl.NT) : own_fn<__nv_bfloat16>(pl.DP, pl.NT);
     // the prefix: as many parts as give every SM a block
     const int64_t rows = (int64_t)a.batch * a.group;
@@ -878,7 +891,7 @@ int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out) {
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, pl.own) == cudaSuccess) {
         out->regs_per_thread = (uint32_t)fa.numRegs;
-        out->smem_per_block = (uint32_t)fa.sharedSizeBytes;
+        out->smem_per_block = (uint32_t)fa.sharedSizeBytes + pl.own_smem;
     } else {
         cudaGetLastError();
     }
@@ -911,7 +924,8 @@ int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t
         }
         if (e != PB_OK) return e;
     }
-    return lm_launch("pb_prefix_attn", pl.own, dim3((unsigned)pl.own_blocks), dim3(128), 0, st, pl.a.ranks, pl.a, job_id, (FinishedBlockNotifier*)notifier);
+    PB_CUDA(cudaFuncSetAttribute(pl.own, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.own_smem));
+    return lm_launch("pb_prefix_attn", pl.own, dim3((unsigned)pl.own_blocks), dim3(128), pl.own_smem, st, pl.a.ranks, pl.a, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 }  // extern "C"
