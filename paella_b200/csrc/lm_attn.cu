@@ -10,6 +10,7 @@
 #include <cuda.h>
 
 #include <cmath>
+#include <cstdlib>
 
 #include "lm.cuh"
 #include "umma.cuh"
@@ -31,7 +32,8 @@ struct AttnArgs {
     float* part_o;             // [row_tiles][kv_heads][splits][128][DP], a row's 16-byte piece i at i ^ (row % 32)
     float2* part_ml;           // the same without DP: (m, l)
     // own tokens
-    int kv_heads, row_groups, ranks, early, out_vec;
+    int kv_heads, row_groups, ranks, early, out_vec;     // early: behind a prefix_kernel, beside whose end it starts
+    int ahead;                 // tokens of the prefix that own_kernel takes as if they were each sequence's own: all of them, or none
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -313,17 +315,23 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
             constexpr int kPerRow = DP / 8, kMine = kPerRow;
             const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
             const int row0 = row - in_tile, thread = threadIdx.x & 127;
+            constexpr int kStep = 128 / kPerRow;                                 // rows from one of a thread's pieces to the next
             uint4 v[kMine];
+            int r = row0 + thread / kPerRow, b = r / a.group, h = r - b * a.group;   // (quotients in the loop took 2 us)
+            const int b_step = kStep / a.group, h_step = kStep - b_step * a.group, c = thread % kPerRow;
+            const T* src = static_cast<const T*>(a.q) + (int64_t)kvh * a.group * a.q_head + 8 * c;
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
-                const int r = row0 + (i * 128 + thread) / kPerRow, c = thread % kPerRow;
                 v[i] = make_uint4(0, 0, 0, 0);
-                if (r < rows && 8 * c < a.D)
-                    v[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(r / a.group) * a.q_stride + (int64_t)(kvh * a.group + r % a.group) * a.q_head + 8 * c));
+                if (r < rows && 8 * c < a.D) v[i] = __ldcg(reinterpret_cast<const uint4*>(src + b * a.q_stride + h * a.q_head));
+                r += kStep;
+                b += b_step;
+                h += h_step;
+                if (h >= a.group) { h -= a.group; ++b; }
             }
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
-                const int r = (i * 128 + thread) / kPerRow, c = thread % kPerRow;
+                const int r = (i * 128 + thread) / kPerRow;
                 st_shared_v4(q_smem + g * kTile + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
             }
         }
@@ -536,6 +544,19 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     unit /= a.row_groups;
     const int kvh = unit % a.kv_heads, b = unit / a.kv_heads;
     const int row0 = zg * R, rows = b < a.batch ? min(R, a.group - row0) : 0;
+    // Chunks of 16 tokens: those of the prefix that are taken here, then the sequence's own.  A lane looks a chunk's two halves of 8 tokens up (a page holds a
+    // multiple of 8), for 32 chunks at a time; the first of them before the sequence's length is known, whatever it is: entries up to max_own may be read.
+    const int chunks_ahead = (a.ahead + 15) / 16;
+    const auto page_of = [&](int chunk, int half) {
+        const int token = 16 * (chunk < chunks_ahead ? chunk : chunk - chunks_ahead) + 8 * half;
+        if (b >= a.batch || token >= (chunk < chunks_ahead ? a.ahead : a.max_own)) return 0;
+        return __ldcg((chunk < chunks_ahead ? a.prefix_pages : a.block_table + b * a.table_stride) + token / a.page);
+    };
+    int page_lo = 0, page_hi = 0;
+    if (a.ranks == 1) {
+        page_lo = page_of(warp + 4 * lane, 0);
+        page_hi = page_of(warp + 4 * lane, 1);
+    }
     int own = 0;
     if (b < a.batch && a.max_own > 0) {
         own = __ldcg(a.own_lens + b);
@@ -544,7 +565,9 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             own = own < 0 ? 0 : a.max_own;
         }
     }
-    const int chunks = (own + 15) / 16, first = (int)((int64_t)chunks * rank / a.ranks) + warp, last = (int)((int64_t)chunks * (rank + 1) / a.ranks);
+    const int chunks = b < a.batch ? chunks_ahead + (own + 15) / 16 : 0, first = (int)((int64_t)chunks * rank / a.ranks) + warp, last = (int)((int64_t)chunks * (rank + 1) / a.ranks);
+    const auto token_of = [&](int chunk) { return 16 * (chunk < chunks_ahead ? chunk : chunk - chunks_ahead); };
+    const auto limit_of = [&](int chunk) { return chunk < chunks_ahead ? a.ahead : own; };
     float o[VB][4][NT][4] = {};
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -559,23 +582,25 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                 if (t * 8 + g < rows && 32 * i + 8 * c < a.D)
                     q[t][i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)(kvh * a.group + row0 + t * 8 + g) * a.q_head + 32 * i + 8 * c));
             }
-        // Where this warp's chunks lie, two halves of 8 tokens each (a page holds a multiple of 8), or -1: zeros.  A lane looks a chunk's pages up, for 32
-        // chunks at a time: their latency is paid once.
-        int64_t at_lo = -1, at_hi = -1;
-        const auto look_up = [&](int token) -> int64_t {
-            if (token >= own) return -1;
-            const int at = token / a.page, page = __ldcg(a.block_table + b * a.table_stride + at);
+        int64_t at_lo = -1, at_hi = -1;                                        // where a half lies, or -1: zeros
+        const auto place = [&](int chunk, int half, int page) -> int64_t {
+            const int token = token_of(chunk) + 8 * half;
+            if (chunk >= last || token >= limit_of(chunk)) return -1;
             if (page < 0 || page >= a.n_pages) {
                 atomicExch(&g_attn_flag, kFlagLmPage);
                 return -1;
             }
-            return page * a.page_stride + (token - at * a.page) * a.token_stride + (int64_t)kvh * a.head_stride;
+            return page * a.page_stride + (token % a.page) * a.token_stride + (int64_t)kvh * a.head_stride;
         };
         const auto where = [&](int turn, int64_t& lo, int64_t& hi) {           // of chunk first + 4 turn, turns in order
             if ((turn & 31) == 0) {
                 const int chunk = first + 4 * (turn + lane);
-                at_lo = chunk < last ? look_up(16 * chunk) : -1;
-                at_hi = chunk < last ? look_up(16 * chunk + 8) : -1;
+                if (turn > 0 || a.ranks > 1) {
+                    page_lo = chunk < last ? page_of(chunk, 0) : 0;
+                    page_hi = chunk < last ? page_of(chunk, 1) : 0;
+                }
+                at_lo = place(chunk, 0, page_lo);
+                at_hi = place(chunk, 1, page_hi);
             }
             lo = __shfl_sync(0xffffffffu, at_lo, turn & 31);
             hi = __shfl_sync(0xffffffffu, at_hi, turn & 31);
@@ -590,12 +615,13 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                 int64_t lo, hi;
                 where(turn, lo, hi);
                 const uint32_t to = ring + (turn % kStages) * (2 * kHalf);
+                const int left = limit_of(chunk) - token_of(chunk);
                 const bool col = 8 * piece < a.D;
 #pragma unroll
                 for (int i = 0; i < 16 / kRows; ++i) {
                     const int row = i * kRows + row0;
                     const int64_t base = row < 8 ? lo : hi;
-                    const bool there = col && base >= 0 && 16 * chunk + row < own;
+                    const bool there = col && base >= 0 && row < left;
                     const int64_t at = there ? base + (row & 7) * a.token_stride + 8 * piece : 0;
                     const uint32_t bytes = there ? 16 : 0, dst = to + row * (DP * 2);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + ((piece ^ ((row & 1) << 2)) << 4)), "l"(static_cast<const T*>(a.k) + at), "r"(bytes) : "memory");
@@ -623,7 +649,8 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                     mma_16x8x16<T>(s[t], a1, q[t][i].z, q[t][i].w);
                 }
             }
-            const bool in0 = 16 * chunk + g < own, in1 = 16 * chunk + g + 8 < own;
+            const int left = limit_of(chunk) - token_of(chunk);
+            const bool in0 = g < left, in1 = g + 8 < left;
             float up[NT][2];
             bool grown = false;
 #pragma unroll
@@ -705,7 +732,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
 
     // The parts joined.  First the weights 2^(m_i - M) / sum 2^(m_i - M) l_i of each row's parts, a row a warp, a part a lane; then a float4 of a row for
     // `lanes` neighbouring threads, which deal the parts out among themselves.
-    const int ahead = a.prefix_len > 0 ? a.splits : 0, parts = ahead + (own > 0 ? 4 * a.ranks : 0);
+    const int ahead = a.early ? a.splits : 0, parts = ahead + (chunks > 0 ? 4 * a.ranks : 0);
     const auto first_part = [&](int row) {             // of the prefix for this row, as a row of part_ml
         const int flat = b * a.group + row0 + row;
         return (((int64_t)(flat >> 7) * a.kv_heads + kvh) * a.splits << 7) + (flat & 127);
@@ -839,23 +866,34 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     a.key_tiles = ceil_div(a.prefix_len, 128);
     a.box_rows = 8;
     while (a.box_rows < 128 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
+    // Own tokens: enough blocks of a cluster on a sequence and key head to use the GPU, no more than fit it at once, 128 tokens each at least.
+    a.row_groups = ceil_div(a.group, 8 * pl.NT);
+    const int64_t own_units = (int64_t)a.batch * a.kv_heads * a.row_groups;
+    constexpr int kAtOnce = 3 * 148;
+    const auto ranks_of = [&](int64_t tokens) {
+        int ranks = 1;
+        while (ranks < kMaxRanks && own_units * ranks * 2 <= kAtOnce && tokens / (2 * ranks) >= 128) ranks *= 2;
+        return ranks;
+    };
+    // A short prefix is taken as if it were each sequence's own where that is less than 8 us of a block's 46 bytes a nanosecond: the other kernel and the parts
+    // that it leaves take 10 at least.  (TIMES)
+    const int64_t tokens = (int64_t)a.prefix_len + a.max_own;
+    const double here_us = ceil_div<int64_t>(own_units * ranks_of(tokens), kAtOnce) * ((double)a.prefix_len / ranks_of(tokens)) * 4 * a.D / 46e3;
+    const char* force = getenv("PB_ATTN_PREFIX");          // 1 = prefix_kernel wherever there is a prefix, 0 = never; by rule otherwise
+    a.ahead = (force && force[0] ? force[0] == '0' : here_us < 8.0) ? a.prefix_len : 0;
+    a.early = a.prefix_len > a.ahead && own_units > 0;
+    a.ranks = ranks_of(a.ahead + (int64_t)a.max_own);
+    pl.own_blocks = own_units > 0 ? own_units * a.ranks : 1;
     const int64_t units = (int64_t)a.pairs * a.kv_heads;
     a.splits = 1;
     if (units > 0 && units < kMaxSplits) a.splits = (int)(kMaxSplits / units);
     if (a.splits > a.key_tiles) a.splits = a.key_tiles > 0 ? a.key_tiles : 1;
-    pl.prefix_blocks = a.prefix_len > 0 ? units * a.splits : 0;
-    const uint64_t parts = pl.prefix_blocks > 0 ? (uint64_t)a.row_tiles * a.kv_heads * a.splits * 128 : 0;
+    pl.prefix_blocks = a.early ? units * a.splits : 0;
+    const uint64_t parts = a.early ? (uint64_t)a.row_tiles * a.kv_heads * a.splits * 128 : 0;
     pl.scratch = parts * ((uint64_t)pl.DP * 4 + 8);
     a.part_o = (float*)p->scratch;
     a.part_ml = (float2*)((char*)p->scratch + parts * pl.DP * 4);
-    // own tokens
-    a.row_groups = ceil_div(a.group, 8 * pl.NT);
-    const int64_t own_units = (int64_t)a.batch * a.kv_heads * a.row_groups;
-    a.ranks = 1;
-    while (a.ranks < kMaxRanks && own_units * a.ranks < 2 * 148 && a.max_own / (2 * a.ranks) >= 128) a.ranks *= 2;
-    pl.own_blocks = own_units > 0 ? own_units * a.ranks : 1;
     PB_REQUIRE(pl.prefix_blocks <= 0x7fffffff && pl.own_blocks <= 0x7fffffff, "%s: too many blocks for one launch", who);
-    a.early = pl.prefix_blocks > 0;
     a.out_vec = aligned(p->out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
     return PB_OK;
 }

@@ -15,7 +15,17 @@ from paella_b200 import capi
 from tests import gpu_util as gu
 from tests import lm_util as lu
 
-pytestmark = pytest.mark.gpu
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("prefix_kernel")]
+
+
+@pytest.fixture(params=["rule", "0", "1"])
+def prefix_kernel(request, monkeypatch):
+    """Which kernel takes the prefix: by rule, the one of the sequences' own tokens, or that of the whole batch."""
+    if request.param == "rule":
+        monkeypatch.delenv("PB_ATTN_PREFIX", raising=False)
+    else:
+        monkeypatch.setenv("PB_ATTN_PREFIX", request.param)
+    return request.param
 
 
 class Problem:
