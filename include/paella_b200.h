@@ -214,7 +214,8 @@ PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
  * reference, whose adapters serve image models.  In the manner of the operators above: a params structure filled by the
  * caller, `_info` for the geometry a job stage declares, `_launch` to enqueue on `stream` (a cudaStream_t of the current
  * device, where all buffers live).
- *  - Each launcher enqueues one kernel, whose every block reports start/end on `notifier` (may be NULL) for `job_id`.
+ *  - Each launcher enqueues one kernel, pb_prefix_attn_launch up to three.  Every block of the only, or last, kernel reports
+ *    start/end on `notifier` (may be NULL) for `job_id`; that kernel is what `_info` describes.
  *  - Strides are in elements.  Buffers may lie anywhere inside larger ones; outputs do not overlap inputs unless a text says so.
  *  - Launches allocate nothing and may be captured into a CUDA graph, the first one included.  The pointers and sizes of the
  *    params are read at the launch, what they point to when the kernels run.

@@ -29,7 +29,8 @@ struct AttnArgs {
     float scale;
     // the prefix's split
     int row_tiles, pairs, splits, key_tiles, box_rows;
-    float* part_o;             // [row_tiles][kv_heads][splits][128][DP], a row's 16-byte piece i at i ^ (row % 32)
+    int row_parts;             // splits, and one more where own tokens leave a part as well
+    float* part_o;             // [row_tiles][kv_heads][row_parts][128][DP], a row's 16-byte piece i at i ^ (row % 32)
     float2* part_ml;           // the same without DP: (m, l)
     // own tokens
     int kv_heads, row_groups, ranks, early, out_vec;     // early: behind a prefix_kernel, beside whose end it starts
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
             __syncwarp();
         }
         if (ok && live_warp && (two || g == 0)) {
-            const int64_t part = ((int64_t)(2 * pair + (two ? g : 0)) * a.kv_heads + kvh) * a.splits + split;
+            const int64_t part = ((int64_t)(2 * pair + (two ? g : 0)) * a.kv_heads + kvh) * a.row_parts + split;
             if (row < rows) a.part_ml[part * 128 + in_tile] = make_float2(m, l);
             if (lane == 0) {
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + (part * 128 + in_tile) * DP), "r"(my_row + (two ? g * (128 * DP * 4) : 0)), "n"(32 * DP * 4) : "memory");
@@ -526,7 +527,10 @@ template <int DP> struct OwnShape {
     static constexpr int stages = DP == 128 ? 2 : 4;
     static constexpr uint32_t smem = 4 * stages * 2 * half;
 };
-template <typename T, int DP, int NT>
+// Phase 0 does all of it.  Where there are more blocks than fit the GPU at once, beside a prefix_kernel, phase 1 leaves its part to phase 2, a launch of its
+// own: its blocks then go on while the prefix is worked on, on the SMs that are left over and on those that become free, where blocks that wait for
+// the prefix's parts would hold them.
+template <typename T, int DP, int NT, int PHASE>
 __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64, kStages = OwnShape<DP>::stages;
     constexpr uint32_t kHalf = OwnShape<DP>::half;
@@ -535,7 +539,8 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     float (*s_o)[R][DP] = reinterpret_cast<float (*)[R][DP]>(smem_raw);
     __shared__ __align__(8) float2 s_ml[4][R];
     __shared__ float s_w[R][kMaxParts];
-    if (!a.early) griddep_wait();
+    if (PHASE == 2 || !a.early) griddep_wait();
+    if (PHASE == 1) griddep_launch();
     if (nf) nf->start(job_id);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = blockIdx.x % a.ranks;
@@ -553,26 +558,26 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         return __ldcg((chunk < chunks_ahead ? a.prefix_pages : a.block_table + b * a.table_stride) + token / a.page);
     };
     int page_lo = 0, page_hi = 0;
-    if (a.ranks == 1) {
+    if (PHASE != 2 && a.ranks == 1) {
         page_lo = page_of(warp + 4 * lane, 0);
         page_hi = page_of(warp + 4 * lane, 1);
     }
     int own = 0;
-    if (b < a.batch && a.max_own > 0) {
+    if (PHASE != 2 && b < a.batch && a.max_own > 0) {
         own = __ldcg(a.own_lens + b);
         if (own < 0 || own > a.max_own) {
             if (threadIdx.x == 0) atomicExch(&g_attn_flag, kFlagLmLength);
             own = own < 0 ? 0 : a.max_own;
         }
     }
-    const int chunks = b < a.batch ? chunks_ahead + (own + 15) / 16 : 0, first = (int)((int64_t)chunks * rank / a.ranks) + warp, last = (int)((int64_t)chunks * (rank + 1) / a.ranks);
+    const int chunks = PHASE != 2 && b < a.batch ? chunks_ahead + (own + 15) / 16 : 0, first = (int)((int64_t)chunks * rank / a.ranks) + warp, last = (int)((int64_t)chunks * (rank + 1) / a.ranks);
     const auto token_of = [&](int chunk) { return 16 * (chunk < chunks_ahead ? chunk : chunk - chunks_ahead); };
     const auto limit_of = [&](int chunk) { return chunk < chunks_ahead ? a.ahead : own; };
     float o[VB][4][NT][4] = {};
     float m[NT][2], l[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
-    if (first < last) {
+    if (PHASE != 2 && first < last) {
         uint4 q[NT][KB];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -708,35 +713,63 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    __syncthreads();                                                      // the rings become the warps' parts
-    // this warp's part: (m, l) and O of its rows, values 64 i + 8 g + 2 e and + 1
+    const auto first_part = [&](int row) {             // of this row's, as a row of part_ml
+        const int flat = b * a.group + row0 + row;
+        return (((int64_t)(flat >> 7) * a.kv_heads + kvh) * a.row_parts << 7) + (flat & 127);
+    };
+    constexpr int kPieces = DP / 4;
+    if constexpr (PHASE != 2) {
+        __syncthreads();                                                  // the rings become the warps' parts
+        // this warp's part: (m, l) and O of its rows, values 64 i + 8 g + 2 e and + 1
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float x = l[t][j];
-            x += __shfl_xor_sync(0xffffffffu, x, 4);
-            x += __shfl_xor_sync(0xffffffffu, x, 8);
-            x += __shfl_xor_sync(0xffffffffu, x, 16);
-            const int row = 8 * t + 2 * c + j;
-            if (g == 0) s_ml[warp][row] = make_float2(m[t][j], x);
+            for (int j = 0; j < 2; ++j) {
+                float x = l[t][j];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int row = 8 * t + 2 * c + j;
+                if (g == 0) s_ml[warp][row] = make_float2(m[t][j], x);
 #pragma unroll
-            for (int i = 0; i < VB; ++i)
+                for (int i = 0; i < VB; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(&s_o[warp][row][64 * i + 8 * g + 2 * e]) = make_float2(o[i][e][t][j], o[i][e][t][2 + j]);
+                    for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(&s_o[warp][row][64 * i + 8 * g + 2 * e]) = make_float2(o[i][e][t][j], o[i][e][t][2 + j]);
+            }
+    }
+    if constexpr (PHASE == 1) {
+        __syncthreads();
+        // the four warps' parts as one (a block has the sequence to itself here)
+        for (int item = threadIdx.x; item < rows * kPieces; item += 128) {
+            const int row = item / kPieces, i4 = item % kPieces;
+            float top = -INFINITY, sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][row].x);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 ml = s_ml[w][row];
+                const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][4 * i4]);
+                sum = fmaf(f, ml.y, sum);
+                acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+            }
+            const int64_t at = first_part(row) + (int64_t)a.splits * 128;
+            if (i4 == 0) a.part_ml[at] = make_float2(top, sum);
+            reinterpret_cast<float4*>(a.part_o + at * DP)[i4 ^ ((int)at & 31 & (kPieces - 1))] = acc;
         }
-    if (a.early) griddep_wait();                                          // the prefix's parts
+        if (blockIdx.x == gridDim.x - 1) griddep_wait();                  // so that this launch ends behind the prefix's
+        if (nf) nf->end(job_id);
+        return;
+    }
+    if (PHASE == 0 && a.early) griddep_wait();                            // the prefix's parts
     griddep_launch();
     if (a.ranks > 1) { cluster_arrive(); cluster_wait(); }
     else __syncthreads();
 
     // The parts joined.  First the weights 2^(m_i - M) / sum 2^(m_i - M) l_i of each row's parts, a row a warp, a part a lane; then a float4 of a row for
     // `lanes` neighbouring threads, which deal the parts out among themselves.
-    const int ahead = a.early ? a.splits : 0, parts = ahead + (chunks > 0 ? 4 * a.ranks : 0);
-    const auto first_part = [&](int row) {             // of the prefix for this row, as a row of part_ml
-        const int flat = b * a.group + row0 + row;
-        return (((int64_t)(flat >> 7) * a.kv_heads + kvh) * a.splits << 7) + (flat & 127);
-    };
+    const int ahead = a.early ? a.row_parts : 0, parts = ahead + (chunks > 0 ? 4 * a.ranks : 0);
     for (int row = warp; row < rows; row += 4) {
         const float2* ml = a.part_ml + first_part(row);
         float2 x[kMaxParts / 32];
@@ -765,7 +798,6 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;
     }
     __syncthreads();
-    constexpr int kPieces = DP / 4;
     const int items = rows * kPieces;
     int lanes = 1;
     while (lanes < 32 && items * lanes * 2 <= 128 * a.ranks) lanes *= 2;
@@ -811,9 +843,9 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
 
 typedef void (*OwnFn)(AttnArgs, uint32_t, FinishedBlockNotifier*);
 
-template <typename T> OwnFn own_fn(int DP, int NT) {
-    if (DP == 64) return NT == 1 ? own_kernel<T, 64, 1> : own_kernel<T, 64, 2>;
-    return NT == 1 ? own_kernel<T, 128, 1> : own_kernel<T, 128, 2>;
+template <typename T, int PHASE> OwnFn own_fn(int DP, int NT) {
+    if (DP == 64) return NT == 1 ? own_kernel<T, 64, 1, PHASE> : own_kernel<T, 64, 2, PHASE>;
+    return NT == 1 ? own_kernel<T, 128, 1, PHASE> : own_kernel<T, 128, 2, PHASE>;
 }
 
 struct AttnPlan {
@@ -822,7 +854,7 @@ struct AttnPlan {
     bool half;
     int64_t prefix_blocks, own_blocks;
     uint64_t scratch;
-    OwnFn own;
+    OwnFn own, join;           // join: NULL, or phase 2 behind own, phase 1
     uint32_t own_smem;
 };
 
@@ -857,7 +889,6 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     pl.NT = a.group <= 8 ? 1 : 2;
     pl.half = p->dtype == PB_F16;
     pl.own_smem = pl.DP == 64 ? OwnShape<64>::smem : OwnShape<128>::smem;
-    pl.own = pl.half ? own_fn<__half>(pl.DP, pl.NT) : own_fn<__nv_bfloat16>(pl.DP, pl.NT);
     // the prefix: as many parts as give every SM a block
     const int64_t rows = (int64_t)a.batch * a.group;
     PB_REQUIRE(rows <= (1 << 24), "%s: %lld query rows for a key head", who, (long long)rows);
@@ -889,7 +920,11 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     if (units > 0 && units < kMaxSplits) a.splits = (int)(kMaxSplits / units);
     if (a.splits > a.key_tiles) a.splits = a.key_tiles > 0 ? a.key_tiles : 1;
     pl.prefix_blocks = a.early ? units * a.splits : 0;
-    const uint64_t parts = a.early ? (uint64_t)a.row_tiles * a.kv_heads * a.splits * 128 : 0;
+    const bool apart = a.early && own_units > kAtOnce && a.max_own > 0;
+    a.row_parts = a.splits + (apart ? 1 : 0);
+    pl.own = pl.half ? (apart ? own_fn<__half, 1> : own_fn<__half, 0>)(pl.DP, pl.NT) : (apart ? own_fn<__nv_bfloat16, 1> : own_fn<__nv_bfloat16, 0>)(pl.DP, pl.NT);
+    pl.join = !apart ? nullptr : pl.half ? own_fn<__half, 2>(pl.DP, pl.NT) : own_fn<__nv_bfloat16, 2>(pl.DP, pl.NT);
+    const uint64_t parts = a.early ? (uint64_t)a.row_tiles * a.kv_heads * a.row_parts * 128 : 0;
     pl.scratch = parts * ((uint64_t)pl.DP * 4 + 8);
     a.part_o = (float*)p->scratch;
     a.part_ml = (float2*)((char*)p->scratch + parts * pl.DP * 4);
@@ -927,9 +962,9 @@ int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out) {
     out->num_blocks = (uint32_t)pl.own_blocks;
     out->threads_per_block = 128;
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, pl.own) == cudaSuccess) {
+    if (cudaFuncGetAttributes(&fa, pl.join ? pl.join : pl.own) == cudaSuccess) {
         out->regs_per_thread = (uint32_t)fa.numRegs;
-        out->smem_per_block = (uint32_t)fa.sharedSizeBytes + pl.own_smem;
+        out->smem_per_block = (uint32_t)fa.sharedSizeBytes + (pl.join ? 0 : pl.own_smem);
     } else {
         cudaGetLastError();
     }
@@ -963,7 +998,12 @@ int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t
         if (e != PB_OK) return e;
     }
     PB_CUDA(cudaFuncSetAttribute(pl.own, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.own_smem));
-    return lm_launch("pb_prefix_attn", pl.own, dim3((unsigned)pl.own_blocks), dim3(128), pl.own_smem, st, pl.a.ranks, pl.a, job_id, (FinishedBlockNotifier*)notifier);
+    FinishedBlockNotifier* nf = (FinishedBlockNotifier*)notifier;
+    const dim3 blocks((unsigned)pl.own_blocks);
+    if (!pl.join) return lm_launch("pb_prefix_attn", pl.own, blocks, dim3(128), pl.own_smem, st, pl.a.ranks, pl.a, job_id, nf);
+    const int e = lm_launch("pb_prefix_attn (own tokens)", pl.own, blocks, dim3(128), pl.own_smem, st, 1, pl.a, job_id, (FinishedBlockNotifier*)nullptr);
+    if (e != PB_OK) return e;
+    return lm_launch("pb_prefix_attn (parts)", pl.join, blocks, dim3(128), 0, st, 1, pl.a, job_id, nf);
 }
 
 }  // extern "C"

@@ -112,7 +112,8 @@ class Problem:
     ([1, 2, 127, 128, 129, 255, 256, 257], 1, 8, 128, 128, 64), ([33] * 5, 8, 5, 80, 257, 32), ([0, 700], 1, 16, 96, 127, 8), ([40, 41], 4, 1, 128, 4096, 128),
     ([9] * 64, 2, 4, 64, 1000, 16), ([0, 64, 3] * 11, 1, 7, 112, 129, 24), ([20] * 17, 1, 8, 128, 640, 64), ([100] * 3, 2, 2, 8, 50, 8), ([7] * 40, 3, 8, 128, 2049, 256),
     ([1000, 0, 5, 2500], 2, 8, 128, 0, 64), ([600] * 2, 1, 32, 64, 333, 40), ([0] * 130, 1, 2, 128, 515, 32), ([3] * 300, 1, 1, 40, 77, 16), ([11] * 2, 1, 128, 128, 200, 16),
-    ([5] * 3, 1, 71, 64, 5000, 64), ([2] * 100, 1, 6, 128, 9001, 128)])
+    ([5] * 3, 1, 71, 64, 5000, 64), ([2] * 100, 1, 6, 128, 9001, 128),
+    ([0, 17, 40, 1] * 75, 2, 3, 64, 515, 16), ([33, 0] * 65, 8, 2, 128, 300, 24), ([1] * 64, 1, 128, 112, 200, 32)])
 @pytest.mark.parametrize("ty,heads_first", [("bf16", False), ("f16", True)])
 def test_attention(ty, heads_first, lens, hkv, group, d, prefix, page):
     p = Problem(lens, hkv, group, d, prefix, page, ty, heads_first)
@@ -195,7 +196,7 @@ def test_cache_behind_four_billion_elements():
     assert torch.equal(p.run(), ref)
 
 
-@pytest.mark.parametrize("lens,prefix", [([5, 0, 300], 1000), ([5, 0, 300], 0), ([0, 0, 0], 1000), ([17] * 50, 3000)])
+@pytest.mark.parametrize("lens,prefix", [([5, 0, 300], 1000), ([5, 0, 300], 0), ([0, 0, 0], 1000), ([17] * 50, 3000), ([40, 3] * 150, 700)])
 def test_captured_with_other_lengths_and_the_same_bits_again(lens, prefix):
     """A graph's launches read lengths, tables and queries at each replay; the same inputs give the same bits."""
     p = Problem(lens, 2, 4, 128, prefix, 32, most=max(lens))
@@ -222,7 +223,7 @@ def test_captured_with_other_lengths_and_the_same_bits_again(lens, prefix):
     assert gu.error_flag() == 0
 
 
-@pytest.mark.parametrize("lens,prefix", [([5, 0, 300], 1000), ([5, 0, 300], 0), ([0, 0, 0], 1000), ([2] * 100, 50), ([], 100)])
+@pytest.mark.parametrize("lens,prefix", [([5, 0, 300], 1000), ([5, 0, 300], 0), ([0, 0, 0], 1000), ([2] * 100, 50), ([], 100), ([9, 0] * 150, 400)])
 def test_notifications_count_the_declared_blocks(lens, prefix):
     p = Problem(lens or [1], 2, 4, 128, prefix, 32)
     params = p.params()
