@@ -128,6 +128,7 @@ struct DenseArgs {
 
 constexpr uint32_t kABytes = 128 * 128;
 constexpr int kMaxInt8Stages = 16;
+constexpr int kMaxInt8Smem = 224 * 1024;
 
 
 template <bool PAIR>
@@ -593,7 +594,7 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
     if (!pl.many) a.kblocks = ceil_div(a.K, 128 * halves);
     const uint32_t stage = pl.many ? kABytes + (uint32_t)a.BN * 64 : (kABytes + (uint32_t)a.BN * 128) * halves;
     if (pl.many) {
-        a.stages = (int)std::min<uint32_t>(kMaxInt8Stages, (227 * 1024 - 4096 - kOutBytes) / stage);
+        a.stages = (int)std::min<uint32_t>(kMaxInt8Stages, (kMaxInt8Smem - 1024 - kOutBytes) / stage);
         pl.smem = 1024 + a.stages * stage + kOutBytes;
         const int64_t tiles = (int64_t)a.channel_tiles * a.token_tiles;
         PB_REQUIRE(tiles <= 0x3fffffff, "pb_int8_dense: too many results for one launch");
@@ -689,7 +690,7 @@ int pb_int8_dense_launch(const pb_int8_dense_params* p, void* stream, uint32_t j
     int e = encode_tiled_sw128(CU_TENSOR_MAP_DATA_TYPE_UINT8, p->w, 2, wdims, &wstride, wbox, &wmap);
     if (e == PB_OK) e = encode_tiled_sw128(CU_TENSOR_MAP_DATA_TYPE_UINT8, p->x, 2, xdims, &xstride, xbox, &xmap);
     if (e != PB_OK) return e;
-    PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem));
+    PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInt8Smem));      // (the same for every launch: other threads' may be on their way)
     return lm_launch("pb_int8_dense", pl.fn, dim3(pl.blocks), dim3(192), pl.smem, (cudaStream_t)stream, pl.a.splits, pl.a, wmap, xmap, job_id, (FinishedBlockNotifier*)notifier);
 }
 

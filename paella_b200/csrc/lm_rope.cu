@@ -574,7 +574,7 @@ int rope_info(const RopePlan& pl, int dtype, pb_launch_info* out) {
 }
 
 int launch_rope(const char* who, const RopePlan& pl, void* stream, uint32_t job_id, void* notifier) {
-    if (pl.smem > 48 * 1024) PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));
+    if (pl.smem > 48 * 1024) PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (8192 + 1024)));
     return lm_launch(who, pl.fn, dim3(pl.blocks), dim3(256), (size_t)pl.smem, (cudaStream_t)stream, 1, pl.a, job_id, (FinishedBlockNotifier*)notifier);
 }
 
