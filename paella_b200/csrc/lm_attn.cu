@@ -906,12 +906,13 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
         while (ranks < kMaxRanks && own_units * ranks * 2 <= kAtOnce && tokens / (2 * ranks) >= 128) ranks *= 2;
         return ranks;
     };
-    // A short prefix is taken as if it were each sequence's own where that is less than 8 us of a block's 46 bytes a nanosecond: the other kernel and the parts
-    // that it leaves take 10 at least.  (TIMES)
+    // A short prefix is taken as if it were each sequence's own, where that costs little: a block's tokens come at some 70 bytes a nanosecond, those of all
+    // blocks from the L2 cache at 9 KB.  (8 key heads of 128, with the own kernel alone / with both: one sequence behind 512, 4096, 8192 tokens 6.8 / 9.6 us,
+    // 10.3 / 12.6, 16.1 / 15.5; 8 behind 256 and 1024 6.9 / 9.3, 10.8 / 9.2; 32 behind 256 and 512 10.2 / 10.4, 13.4 / 11.0.)
     const int64_t tokens = (int64_t)a.prefix_len + a.max_own;
-    const double here_us = ceil_div<int64_t>(own_units * ranks_of(tokens), kAtOnce) * ((double)a.prefix_len / ranks_of(tokens)) * 4 * a.D / 46e3;
+    const double bytes = 4.0 * a.D * a.prefix_len, block_us = bytes / ranks_of(tokens) / 70e3, all_us = bytes * own_units / 9e6;
     const char* force = getenv("PB_ATTN_PREFIX");          // 1 = prefix_kernel wherever there is a prefix, 0 = never; by rule otherwise
-    a.ahead = (force && force[0] ? force[0] == '0' : here_us < 8.0) ? a.prefix_len : 0;
+    a.ahead = (force && force[0] ? force[0] == '0' : block_us < 6.0 && all_us < 3.5) ? a.prefix_len : 0;
     a.early = a.prefix_len > a.ahead && own_units > 0;
     a.ranks = ranks_of(a.ahead + (int64_t)a.max_own);
     pl.own_blocks = own_units > 0 ? own_units * a.ranks : 1;

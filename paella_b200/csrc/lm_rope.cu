@@ -39,8 +39,8 @@ struct RopeArgs {
     int wide_weights;          // weights are 16-byte aligned
 };
 
-// V values are an access, a lane takes CH chunks of 2 V values, a group HEADS neighbouring heads of a token, in registers: few heads, or any alignment.
-template <typename T, int V, int CH, int HEADS>
+// V values are an access, a lane takes CH chunks of 2 V values, a group one head of a token: few heads, or any alignment.
+template <typename T, int V, int CH>
 __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     using Vt = LmVec<T, V>;
     griddep_wait();
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
     const int lane = threadIdx.x & (a.lanes - 1);
     const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / a.lanes;
     const int64_t token = group >> 32 ? group / a.slices : (uint32_t)group / (uint32_t)a.slices;    // (a 64-bit quotient takes some 70 instructions)
-    const int head0 = (int)(group - token * a.slices) * HEADS;
+    const int head = (int)(group - token * a.slices);
     bool live = token < a.tokens;
     int pos = 0;
     int64_t slot = 0;
@@ -71,20 +71,17 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
         if (lo[c] >= a.head_dim) lo[c] = -1;
         if (hi[c] >= a.head_dim) hi[c] = -1;
     }
-    Vt x[HEADS][CH][2];
-    const auto set_of = [&](int head) { return head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2; };
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h) {
-        const int head = head0 + h;
-        if (!live || head >= a.first[2]) continue;
-        const int w = set_of(head);
-        const T* src = static_cast<const T*>(a.set[w].src) + token * a.set[w].src_token + (head - (w ? a.first[w - 1] : 0)) * a.set[w].src_head;
+    Vt x[CH][2];
+    const int kind = head < a.first[0] ? 0 : head < a.first[1] ? 1 : 2, within = head - (kind ? a.first[kind - 1] : 0);
+    const HeadSet& s = a.set[kind];
+    if (live) {
+        const T* src = static_cast<const T*>(s.src) + token * s.src_token + within * s.src_head;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int at = p ? hi[c] : lo[c];
-                if (at >= 0) x[h][c][p] = *reinterpret_cast<const Vt*>(src + at);
+                if (at >= 0) x[c][p] = *reinterpret_cast<const Vt*>(src + at);
             }
     }
     bool store = true;                                   // keys and values of this token are stored
@@ -121,16 +118,10 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
             for (int j = 0; j < V; ++j) { co[c][j] = 1.f; si[c][j] = 0.f; }
         }
     }
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h) {
-        const int head = head0 + h;
-        int w = set_of(head);
-        if (!live || head >= a.first[2] || (w && !store)) w = -1;
-        if (__all_sync(0xffffffffu, w < 0)) continue;
-        const HeadSet& s = a.set[w < 0 ? 0 : w];
+    const int w = live && (kind == 0 || store) ? kind : -1;
+    if (!__all_sync(0xffffffffu, w < 0)) {
         const float* weight = w < 0 ? nullptr : s.weight;
-        T* dst = static_cast<T*>(s.dst) + (head - (w > 0 ? a.first[w - 1] : 0)) * s.dst_head +
-                 (w > 0 && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
+        T* dst = static_cast<T*>(s.dst) + within * s.dst_head + (kind && a.slots ? page * a.page_stride + slot * a.row_stride : token * s.dst_token);
         float z[CH][2][V];
         float sum = 0.f;
 #pragma unroll
@@ -140,13 +131,12 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
                 const bool there = w >= 0 && (p ? hi[c] : lo[c]) >= 0;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    z[c][p][j] = there ? lm_to_f<T>(x[h][c][p].v[j]) : 0.f;
+                    z[c][p][j] = there ? lm_to_f<T>(x[c][p].v[j]) : 0.f;
                     sum += z[c][p][j] * z[c][p][j];
                 }
             }
         if (__any_sync(0xffffffffu, weight != nullptr))
             for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (w < 0) continue;
         if (weight) {
             const float r = rsqrtf(sum * a.inv_dim + a.eps);
             constexpr int W = V < 4 ? V : 4;             // (weights may lie at any float: wide accesses only where they do not)
@@ -196,11 +186,11 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
                     out[1].v[j] = lm_from_f<T>(z[c][1][j]);
                 }
             } else {                                     // as it was, a NaN's bits too
-                out[0] = x[h][c][0];
-                out[1] = x[h][c][1];
+                out[0] = x[c][0];
+                out[1] = x[c][1];
             }
-            if (lo[c] >= 0) *reinterpret_cast<Vt*>(dst + lo[c]) = out[0];
-            if (hi[c] >= 0) *reinterpret_cast<Vt*>(dst + hi[c]) = out[1];
+            if (w >= 0 && lo[c] >= 0) *reinterpret_cast<Vt*>(dst + lo[c]) = out[0];
+            if (w >= 0 && hi[c] >= 0) *reinterpret_cast<Vt*>(dst + hi[c]) = out[1];
         }
     }
     if (nf) nf->end(job_id);
@@ -460,10 +450,10 @@ bool vectors_fit(const HeadSet& s, int heads, int V, size_t es) {
 template <typename T>
 RopeFn pick(bool wide, int heads, bool interleaved) {
     constexpr int VN = 16 / (int)sizeof(T);
-    if (!wide) return rope_kernel<T, 1, 4, 1>;
+    if (!wide) return rope_kernel<T, 1, 4>;
     if (heads == 8) return interleaved ? rope_many_kernel<T, 8, true> : rope_many_kernel<T, 8, false>;
     if (heads == 4) return interleaved ? rope_many_kernel<T, 4, true> : rope_many_kernel<T, 4, false>;
-    return heads == 2 ? rope_kernel<T, VN, 1, 2> : rope_kernel<T, VN, 1, 1>;
+    return rope_kernel<T, VN, 1>;
 }
 
 int plan_rope(const char* who, int dtype, RopePlan& pl) {
@@ -486,11 +476,10 @@ int plan_rope(const char* who, int dtype, RopePlan& pl) {
     a.lanes = 1;
     while (a.lanes * per_lane < chunks) a.lanes *= 2;
     const int heads = a.first[2];
-    // Heads of a group: as many as leave the GPU two waves of threads.
+    // Heads of a group: eight (four of few) once that gives every SM a block and a half, one below.  (40 heads of 128 in bf16, one / four / eight: 700 tokens
+    // 5.8 / 5.8 / 6.2 us, 1500 12.7 / 11.8 / 11.8, 3000 24 / 20 / 20, 16384 118 / 80 / 72.)
     int each = 1;
-    if (wide)
-        for (int e = 8; e > 1; e /= 2)
-            if (heads >= e && (int64_t)a.tokens * ceil_div(heads, e) * a.lanes >= 2 * 148 * 768) { each = e; break; }
+    if (wide && heads > 1 && (int64_t)a.tokens * ceil_div(heads, heads > 4 ? 8 : 4) * a.lanes >= 148 * 384) each = heads > 4 ? 8 : 4;
     a.slices = ceil_div(heads, each);
     const int64_t blocks = ceil_div<int64_t>((int64_t)a.tokens * a.slices * a.lanes, 256);
     PB_REQUIRE(blocks <= 0x7fffffff, "%s: %d tokens of %d heads are too many for one launch", who, a.tokens, heads);
