@@ -570,24 +570,27 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
     const int T = a.T > 0 ? a.T : 1;
     double best = 1e300;
     int halves = 1;            // of 128 bytes of a row in a stage of int8_few_kernel
-    // One block a tile, up to 8 blocks on its reduction.  Beside what an SM does: the weights from memory, at 3050 bytes a clock where every SM asks for them
-    // and 2700 otherwise, and 2600 clocks for parts that meet.  (24 tokens, 16384 -> 14336: 112 blocks 52 us, 224 that share 42; 4096 -> 14336: 13.7
-    // against 17.7; one token, 4096 -> 4096: 128 blocks that share 6.2 us, 64 6.7.)
-    for (int tt = ceil_div(T, 128); tt <= ceil_div(T, 128) + 1; ++tt) {
+    // One block a tile; narrower tiles, and up to 8 blocks on a reduction, only where SMs would be idle otherwise (two blocks an SM for long reductions).
+    // Beside what an SM does: the weights from memory, at 3050 bytes a clock where every SM asks for them and 2700 otherwise, and for parts that meet 2600
+    // clocks and 70 a token.  (24 tokens, 4096 -> 14336: 112 blocks 13.6 us, 224 that share 17.9, 224 of twelve tokens 16.8; 16384 -> 14336: 112 blocks 52, 224
+    // that share 42; 64 tokens, 1024 -> 1024: 8 blocks 4.5, 16 of half the tokens 3.6, 64 that share 5.5.)
+    for (int tt = ceil_div(T, 128); tt <= ceil_div(T, 16); ++tt) {
         const int BN = round_up(ceil_div(T, tt), 16), tiles = ceil_div(T, BN), pieces = BN <= 32 ? 2 : 1, few = ceil_div(a.K, 128 * pieces);
+        if (tt > ceil_div(T, 128) && (int64_t)ceil_div(a.N, 128) * tiles > 148) break;
         for (int S = 1; S <= 8 && S <= few; S *= 2) {
             const double blocks = (double)ceil_div(a.N, 128) * tiles * S;
+            if (S > 1 && blocks > (a.K >= 8192 ? 296 : 148)) break;
             const double work = std::ceil(blocks / 148) * ceil_div(few, S) * pieces * kblock_clocks(BN, BN), memory = (double)a.N * a.K / (blocks >= 148 ? 3050 : 2700);
-            const double clocks = std::max(work, memory) + (S > 1 ? 2600 + 8.0 * BN : 0) + 10.0 * BN;
+            const double clocks = std::max(work, memory) + (S > 1 ? 2600 + 70.0 * std::min(BN, T) : 0) + 10.0 * BN;
             if (clocks < best) { best = clocks; pl.many = false; a.BN = BN; a.token_tiles = tiles; a.splits = S; halves = pieces; }
         }
     }
     // pairs of SMs on 256 channels
     if (T > 64)
-        for (int BN = 64; BN <= 256; BN += 32) {
-            const int tiles = ceil_div(T, BN);
-            const double clocks = std::ceil((double)ceil_div(a.N, 256) * tiles / 74) * a.kblocks * kblock_clocks(BN, BN / 2) + 2000 + 10.0 * BN;
-            if (clocks < best) { best = clocks; pl.many = true; a.BN = BN; a.token_tiles = tiles; a.splits = 1; }
+        for (int wide = 64; wide <= 256; wide += 32) {
+            const int tiles = ceil_div(T, wide);
+            const double clocks = std::ceil((double)ceil_div(a.N, 256) * tiles / 74) * a.kblocks * kblock_clocks(wide, wide / 2) + 2000 + 10.0 * wide;
+            if (clocks < best) { best = clocks; pl.many = true; a.BN = wide; a.token_tiles = tiles; a.splits = 1; }
         }
     a.channel_tiles = ceil_div(a.N, pl.many ? 256 : 128);
     // Narrow tiles take 256 bytes of a row a stage: what a stage costs beside its copies and products, 230 clocks, comes half as often.
