@@ -217,6 +217,7 @@ PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
  *  - Each launcher enqueues one kernel, pb_prefix_attn_launch up to three.  Every block of the only, or last, kernel reports
  *    start/end on `notifier` (may be NULL) for `job_id`; that kernel is what `_info` describes.
  *  - Strides are in elements.  Buffers may lie anywhere inside larger ones; outputs do not overlap inputs unless a text says so.
+ *    Alignment to the element is enough where no more is asked for; rows and heads that start on 16 bytes are moved faster.
  *  - Launches allocate nothing and may be captured into a CUDA graph, the first one included.  The pointers and sizes of the
  *    params are read at the launch, what they point to when the kernels run.
  *  - What the host can see to be wrong is refused with PB_ERR_INVALID before anything is enqueued.  What only the device can
@@ -237,7 +238,7 @@ typedef struct pb_int8_quantize_params {
     int32_t tokens, channels;    /* rows (0 = nothing to do) and their length (>= 1) */
     int32_t x_dtype;             /* PB_F32, PB_BF16 or PB_F16 */
     int32_t reserved;            /* 0 */
-    int64_t x_stride, q_stride;  /* from row to row */
+    int64_t x_stride, q_stride;  /* from row to row; pb_int8_dense takes rows of q that start on 16 bytes */
     const void* x;
     int8_t* q;
     float* scale;                /* [tokens] */
@@ -332,7 +333,7 @@ typedef struct pb_prefix_attn_params {
     int32_t q_heads, kv_heads;   /* q_heads a multiple of kv_heads */
     int32_t head_dim;            /* a multiple of 8, 8 to 128 */
     int32_t page_size;           /* a multiple of 8 */
-    int32_t max_blocks;          /* entries of a row of block_table that may be read */
+    int32_t max_blocks;          /* entries of a row of block_table; those of max_own_len tokens are read, whatever own_lens says */
     int32_t prefix_len;          /* tokens, >= 0; ends anywhere in its last page */
     int32_t max_own_len;         /* the most that own_lens holds; <= max_blocks * page_size */
     float scale;

@@ -2,11 +2,16 @@
 //
 //   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j   over the prefix's tokens and the sequence's own
 //
-// Two kernels.  The prefix is one matrix for the whole batch: the rows of all sequences' query heads that share a key head
-// meet it in tiles of 128 rows x 128 keys on the tensor cores (prefix_kernel), and its keys and values are read once for 256
-// rows.  A sequence's own tokens meet only its `group` query rows: that is bound by reading them, a block for each sequence and
-// key head (own_kernel), which also joins the parts of the prefix with its own.  Softmax runs along with the sums: each part
-// has its rows' maximum m, sum l and unscaled O, and parts join as sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.
+// The prefix is one matrix for the whole batch: the rows of all sequences' query heads that share a key head meet it in tiles of 128 rows x
+// 128 keys on the tensor cores (prefix_kernel), and its keys and values are read once for 256 rows.  A sequence's own tokens meet only its `group`
+// query rows: that is bound by reading them, a block for each sequence and key head (own_kernel), which also joins the parts of the prefix with
+// its own.  Softmax runs along with the sums, in fp32: each part has its rows' maximum m, sum l and unscaled O, and parts join as
+// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.  The softmax's values are rounded to the cache's type, as the tensor cores take them; the sums l are of what they
+// were before.
+//
+// What bounds it: few rows, the cache's bytes (16 sequences of 8 heads a key head behind 130001 tokens, 556 MB: 104 to 108 us, 5.2 TB/s); many, the tensor cores
+// and the exponentials together (2048 rows a key head behind 16384 tokens: the tensor pipe is busy 71 % of the time on the SMs that take part).  256
+// sequences of 8 heads a key head behind 16384 tokens with up to 1024 of their own: 200 to 206 us.
 #include <cuda.h>
 
 #include <cmath>
@@ -88,7 +93,8 @@ constexpr float kSlack = 8.f;
 // fp16 has few exponents below 1: its values are scaled up by 2^5 (2^13 with the slack; the sums with them).
 template <typename T> __device__ __forceinline__ constexpr float p_shift() { return sizeof(T) == 2 && std::is_same<T, __half>::value ? 5.f : 0.f; }
 
-// 64 keys: 2^(s c + base) from their scores, rounded to pairs, and the sum of what they were.  One pair in four on the multipliers.
+// 64 keys: 2^(s c + base) from their scores, rounded to pairs, and the sum of what they were.  One pair in four on the multipliers (none, one in eight, three, two:
+// 156, 168, 144, 158 us against 139 behind 16384 tokens).
 template <typename T>
 __device__ __forceinline__ float values_of(const uint32_t* s, float c, float base, uint32_t (&p)[32]) {
     const uint64_t c2 = pack_f32x2(__float_as_uint(c), __float_as_uint(c)), base2 = pack_f32x2(__float_as_uint(base), __float_as_uint(base));
@@ -115,12 +121,14 @@ __device__ __forceinline__ float values_of(const uint32_t* s, float c, float bas
 
 // ---- the prefix ----------------------------------------------------------------------------------------------
 // A block takes a range of the prefix's keys for one key head and a pair of row tiles, or, where the last row tile is alone, that tile with its
-// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warp 8 loads keys and values, warps 9 and 10
-// issue the products of one of the pair each: S = Q K^T of the one tile runs while the other's softmax does.  S (128 columns) becomes P in place (64 columns of 16-bit pairs), the A
-// operand of O += P V, whose first half starts when half of P is there.  Tensor memory: S0 S1 O0 O1.
+// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warp 8 copies keys and values, warps 9 and 10
+// issue the products of one of the pair each, 64 keys at a time: S = Q K^T into 64 columns of tensor memory, where P of 16-bit pairs takes its place as the A operand
+// of O += P V, while softmax is at the other 64.  Tensor memory: S0 S1 O0 O1, all of it at 128 values a head.
+// (Scores of 128 keys at once, which cost the tensor cores 512 clocks instead of 778, leave no second place for them: a tile of the pair took 4100 clocks
+// from one softmax to the next instead of 3300.  A lone issuing warp for both: 4800, its waits of 100 to 200 clocks each in a row.)
 template <int DP> struct PrefixShape {
     static constexpr uint32_t tile = 128 * DP * 2;                   // bytes of 128 rows
-    static constexpr int stages = DP == 128 ? 5 : 10;                // tiles of keys or values in flight
+    static constexpr int stages = DP == 128 ? 5 : 10;                // tiles of keys or values in flight (three: 215 instead of 205 us)
     static constexpr uint32_t smem = 1024 + (2 + stages) * tile;     // two tiles of queries in front of them
 };
 
@@ -515,8 +523,8 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
 }
 
 // A block (or a cluster of `ranks` blocks, each a range of the tokens) takes 8 NT query rows of one sequence and key head.  A warp takes 16 tokens at a
-// time, copied into a ring of its own two to four chunks ahead: 12 warps of an SM have 96 to 192 KB on the way.  (In registers, a chunk ahead, it was 60: 1024
-// sequences' worth of 16 tokens a head came at 3.9 TB/s.)  The order of a head's values within a product's 16 is free as long as both operands have the
+// time, copied into a ring of its own two to four chunks ahead: 12 warps of an SM have 96 to 192 KB on the way.  (In registers, a chunk ahead, it was some 60: 537 MB
+// of own tokens took 141 us instead of 88 to 98.)  The order of a head's values within a product's 16 is free as long as both operands have the
 // same, and so is the order of O's rows, hence each lane reads 16 bytes as they lie:
 //   S^T[token][row] = K Q^T:  lane (g, c) = (lane / 4, lane % 4) holds 8 values at 8 c of every 32 of tokens g and g + 8
 //   O^T[value][row] = V^T P^T: 8 values at 8 g of every 64 of tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
@@ -529,7 +537,7 @@ template <int DP> struct OwnShape {
 };
 // Phase 0 does all of it.  Where there are more blocks than fit the GPU at once, beside a prefix_kernel, phase 1 leaves its part to phase 2, a launch of its
 // own: its blocks then go on while the prefix is worked on, on the SMs that are left over and on those that become free, where blocks that wait for
-// the prefix's parts would hold them.
+// the prefix's parts would hold them (220 -> 200 us).
 template <typename T, int DP, int NT, int PHASE>
 __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64, kStages = OwnShape<DP>::stages;

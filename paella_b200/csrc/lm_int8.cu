@@ -16,8 +16,9 @@ namespace {
 __device__ uint32_t g_int8_flag;
 
 // ---- activations to 8 bits ---------------------------------------------------------------
-// Bound by memory: a row is read once, stays in registers, and leaves as a quarter or half of its bytes.  `Row` threads take a row (a warp a
-// short one, the block a long one) in vectors of 16 bytes; what does not fit the registers is read a second time, from the caches.
+// Bound by memory (8192 rows of 8192 in fp16, 201 MB: 38 us, 5.2 TB/s): a row is read once, stays in registers, and leaves as a quarter or half of its bytes.
+// `ROW` threads take a row (a warp a short one, the block a long one) in vectors of 16 bytes; what does not fit the registers is read a second time, from the
+// caches.
 struct QuantizeArgs {
     const void* x;
     int8_t* q;
@@ -26,7 +27,9 @@ struct QuantizeArgs {
     int tokens, channels;
 };
 
-__device__ __forceinline__ int8_t to_int8(float v, float inv) { return (int8_t)__float2int_rn(v * inv); }
+// rint(v * inv) for products up to 2^22: behind 1.5 x 2^23 the sum's last bits are the whole number, halves to even as rint has them.  (Conversions on the
+// special-function unit kept it busy 45 % of the time.)
+__device__ __forceinline__ int8_t to_int8(float v, float inv) { return (int8_t)__float_as_int(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); }
 
 template <typename T, bool WIDE, int ROW>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(const __grid_constant__ QuantizeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
@@ -112,10 +115,11 @@ template <typename T> QuantizeFn quantize_fn(bool wide, bool warp) {
 // lanes hold neighbouring values of y.
 //
 // Few tokens are bound by reading the weights, many by the tensor cores.  int8_few_kernel: a tile of 128 channels for each block, its
-// reduction shared by the blocks of a cluster where the tiles alone leave SMs idle; the sums meet in shared memory (whole numbers:
-// their order changes nothing).  int8_many_kernel: a pair of SMs on a tile of 256 channels, each block with its own half of the
-// channels and half of the tokens: 32 KB a k-block and SM for 512 clocks of products, which the path from the L2 cache into an SM (some 60 bytes a
-// clock) feeds; a lone SM on 128 x 256 would need 48 KB.
+// reduction shared by the blocks of a cluster where the tiles alone leave SMs idle; they send their sums to the blocks that own the tokens (whole numbers:
+// their order changes nothing).  24 tokens, 4096 -> 14336: 13.6 us with the quantiser, 4.4 TB/s, 67 % of the copy rate; 64 tokens, 8192 -> 28672 40 to 42 us,
+// 87 to 90 %.  int8_many_kernel: a pair of SMs on a tile of 256 channels, each block with its own half of the channels and half of the tokens: 32 KB a
+// k-block and SM for 512 clocks of products, which the path from the L2 cache into an SM (some 60 bytes a clock) feeds; a lone SM on 128 x 256 would need
+// 48 KB.  8192 tokens, 8192 -> 8192: 337 us at full clocks, 3261 TOP/s, twice the measured bf16 rate to 1 %; 390 to 400 where power holds the clocks down.
 struct DenseArgs {
     const float *x_scale, *w_scale, *bias;
     void* y;
@@ -580,7 +584,7 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
         for (int S = 1; S <= 8 && S <= few; S *= 2) {
             const double blocks = (double)ceil_div(a.N, 128) * tiles * S;
             if (S > 1 && blocks > (a.K >= 8192 ? 296 : 148)) break;
-            const double work = std::ceil(blocks / 148) * ceil_div(few, S) * pieces * kblock_clocks(BN, BN), memory = (double)a.N * a.K / (blocks >= 148 ? 3050 : 2700);
+            const double work = std::ceil(blocks / 148) * ceil_div(few, S) * pieces * kblock_clocks(BN, BN), memory = (double)a.N * a.K / (22 * std::min(blocks, 148.0));
             const double clocks = std::max(work, memory) + (S > 1 ? 2600 + 70.0 * std::min(BN, T) : 0) + 10.0 * BN;
             if (clocks < best) { best = clocks; pl.many = false; a.BN = BN; a.token_tiles = tiles; a.splits = S; halves = pieces; }
         }
