@@ -14,6 +14,7 @@
 // sequences of 8 heads a key head behind 16384 tokens with up to 1024 of their own: 200 to 206 us.
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 
@@ -877,7 +878,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     PB_REQUIRE(p->prefix_len >= 0 && p->prefix_len <= (1 << 30) && p->max_own_len >= 0 && p->max_own_len <= (1 << 30), "%s: prefix of %d tokens, at most %d own", who, p->prefix_len, p->max_own_len);
     PB_REQUIRE(p->max_blocks >= 0 && p->max_own_len <= (int64_t)p->max_blocks * p->page_size, "%s: %d own tokens do not fit %d pages of %d", who, p->max_own_len, p->max_blocks, p->page_size);
     PB_REQUIRE(p->n_pages > 0 || (p->prefix_len == 0 && p->max_own_len == 0) || p->batch == 0, "%s: a cache without pages", who);
-    PB_REQUIRE(p->scale == p->scale && fabsf(p->scale) <= 3.402823466e38f, "%s: scale is not finite", who);
+    PB_REQUIRE(fabsf(p->scale) <= 2e38f, "%s: scale is not finite, or above 2e38", who);        // (which in powers of two is finite, too)
     PB_REQUIRE(p->page_stride % 8 == 0 && p->token_stride % 8 == 0 && p->head_stride % 8 == 0 && p->page_stride > 0 && p->token_stride > 0 && p->head_stride > 0, "%s: strides of the cache are positive multiples of 8", who);
     PB_REQUIRE(p->q_stride % 8 == 0 && p->q_head_stride % 8 == 0, "%s: rows of q start on 16 bytes", who);
     if (p->batch > 0) {
@@ -922,8 +923,8 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     const char* force = getenv("PB_ATTN_PREFIX");          // 1 = prefix_kernel wherever there is a prefix, 0 = never; by rule otherwise
     a.ahead = (force && force[0] ? force[0] == '0' : block_us < 6.0 && all_us < 3.5) ? a.prefix_len : 0;
     a.early = a.prefix_len > a.ahead && own_units > 0;
-    a.ranks = ranks_of(a.ahead + (int64_t)a.max_own);
-    pl.own_blocks = own_units > 0 ? own_units * a.ranks : 1;
+    a.ranks = own_units > 0 ? ranks_of(a.ahead + (int64_t)a.max_own) : 1;
+    pl.own_blocks = std::max<int64_t>(own_units * a.ranks, 1);
     const int64_t units = (int64_t)a.pairs * a.kv_heads;
     a.splits = 1;
     if (units > 0 && units < kMaxSplits) a.splits = (int)(kMaxSplits / units);

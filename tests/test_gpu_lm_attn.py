@@ -236,6 +236,42 @@ def test_notifications_count_the_declared_blocks(lens, prefix):
         assert bool((p.out == 9.0).all())
 
 
+@pytest.mark.parametrize("most", [0, 64, 5000])
+def test_no_tokens_at_all_and_no_sequences(most):
+    p = Problem([0, 0, 0], 2, 4, 64, 0, 16, most=most)
+    p.check(p.run())
+    params = p.params()
+    params.batch = 0
+    p.out.fill_(9.0)
+    n = lu.info("prefix_attn", params).num_blocks
+    assert lu.records("prefix_attn", params) == (n, n)
+    assert bool((p.out == 9.0).all()) and gu.error_flag() == 0
+
+
+def test_sequences_that_share_pages():
+    """The same page for several sequences, twice for one, and for the prefix too."""
+    p = Problem([40, 64, 33], 2, 4, 64, 70, 16)
+    p.table[1, :4], p.table[2, :3] = p.table[0, 0], p.prefix_pages[1]
+    p.check(p.run())
+
+
+def test_two_streams_at_once():
+    """Calls with scratch memory of their own on two streams and the current one give what they give alone."""
+    ps = [Problem([30, 0, 500], 2, 4, 128, 5000, 32), Problem([7] * 160, 4, 4, 64, 900, 16, ty="f16"), Problem([3, 90], 2, 8, 128, 300, 64)]
+    alone = [p.run().clone() for p in ps]
+    params, streams = [p.params() for p in ps], [torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.current_stream()]
+    for p in ps:
+        p.out.fill_(9.0)
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for pa, st in zip(params, streams):
+            lu.launch("prefix_attn", pa, st)
+    torch.cuda.synchronize()
+    for p, ref in zip(ps, alone):
+        assert torch.equal(p.out[:-1], ref)
+    assert gu.error_flag() == 0
+
+
 def test_a_decode_step_of_the_operators_together():
     """Dense layer in 8-bit integers -> norms, rotation and append -> attention, two steps in a row: what a layer does to serve a token.  The second step
     reads what the first appended.  Compared with the operators' formulas on each operator's own inputs, so that each error counts once."""
