@@ -522,7 +522,7 @@ int check_quantize(const pb_int8_quantize_params* p) {
     const char* who = "pb_int8_quantize";
     PB_REQUIRE(p != nullptr, "%s: NULL params", who);
     PB_REQUIRE(is_float_dtype(p->x_dtype), "%s: x_dtype %d (PB_F32, PB_BF16 or PB_F16)", who, p->x_dtype);
-    PB_REQUIRE(p->tokens >= 0 && p->channels >= 1, "%s: %d tokens of %d channels", who, p->tokens, p->channels);
+    PB_REQUIRE(p->tokens >= 0 && p->tokens <= (1 << 30) && p->channels >= 1 && p->channels <= (1 << 30), "%s: %d tokens of %d channels", who, p->tokens, p->channels);
     PB_REQUIRE(p->tokens == 0 || (p->x && p->q && p->scale), "%s: NULL buffer", who);
     PB_REQUIRE(aligned(p->x, dtype_bytes(p->x_dtype)) && aligned(p->scale, 4), "%s: a buffer is not aligned to its elements", who);
     return PB_OK;
@@ -532,7 +532,7 @@ int check_dense(const pb_int8_dense_params* p) {
     const char* who = "pb_int8_dense";
     PB_REQUIRE(p != nullptr, "%s: NULL params", who);
     PB_REQUIRE(is_float_dtype(p->y_dtype), "%s: y_dtype %d (PB_F32, PB_BF16 or PB_F16)", who, p->y_dtype);
-    PB_REQUIRE(p->tokens >= 0 && p->in_channels >= 1 && p->out_channels >= 1, "%s: %d tokens, %d -> %d channels", who, p->tokens, p->in_channels, p->out_channels);
+    PB_REQUIRE(p->tokens >= 0 && p->tokens <= (1 << 30) && p->in_channels >= 1 && p->out_channels >= 1 && p->out_channels <= (1 << 30), "%s: %d tokens, %d -> %d channels", who, p->tokens, p->in_channels, p->out_channels);
     PB_REQUIRE(p->in_channels <= 131071, "%s: %d input channels could pass 32 bits (at most 131071)", who, p->in_channels);
     PB_REQUIRE(p->act >= 0 && p->act <= 2, "%s: activation %d (0 none, 1 relu, 2 relu6)", who, p->act);
     PB_REQUIRE(p->x_stride % 16 == 0 && p->w_stride % 16 == 0, "%s: rows of x and w start on 16 bytes (strides %lld, %lld)", who, (long long)p->x_stride, (long long)p->w_stride);
@@ -575,8 +575,8 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
     double best = 1e300;
     int halves = 1;            // of 128 bytes of a row in a stage of int8_few_kernel
     // One block a tile; narrower tiles, and up to 8 blocks on a reduction, only where SMs would be idle otherwise (two blocks an SM for long reductions).
-    // Beside what an SM does: the weights from memory, at 3050 bytes a clock where every SM asks for them and 2700 otherwise, and for parts that meet 2600
-    // clocks and 70 a token.  (24 tokens, 4096 -> 14336: 112 blocks 13.6 us, 224 that share 17.9, 224 of twelve tokens 16.8; 16384 -> 14336: 112 blocks 52, 224
+    // Beside what an SM does: the weights from memory, at 22 bytes a clock for each SM that asks for them, and for parts that meet 2600 clocks and 70 a
+    // token.  (24 tokens, 4096 -> 14336: 112 blocks 13.6 us, 224 that share 17.9, 224 of twelve tokens 16.8; 16384 -> 14336: 112 blocks 52, 224
     // that share 42; 64 tokens, 1024 -> 1024: 8 blocks 4.5, 16 of half the tokens 3.6, 64 that share 5.5.)
     for (int tt = ceil_div(T, 128); tt <= ceil_div(T, 16); ++tt) {
         const int BN = round_up(ceil_div(T, tt), 16), tiles = ceil_div(T, BN), pieces = BN <= 32 ? 2 : 1, few = ceil_div(a.K, 128 * pieces);

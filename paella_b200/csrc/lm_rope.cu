@@ -510,7 +510,7 @@ int rope_plan(const pb_qk_rope_params* p, RopePlan& pl) {
     if (p->tokens > 0) {
         PB_REQUIRE(p->q_heads == 0 || (p->q && p->q_out), "%s: NULL q or q_out", who);
         PB_REQUIRE(p->kv_heads == 0 || (p->k && p->k_out), "%s: NULL k or k_out", who);
-        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->k_out, es), "%s: a buffer is not aligned to its elements", who);
+        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->k_out, es) && aligned(p->q_weight, 4) && aligned(p->k_weight, 4), "%s: a buffer is not aligned to its elements", who);
     }
     RopeArgs& a = pl.a;
     memset(&a, 0, sizeof(a));
@@ -534,7 +534,7 @@ int append_plan(const pb_kv_append_params* p, RopePlan& pl) {
     if (p->tokens > 0) {
         PB_REQUIRE(p->k && p->v && p->k_cache && p->v_cache && p->slots && aligned(p->slots, 8), "%s: NULL k, v, cache or slots", who);
         PB_REQUIRE(p->q_heads == 0 || (p->q && p->q_out), "%s: NULL q or q_out", who);
-        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->v, es) && aligned(p->k_cache, es) && aligned(p->v_cache, es), "%s: a buffer is not aligned to its elements", who);
+        PB_REQUIRE(aligned(p->q, es) && aligned(p->q_out, es) && aligned(p->k, es) && aligned(p->v, es) && aligned(p->k_cache, es) && aligned(p->v_cache, es) && aligned(p->q_weight, 4) && aligned(p->k_weight, 4), "%s: a buffer is not aligned to its elements", who);
     }
     RopeArgs& a = pl.a;
     memset(&a, 0, sizeof(a));

@@ -154,6 +154,22 @@ def test_rope_in_place_at_any_element(shift, interleaved):
     check(k, *rk, "bf16")
 
 
+@pytest.mark.parametrize("interleaved", [0, 1])
+def test_rope_of_many_tokens_in_place(interleaved):
+    """Queries and keys inside a fused projection's rows, turned where they lie; the values between them stay."""
+    g, t, d = lu.gen(11), 21000, 64
+    x = heads(g, t, 14, d, "bf16")
+    q, k, v = x[:, :9], x[:, 9:11], x[:, 11:]
+    qw, kw, tab, v0 = 1 + 0.3 * lu.randn(g, d), 1 + 0.3 * lu.randn(g, d), table(64, d), v.clone()
+    pos = torch.randint(0, 64, (t,), generator=g, device="cuda", dtype=torch.int32)
+    rq, rk = ref_heads(q, qw, tab, pos, d, interleaved), ref_heads(k, kw, tab, pos, d, interleaved)
+    lu.launch("qk_rope", rope_params("bf16", q, k, q, k, qw, kw, tab, pos, d, interleaved))
+    gu.sync()
+    check(q, *rq, "bf16")
+    check(k, *rk, "bf16")
+    assert torch.equal(v, v0)
+
+
 def test_rope_values_at_the_ends_of_the_range():
     """Zeros stay zeros, the type's largest values are normed without overflow of the mean, a NaN stays in its head."""
     d, t = 128, 4

@@ -114,3 +114,12 @@ def test_attention_struct_size_and_declared_work():
     assert lu.info("prefix_attn", attn(max_own_len=0, block_table=None, own_lens=None, max_blocks=0)).num_blocks >= 1
     L = capi.load()
     assert L.pb_prefix_attn_info(None, C.byref(li)) == -2 and L.pb_prefix_attn_launch(None, None, 0, None) == -2
+
+
+# sizes whose sums with a tile would pass 32 bits, weights between floats, a scale that is infinite in powers of two
+@pytest.mark.parametrize("name,params", [("int8_quantize", quantize(tokens=2 ** 31 - 1)), ("int8_quantize", quantize(channels=2 ** 31 - 1)), ("int8_dense", dense(tokens=2 ** 31 - 1)),
+                                         ("int8_dense", dense(out_channels=2 ** 31 - 1)), ("qk_rope", rope(q_weight=A + 2)), ("qk_rope", rope(k_weight=A + 2)),
+                                         ("kv_append", append(q_weight=A + 1)), ("kv_append", append(k_weight=A + 2)), ("prefix_attn", attn(scale=3e38)),
+                                         ("prefix_attn", attn(scale=-3e38))])
+def test_more_refusals(name, params):
+    assert lu.refused(name, params).startswith("pb_" + name)
