@@ -120,6 +120,8 @@ template <typename T> QuantizeFn quantize_fn(bool wide, bool warp) {
 // 87 to 90 %.  int8_many_kernel: a pair of SMs on a tile of 256 channels, each block with its own half of the channels and half of the tokens: 32 KB a
 // k-block and SM for 512 clocks of products, which the path from the L2 cache into an SM (some 60 bytes a clock) feeds; a lone SM on 128 x 256 would need
 // 48 KB.  8192 tokens, 8192 -> 8192: 337 us at full clocks, 3261 TOP/s, twice the measured bf16 rate to 1 %; 390 to 400 where power holds the clocks down.
+// 777 tokens, 2000 -> 5001 in fp32: 13.8 us (16.0 with one width for all tiles, 160 of them of 128 for 74 pairs): 1 for the first operands, 6 for the products, which
+// wait for the L2 cache (11 TB/s), 3 for the results of all SMs at once.
 struct DenseArgs {
     const float *x_scale, *w_scale, *bias;
     void* y;
@@ -127,6 +129,7 @@ struct DenseArgs {
     int T, K, N, act;
     int kblocks, BN, stages, splits;       // BN: tokens of a tile
     int channel_tiles, token_tiles;
+    int last, extra;                       // int8_many_kernel: tokens of the last tile, a multiple of 32; narrow tiles of a pair before all pairs take some
     int y_vec;                             // rows of y take 16-byte stores
 };
 
@@ -330,18 +333,18 @@ __device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-__device__ __forceinline__ bool all_of_128(bool ok) {
+__device__ __forceinline__ bool all_of_256(bool ok) {
     uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
     return all != 0;
 }
 
-constexpr uint32_t kOutBytes = 16 * 128 * 4;           // 32 tokens of 128 channels in 16 bits on their way out
+constexpr uint32_t kOutBytes = 2 * 16 * 128 * 4;       // twice 32 tokens of 128 channels in 16 bits on their way out
 
-// A pair of blocks walks its share of the tiles.  Warps 0-3: results, a lane a channel; warp 4: copies of this block's operands; warp 5 of the first
-// block: the products of both.  Two accumulators: the results of a tile leave under the products of the next.
+// A pair of blocks walks its share of the tiles.  Warps 0-3 and 4-7: results, a lane a channel, 32 tokens each in turn; warp 8: copies of this block's operands; warp
+// 9 of the first block: the products of both.  Two accumulators: the results of a tile leave under the products of the next.
 template <typename Y>
-__global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+__global__ void __launch_bounds__(320, 1) int8_many_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                                                            uint32_t job_id, FinishedBlockNotifier* nf) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t s_full[kMaxInt8Stages], s_empty[kMaxInt8Stages], s_sums[2], s_read[2];
@@ -350,8 +353,8 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
     __shared__ float s_xs[256];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, stage_bytes = kABytes + (uint32_t)a.BN * 64u, out = ring + a.stages * stage_bytes;
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int rank = blockIdx.x & 1, pairs = gridDim.x / 2, tiles = a.channel_tiles * a.token_tiles;
-    if (warp == 5) {
+    const int rank = blockIdx.x & 1, pairs = gridDim.x / 2;
+    if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -377,13 +380,27 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
     if (nf) nf->start(job_id);
     griddep_launch();
 
-    // Neighbouring pairs take the tokens of the same channels, then the next channels: all of them together read few rows of both operands.
-    if (warp == 4) {
+    // Neighbouring pairs take the tokens of the same channels, then the next channels: all of them together read few rows of both operands.  The narrower tiles of
+    // the last tokens come last: `extra` for each pair that has a wide tile less than others, the rest for all.
+    struct Tile { int n0, t0, width; };
+    const int wide = a.last < a.BN ? a.token_tiles - 1 : a.token_tiles, all = wide * a.channel_tiles, pair = blockIdx.x >> 1, short_of = all % pairs;
+    const auto tile_at = [&](int turn, Tile& tile) {
+        const int i = pair + turn * pairs, k = turn - (all - pair + pairs - 1) / pairs, given = a.extra * (pairs - short_of);
+        if (i < all) {
+            tile = {i / wide * 256, i % wide * a.BN, a.BN};
+            return true;
+        }
+        const int n = pair < short_of ? given + k * pairs + pair : k < a.extra ? k * (pairs - short_of) + pair - short_of : given + (k - a.extra) * pairs + pair;
+        tile = {n * 256, wide * a.BN, a.last};
+        return a.last < a.BN && n < a.channel_tiles;
+    };
+    Tile tile;
+    if (warp == 8) {
         uint32_t st = 0, parity = 1;
         int filled = 0;
         bool ok = true;
-        for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
-            const int n0 = tile / a.token_tiles * 256 + 128 * rank, t0 = tile % a.token_tiles * a.BN + (a.BN / 2) * rank;
+        for (int turn = 0; ok && tile_at(turn, tile); ++turn) {
+            const int n0 = tile.n0 + 128 * rank, t0 = tile.t0 + tile.width / 2 * rank;
             for (int i = 0; i < a.kblocks; ++i) {
                 if (filled == a.stages) {
                     ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_int8_flag, kFlagLmWait));
@@ -401,16 +418,15 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
                 if (++st == (uint32_t)a.stages) { st = 0; parity ^= 1; }
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         if (rank == 0) {
-            const uint32_t idesc = uniform(i8_idesc(256, a.BN)), step = uniform(stage_bytes >> 4), stages = uniform((uint32_t)a.stages);
+            const uint32_t step = uniform(stage_bytes >> 4), stages = uniform((uint32_t)a.stages);
             const uint64_t desc = umma_desc_sw128(uniform(ring));
             const uint32_t high = (uint32_t)(desc >> 32);
             uint32_t st = 0, parity = 0, low = (uint32_t)desc;
-            int turn = 0;
             bool ok = true;
-            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs, ++turn) {
-                const uint32_t acc = turn & 1, sums = tmem + 256 * acc;
+            for (int turn = 0; ok && tile_at(turn, tile); ++turn) {
+                const uint32_t acc = turn & 1, sums = tmem + 256 * acc, idesc = uniform(i8_idesc(256, tile.width));
                 if (turn >= 2) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_read[acc]), (uint32_t)(turn / 2 - 1) & 1, &s_abort, &g_int8_flag, kFlagLmWait));
                 if (!ok) break;
                 tcgen05_fence_after();
@@ -432,22 +448,21 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
             }
         }
     } else {
-        int turn = 0;
-        for (int tile = blockIdx.x >> 1; tile < tiles; tile += pairs, ++turn) {
-            const int acc = turn & 1, n0 = tile / a.token_tiles * 256 + 128 * rank, t0 = tile % a.token_tiles * a.BN, tokens = min(a.BN, a.T - t0);
-            const int n = n0 + 32 * warp + lane;
+        const int quarter = warp & 3, group = warp >> 2;
+        for (int turn = 0; tile_at(turn, tile); ++turn) {
+            const int acc = turn & 1, n0 = tile.n0 + 128 * rank, t0 = tile.t0, tokens = min(tile.width, a.T - t0);
+            const int n = n0 + 32 * quarter + lane;
             const float ws = n < a.N ? __ldg(a.w_scale + n) : 0.f, bias = n < a.N && a.bias ? __ldg(a.bias + n) : 0.f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");                         // the last tile's scales and values have been read
-            for (int j = threadIdx.x; j < a.BN; j += 128) s_xs[j] = j < tokens ? __ldcg(a.x_scale + t0 + j) : 0.f;
-            // (the four warps go on together or not at all: they meet at barriers)
-            if (!all_of_128(mbar_wait(smem_u32(&s_sums[acc]), (turn / 2) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) break;
+            asm volatile("bar.sync 1, 256;" ::: "memory");                         // the last tile's scales and values have been read
+            if (threadIdx.x < tokens) s_xs[threadIdx.x] = __ldcg(a.x_scale + t0 + threadIdx.x);
+            // (the eight warps go on together or not at all: they meet at barriers)
+            if (!all_of_256(mbar_wait(smem_u32(&s_sums[acc]), (turn / 2) & 1, &s_abort, &g_int8_flag, kFlagLmWait))) break;
             tcgen05_fence_after();
-            for (int j0 = 0; j0 < a.BN; j0 += 32) {
-                if (j0 >= tokens) break;
+            for (int j0 = 32 * group; j0 < tokens; j0 += 64) {
                 uint32_t v[32];
-                tcgen05_ld32(tmem + ((uint32_t)warp << 21) + 256 * acc + j0, v);
+                tcgen05_ld32(tmem + ((uint32_t)quarter << 21) + 256 * acc + j0, v);
                 tcgen05_wait_ld();
-                if (j0 + 32 >= tokens) tcgen05_fence_before();                      // the accumulator's last columns: it may be written again
+                if (j0 + 64 >= tokens) tcgen05_fence_before();                      // this warp's last columns: they may be written again
                 const int left = min(32, tokens - j0);
                 if (sizeof(Y) == 4 || !a.y_vec || n0 + 128 > a.N) {
                     // a warp's 32 channels of a token are 128 (64) bytes of a row, wherever it starts
@@ -466,25 +481,25 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
                     continue;
                 }
                 if constexpr (sizeof(Y) == 2) {        // two tokens a word in shared memory, [token / 2][channel], and out 16 bytes a thread
-                    const uint32_t me = out + (uint32_t)(32 * warp + lane) * 4u;
+                    const uint32_t mine = out + group * (kOutBytes / 2), me = mine + (uint32_t)(32 * quarter + lane) * 4u;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2)
                         asm volatile("st.shared.b32 [%0], %1;" ::"r"(me + j * 256),
                                      "r"(lm_pack2<Y>(int8_result(a.act, (int)v[j], s_xs[j0 + j] * ws, bias), int8_result(a.act, (int)v[j + 1], s_xs[j0 + j + 1] * ws, bias))) : "memory");
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
                     Y* dst = static_cast<Y*>(a.y) + (int64_t)(t0 + j0) * a.y_stride + n0;
-                    for (int i = threadIdx.x; i < 16 * 16; i += 128) {             // tokens 2 (i / 16) and + 1, channels 8 (i % 16) and up
-                        const uint4 p = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32), q = ld_shared_v4(out + (i >> 4) * 512 + (i & 15) * 32 + 16);
+                    for (int i = threadIdx.x & 127; i < 16 * 16; i += 128) {             // tokens 2 (i / 16) and + 1, channels 8 (i % 16) and up
+                        const uint4 p = ld_shared_v4(mine + (i >> 4) * 512 + (i & 15) * 32), q = ld_shared_v4(mine + (i >> 4) * 512 + (i & 15) * 32 + 16);
                         Y* at = dst + (i >> 4) * 2 * a.y_stride + (i & 15) * 8;
                         if ((i >> 4) * 2 < left)
                             *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(p.x, p.y, 0x5410), __byte_perm(p.z, p.w, 0x5410), __byte_perm(q.x, q.y, 0x5410), __byte_perm(q.z, q.w, 0x5410));
                         if ((i >> 4) * 2 + 1 < left)
                             *reinterpret_cast<uint4*>(at + a.y_stride) = make_uint4(__byte_perm(p.x, p.y, 0x7632), __byte_perm(p.z, p.w, 0x7632), __byte_perm(q.x, q.y, 0x7632), __byte_perm(q.z, q.w, 0x7632));
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory");
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");                         // all four warps have read the accumulator
+            asm volatile("bar.sync 1, 256;" ::: "memory");                         // all warps have read the accumulator
             if (threadIdx.x == 0)
                 asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_u32(&s_read[acc]), 0u)) : "memory");
         }
@@ -494,7 +509,7 @@ __global__ void __launch_bounds__(192, 1) int8_many_kernel(const __grid_constant
     if (s_abort) wait_for_copies();
     cluster_arrive();
     cluster_wait();                                    // neither block's memory goes before both have finished
-    if (warp == 5) {
+    if (warp == 9) {
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -592,9 +607,16 @@ int plan_dense(const pb_int8_dense_params* p, DensePlan& pl) {
     // pairs of SMs on 256 channels
     if (T > 64)
         for (int wide = 64; wide <= 256; wide += 32) {
-            const int tiles = ceil_div(T, wide);
-            const double clocks = std::ceil((double)ceil_div(a.N, 256) * tiles / 74) * a.kblocks * kblock_clocks(wide, wide / 2) + 2000 + 10.0 * wide;
-            if (clocks < best) { best = clocks; pl.many = true; a.BN = wide; a.token_tiles = tiles; a.splits = 1; }
+            const int tiles = ceil_div(T, wide), last = round_up(T - (tiles - 1) * wide, 32);
+            const int64_t rows = ceil_div(a.N, 256), full = rows * (last < wide ? tiles - 1 : tiles), narrow = rows * tiles - full;
+            // (as the kernel deals them out: the most have the first pair, and the first that has a wide tile less than others)
+            const double of_wide = a.kblocks * kblock_clocks(wide, wide / 2), of_narrow = a.kblocks * kblock_clocks(last, last / 2);
+            for (int extra = 0; extra <= (narrow ? 4 : 0); ++extra) {
+                const int64_t rest = std::max<int64_t>(narrow - extra * (74 - full % 74), 0);
+                const double first = ceil_div<int64_t>(full, 74) * of_wide + ceil_div<int64_t>(rest, 74) * of_narrow, other = full / 74 * of_wide + (std::min<int64_t>(extra, narrow) + ceil_div<int64_t>(rest, 74)) * of_narrow;
+                const double clocks = std::max(first, other) + 2000 + 10.0 * wide;
+                if (clocks < best) { best = clocks; pl.many = true; a.BN = wide; a.token_tiles = tiles; a.last = last; a.extra = extra; a.splits = 1; }
+            }
         }
     a.channel_tiles = ceil_div(a.N, pl.many ? 256 : 128);
     // Narrow tiles take 256 bytes of a row a stage: what a stage costs beside its copies and products, 230 clocks, comes half as often.
@@ -675,7 +697,7 @@ int pb_int8_dense_info(const pb_int8_dense_params* p, pb_launch_info* out) {
     memset(out, 0, sizeof(*out));
     const uint64_t t = (uint64_t)p->tokens, k = (uint64_t)p->in_channels, n = (uint64_t)p->out_channels;
     out->num_blocks = p->tokens > 0 ? pl.blocks : 1;
-    out->threads_per_block = 192;
+    out->threads_per_block = pl.many ? 320 : 192;
     out->smem_per_block = pl.smem;
     out->regs_per_thread = lm_regs(pl.fn);
     out->tmem_cols_per_block = pl.tmem_cols;
@@ -698,7 +720,7 @@ int pb_int8_dense_launch(const pb_int8_dense_params* p, void* stream, uint32_t j
     if (e == PB_OK) e = encode_tiled_sw128(CU_TENSOR_MAP_DATA_TYPE_UINT8, p->x, 2, xdims, &xstride, xbox, &xmap);
     if (e != PB_OK) return e;
     PB_CUDA(cudaFuncSetAttribute(pl.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxInt8Smem));      // (the same for every launch: other threads' may be on their way)
-    return lm_launch("pb_int8_dense", pl.fn, dim3(pl.blocks), dim3(192), pl.smem, (cudaStream_t)stream, pl.a.splits, pl.a, wmap, xmap, job_id, (FinishedBlockNotifier*)notifier);
+    return lm_launch("pb_int8_dense", pl.fn, dim3(pl.blocks), dim3(pl.many ? 320 : 192), pl.smem, (cudaStream_t)stream, pl.a.splits, pl.a, wmap, xmap, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 }  // extern "C"

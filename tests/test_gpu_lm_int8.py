@@ -94,6 +94,19 @@ def test_dense(ty, bias, act, gap, t, k, n):
     assert gu.error_flag() == 0
 
 
+# more tiles than pairs of SMs, and a narrower last one: pairs that have a wide tile less than others take one or more of those, then all do
+@pytest.mark.parametrize("t,k,n", [(257, 64, 20000), (519, 144, 40000), (777, 200, 5001), (777, 32, 9472), (1030, 272, 19001), (3000, 128, 2600), (333, 16, 30000), (290, 48, 37888), (1000, 96, 12345)])
+def test_dense_of_many_tiles(t, k, n):
+    g = lu.gen(t + n)
+    x, w, xs, ws = operands(g, t, k, n)
+    y = torch.full((t + 1, n), 9.0, device="cuda")
+    for _ in range(2):
+        lu.launch("int8_dense", dense_params(x, xs, w, ws, k, None, y[:t], "f32"))
+    gu.sync()
+    check_dense(y[:t], x, xs, w, ws, k, None, "f32", 0)
+    assert bool((y[t] == 9.0).all()) and gu.error_flag() == 0
+
+
 @pytest.mark.parametrize("t,k,n", [(1, 131071, 128), (40, 131071, 128), (200, 131071, 256)])
 @pytest.mark.parametrize("a,b", [(-128, -128), (-128, 127), (127, 127)])
 def test_dense_sums_reach_32_bits(t, k, n, a, b):
