@@ -122,7 +122,7 @@ __device__ __forceinline__ float values_of(const uint32_t* s, float c, float bas
 
 // ---- the prefix ----------------------------------------------------------------------------------------------
 // A block takes a range of the prefix's keys for one key head and a pair of row tiles, or, where the last row tile is alone, that tile with its
-// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warp 8 copies keys and values, warps 9 and 10
+// even and odd key tiles as a pair.  Warps 0-3 and 4-7: softmax of one of the pair each, a row a thread; warps 8 and 11 copy keys and values, warps 9 and 10
 // issue the products of one of the pair each, 64 keys at a time: S = Q K^T into 64 columns of tensor memory, where P of 16-bit pairs takes its place as the A operand
 // of O += P V, while softmax is at the other 64.  Tensor memory: S0 S1 O0 O1, all of it at 128 values a head.
 // (Scores of 128 keys at once, which cost the tensor cores 512 clocks instead of 778, leave no second place for them: a tile of the pair took 4100 clocks
@@ -134,11 +134,11 @@ template <int DP> struct PrefixShape {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(384, 1) prefix_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages + 1;
-    constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
+    constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128, kHalfTile = kTile / 2;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_q;
+    __shared__ uint64_t s_full[2 * kStages], s_empty[2 * kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_q;
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
     const int pair = blockIdx.x % a.pairs, split = (blockIdx.x / a.pairs) % a.splits, kvh = blockIdx.x / (a.pairs * a.splits);
     const int kt0 = (int)((int64_t)a.key_tiles * split / a.splits), n = (int)((int64_t)a.key_tiles * (split + 1) / a.splits) - kt0;
     const bool two = 2 * pair + 1 < a.row_tiles;      // two row tiles; otherwise one, its key tiles dealt to both softmax groups
-    const uint32_t ring = q_smem + (two ? 2 : 1) * kTile, stages = two ? kStages - 1 : kStages;      // a lone tile leaves its partner's place to the ring
+    const uint32_t ring = q_smem + (two ? 2 : 1) * kTile;                // (a lone tile leaves its partner's place to the rings)
     const int tail = min(128, a.prefix_len - (kt0 + n - 1) * 128);       // keys of the last tile
 
     if (warp == 9) {
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
     }
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < 2 * kStages; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_empty[i]), two ? 2 : 1);       // groups that use a tile
         }
@@ -179,59 +179,90 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
     griddep_wait();
     griddep_launch();          // own_kernel, which reads nothing that precedes this launch in the stream but what has ended here
 
-    if (warp == 8) {
-        // Keys and values in the order in which the products ask for them.  A lane copies a box: `box_rows` tokens of a page, 64 values of each.  Its page is
-        // looked up four copies ahead (each on its own took 1500 clocks, which was the time of a tile).
-        const int box = lane / kBlocks, blk = lane % kBlocks;
-        const auto tile_of = [&](int pos, bool& values) {
-            if (two) { values = pos & 1; return pos >> 1; }
-            values = pos == 2 * n - 1 || (pos > 0 && !(pos & 1));
-            return pos == 0 ? 0 : pos == 2 * n - 1 ? n - 1 : values ? (pos - 2) >> 1 : (pos + 1) >> 1;
+    // Keys and values come through rings.  With two row tiles: one ring of tiles of 128 keys or values, tile t's at 2 t and 2 t + 1, which both groups use.  With
+    // a lone one: a ring for each group, of halves of tiles in the order in which its products take them.  Whoever waits for an entry has used the one before it
+    // in its place (in a ring that two groups share by turns, the parity of a barrier two phases behind would let a group go on).
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &s_abort, &g_attn_flag, kFlagLmWait)); };
+    // (For two row tiles and for a lone one apart, so that strides are constants.)
+    const auto copies = [&](auto kind) __attribute__((always_inline)) {
+        constexpr bool TWO = decltype(kind)::value;
+        // With two row tiles one warp copies keys, one values, otherwise each what one group takes.  A lane copies a box: `box_rows` tokens of a page, 64 values of
+        // each.  Its page is looked up a copy ahead.  (One warp for all: 1250 clocks a copy beside the softmax warps, 2500 for a tile's keys and values, where
+        // all else takes 1650.)
+        const int box = lane / kBlocks, blk = lane % kBlocks, which = warp == 11;
+        struct Side {                                  // keys or values: the copy to come, and where it lies for this lane
+            int first, at, row, page;
         };
-        int page[4], row[4];
-        const auto look_up = [&](int pos, int& page, int& row) {
-            bool values;
-            const int key = (kt0 + tile_of(pos, values)) * 128 + box * a.box_rows;
-            if (pos < 2 * n && box * a.box_rows < 128 && key < a.prefix_len) {
-                const int at = key / a.page;
-                page = __ldcg(a.prefix_pages + at);
-                row = key - at * a.page;
-            }
+        const auto look_up = [&](Side& s, int tokens) {
+            s.page = 0;
+            if (box * a.box_rows < tokens && s.first + box * a.box_rows < a.prefix_len) s.page = __ldcg(a.prefix_pages + s.at);
         };
-#pragma unroll
-        for (int k = 0; k < 4; ++k) look_up(k, page[k], row[k]);
-        uint32_t st = 0, parity = 1;
-        bool ok = true;
-        for (int pos0 = 0; pos0 < 2 * n && ok; pos0 += 4) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int pos = pos0 + k;
-                if (pos >= 2 * n || !ok) break;
-                bool values;
-                const int left = min(128, a.prefix_len - (kt0 + tile_of(pos, values)) * 128), boxes = (left + a.box_rows - 1) / a.box_rows;
-                if (pos >= (int)stages) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[st]), parity, &s_abort, &g_attn_flag, kFlagLmWait));
-                if (!ok) break;
-                const uint32_t bar = smem_u32(&s_full[st]);
-                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
-                __syncwarp();
-                if (lane < boxes * kBlocks) {
-                    if (page[k] < 0 || page[k] >= a.n_pages) {
-                        atomicExch(&g_attn_flag, kFlagLmPage);
-                        page[k] = a.n_pages;          // outside of the map: zeros
-                    }
-                    tma_load_4d(ring + st * kTile + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, row[k], kvh, page[k], bar);
+        const auto start = [&](int first, int tokens) {
+            Side s;
+            s.first = first;
+            s.at = (first + box * a.box_rows) / a.page;
+            s.row = first + box * a.box_rows - s.at * a.page;
+            look_up(s, tokens);
+            return s;
+        };
+        // Copies `tokens` from s.first into an entry, and looks up what lies `pages` pages and `rows` rows on.
+        const auto copy = [&](Side& s, const CUtensorMap* map, int tokens, int by, int pages, int rows, int entry, uint32_t parity) {
+            const int boxes = (max(min(tokens, a.prefix_len - s.first), 0) + a.box_rows - 1) / a.box_rows;
+            if (!wait(&s_empty[entry], parity)) return false;                     // (the first time round at once)
+            const uint32_t bar = smem_u32(&s_full[entry]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
+            __syncwarp();
+            if (box < boxes) {
+                if ((uint32_t)s.page >= (uint32_t)a.n_pages) {
+                    atomicExch(&g_attn_flag, kFlagLmPage);
+                    s.page = a.n_pages;                // outside of the map: zeros
                 }
-                look_up(pos + 4, page[k], row[k]);
-                if (++st == stages) { st = 0; parity ^= 1; }
+                const uint32_t to = TWO ? ring + entry * kTile + blk * kBlock : ring + entry * kHalfTile + blk * (kBlock / 2);
+                tma_load_4d(to + box * a.box_rows * 128, map, blk * 64, s.row, kvh, s.page, bar);
+            }
+            __syncwarp();
+            s.first += by;
+            s.at += pages;
+            s.row += rows;
+            if (s.row >= a.page) { s.row -= a.page; ++s.at; }
+            look_up(s, tokens);
+            return true;
+        };
+        if constexpr (TWO) {
+            const int pages = 128 / a.page, rows = 128 % a.page;
+            Side s = start(kt0 * 128, 128);
+            uint32_t st = which, parity = 1;
+            for (int t = 0; t < n; ++t) {
+                if (!copy(s, which ? &vmap : &kmap, 128, 128, pages, rows, (int)st, parity)) break;
+                st += 2;
+                if (st >= kStages - 1) { st -= kStages - 1; parity ^= 1; }
+            }
+        } else {
+            const int mine = (n - which + 1) / 2, pages_1 = 64 / a.page, rows_1 = 64 % a.page, pages_3 = 192 / a.page, rows_3 = 192 % a.page;      // to a tile's other half, to the next tile
+            Side k = start((kt0 + which) * 128, 64), v = k;
+            uint32_t st = 0, parity = 1;
+            const auto next = [&](Side& s, const CUtensorMap* map, int h) {
+                const bool ok = copy(s, map, 64, h ? 192 : 64, h ? pages_3 : pages_1, h ? rows_3 : rows_1, which * kStages + (int)st, parity);
+                if (++st == kStages) { st = 0; parity ^= 1; }
+                return ok;
+            };
+            bool ok = mine > 0 && next(k, &kmap, 0) && next(k, &kmap, 1);
+            for (int u = 0; ok && u < mine; ++u) {
+                const bool last = u == mine - 1;
+                ok = next(v, &vmap, 0) && (last || next(k, &kmap, 0)) && next(v, &vmap, 1) && (last || next(k, &kmap, 1));
             }
         }
-    } else if (warp == 9 || warp == 10) {
+    };
+    const auto products = [&](auto kind) __attribute__((always_inline)) {
+        constexpr bool TWO = decltype(kind)::value;
         // The products of one softmax group: two warps, so that the waits of one lie under the products of the other.
         constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t idesc_s = (1u << 4) | kType | ((64u >> 3) << 17) | ((128u >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
-        // The ring's entries of key tile t and its values: 2 t and 2 t + 1 with two row tiles; otherwise keys are entries 0, 1, 3, 5 ..., values 2, 4, 6
-        // ... and the last one.
+        const int g = warp - 9, mine = TWO ? n : (n - g + 1) / 2;      // key tiles of this group: all, or g, g + 2 ...
+        const uint32_t d_s = tmem + g * 128, d_o = tmem + 256 + g * DP, block = TWO ? kBlock : kBlock / 2, entry = TWO ? kTile : kHalfTile, first = TWO ? 0 : g * kStages;
+        const uint64_t desc_q = umma_desc_sw128(q_smem + (TWO ? g * kTile : 0)), desc_k = umma_desc_sw128(ring + first * entry), desc_v = umma_desc_sw128_mn(ring + first * entry, block);
+        const uint32_t high_k = (uint32_t)(desc_k >> 32), high_v = (uint32_t)(desc_v >> 32), low_q = (uint32_t)desc_q;
         struct Place {
             uint32_t st, parity;
             __device__ __forceinline__ void on(uint32_t by, uint32_t stages) {
@@ -239,82 +270,89 @@ __global__ void __launch_bounds__(352, 1) prefix_kernel(const __grid_constant__ 
                 if (st >= stages) { st -= stages; parity ^= 1; }
             }
         };
-        const int g = warp - 9, mine = two ? n : (n - g + 1) / 2;      // key tiles of this group: g, g + 2 ... or all
-        Place keys = {two ? 0u : (uint32_t)g, 0}, values = {two ? 1u : g == n - 1 ? 2u * n - 1u : 2u * g + 2u, 0};
-        const uint32_t d_s = tmem + g * 128, d_o = tmem + 256 + g * DP;
-        const uint64_t desc_q = umma_desc_sw128(q_smem + (two ? g * kTile : 0)), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
-        const uint32_t high_k = (uint32_t)(desc_k >> 32), high_v = (uint32_t)(desc_v >> 32), low_q = (uint32_t)desc_q;
-        const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &s_abort, &g_attn_flag, kFlagLmWait)); };
+        Place keys = {0, 0}, values = {1, 0};          // (with a lone row tile `keys` alone, for both)
         // With two row tiles the groups take turns at the tensor cores, a half's values and the next scores in its place at a time: one's softmax then lies under
         // the other's products.  (Left alone they fall into step: products of both mixed, then softmax of both.)  The turn goes on with half of the scores still
         // to be issued, so that the other warp has seen it when they have been.
         uint32_t turn = 0;
         const auto take_turn = [&]() {
-            if (!two) return true;
+            if (!TWO) return true;
             const bool now = wait(&s_turn[g], turn);
             turn ^= 1;
             return now;
         };
         // Scores of 64 keys, the first or second half of a tile, into their own 64 columns.
-        const auto scores = [&](int u, uint32_t h) {
-            if (h == 0 && !wait(&s_full[keys.st], keys.parity)) return false;
+        const auto scores = [&](uint32_t h) {
+            if ((h == 0 || !TWO) && !wait(&s_full[first + keys.st], keys.parity)) return false;
             tcgen05_fence_after();
-            const uint32_t low = (uint32_t)desc_k + keys.st * (kTile >> 4) + h * (8192 >> 4);
+            const uint32_t low = (uint32_t)desc_k + keys.st * (entry >> 4) + (TWO ? h * (8192 >> 4) : 0);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
-                    if (two && k == DP / 32) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
-                    const uint32_t at = (k >> 2) * (kBlock >> 4) + (k & 3) * 2;
-                    tcgen05_mma_bf16(d_s + h * 64, pack_f32x2(low_q + at, high_k), pack_f32x2(low + at, high_k), idesc_s, k > 0);
+                    if (TWO && k == DP / 32) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
+                    tcgen05_mma_bf16(d_s + h * 64, pack_f32x2(low_q + (k >> 2) * (kBlock >> 4) + (k & 3) * 2, high_k), pack_f32x2(low + (k >> 2) * (block >> 4) + (k & 3) * 2, high_k), idesc_s, k > 0);
                 }
                 tcgen05_commit(smem_u32(&s_scores[g][h]));
-                if (h == 1) tcgen05_commit(smem_u32(&s_empty[keys.st]));
+                if (h == 1 || !TWO) tcgen05_commit(smem_u32(&s_empty[first + keys.st]));
             }
             __syncwarp();
-            if (h == 1) keys.on(two ? 2 : u == 0 && g == 0 ? 3 : 4, stages);
+            if (!TWO) keys.on(1, kStages);
+            else if (h == 1) keys.on(2, kStages - 1);
             return true;
         };
         bool ok = wait(&s_q, 0);
         if (ok && g == 1) ok = take_turn();
-        if (ok && mine > 0) ok = scores(0, 0);
+        if (ok && mine > 0) ok = scores(0);
         if (ok) ok = take_turn();
-        if (ok && mine > 0) ok = scores(0, 1);
+        if (ok && mine > 0) ok = scores(1);
         for (int u = 0; ok && u < mine; ++u) {
-            const bool last = u == mine - 1;
-            ok = wait(&s_full[values.st], values.parity);
-            if (!ok) break;
-            if ((two ? u : g + 2 * u) == n - 1 && tail < 128) {
-                // Rows behind the prefix's last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.  (With two row tiles
-                // both warps write these zeros before they use them.)
-                const uint32_t v_smem = ring + values.st * kTile;
-                for (int c = lane; c < (128 - tail) * 8 * kBlocks; c += 32) {
-                    const int blk = c / ((128 - tail) * 8), at = c % ((128 - tail) * 8);
-                    st_shared_v4(v_smem + blk * kBlock + tail * 128 + at * 16, 0, 0, 0, 0);
-                }
-                fence_proxy_async();
-                __syncwarp();
-            }
-            const uint32_t low = (uint32_t)desc_v + values.st * (kTile >> 4), more = u > 0;
+            const bool last = u == mine - 1, cut = (TWO ? u : g + 2 * u) == n - 1 && tail < 128;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
+                Place& at = TWO ? values : keys;
+                if (h == 0 || !TWO) {
+                    ok = wait(&s_full[first + at.st], at.parity);
+                    if (!ok) break;
+                    if (cut) {
+                        // Rows behind the prefix's last token: their P is zero, and so is what they hold, which nobody wrote or which may be NaNs.  (With two row
+                        // tiles both warps write these zeros before they use them.)
+                        const uint32_t v_smem = ring + (first + at.st) * entry;
+                        const int all = TWO ? 128 : 64, live = TWO ? tail : min(max(tail - 64 * (int)h, 0), 64);
+                        for (int c = lane; c < (all - live) * 8 * kBlocks; c += 32) {
+                            const int blk = c / ((all - live) * 8), piece = c % ((all - live) * 8);
+                            st_shared_v4(v_smem + blk * block + live * 128 + piece * 16, 0, 0, 0, 0);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                }
                 ok = wait(&s_probs[g][h], (uint32_t)u & 1) && take_turn();
                 if (!ok) break;
                 tcgen05_fence_after();
+                const uint32_t low = (uint32_t)desc_v + at.st * (entry >> 4) + (TWO ? h * (8192 >> 4) : 0), more = u > 0;
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tcgen05_mma_f16_ts(d_o, d_s + h * 64 + k * 8, pack_f32x2(low + (4 * h + k) * (2048 >> 4), high_v), idesc_o, more | (uint32_t)(h > 0 || k > 0));
-                    if (h == 1) tcgen05_commit(smem_u32(&s_empty[values.st]));
+                        tcgen05_mma_f16_ts(d_o, d_s + h * 64 + k * 8, pack_f32x2(low + k * (2048 >> 4), high_v), idesc_o, more | (uint32_t)(h > 0 || k > 0));
+                    if (h == 1 || !TWO) tcgen05_commit(smem_u32(&s_empty[first + at.st]));
                     if (last) tcgen05_commit(smem_u32(h == 0 ? &s_half[g] : &s_done[g]));
                 }
                 __syncwarp();
-                if (!last) ok = scores(u + 1, h);
-                else if (two && elect_one()) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
+                if (!TWO) keys.on(1, kStages);
+                if (!last) ok = scores(h);
+                else if (TWO && elect_one()) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
                 __syncwarp();
                 if (!ok) break;
             }
-            values.on(two ? 2 : g + (u + 1) * 2 == n - 1 ? 3 : 4, stages);
+            if (TWO) values.on(2, kStages - 1);
         }
+    };
+    if (warp == 8 || warp == 11) {
+        if (two) copies(std::true_type());
+        else copies(std::false_type());
+    } else if (warp == 9 || warp == 10) {
+        if (two) products(std::true_type());
+        else products(std::false_type());
     } else if (warp < 8) {
         const int g = warp >> 2, in_tile = (warp & 3) * 32 + lane, rows = a.batch * a.group;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                       // this warp's lanes of tensor memory
@@ -905,7 +943,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     a.pairs = ceil_div(a.row_tiles, 2);
     a.key_tiles = ceil_div(a.prefix_len, 128);
     a.box_rows = 8;
-    while (a.box_rows < 128 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
+    while (a.box_rows < 64 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
     // Own tokens: enough blocks of a cluster on a sequence and key head to use the GPU, no more than fit it at once, 128 tokens each at least.
     a.row_groups = ceil_div(a.group, 8 * pl.NT);
     const int64_t own_units = (int64_t)a.batch * a.kv_heads * a.row_groups;
@@ -946,7 +984,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
 template <typename T, int DP>
 int launch_prefix(const AttnPlan& pl, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
     PB_CUDA(cudaFuncSetAttribute(prefix_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrefixShape<DP>::smem));
-    return lm_launch("pb_prefix_attn (prefix)", prefix_kernel<T, DP>, dim3((unsigned)pl.prefix_blocks), dim3(352), PrefixShape<DP>::smem, st, 1, pl.a, km, vm);
+    return lm_launch("pb_prefix_attn (prefix)", prefix_kernel<T, DP>, dim3((unsigned)pl.prefix_blocks), dim3(384), PrefixShape<DP>::smem, st, 1, pl.a, km, vm);
 }
 
 }  // namespace

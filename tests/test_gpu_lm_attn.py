@@ -272,6 +272,19 @@ def test_two_streams_at_once():
     assert gu.error_flag() == 0
 
 
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_long_prefix_of_one_row_tile(page):
+    """Many tiles through the rings of a block whose groups take every other tile; the same bits each time."""
+    p = Problem([1] * 16, 2, 8, 128, 70001, page)
+    first = p.run().clone()
+    p.check(first, only=(0, 15))
+    params = p.params()
+    for _ in range(40):
+        lu.launch("prefix_attn", params)
+    gu.sync()
+    assert torch.equal(p.out[:-1], first) and gu.error_flag() == 0
+
+
 def test_a_decode_step_of_the_operators_together():
     """Dense layer in 8-bit integers -> norms, rotation and append -> attention, two steps in a row: what a layer does to serve a token.  The second step
     reads what the first appended.  Compared with the operators' formulas on each operator's own inputs, so that each error counts once."""
