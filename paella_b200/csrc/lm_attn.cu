@@ -9,9 +9,9 @@
 // sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.  The softmax's values are rounded to the cache's type, as the tensor cores take them; the sums l are of what they
 // were before.
 //
-// What bounds it: few rows, the cache's bytes (16 sequences of 8 heads a key head behind 130001 tokens, 556 MB: 104 to 108 us, 5.2 TB/s); many, the tensor cores
-// and the exponentials together (2048 rows a key head behind 16384 tokens: the tensor pipe is busy 71 % of the time on the SMs that take part).  256
-// sequences of 8 heads a key head behind 16384 tokens with up to 1024 of their own: 200 to 206 us.
+// What bounds it: few rows, the cache's bytes (16 sequences of 8 heads a key head behind 130001 tokens, 556 MB: 99 to 102 us, 5.5 TB/s); many, the tensor cores
+// and the exponentials together (2048 rows a key head behind 16384 tokens: the tensor pipe is busy 71 % of the time on the SMs that take part, 139 us cool and up to 160 where power holds the clocks down).  256
+// sequences of 8 heads a key head behind 16384 tokens with up to 1024 of their own: 200 to 224 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(384, 1) prefix_kernel(const __grid_constant__ 
     constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128, kHalfTile = kTile / 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t s_full[2 * kStages], s_empty[2 * kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_q;
+    __shared__ int s_pages[2][4][32];
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -187,71 +188,72 @@ __global__ void __launch_bounds__(384, 1) prefix_kernel(const __grid_constant__ 
     const auto copies = [&](auto kind) __attribute__((always_inline)) {
         constexpr bool TWO = decltype(kind)::value;
         // With two row tiles one warp copies keys, one values, otherwise each what one group takes.  A lane copies a box: `box_rows` tokens of a page, 64 values of
-        // each.  Its page is looked up a copy ahead.  (One warp for all: 1250 clocks a copy beside the softmax warps, 2500 for a tile's keys and values, where
-        // all else takes 1650.)
-        const int box = lane / kBlocks, blk = lane % kBlocks, which = warp == 11;
-        struct Side {                                  // keys or values: the copy to come, and where it lies for this lane
-            int first, at, row, page;
+        // each.  Its pages are looked up two copies ahead, by asynchronous copies into its own words: a load into a register is waited for as soon as the
+        // register is moved, 1300 clocks a copy.  (One warp for all: 2500 clocks for a tile's keys and values, where all else takes 1650.)  Rolled up: what runs
+        // once comes from memory, too, and cost a short prefix 4 us.
+        constexpr int tokens = TWO ? 128 : 64, kAhead = 2;                        // of a copy
+        const int box = lane / kBlocks, blk = lane % kBlocks, which = warp == 11, mine = TWO ? n : 2 * ((n - which + 1) / 2);
+        const int pages_1 = tokens / a.page, rows_1 = tokens % a.page, pages_3 = 192 / a.page, rows_3 = 192 % a.page;
+        struct Where {                                 // a copy's first token, and where it lies for this lane
+            int first, at, row;
         };
-        const auto look_up = [&](Side& s, int tokens) {
-            s.page = 0;
-            if (box * a.box_rows < tokens && s.first + box * a.box_rows < a.prefix_len) s.page = __ldcg(a.prefix_pages + s.at);
+        const auto advance = [&](Where& w, int i) {    // from copy i: the halves of a tile are neighbours, the group's tiles are not
+            const bool far = !TWO && (i & 1);
+            w.first += far ? 192 : tokens;
+            w.at += far ? pages_3 : pages_1;
+            w.row += far ? rows_3 : rows_1;
+            if (w.row >= a.page) { w.row -= a.page; ++w.at; }
         };
-        const auto start = [&](int first, int tokens) {
-            Side s;
-            s.first = first;
-            s.at = (first + box * a.box_rows) / a.page;
-            s.row = first + box * a.box_rows - s.at * a.page;
-            look_up(s, tokens);
-            return s;
+        const uint32_t words = smem_u32(&s_pages[which][0][lane]);
+        Where ahead = {(TWO ? kt0 : kt0 + which) * 128, 0, 0};
+        ahead.at = (ahead.first + box * a.box_rows) / a.page;
+        ahead.row = ahead.first + box * a.box_rows - ahead.at * a.page;
+        Where keys = ahead, values = ahead;
+        const auto look_up = [&](int i) {
+            if (i < mine && box * a.box_rows < tokens && ahead.first + box * a.box_rows < a.prefix_len)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + (i & 3) * 128), "l"(a.prefix_pages + ahead.at) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            advance(ahead, i);
         };
-        // Copies `tokens` from s.first into an entry, and looks up what lies `pages` pages and `rows` rows on.
-        const auto copy = [&](Side& s, const CUtensorMap* map, int tokens, int by, int pages, int rows, int entry, uint32_t parity) {
-            const int boxes = (max(min(tokens, a.prefix_len - s.first), 0) + a.box_rows - 1) / a.box_rows;
+        uint32_t st = TWO ? which : 0, parity = 1;
+        const auto copy = [&](const Where& w, int i, const CUtensorMap* map) {
+            const int boxes = (max(min(tokens, a.prefix_len - w.first), 0) + a.box_rows - 1) / a.box_rows, entry = TWO ? (int)st : which * kStages + (int)st;
             if (!wait(&s_empty[entry], parity)) return false;                     // (the first time round at once)
             const uint32_t bar = smem_u32(&s_full[entry]);
             if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
             __syncwarp();
             if (box < boxes) {
-                if ((uint32_t)s.page >= (uint32_t)a.n_pages) {
+                int page;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(page) : "r"(words + (i & 3) * 128) : "memory");
+                if ((uint32_t)page >= (uint32_t)a.n_pages) {
                     atomicExch(&g_attn_flag, kFlagLmPage);
-                    s.page = a.n_pages;                // outside of the map: zeros
+                    page = a.n_pages;                  // outside of the map: zeros
                 }
                 const uint32_t to = TWO ? ring + entry * kTile + blk * kBlock : ring + entry * kHalfTile + blk * (kBlock / 2);
-                tma_load_4d(to + box * a.box_rows * 128, map, blk * 64, s.row, kvh, s.page, bar);
+                tma_load_4d(to + box * a.box_rows * 128, map, blk * 64, w.row, kvh, page, bar);
             }
             __syncwarp();
-            s.first += by;
-            s.at += pages;
-            s.row += rows;
-            if (s.row >= a.page) { s.row -= a.page; ++s.at; }
-            look_up(s, tokens);
+            st += TWO ? 2 : 1;
+            if (st >= (TWO ? kStages - 1 : kStages)) { st -= TWO ? kStages - 1 : kStages; parity ^= 1; }
             return true;
         };
-        if constexpr (TWO) {
-            const int pages = 128 / a.page, rows = 128 % a.page;
-            Side s = start(kt0 * 128, 128);
-            uint32_t st = which, parity = 1;
-            for (int t = 0; t < n; ++t) {
-                if (!copy(s, which ? &vmap : &kmap, 128, 128, pages, rows, (int)st, parity)) break;
-                st += 2;
-                if (st >= kStages - 1) { st -= kStages - 1; parity ^= 1; }
+#pragma unroll 1
+        for (int i = 0; i < kAhead; ++i) look_up(i);
+        bool ok = true;
+#pragma unroll 1
+        for (int i = 0; ok && i < mine + (TWO || !mine ? 0 : 2); ++i) {            // keys i and values i - 2 of a group; the one or the other
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+            if (!TWO && i >= 2) {
+                ok = copy(values, i - 2, &vmap);
+                advance(values, i - 2);
             }
-        } else {
-            const int mine = (n - which + 1) / 2, pages_1 = 64 / a.page, rows_1 = 64 % a.page, pages_3 = 192 / a.page, rows_3 = 192 % a.page;      // to a tile's other half, to the next tile
-            Side k = start((kt0 + which) * 128, 64), v = k;
-            uint32_t st = 0, parity = 1;
-            const auto next = [&](Side& s, const CUtensorMap* map, int h) {
-                const bool ok = copy(s, map, 64, h ? 192 : 64, h ? pages_3 : pages_1, h ? rows_3 : rows_1, which * kStages + (int)st, parity);
-                if (++st == kStages) { st = 0; parity ^= 1; }
-                return ok;
-            };
-            bool ok = mine > 0 && next(k, &kmap, 0) && next(k, &kmap, 1);
-            for (int u = 0; ok && u < mine; ++u) {
-                const bool last = u == mine - 1;
-                ok = next(v, &vmap, 0) && (last || next(k, &kmap, 0)) && next(v, &vmap, 1) && (last || next(k, &kmap, 1));
+            if (ok && i < mine) {
+                ok = copy(keys, i, TWO && which ? &vmap : &kmap);
+                advance(keys, i);
             }
+            look_up(i + kAhead);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     };
     const auto products = [&](auto kind) __attribute__((always_inline)) {
         constexpr bool TWO = decltype(kind)::value;
@@ -359,28 +361,29 @@ __global__ void __launch_bounds__(384, 1) prefix_kernel(const __grid_constant__ 
         const int row = (2 * pair + (two ? g : 0)) * 128 + in_tile;
         const bool live_warp = row - lane < rows;
         if (two || g == 0) {
-            // 16 bytes at a time, neighbouring lanes on neighbouring bytes of a row; |scale| from here on
-            constexpr int kPerRow = DP / 8, kMine = kPerRow;
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-            const int row0 = row - in_tile, thread = threadIdx.x & 127;
-            constexpr int kStep = 128 / kPerRow;                                 // rows from one of a thread's pieces to the next
-            uint4 v[kMine];
-            int r = row0 + thread / kPerRow, b = r / a.group, h = r - b * a.group;   // (quotients in the loop took 2 us)
-            const int b_step = kStep / a.group, h_step = kStep - b_step * a.group, c = thread % kPerRow;
-            const T* src = static_cast<const T*>(a.q) + (int64_t)kvh * a.group * a.q_head + 8 * c;
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (r < rows && 8 * c < a.D) v[i] = __ldcg(reinterpret_cast<const uint4*>(src + b * a.q_stride + h * a.q_head));
+            // neighbouring lanes on neighbouring bytes of a row
+            constexpr int kPerRow = DP / 8, kStep = 128 / kPerRow;               // 16-byte pieces of a row; rows from one of a thread's pieces to the next
+            const int thread = threadIdx.x & 127, c = thread % kPerRow, r0 = thread / kPerRow, b_step = kStep / a.group, h_step = kStep - b_step * a.group;
+            const uint32_t mine = q_smem + g * kTile + (c >> 3) * kBlock + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4);
+            int r = row - in_tile + r0, h = r % a.group;                          // (quotients in the loop took 2 us)
+            const int64_t step = b_step * a.q_stride + h_step * a.q_head, wrap = a.q_stride - a.group * a.q_head;
+            const T* src = static_cast<const T*>(a.q) + r / a.group * a.q_stride + ((int64_t)kvh * a.group + h) * a.q_head + 8 * c;
+#pragma unroll 2
+            for (int i = 0; i < kPerRow; ++i) {
+                const bool there = r < rows && 8 * c < a.D;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine + i * (kStep * 128)), "l"(there ? src : static_cast<const T*>(a.q)), "r"(there ? 16 : 0) : "memory");
                 r += kStep;
-                b += b_step;
                 h += h_step;
-                if (h >= a.group) { h -= a.group; ++b; }
+                src += step;
+                if (h >= a.group) { h -= a.group; src += wrap; }
             }
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                const int r = (i * 128 + thread) / kPerRow;
-                st_shared_v4(q_smem + g * kTile + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (a.scale < 0.f) {                                                 // |scale| from here on
+#pragma unroll 1
+                for (int i = 0; i < kPerRow; ++i) {
+                    const uint4 v = ld_shared_v4(mine + i * (kStep * 128));
+                    st_shared_v4(mine + i * (kStep * 128), v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                }
             }
         }
         fence_proxy_async();
