@@ -957,8 +957,8 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
         return ranks;
     };
     // A short prefix is taken as if it were each sequence's own, where that costs little: a block's tokens come at some 70 bytes a nanosecond, those of all
-    // blocks from the L2 cache at 9 KB.  (8 key heads of 128, with the own kernel alone / with both: one sequence behind 512, 4096, 8192 tokens 6.8 / 9.6 us,
-    // 10.3 / 12.6, 16.1 / 15.5; 8 behind 256 and 1024 6.9 / 9.3, 10.8 / 9.2; 32 behind 256 and 512 10.2 / 10.4, 13.4 / 11.0.)
+    // blocks from the L2 cache at 9 KB.  (8 key heads of 128, with the own kernel alone / with both: one sequence behind 512, 4096, 8192 tokens 6.8 / 9.5 us,
+    // 10.3 / 11.4, 16.1 / 14.7; 8 behind 256 and 1024 6.9 / 9.1, 10.8 / 9.2; 32 behind 256 and 512 10.2 / 10.0, 13.4 / 10.7.)
     const int64_t tokens = (int64_t)a.prefix_len + a.max_own;
     const double bytes = 4.0 * a.D * a.prefix_len, block_us = bytes / ranks_of(tokens) / 70e3, all_us = bytes * own_units / 9e6;
     const char* force = getenv("PB_ATTN_PREFIX");          // 1 = prefix_kernel wherever there is a prefix, 0 = never; by rule otherwise
