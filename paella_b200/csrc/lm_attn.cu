@@ -63,7 +63,8 @@ __device__ __forceinline__ bool all_of_256(bool ok) {
 
 // 2^x of a pair on the multipliers, beside ex2 on the special-function unit, which alone would take as long as the products: x = i + f with |f| <= 1/2
 // (the sum with 1.5 x 2^23 rounds to a whole number), 2^f as the polynomial of degree 5 with the least largest relative error (Remez's exchange;
-// 2^-23.7, 2^-22.2 with fp32's roundings), i added to its exponent.  Below 2^-126: nothing.  For x < 127; a NaN stays one.
+// 2^-23.7, 2^-22.2 with fp32's roundings), i added to its exponent.  Up to 2^-126: nothing.  For x < 127; a NaN stays one: the
+// exponent's sum makes a finite number of it, so x comes into the last sum once more.
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     const auto both = [](float v) { return pack_f32x2(__float_as_uint(v), __float_as_uint(v)); };
     float lo, hi;
@@ -78,7 +79,7 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     r = fma_f32x2(r, f, both(0.6931469440460205f));
     r = fma_f32x2(r, f, both(1.0000001192092896f));
     r = pack_f32x2((uint32_t)r + ((uint32_t)t << 23), (uint32_t)(r >> 32) + ((uint32_t)(t >> 32) << 23));
-    return add_f32x2(r, both(-0x1p-126f));
+    return add_f32x2(r, fma_f32x2(x, both(0.f), both(-0x1.000002p-126f)));
 }
 
 __device__ __forceinline__ float max3(float x, float y, float z) {        // (NaNs lose, as in fmaxf)
