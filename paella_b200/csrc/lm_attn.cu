@@ -63,7 +63,7 @@ __device__ __forceinline__ bool all_of_256(bool ok) {
 
 // 2^x of a pair on the multipliers, beside ex2 on the special-function unit, which alone would take as long as the products: x = i + f with |f| <= 1/2
 // (the sum with 1.5 x 2^23 rounds to a whole number), 2^f as the polynomial of degree 5 with the least largest relative error (Remez's exchange;
-// 2^-23.7, 2^-22.2 with fp32's roundings), i added to its exponent.  Up to 2^-126: nothing.  For x < 127; a NaN stays one: the
+// 2^-22.6 with the coefficients in fp32, 2^-22.1 with fp32's roundings), i added to its exponent.  Up to 2^-126: nothing.  For x < 127; a NaN stays one: the
 // exponent's sum makes a finite number of it, so x comes into the last sum once more.
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     const auto both = [](float v) { return pack_f32x2(__float_as_uint(v), __float_as_uint(v)); };
