@@ -40,6 +40,7 @@ struct AttnArgs {
     float2* part_ml;           // the same without DP: (m, l)
     // own tokens
     int kv_heads, row_groups, ranks, early, out_vec;     // early: behind a prefix_kernel, beside whose end it starts
+    uint32_t per_piece;        // 2^16 / (D / 4), rounded up
     int ahead;                 // tokens of the prefix that own_kernel takes as if they were each sequence's own: all of them, or none
 };
 
@@ -768,7 +769,9 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         const int flat = b * a.group + row0 + row;
         return (((int64_t)(flat >> 7) * a.kv_heads + kvh) * a.row_parts << 7) + (flat & 127);
     };
-    constexpr int kPieces = DP / 4;
+    constexpr int kPieces = DP / 4;                                       // 16-byte pieces of a row as it lies,
+    const int pieces = a.D / 4;                                           // those that hold values
+    const auto row_of = [&](int item) { return (int)((uint32_t)item * a.per_piece >> 16); };       // item / pieces, exact below 2048
     if constexpr (PHASE != 2) {
         __syncthreads();                                                  // the rings become the warps' parts
         // this warp's part: (m, l) and O of its rows, values 64 i + 8 g + 2 e and + 1
@@ -791,8 +794,8 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     if constexpr (PHASE == 1) {
         __syncthreads();
         // the four warps' parts as one (a block has the sequence to itself here)
-        for (int item = threadIdx.x; item < rows * kPieces; item += 128) {
-            const int row = item / kPieces, i4 = item % kPieces;
+        for (int item = threadIdx.x; item < rows * pieces; item += 128) {
+            const int row = row_of(item), i4 = item - row * pieces;
             float top = -INFINITY, sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -849,14 +852,14 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;
     }
     __syncthreads();
-    const int items = rows * kPieces;
+    const int items = rows * pieces;
     int lanes = 1;
     while (lanes < 32 && items * lanes * 2 <= 128 * a.ranks) lanes *= 2;
     const int sub = threadIdx.x & (lanes - 1);
     for (int base = 0; base < items; base += 128 * a.ranks / lanes) {
         const int item = base + (rank * 128 + threadIdx.x) / lanes;
         const bool real = item < items;
-        const int row = real ? item / kPieces : 0, i4 = item % kPieces;
+        const int row = real ? row_of(item) : 0, i4 = real ? item - row * pieces : 0;
         const int64_t at = first_part(row);
         const float4* src = reinterpret_cast<const float4*>(a.part_o + at * DP) + (i4 ^ ((int)at & 31 & (kPieces - 1)));
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -880,7 +883,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             acc.x += __shfl_xor_sync(0xffffffffu, acc.x, k); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, k);
             acc.z += __shfl_xor_sync(0xffffffffu, acc.z, k); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, k);
         }
-        if (!real || sub != 0 || 4 * i4 >= a.D) continue;
+        if (!real || sub != 0) continue;
         T* dst = static_cast<T*>(a.out) + b * a.out_stride + (int64_t)(kvh * a.group + row0 + row) * a.out_head + 4 * i4;
         if (a.out_vec) {
             *reinterpret_cast<uint2*>(dst) = make_uint2(lm_pack2<T>(acc.x, acc.y), lm_pack2<T>(acc.z, acc.w));
@@ -888,7 +891,8 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             dst[0] = lm_from_f<T>(acc.x); dst[1] = lm_from_f<T>(acc.y); dst[2] = lm_from_f<T>(acc.z); dst[3] = lm_from_f<T>(acc.w);
         }
     }
-    if (a.ranks > 1) { cluster_arrive_relaxed(); cluster_wait(); }        // the others have read this block's part
+    // The others have read this block's part.  (Whatever a lane has loaded of theirs has gone into a shuffle or a store in front of its arrival: nothing is left to order.)
+    if (a.ranks > 1) { cluster_arrive_relaxed(); cluster_wait(); }
     if (nf) nf->end(job_id);
 }
 
@@ -936,6 +940,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     a.page_stride = p->page_stride; a.token_stride = p->token_stride; a.head_stride = p->head_stride; a.table_stride = p->table_stride;
     a.batch = p->batch; a.group = p->q_heads / p->kv_heads; a.D = p->head_dim; a.page = p->page_size; a.n_pages = (int)p->n_pages; a.prefix_len = p->prefix_len;
     a.max_own = p->max_own_len; a.scale = p->scale; a.kv_heads = p->kv_heads;
+    a.per_piece = (uint32_t)ceil_div(1 << 16, p->head_dim / 4);
     pl.DP = p->head_dim <= 64 ? 64 : 128;
     pl.NT = a.group <= 8 ? 1 : 2;
     pl.half = p->dtype == PB_F16;
