@@ -567,7 +567,7 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
 }
 
 // A block (or a cluster of `ranks` blocks, each a range of the tokens) takes 8 NT query rows of one sequence and key head.  A warp takes 16 tokens at a
-// time, copied into a ring of its own two to four chunks ahead: 12 warps of an SM have 96 to 192 KB on the way.  (In registers, a chunk ahead, it was some 60: 537 MB
+// time, copied into a ring of its own two to four chunks ahead: 12 warps of an SM (8 for more than 8 rows) have 96 to 192 KB (64 to 128) on the way.  (In registers, a chunk ahead, it was some 60: 537 MB
 // of own tokens took 141 us instead of 88 to 98.)  The order of a head's values within a product's 16 is free as long as both operands have the
 // same, and so is the order of O's rows, hence each lane reads 16 bytes as they lie:
 //   S^T[token][row] = K Q^T:  lane (g, c) = (lane / 4, lane % 4) holds 8 values at 8 c of every 32 of tokens g and g + 8
@@ -579,7 +579,7 @@ template <int DP> struct OwnShape {
     static constexpr int stages = DP == 128 ? 2 : 4;
     static constexpr uint32_t smem = 4 * stages * 2 * half;
 };
-// Phase 0 does all of it.  Where there are more blocks than fit the GPU at once, beside a prefix_kernel, phase 1 leaves its part to phase 2, a launch of its
+// Phase 0 does all of it.  Where there are more than three blocks an SM, beside a prefix_kernel, phase 1 leaves its part to phase 2, a launch of its
 // own: its blocks then go on while the prefix is worked on, on the SMs that are left over and on those that become free, where blocks that wait for
 // the prefix's parts would hold them (220 -> 200 us).
 template <typename T, int DP, int NT, int PHASE>
@@ -953,13 +953,17 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     a.key_tiles = ceil_div(a.prefix_len, 128);
     a.box_rows = 8;
     while (a.box_rows < 64 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
-    // Own tokens: enough blocks of a cluster on a sequence and key head to use the GPU, no more than fit it at once, 128 tokens each at least.
+    // Own tokens: enough blocks of a cluster on a sequence and key head to use the GPU, 128 tokens each at least, and no more than three an SM.  Those fit it at once for
+    // groups of up to 8 query heads; larger groups' blocks (79 KB) fit it two at a time, but halving their number there costs more often than it gains, since lengths differ and
+    // shorter ranges even them out.  (16 heads a key head, lengths from 0 to the most, at most three / two an SM: 20 sequences of up to 2048 29.5 / 34.9 us, 25 of 4096
+    // 53.9 / 61.3, 12 of 4096 35.8 / 37.4, 6 of 4096 28.7 / 24.1; behind 8192 tokens, where the number also decides whether the parts are joined apart: 20 of 2048 53.9 / 57.9, 40 of 512
+    // 58.0 / 58.8, 52 of 1024 80.5 / 78.3, and of 32 heads a key head 40 of 512 57.4 / 50.0.)
     a.row_groups = ceil_div(a.group, 8 * pl.NT);
     const int64_t own_units = (int64_t)a.batch * a.kv_heads * a.row_groups;
-    constexpr int kAtOnce = 3 * 148;
+    constexpr int kMaxOwnBlocks = 3 * 148;
     const auto ranks_of = [&](int64_t tokens) {
         int ranks = 1;
-        while (ranks < kMaxRanks && own_units * ranks * 2 <= kAtOnce && tokens / (2 * ranks) >= 128) ranks *= 2;
+        while (ranks < kMaxRanks && own_units * ranks * 2 <= kMaxOwnBlocks && tokens / (2 * ranks) >= 128) ranks *= 2;
         return ranks;
     };
     // A short prefix is taken as if it were each sequence's own, where that costs little: a block's tokens come at some 70 bytes a nanosecond, those of all
@@ -977,7 +981,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     if (units > 0 && units < kMaxSplits) a.splits = (int)(kMaxSplits / units);
     if (a.splits > a.key_tiles) a.splits = a.key_tiles > 0 ? a.key_tiles : 1;
     pl.prefix_blocks = a.early ? units * a.splits : 0;
-    const bool apart = a.early && own_units > kAtOnce && a.max_own > 0;
+    const bool apart = a.early && own_units > kMaxOwnBlocks && a.max_own > 0;
     a.row_parts = a.splits + (apart ? 1 : 0);
     pl.own = pl.half ? (apart ? own_fn<__half, 1> : own_fn<__half, 0>)(pl.DP, pl.NT) : (apart ? own_fn<__nv_bfloat16, 1> : own_fn<__nv_bfloat16, 0>)(pl.DP, pl.NT);
     pl.join = !apart ? nullptr : pl.half ? own_fn<__half, 2>(pl.DP, pl.NT) : own_fn<__nv_bfloat16, 2>(pl.DP, pl.NT);

@@ -24,3 +24,19 @@ def test_parts_of_heads_of_any_size(kernel, d, lens, hkv, group, prefix, monkeyp
     gu.sync()
     assert torch.equal(p.out[:-1], first) and bool((p.out[-1] == 9.0).all())
     assert gu.error_flag() == 0
+
+
+@pytest.mark.parametrize("group,fit", [(1, 3), (8, 3), (9, 2), (16, 2), (40, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks_that_an_sm_holds(d, group, fit):
+    """What the rule for own tokens' blocks says of them: 228 KB of shared memory and 65536 registers for blocks of 128 threads, 1 KB of each reserved."""
+    li = lu.info("prefix_attn", Problem([5], 1, group, d, 0, 16).params())
+    assert min(228 * 1024 // (li.smem_per_block + 1024), 65536 // (-(-li.regs_per_thread // 8) * 8 * 128)) == fit
+
+
+@pytest.mark.parametrize("lens,hkv,group", [([70, 0, 31, 5] * 20, 4, 12), ([9] * 40, 8, 16), ([40, 3] * 41, 2, 20)])
+def test_more_blocks_behind_a_prefix_than_fit_at_once(lens, hkv, group):
+    """300 to 444 blocks of large groups: some come in only when others, which wait for the prefix, have left."""
+    p = Problem(lens, hkv, group, 128, 3000, 32, most=100)
+    p.check(p.run(), only=range(0, len(lens), 13))
+    assert 296 < lu.info("prefix_attn", p.params()).num_blocks <= 444 and gu.error_flag() == 0
