@@ -994,6 +994,11 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     return PB_OK;
 }
 
+const void* prefix_fn(const AttnPlan& pl) {
+    if (pl.DP == 64) return pl.half ? (const void*)prefix_kernel<__half, 64> : (const void*)prefix_kernel<__nv_bfloat16, 64>;
+    return pl.half ? (const void*)prefix_kernel<__half, 128> : (const void*)prefix_kernel<__nv_bfloat16, 128>;
+}
+
 template <typename T, int DP>
 int launch_prefix(const AttnPlan& pl, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
     PB_CUDA(cudaFuncSetAttribute(prefix_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrefixShape<DP>::smem));
@@ -1020,15 +1025,25 @@ int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out) {
     if (rc != PB_OK) return rc;
     PB_REQUIRE(out != nullptr, "pb_prefix_attn_info: NULL out");
     memset(out, 0, sizeof(*out));
+    // The last kernel reports, so its blocks are declared; the scheduler takes what they declare from the launch on, so together they declare the most that any of the launch's
+    // kernels holds.
     out->num_blocks = (uint32_t)pl.own_blocks;
-    out->threads_per_block = 128;
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, pl.join ? pl.join : pl.own) == cudaSuccess) {
-        out->regs_per_thread = (uint32_t)fa.numRegs;
-        out->smem_per_block = (uint32_t)fa.sharedSizeBytes + (pl.join ? 0 : pl.own_smem);
-    } else {
-        cudaGetLastError();
-    }
+    uint64_t threads = 0, smem = 0, regs = 0, columns = 0;
+    const auto holds = [&](const void* fn, int64_t blocks, uint64_t block_threads, uint64_t dynamic, uint64_t block_columns) {
+        cudaFuncAttributes fa = {};
+        if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) cudaGetLastError();       // (without a GPU: what the host knows)
+        threads = std::max<uint64_t>(threads, blocks * block_threads);
+        smem = std::max<uint64_t>(smem, blocks * (fa.sharedSizeBytes + dynamic));
+        regs = std::max<uint64_t>(regs, blocks * block_threads * fa.numRegs);
+        columns = std::max<uint64_t>(columns, blocks * block_columns);
+    };
+    if (pl.prefix_blocks > 0) holds(prefix_fn(pl), pl.prefix_blocks, 384, pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem, 512);
+    holds((const void*)pl.own, pl.own_blocks, 128, pl.own_smem, 0);
+    if (pl.join) holds((const void*)pl.join, pl.own_blocks, 128, 0, 0);
+    out->threads_per_block = (uint32_t)ceil_div<uint64_t>(threads, pl.own_blocks);
+    out->smem_per_block = (uint32_t)ceil_div<uint64_t>(smem, pl.own_blocks);
+    out->regs_per_thread = (uint32_t)ceil_div<uint64_t>(regs, (uint64_t)pl.own_blocks * out->threads_per_block);
+    out->tmem_cols_per_block = (uint32_t)ceil_div<uint64_t>(columns, pl.own_blocks);
     const uint64_t seen = (uint64_t)p->prefix_len + (uint64_t)p->batch * p->max_own_len;
     out->flops = 4ull * p->head_dim * p->q_heads * p->batch * ((uint64_t)p->prefix_len + p->max_own_len);
     out->bytes = p->batch ? 4ull * p->head_dim * (p->kv_heads * seen + (uint64_t)p->batch * p->q_heads) : 0;

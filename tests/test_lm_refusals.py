@@ -123,3 +123,19 @@ def test_attention_struct_size_and_declared_work():
                                          ("prefix_attn", attn(scale=-3e38))])
 def test_more_refusals(name, params):
     assert lu.refused(name, params).startswith("pb_" + name)
+
+
+def test_attention_declares_what_its_largest_kernel_holds():
+    """The last kernel's blocks report, and together they declare the most that any kernel of the launch holds: the prefix's takes whole SMs, with all of their tensor memory."""
+    sizes = dict(head_dim=128, page_stride=2 ** 15, token_stride=1024, head_stride=128, q_stride=2 ** 14, out_stride=2 ** 14, q_head_stride=128, out_head_stride=128, n_pages=2 ** 20,
+                 page_size=32, max_blocks=32, table_stride=32, max_own_len=512)
+    for batch, q_heads, kv_heads, prefix, blocks in ((32, 32, 8, 8192, 144), (1, 8, 1, 130001, 148), (256, 64, 8, 16384, 128)):
+        li = lu.info("prefix_attn", attn(batch=batch, q_heads=q_heads, kv_heads=kv_heads, prefix_len=prefix, **sizes))
+        assert li.num_blocks * li.threads_per_block >= blocks * 384
+        assert li.num_blocks * li.smem_per_block >= blocks * 225 * 1024
+        assert li.num_blocks * li.tmem_cols_per_block >= blocks * 512
+    # where the sequences' own tokens have more blocks than fit at once, those hold more shared memory than the prefix's, and the join, which reports, less than either
+    li = lu.info("prefix_attn", attn(batch=256, q_heads=64, kv_heads=8, prefix_len=16384, **sizes))
+    assert li.num_blocks == 2048 and li.smem_per_block >= 64 * 1024 and li.threads_per_block == 128
+    li = lu.info("prefix_attn", attn(batch=4, q_heads=32, kv_heads=8, prefix_len=0, **sizes))
+    assert li.threads_per_block == 128 and li.tmem_cols_per_block == 0 and li.smem_per_block >= 64 * 1024
