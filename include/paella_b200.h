@@ -218,7 +218,8 @@ PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
  *    start/end on `notifier` (may be NULL) for `job_id`.  `_info` declares that kernel's blocks; where an earlier kernel of the
  *    launch holds more threads, registers, shared or tensor memory, a block is declared with so much more that num_blocks
  *    times it is what that kernel holds.
- *  - Strides are in elements.  Buffers may lie anywhere inside larger ones; outputs do not overlap inputs unless a text says so.
+ *  - Strides are in elements and may be negative where no more is asked for; those of outputs keep neighbouring rows and heads
+ *    apart.  Buffers may lie anywhere inside larger ones; outputs do not overlap inputs unless a text says so.
  *    Alignment to the element is enough where no more is asked for; rows and heads that start on 16 bytes are moved faster.
  *  - Launches allocate nothing and may be captured into a CUDA graph, the first one included.  The pointers and sizes of the
  *    params are read at the launch, what they point to when the kernels run.

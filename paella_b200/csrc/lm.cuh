@@ -22,6 +22,8 @@ constexpr uint32_t kFlagLmPosition = 0x301, kFlagLmSlot = 0x302, kFlagLmLength =
 inline size_t dtype_bytes(int dtype) { return dtype == PB_F32 ? 4 : 2; }
 inline bool is_float_dtype(int dtype) { return dtype == PB_F32 || dtype == PB_BF16 || dtype == PB_F16; }
 inline bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+// Rows of `length` elements, `stride` apart in either direction, do not lie over their neighbours.
+inline bool rows_apart(int64_t count, int64_t stride, int64_t length) { return count <= 1 || stride >= length || stride <= -length; }
 
 template <typename F>
 uint32_t lm_regs(F fn) {

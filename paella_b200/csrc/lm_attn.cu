@@ -927,6 +927,7 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     PB_REQUIRE(fabsf(p->scale) <= 2e38f, "%s: scale is not finite, or above 2e38", who);        // (which in powers of two is finite, too)
     PB_REQUIRE(p->page_stride % 8 == 0 && p->token_stride % 8 == 0 && p->head_stride % 8 == 0 && p->page_stride > 0 && p->token_stride > 0 && p->head_stride > 0, "%s: strides of the cache are positive multiples of 8", who);
     PB_REQUIRE(p->q_stride % 8 == 0 && p->q_head_stride % 8 == 0, "%s: rows of q start on 16 bytes", who);
+    PB_REQUIRE(rows_apart(p->batch, p->out_stride, p->head_dim) && rows_apart(p->q_heads, p->out_head_stride, p->head_dim), "%s: rows of out overlap (strides %lld, %lld)", who, (long long)p->out_stride, (long long)p->out_head_stride);
     if (p->batch > 0) {
         PB_REQUIRE(p->q && p->out && p->k_cache && p->v_cache, "%s: NULL buffer", who);
         PB_REQUIRE(aligned(p->q, 16) && aligned(p->k_cache, 16) && aligned(p->v_cache, 16) && aligned(p->out, 2), "%s: q and the cache must be 16-byte aligned", who);

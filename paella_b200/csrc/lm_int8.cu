@@ -540,6 +540,7 @@ int check_quantize(const pb_int8_quantize_params* p) {
     PB_REQUIRE(p->tokens >= 0 && p->tokens <= (1 << 30) && p->channels >= 1 && p->channels <= (1 << 30), "%s: %d tokens of %d channels", who, p->tokens, p->channels);
     PB_REQUIRE(p->tokens == 0 || (p->x && p->q && p->scale), "%s: NULL buffer", who);
     PB_REQUIRE(aligned(p->x, dtype_bytes(p->x_dtype)) && aligned(p->scale, 4), "%s: a buffer is not aligned to its elements", who);
+    PB_REQUIRE(rows_apart(p->tokens, p->q_stride, p->channels), "%s: rows of q overlap (stride %lld)", who, (long long)p->q_stride);
     return PB_OK;
 }
 
@@ -552,6 +553,7 @@ int check_dense(const pb_int8_dense_params* p) {
     PB_REQUIRE(p->act >= 0 && p->act <= 2, "%s: activation %d (0 none, 1 relu, 2 relu6)", who, p->act);
     PB_REQUIRE(p->x_stride % 16 == 0 && p->w_stride % 16 == 0, "%s: rows of x and w start on 16 bytes (strides %lld, %lld)", who, (long long)p->x_stride, (long long)p->w_stride);
     PB_REQUIRE((p->x_stride >= p->in_channels || p->tokens <= 1) && (p->w_stride >= p->in_channels || p->out_channels == 1), "%s: rows overlap (strides %lld, %lld)", who, (long long)p->x_stride, (long long)p->w_stride);
+    PB_REQUIRE(rows_apart(p->tokens, p->y_stride, p->out_channels), "%s: rows of y overlap (stride %lld)", who, (long long)p->y_stride);
     if (p->tokens > 0) {
         PB_REQUIRE(p->x && p->x_scale && p->w && p->w_scale && p->y, "%s: NULL buffer", who);
         PB_REQUIRE(aligned(p->x, 16) && aligned(p->w, 16), "%s: x and w must be 16-byte aligned", who);

@@ -500,12 +500,18 @@ int check_heads(const char* who, int dtype, int tokens, int q_heads, int kv_head
     return PB_OK;
 }
 
+bool heads_apart(int64_t tokens, int heads, int head_dim, int64_t stride, int64_t head_stride) {
+    return heads == 0 || (rows_apart(tokens, stride, head_dim) && rows_apart(heads, head_stride, head_dim));
+}
+
 int rope_plan(const pb_qk_rope_params* p, RopePlan& pl) {
     const char* who = "pb_qk_rope";
     PB_REQUIRE(p != nullptr, "%s: NULL params", who);
     const int rc = check_heads(who, p->dtype, p->tokens, p->q_heads, p->kv_heads, p->head_dim, p->rot_dim, p->max_position, p->cos_sin, p->positions);
     if (rc != PB_OK) return rc;
     PB_REQUIRE(p->q_heads + p->kv_heads > 0, "%s: no heads", who);
+    PB_REQUIRE(heads_apart(p->tokens, p->q_heads, p->head_dim, p->q_out_stride, p->q_out_head_stride) && heads_apart(p->tokens, p->kv_heads, p->head_dim, p->k_out_stride, p->k_out_head_stride),
+               "%s: rows of q_out or k_out overlap", who);
     const size_t es = dtype_bytes(p->dtype);
     if (p->tokens > 0) {
         PB_REQUIRE(p->q_heads == 0 || (p->q && p->q_out), "%s: NULL q or q_out", who);
@@ -530,6 +536,8 @@ int append_plan(const pb_kv_append_params* p, RopePlan& pl) {
     if (rc != PB_OK) return rc;
     PB_REQUIRE(p->kv_heads > 0, "%s: no key heads", who);
     PB_REQUIRE(p->page_size >= 1 && p->n_pages >= 0 && p->n_pages <= INT64_MAX / p->page_size, "%s: %lld pages of %d rows", who, (long long)p->n_pages, p->page_size);
+    PB_REQUIRE(rows_apart(p->n_pages, p->page_stride, p->head_dim) && heads_apart(p->page_size, p->kv_heads, p->head_dim, p->token_stride, p->head_stride), "%s: rows of the cache overlap", who);
+    PB_REQUIRE(heads_apart(p->tokens, p->q_heads, p->head_dim, p->q_out_stride, p->q_out_head_stride), "%s: rows of q_out overlap", who);
     const size_t es = dtype_bytes(p->dtype);
     if (p->tokens > 0) {
         PB_REQUIRE(p->k && p->v && p->k_cache && p->v_cache && p->slots && aligned(p->slots, 8), "%s: NULL k, v, cache or slots", who);

@@ -125,6 +125,25 @@ def test_more_refusals(name, params):
     assert lu.refused(name, params).startswith("pb_" + name)
 
 
+# rows of results that lie over one another, forgotten strides among them; where there is only one row its stride does not matter
+@pytest.mark.parametrize("name,params", [("int8_quantize", quantize(q_stride=0)), ("int8_quantize", quantize(q_stride=63)), ("int8_quantize", quantize(q_stride=-63)), ("int8_dense", dense(y_stride=0)),
+                                         ("int8_dense", dense(y_stride=31)), ("int8_dense", dense(y_stride=-31)),
+                                         ("qk_rope", rope(q_out_stride=0)), ("qk_rope", rope(q_out_head_stride=63)), ("qk_rope", rope(k_out_stride=-63)), ("qk_rope", rope(k_out_head_stride=0)),
+                                         ("kv_append", append(page_stride=0)), ("kv_append", append(token_stride=63)), ("kv_append", append(head_stride=0)), ("kv_append", append(q_out_stride=8)),
+                                         ("kv_append", append(q_out_head_stride=0)), ("prefix_attn", attn(out_stride=0)), ("prefix_attn", attn(out_stride=63)), ("prefix_attn", attn(out_head_stride=-63))])
+def test_rows_of_results_that_overlap_are_refused(name, params):
+    assert lu.refused(name, params).startswith("pb_" + name)
+
+
+@pytest.mark.parametrize("name,params", [("int8_quantize", quantize(tokens=1, q_stride=0)), ("int8_quantize", quantize(q_stride=-64)), ("int8_quantize", quantize(x_stride=0)),
+                                         ("int8_dense", dense(tokens=1, y_stride=0)), ("int8_dense", dense(y_stride=-2 ** 63)), ("qk_rope", rope(tokens=1, q_out_stride=0, k_out_stride=0)),
+                                         ("qk_rope", rope(kv_heads=1, k_out_head_stride=0)), ("qk_rope", rope(kv_heads=0, k_out_stride=0)), ("qk_rope", rope(q_stride=0, k_head_stride=0)),
+                                         ("kv_append", append(n_pages=1, page_stride=0)), ("kv_append", append(page_size=1, token_stride=0)), ("kv_append", append(kv_heads=1, head_stride=0)),
+                                         ("kv_append", append(q_heads=0, q_out_stride=0)), ("prefix_attn", attn(batch=1, out_stride=0)), ("prefix_attn", attn(q_heads=1, kv_heads=1, out_head_stride=0))])
+def test_strides_of_lone_rows_and_of_inputs_are_free(name, params):
+    lu.info(name, params)
+
+
 def test_attention_declares_what_its_largest_kernel_holds():
     """The last kernel's blocks report, and together they declare the most that any kernel of the launch holds: the prefix's takes whole SMs, with all of their tensor memory."""
     sizes = dict(head_dim=128, page_stride=2 ** 15, token_stride=1024, head_stride=128, q_stride=2 ** 14, out_stride=2 ** 14, q_head_stride=128, out_head_stride=128, n_pages=2 ** 20,
