@@ -105,17 +105,6 @@ __device__ __forceinline__ void tcgen05_st8(uint32_t taddr, const uint32_t (&r)[
                  ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-__device__ __forceinline__ void tcgen05_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // lo and hi less the bf16 values of the pair, exactly.  (The mixed multiply-add reads a half of a register: two instructions where widening the
 // halves and subtracting takes three.)

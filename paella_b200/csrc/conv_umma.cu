@@ -761,11 +761,6 @@ constexpr int kWarpB = 3;          // issues operand B's copies
 // operand A's warp stores a stage through TMA before it loads the next tile there, and the blocks of a row tile, which normalise the same
 // k-blocks, take turns at that.  (DenseNet-121 of three images: 622 us without these stores, 637 with them, 670 when the normalising
 // threads store.)
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
 // consts: [k-block][64 scales, 64 biases] of this rank's k-blocks, in shared memory.
 __device__ __forceinline__ void normalise_constants(const ConvArgs& a, float* consts, int kb_begin, int nkb) {
     for (int i = threadIdx.x; i < nkb * 32; i += 128) {
@@ -1174,12 +1169,6 @@ conv_umma_pre_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // issues for the pair and commits to the barriers of both ("empty", "accumulator complete").  Each block has its own rows of
 // the accumulator in its tensor memory and finishes them as a lone block does.  Two pairs share a pair of SMs, so one's epilogue
 // and barrier latencies lie under the other's multiplications.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar)
-        : "memory");
-}
 __device__ __forceinline__ void tma_load_im2col_4d_pair(uint32_t dst, const CUtensorMap* map, int c, int w, int h, int n, uint16_t w_off, uint16_t h_off,
                                                         uint32_t leader_bar) {
     asm volatile(
@@ -1195,10 +1184,6 @@ __device__ __forceinline__ void tcgen05_mma_bf16_pair(uint32_t d_tmem, uint64_t 
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
-}
-// Arrives on the barrier at this offset in both blocks once the pair's multiplications so far are complete.
-__device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
 __global__ void __launch_bounds__(kThreadsTma, 2)

@@ -50,18 +50,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-// Whether it holds for all of the 256 threads of the softmax warps, which meet here.
-__device__ __forceinline__ bool all_of_256(bool ok) {
-    uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
-    return all != 0;
-}
-
 // 2^x of a pair on the multipliers, beside ex2 on the special-function unit, which alone would take as long as the products: x = i + f with |f| <= 1/2
 // (the sum with 1.5 x 2^23 rounds to a whole number), 2^f as the polynomial of degree 5 with the least largest relative error (Remez's exchange;
 // 2^-22.6 with the coefficients in fp32, 2^-22.1 with fp32's roundings), i added to its exponent.  Up to 2^-126: nothing.  For x < 127; a NaN stays one: the

@@ -325,20 +325,6 @@ __global__ void __launch_bounds__(192) int8_few_kernel(const __grid_constant__ D
     if (nf) nf->end(job_id);
 }
 
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar) : "memory");
-}
-// Arrives on the barrier at this offset in both blocks once the pair's products so far are complete.
-__device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-
-__device__ __forceinline__ bool all_of_256(bool ok) {
-    uint32_t all;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
-    return all != 0;
-}
-
 constexpr uint32_t kOutBytes = 2 * 16 * 128 * 4;       // twice 32 tokens of 128 channels in 16 bits on their way out
 
 // A pair of blocks walks its share of the tiles.  Warps 0-3 and 4-7: results, a lane a channel, 32 tokens each in turn; warp 8: copies of this block's operands; warp

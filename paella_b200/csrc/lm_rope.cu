@@ -196,16 +196,6 @@ __global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeA
     if (nf) nf->end(job_id);
 }
 
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
 __device__ __forceinline__ uint64_t two(float x, float y) { return pack_f32x2(__float_as_uint(x), __float_as_uint(y)); }
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }

@@ -73,6 +73,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// One block of a pair (cta_group::2): the copy into its own memory, counted on the first block's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar)
+        : "memory");
+}
+
 // im2col-mode TMA: 128 consecutive output pixels (traversed W, then H, then N inside the bounding
 // box of filter-window origins) x 64 channels, at filter offset (w_off, h_off); elements outside
 // the tensor arrive as zeros.
@@ -152,6 +160,10 @@ __device__ __forceinline__ void tcgen05_st32(uint32_t taddr, const uint32_t* r) 
         "r"(r[31]), "r"(taddr)
         : "memory");
 }
+// Arrives on the barrier at this offset in both blocks of a pair once its multiplications so far are complete.
+__device__ __forceinline__ void tcgen05_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
 __device__ __forceinline__ void tcgen05_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // The A operand from tensor memory: 16-bit values, two a column.
 __device__ __forceinline__ void tcgen05_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -161,6 +173,12 @@ __device__ __forceinline__ void tcgen05_mma_f16_ts(uint32_t d_tmem, uint32_t a_t
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+// Whether it holds for all of the 256 threads of eight warps, which meet here (barrier 1).
+__device__ __forceinline__ bool all_of_256(bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
 }
 // One lane of a converged warp, the same one every time.  Loops that issue tensor-core or copy instructions run
 // warp-uniformly and only the instruction itself is predicated on this: under `if (lane == 0)` the compiler cannot
@@ -230,6 +248,11 @@ __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t x, uint64_t y) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
 __device__ __forceinline__ uint64_t fma_f32x2(uint64_t x, uint64_t y, uint64_t z) {
