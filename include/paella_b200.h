@@ -272,7 +272,8 @@ PB_API int pb_int8_dense_launch(const pb_int8_dense_params* p, void* stream, uin
  * z = x * weight / sqrt(mean(x^2) + eps) over a head's head_dim values (weight NULL: z = x), then for each pair (a, b) of
  * the first rot_dim values of z, with c and s of the pair at the token's position: (a c - b s, b c + a s).  Pairs are
  * (i, i + rot_dim / 2), or (2 i, 2 i + 1) with `interleaved`.  In fp32, rounded once; a head whose sum of squares passes
- * fp32's range (3.4e38: 128 values of 1.6e18) becomes zeros.
+ * fp32's range (3.4e38: 128 values of 1.6e18) becomes zeros.  Few tokens and many take different kernels, which round in
+ * different orders: the same token may differ by its last bit between launches of different sizes.
  * A token whose position lies outside of [0, max_position) is left out: its outputs stay as they were. */
 typedef struct pb_qk_rope_params {
     int32_t dtype;               /* PB_F32, PB_BF16 or PB_F16: q, k and their outputs */

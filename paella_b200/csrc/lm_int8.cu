@@ -116,7 +116,7 @@ template <typename T> QuantizeFn quantize_fn(bool wide, bool warp) {
 //
 // Few tokens are bound by reading the weights, many by the tensor cores.  int8_few_kernel: a tile of 128 channels for each block, its
 // reduction shared by the blocks of a cluster where the tiles alone leave SMs idle; they send their sums to the blocks that own the tokens (whole numbers:
-// their order changes nothing).  24 tokens, 4096 -> 14336: 13.6 us with the quantiser, 4.4 TB/s, 67 % of the copy rate; 64 tokens, 8192 -> 28672 40 to 42 us,
+// their order changes nothing).  Figures here and below are of launches back to back in a graph.  24 tokens, 4096 -> 14336: 13.6 us with the quantiser, 4.4 TB/s, 67 % of the copy rate; 64 tokens, 8192 -> 28672 40 to 42 us,
 // 87 to 90 %.  int8_many_kernel: a pair of SMs on a tile of 256 channels, each block with its own half of the channels and half of the tokens: 32 KB a
 // k-block and SM for 512 clocks of products, which the path from the L2 cache into an SM (some 60 bytes a clock) feeds; a lone SM on 128 x 256 would need
 // 48 KB.  8192 tokens, 8192 -> 8192: 337 us at full clocks, 3261 TOP/s, twice the measured bf16 rate to 1 %; 390 to 400 where power holds the clocks down.

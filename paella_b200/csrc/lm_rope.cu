@@ -5,7 +5,8 @@
 // Both are bound by memory: every head is read once and written once, 4 operations a byte.  A group of lanes takes a head, each
 // lane both halves of its pairs, so that the rotation needs no exchange and only the norm's sum does (three shuffles for a head
 // of 128 values in 16 bits, whose group is eight lanes).  Everything is in fp32 and rounded once.  Few tokens are a chain of latencies (one token into
-// the cache: 2.5 us, 48 tokens of 40 heads 2.6); for many a group takes up to eight neighbouring heads of a token.
+// the cache: 2.5 us, 48 tokens of 40 heads 2.5 to 4; launches back to back in a graph, as all figures here); for many a group takes up to eight neighbouring heads of a token.
+// The two kernels add squares and multiply norm, weight and rotation in different orders, so a token's last fp32 bit depends on which of them takes it.
 #include <cuda.h>
 
 #include "lm.cuh"
@@ -260,7 +261,8 @@ __device__ __forceinline__ void gather(const uint64_t (&A)[8 / sizeof(T)], const
 // and an SM 96 or 192 KB, which cover the latency of x and, behind the position, of the rotation's row.  What the general kernel spends most on beside the
 // transfers, weights and rotation for each head, is found once here: products of weight and cosine or sine of a lane's pairs, again only where
 // queries end and keys begin.  16384 tokens of 40 heads of 128 in bf16, 344 MB: 72 us, 4.8 TB/s, 74 % of the copy rate (118 by the general kernel);
-// what is left is a block's chain of copies, norms and heads one after the other.
+// what is left is a block's chain of copies, norms and heads one after the other.  Three blocks an SM leave a thread 80 registers, of which 16-bit types need 18 or 19 more and fp32
+// in halves 3: those are kept in local memory.
 template <typename T, int HEADS, bool interleaved>
 __global__ void __launch_bounds__(256, 3) rope_many_kernel(const __grid_constant__ RopeArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr int V = 16 / (int)sizeof(T), N = V / 2;
