@@ -358,6 +358,33 @@ typedef struct pb_prefix_attn_params {
 PB_API int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out);
 PB_API int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t job_id, void* notifier);
 
+/* What stands between a block of a layer and the next one, in one pass.  For a token's row x of the block's output:
+ *     a = x * post_weight / sqrt(mean(x^2) + eps)     the norm behind the block (post_weight NULL: a = x)
+ *     h = residual + scale * (gate * a)               gate NULL: ones; residual NULL: zeros
+ *     y = h * weight / sqrt(mean(h^2) + eps)          the norm in front of the next block (weight NULL: ones)
+ * Means are over a row's `channels` values.  In fp32; h and y are rounded once each, y from the h in front of its rounding.
+ * A row whose sum of squares passes fp32's range (3.4e38) becomes zeros behind that norm. */
+typedef struct pb_residual_norm_params {
+    int32_t tokens;              /* 0 = nothing to do */
+    int32_t channels;            /* 1 to 32768 */
+    int32_t dtype;               /* PB_F32, PB_BF16 or PB_F16: x, gate and y */
+    int32_t h_dtype;             /* residual and h: dtype or PB_F32 */
+    float scale;
+    float eps;                   /* >= 0 */
+    int64_t x_stride;            /* from token to token, as all of these */
+    int64_t gate_stride;         /* 0: one gate for all tokens */
+    int64_t residual_stride, h_stride, y_stride;
+    const void* x;
+    const float* post_weight;    /* [channels] or NULL */
+    const void* gate;            /* [tokens][channels] or NULL */
+    const void* residual;        /* or NULL */
+    void* h;                     /* or NULL where it is not wanted; may be residual, with its stride */
+    const float* weight;         /* [channels] or NULL */
+    void* y;                     /* or NULL: no norm in front of a next block; may be x, with its stride */
+} pb_residual_norm_params;
+PB_API int pb_residual_norm_info(const pb_residual_norm_params* p, pb_launch_info* out);
+PB_API int pb_residual_norm_launch(const pb_residual_norm_params* p, void* stream, uint32_t job_id, void* notifier);
+
 /* ------------------------------------------------------------------------ *
  * Model packs and instances: the graph executor behind the model job adapters
  * (replaces tvm::runtime::Module::LoadFromFile + "run"/"get_input"/"get_output",

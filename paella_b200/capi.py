@@ -75,6 +75,12 @@ class PrefixAttnParams(C.Structure):
                [("scratch_bytes", C.c_uint64)]
 
 
+class ResidualNormParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "channels", "dtype", "h_dtype")] + [(n, C.c_float) for n in ("scale", "eps")] + \
+               [(n, C.c_int64) for n in ("x_stride", "gate_stride", "residual_stride", "h_stride", "y_stride")] + \
+               [(n, C.c_void_p) for n in ("x", "post_weight", "gate", "residual", "h", "weight", "y")]
+
+
 class ServerConfig(C.Structure):
     _fields_ = [("device", C.c_int32), ("num_streams", C.c_uint32), ("extra_kernels", C.c_uint32),
                 ("unfairness_threshold", C.c_float), ("sched_sleep", C.c_uint32), ("ring_capacity", C.c_uint64),
@@ -185,6 +191,8 @@ SIGNATURES = {
     "pb_kv_append_launch": (_I, [C.POINTER(KvAppendParams), _VP, _U32, _VP]),
     "pb_prefix_attn_info": (_I, [C.POINTER(PrefixAttnParams), C.POINTER(LaunchInfo)]),
     "pb_prefix_attn_launch": (_I, [C.POINTER(PrefixAttnParams), _VP, _U32, _VP]),
+    "pb_residual_norm_info": (_I, [C.POINTER(ResidualNormParams), C.POINTER(LaunchInfo)]),
+    "pb_residual_norm_launch": (_I, [C.POINTER(ResidualNormParams), _VP, _U32, _VP]),
     "pb_device_error_flag": (_I, [_I, C.POINTER(_U32), _I]),
     "pb_set_conv_split_gain_us": (None, [C.c_double]),
     "pb_conv_umma_time": (_I, [C.POINTER(OpParams), _I, _I, _SZ, C.POINTER(C.c_double)]),
