@@ -385,6 +385,34 @@ typedef struct pb_residual_norm_params {
 PB_API int pb_residual_norm_info(const pb_residual_norm_params* p, pb_launch_info* out);
 PB_API int pb_residual_norm_launch(const pb_residual_norm_params* p, void* stream, uint32_t job_id, void* notifier);
 
+/* What a model's logits say of a token: for each row x of logits, with s = scale (1 / temperature) and p = softmax(s x) over its
+ * `vocab` values,
+ *     logprobs = log p[target],  ranks = 1 + the number of tokens in front of the target,  entropy = -sum p log p,
+ *     top_ids, top_logprobs: the first `top` tokens and their log p.
+ * Tokens are in order of their logits, equal ones the lower index first, NaNs in front of all numbers.  A logit of -infinity is a token that is
+ * masked: p is 0.  A row of such tokens alone has entropy 0 and -infinity for every log p.  A NaN or +infinity among a row's
+ * logits makes its logprobs, entropy and top_logprobs NaN.  Softmax and sums are in fp32.
+ * A negative target marks a row without one: logprob 0, rank 0.  A target of `vocab` or more has logprob NaN and rank 0. */
+typedef struct pb_logprobs_params {
+    int32_t tokens;              /* rows, 0 = nothing to do */
+    int32_t vocab;               /* 1 to 2^30 */
+    int32_t dtype;               /* PB_F32, PB_BF16 or PB_F16: logits */
+    int32_t top;                 /* 0 to 32, at most vocab */
+    float scale;                 /* > 0 */
+    int32_t reserved;            /* 0 */
+    int64_t logits_stride;
+    int64_t top_stride;          /* of top_ids and top_logprobs, from row to row */
+    const void* logits;          /* [tokens][vocab] */
+    const int32_t* targets;      /* [tokens]; or NULL: no logprobs, no ranks */
+    float* logprobs;             /* [tokens] or NULL, as the following */
+    int32_t* ranks;
+    float* entropy;
+    int32_t* top_ids;            /* [tokens][top] */
+    float* top_logprobs;         /* [tokens][top] */
+} pb_logprobs_params;
+PB_API int pb_logprobs_info(const pb_logprobs_params* p, pb_launch_info* out);
+PB_API int pb_logprobs_launch(const pb_logprobs_params* p, void* stream, uint32_t job_id, void* notifier);
+
 /* ------------------------------------------------------------------------ *
  * Model packs and instances: the graph executor behind the model job adapters
  * (replaces tvm::runtime::Module::LoadFromFile + "run"/"get_input"/"get_output",

@@ -81,6 +81,12 @@ class ResidualNormParams(C.Structure):
                [(n, C.c_void_p) for n in ("x", "post_weight", "gate", "residual", "h", "weight", "y")]
 
 
+class LogprobsParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "vocab", "dtype", "top")] + [("scale", C.c_float), ("reserved", C.c_int32)] + \
+               [(n, C.c_int64) for n in ("logits_stride", "top_stride")] + \
+               [(n, C.c_void_p) for n in ("logits", "targets", "logprobs", "ranks", "entropy", "top_ids", "top_logprobs")]
+
+
 class ServerConfig(C.Structure):
     _fields_ = [("device", C.c_int32), ("num_streams", C.c_uint32), ("extra_kernels", C.c_uint32),
                 ("unfairness_threshold", C.c_float), ("sched_sleep", C.c_uint32), ("ring_capacity", C.c_uint64),
@@ -193,6 +199,8 @@ SIGNATURES = {
     "pb_prefix_attn_launch": (_I, [C.POINTER(PrefixAttnParams), _VP, _U32, _VP]),
     "pb_residual_norm_info": (_I, [C.POINTER(ResidualNormParams), C.POINTER(LaunchInfo)]),
     "pb_residual_norm_launch": (_I, [C.POINTER(ResidualNormParams), _VP, _U32, _VP]),
+    "pb_logprobs_info": (_I, [C.POINTER(LogprobsParams), C.POINTER(LaunchInfo)]),
+    "pb_logprobs_launch": (_I, [C.POINTER(LogprobsParams), _VP, _U32, _VP]),
     "pb_device_error_flag": (_I, [_I, C.POINTER(_U32), _I]),
     "pb_set_conv_split_gain_us": (None, [C.c_double]),
     "pb_conv_umma_time": (_I, [C.POINTER(OpParams), _I, _I, _SZ, C.POINTER(C.c_double)]),

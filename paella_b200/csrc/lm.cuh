@@ -17,7 +17,7 @@ namespace pb {
 using llis::job::FinishedBlockNotifier;
 
 // Codes of the error flag.
-constexpr uint32_t kFlagLmPosition = 0x301, kFlagLmSlot = 0x302, kFlagLmLength = 0x303, kFlagLmPage = 0x304, kFlagLmWait = 0x310;
+constexpr uint32_t kFlagLmPosition = 0x301, kFlagLmSlot = 0x302, kFlagLmLength = 0x303, kFlagLmPage = 0x304, kFlagLmToken = 0x305, kFlagLmWait = 0x310;
 
 inline size_t dtype_bytes(int dtype) { return dtype == PB_F32 ? 4 : 2; }
 inline bool is_float_dtype(int dtype) { return dtype == PB_F32 || dtype == PB_BF16 || dtype == PB_F16; }

@@ -37,3 +37,32 @@ def test_norm_struct_size_and_declared_work():
     assert lu.info("residual_norm", norm(tokens=0)).bytes == 0
     L = capi.load()
     assert L.pb_residual_norm_info(None, C.byref(li)) == -2 and L.pb_residual_norm_launch(None, None, 0, None) == -2
+
+
+def logprobs(**over):
+    f = dict(tokens=4, vocab=100, dtype=capi.BF16, top=5, scale=1.0, logits_stride=100, top_stride=5, logits=A, targets=A, logprobs=A, ranks=A, entropy=A, top_ids=A, top_logprobs=A)
+    return capi.LogprobsParams(**{**f, **over})
+
+
+@pytest.mark.parametrize("over", [dict(tokens=-1), dict(vocab=0), dict(vocab=-5), dict(vocab=2 ** 30 + 1), dict(dtype=3), dict(dtype=-1), dict(top=-1), dict(top=33), dict(vocab=4), dict(scale=0.0), dict(scale=-1.0),
+                                  dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2e6), dict(scale=1e-7), dict(logits=None), dict(logits=A + 1), dict(dtype=capi.F32, logits=A + 2), dict(targets=None),
+                                  dict(targets=A + 2), dict(logprobs=A + 1), dict(ranks=A + 2), dict(entropy=A + 2), dict(top_ids=A + 2), dict(top_logprobs=A + 3), dict(top=0, top_stride=0), dict(top_stride=4),
+                                  dict(top_stride=0), dict(logprobs=None, ranks=None, entropy=None, top_ids=None, top_logprobs=None), dict(targets=None, ranks=None)])
+def test_logprobs_refusals(over):
+    assert lu.refused("logprobs", logprobs(**over)).startswith("pb_logprobs")
+
+
+@pytest.mark.parametrize("over", [dict(tokens=0, logits=None), dict(tokens=1, top_stride=0), dict(top=0, top_ids=None, top_logprobs=None, top_stride=0), dict(targets=None, logprobs=None, ranks=None),
+                                  dict(top_ids=None), dict(top_stride=-5), dict(logits_stride=0), dict(logits_stride=-100), dict(vocab=5, top=5), dict(scale=1e-6), dict(scale=1e6)])
+def test_logprobs_takes(over):
+    assert lu.info("logprobs", logprobs(**over)).num_blocks >= 1
+
+
+def test_logprobs_struct_size_and_declared_work():
+    assert C.sizeof(capi.LogprobsParams) == 6 * 4 + 2 * 8 + 7 * 8
+    li = lu.info("logprobs", logprobs())
+    assert li.bytes == 4 * (100 * 2 + 4 * 4 + 2 * 4 * 5) and li.num_blocks == 4 and li.flops == 6 * 4 * 100
+    assert lu.info("logprobs", logprobs(tokens=0)).bytes == 0
+    assert lu.info("logprobs", logprobs(vocab=131072)).num_blocks == 32
+    L = capi.load()
+    assert L.pb_logprobs_info(None, C.byref(li)) == -2 and L.pb_logprobs_launch(None, None, 0, None) == -2
