@@ -358,6 +358,43 @@ typedef struct pb_prefix_attn_params {
 PB_API int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out);
 PB_API int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t job_id, void* notifier);
 
+/* Attention of each sequence's new tokens, one or many, over a paged cache that holds them already (pb_kv_append).  Sequence b has
+ * lens[b] tokens in the cache, page after page of block_table[b], the last n = starts[b + 1] - starts[b] of which are new: rows starts[b] to
+ * starts[b + 1] - 1 of q and out.  The i-th of them stands at position p = lens[b] - n + i and sees the tokens 0 to p, with a window those from
+ * p - window + 1 on: out = softmax(scale * q K^T) V, query head h over key head h / (q_heads / kv_heads).  Products of bf16 / fp16 operands in
+ * fp32; softmax in fp32, its values rounded to the cache's type before they meet V.  A row that sees no token (p < 0) gets
+ * zeros.  What a row does not see has no part in it, whatever it holds; a value of V that is not finite makes the same of the rows that see
+ * it.  Rows that belong to no sequence are left as they are.
+ * A length outside of [0, max_len] counts as the nearer end, as does a start outside of [starts[b - 1], tokens]; of more than max_new new
+ * tokens the first max_new rows are computed, at the positions that they have.  A page number outside of [0, n_pages) counts as a page of zeros. */
+typedef struct pb_chunk_attn_params {
+    int32_t dtype;               /* PB_BF16 or PB_F16 */
+    int32_t batch;               /* sequences, 0 = nothing to do */
+    int32_t tokens;              /* rows of q and out */
+    int32_t q_heads, kv_heads;   /* q_heads a multiple of kv_heads */
+    int32_t head_dim;            /* a multiple of 8, 8 to 128 */
+    int32_t page_size;           /* a multiple of 8 */
+    int32_t max_blocks;          /* entries of a row of block_table */
+    int32_t max_new;             /* the most new tokens that a sequence has */
+    int32_t max_len;             /* the most that lens holds; <= max_blocks * page_size */
+    int32_t window;              /* tokens that a row sees, itself the last of them; 0 = all */
+    float scale;
+    int64_t n_pages;
+    int64_t q_stride, q_head_stride, out_stride, out_head_stride;    /* of q and out; those of q multiples of 8 */
+    int64_t page_stride, token_stride, head_stride;                  /* of k_cache and v_cache: positive multiples of 8 */
+    int64_t table_stride;        /* of block_table, from sequence to sequence */
+    const void* q;               /* [tokens][q_heads][head_dim], 16-byte aligned */
+    void* out;
+    const void *k_cache, *v_cache;   /* 16-byte aligned */
+    const int32_t* block_table;  /* [batch][max_blocks] */
+    const int32_t* starts;       /* [batch + 1] */
+    const int32_t* lens;         /* [batch] */
+    void* scratch;               /* pb_launch_info.scratch_bytes of device memory, 16-byte aligned, for one launch in flight at */
+    uint64_t scratch_bytes;      /* a time; written before it is read, so it needs no initialisation */
+} pb_chunk_attn_params;
+PB_API int pb_chunk_attn_info(const pb_chunk_attn_params* p, pb_launch_info* out);
+PB_API int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t job_id, void* notifier);
+
 /* What stands between a block of a layer and the next one, in one pass.  For a token's row x of the block's output:
  *     a = x * post_weight / sqrt(mean(x^2) + eps)     the norm behind the block (post_weight NULL: a = x)
  *     h = residual + scale * (gate * a)               gate NULL: ones; residual NULL: zeros

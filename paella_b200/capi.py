@@ -75,6 +75,15 @@ class PrefixAttnParams(C.Structure):
                [("scratch_bytes", C.c_uint64)]
 
 
+class ChunkAttnParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "batch", "tokens", "q_heads", "kv_heads", "head_dim", "page_size", "max_blocks", "max_new", "max_len", "window")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_int64) for n in ("n_pages", "q_stride", "q_head_stride", "out_stride", "out_head_stride", "page_stride", "token_stride", "head_stride",
+                                         "table_stride")] + \
+               [(n, C.c_void_p) for n in ("q", "out", "k_cache", "v_cache", "block_table", "starts", "lens", "scratch")] + \
+               [("scratch_bytes", C.c_uint64)]
+
+
 class ResidualNormParams(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("tokens", "channels", "dtype", "h_dtype")] + [(n, C.c_float) for n in ("scale", "eps")] + \
                [(n, C.c_int64) for n in ("x_stride", "gate_stride", "residual_stride", "h_stride", "y_stride")] + \
@@ -197,6 +206,8 @@ SIGNATURES = {
     "pb_kv_append_launch": (_I, [C.POINTER(KvAppendParams), _VP, _U32, _VP]),
     "pb_prefix_attn_info": (_I, [C.POINTER(PrefixAttnParams), C.POINTER(LaunchInfo)]),
     "pb_prefix_attn_launch": (_I, [C.POINTER(PrefixAttnParams), _VP, _U32, _VP]),
+    "pb_chunk_attn_info": (_I, [C.POINTER(ChunkAttnParams), C.POINTER(LaunchInfo)]),
+    "pb_chunk_attn_launch": (_I, [C.POINTER(ChunkAttnParams), _VP, _U32, _VP]),
     "pb_residual_norm_info": (_I, [C.POINTER(ResidualNormParams), C.POINTER(LaunchInfo)]),
     "pb_residual_norm_launch": (_I, [C.POINTER(ResidualNormParams), _VP, _U32, _VP]),
     "pb_logprobs_info": (_I, [C.POINTER(LogprobsParams), C.POINTER(LaunchInfo)]),

@@ -997,6 +997,11 @@ int launch_prefix(const AttnPlan& pl, const CUtensorMap& km, const CUtensorMap& 
 }
 
 }  // namespace
+}  // namespace pb
+
+#include "lm_chunk.cuh"
+
+namespace pb {
 
 uint32_t* lm_attn_error_flag_ptr() {
     void* p = nullptr;
@@ -1071,6 +1076,25 @@ int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t
     const int e = lm_launch("pb_prefix_attn (own tokens)", pl.own, blocks, dim3(128), pl.own_smem, st, 1, pl.a, job_id, (FinishedBlockNotifier*)nullptr);
     if (e != PB_OK) return e;
     return lm_launch("pb_prefix_attn (parts)", pl.join, blocks, dim3(128), 0, st, 1, pl.a, job_id, nf);
+}
+
+int pb_chunk_attn_info(const pb_chunk_attn_params* p, pb_launch_info* out) {
+    ChunkArgs a;
+    const int rc = check_chunk(p, a);
+    if (rc != PB_OK) return rc;
+    PB_REQUIRE(out != nullptr, "pb_chunk_attn_info: NULL out");
+    memset(out, 0, sizeof(*out));
+    out->num_blocks = (uint32_t)std::max<int64_t>(1, ceil_div<int64_t>((int64_t)a.batch * a.max_new * a.q_heads, 4));
+    out->threads_per_block = 128;
+    return PB_OK;
+}
+
+int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t job_id, void* notifier) {
+    ChunkArgs a;
+    const int rc = check_chunk(p, a);
+    if (rc != PB_OK) return rc;
+    const int64_t blocks = std::max<int64_t>(1, ceil_div<int64_t>((int64_t)a.batch * a.max_new * a.q_heads, 4));
+    return lm_launch("pb_chunk_attn", p->dtype == PB_F16 ? chunk_simple_kernel<__half> : chunk_simple_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, 1, a, job_id, (FinishedBlockNotifier*)notifier);
 }
 
 }  // extern "C"

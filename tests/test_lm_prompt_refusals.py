@@ -66,3 +66,32 @@ def test_logprobs_struct_size_and_declared_work():
     assert lu.info("logprobs", logprobs(vocab=131072)).num_blocks == 32
     L = capi.load()
     assert L.pb_logprobs_info(None, C.byref(li)) == -2 and L.pb_logprobs_launch(None, None, 0, None) == -2
+
+
+def chunk(**over):
+    f = dict(dtype=capi.BF16, batch=4, tokens=40, q_heads=8, kv_heads=2, head_dim=64, page_size=16, max_blocks=8, max_new=20, max_len=128, window=0, scale=0.125, n_pages=40, q_stride=512, q_head_stride=64,
+             out_stride=512, out_head_stride=64, page_stride=2048, token_stride=128, head_stride=64, table_stride=8, q=A, out=A, k_cache=A, v_cache=A, block_table=A, starts=A, lens=A, scratch=A,
+             scratch_bytes=1 << 40)
+    return capi.ChunkAttnParams(**{**f, **over})
+
+
+@pytest.mark.parametrize("over", [dict(dtype=capi.F32), dict(dtype=3), dict(batch=-1), dict(batch=2 ** 31 - 1), dict(tokens=-1), dict(q_heads=0), dict(kv_heads=0), dict(q_heads=7), dict(q_heads=2 ** 17, kv_heads=1),
+                                  dict(head_dim=136), dict(head_dim=12), dict(head_dim=0), dict(page_size=0), dict(page_size=12), dict(page_size=2 ** 25), dict(max_blocks=-1), dict(max_len=129), dict(max_len=-1),
+                                  dict(max_len=2 ** 30 + 1, max_blocks=2 ** 30), dict(max_new=-1), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(n_pages=-1),
+                                  dict(n_pages=2 ** 31), dict(n_pages=0), dict(page_stride=2050), dict(page_stride=0), dict(token_stride=4), dict(token_stride=-128), dict(head_stride=63), dict(q_stride=12), dict(q_head_stride=4),
+                                  dict(q=A + 8), dict(k_cache=A + 2), dict(v_cache=A + 8), dict(out=A + 1), dict(q=None), dict(out=None), dict(k_cache=None), dict(v_cache=None), dict(block_table=None),
+                                  dict(starts=None), dict(lens=None), dict(starts=A + 1), dict(lens=A + 2), dict(block_table=A + 2), dict(out_stride=0), dict(out_stride=63), dict(out_head_stride=-63)])
+def test_chunk_refusals(over):
+    assert lu.refused("chunk_attn", chunk(**over)).startswith("pb_chunk_attn")
+
+
+@pytest.mark.parametrize("over", [dict(batch=0, q=None), dict(tokens=0, q=None, out=None), dict(max_new=0, starts=None), dict(max_len=0, k_cache=None, block_table=None, n_pages=0, max_blocks=0), dict(tokens=1, out_stride=0),
+                                  dict(q_stride=0), dict(q_stride=-512), dict(out_stride=-512), dict(table_stride=0), dict(window=2 ** 31 - 1), dict(max_new=2 ** 31 - 1), dict(scale=-2e38), dict(max_new=1), dict(max_new=2)])
+def test_chunk_takes(over):
+    assert lu.info("chunk_attn", chunk(**over)).num_blocks >= 1
+
+
+def test_chunk_struct_size_and_null_params():
+    assert C.sizeof(capi.ChunkAttnParams) == 12 * 4 + 9 * 8 + 9 * 8
+    L, li = capi.load(), capi.LaunchInfo()
+    assert L.pb_chunk_attn_info(None, C.byref(li)) == -2 and L.pb_chunk_attn_launch(None, None, 0, None) == -2
