@@ -43,7 +43,21 @@ struct AttnArgs {
     int kv_heads, row_groups, ranks, early, out_vec;     // early: behind a prefix_kernel, beside whose end it starts
     uint32_t per_piece;        // 2^16 / (D / 4), rounded up
     int ahead;                 // tokens of the prefix that own_kernel takes as if they were each sequence's own: all of them, or none
+    // chunks of new tokens (phase 3 of own_kernel): own_lens are whole lengths
+    const int32_t* starts;
+    int tokens, max_new, window, few, beside;      // few: the most rows of a sequence that is taken here; beside: starts beside a kernel of the same launch
 };
+
+// A sequence of a batch of chunks, as its lengths count.
+struct ChunkSeq {
+    int start, rows, first;    // its first row of q, its new tokens, the position of the first of them
+};
+__device__ __forceinline__ ChunkSeq chunk_seq(const int32_t* starts, const int32_t* lens, int b, int tokens, int max_new, int max_len, bool tell) {
+    const int s0 = __ldcg(starts + b), s1 = __ldcg(starts + b + 1), l = __ldcg(lens + b);
+    const int start = min(max(s0, 0), tokens), end = min(max(s1, start), tokens), len = min(max(l, 0), max_len), n = end - start;
+    if (tell && (start != s0 || end != s1 || len != l || n > max_new)) atomicExch(&g_attn_flag, kFlagLmLength);
+    return {start, min(n, max_new), len - n};
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -571,6 +585,8 @@ template <int DP> struct OwnShape {
 // Phase 0 does all of it.  Where there are more than three blocks an SM, beside a prefix_kernel, phase 1 leaves its part to phase 2, a launch of its
 // own: its blocks then go on while the prefix is worked on, on the SMs that are left over and on those that become free, where blocks that wait for
 // the prefix's parts would hold them (220 -> 200 us).
+// Phase 3 takes chunks of new tokens whose rows (tokens x group) are as few as here: row r is head r % group of token r / group, each with an end of its own to
+// what it sees, and with a window a beginning.
 template <typename T, int DP, int NT, int PHASE>
 __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64, kStages = OwnShape<DP>::stages;
@@ -580,8 +596,9 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     float (*s_o)[R][DP] = reinterpret_cast<float (*)[R][DP]>(smem_raw);
     __shared__ __align__(8) float2 s_ml[4][R];
     __shared__ float s_w[R][kMaxParts];
-    if (PHASE == 2 || !a.early) griddep_wait();
-    if (PHASE == 1) griddep_launch();
+    constexpr bool kChunk = PHASE == 3;
+    if (kChunk ? !a.beside : PHASE == 2 || !a.early) griddep_wait();
+    if (PHASE == 1 || (kChunk && a.beside)) griddep_launch();
     if (nf) nf->start(job_id);
     const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = blockIdx.x % a.ranks;
@@ -589,7 +606,20 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     const int zg = unit % a.row_groups;
     unit /= a.row_groups;
     const int kvh = unit % a.kv_heads, b = unit / a.kv_heads;
-    const int row0 = zg * R, rows = b < a.batch ? min(R, a.group - row0) : 0;
+    const int row0 = zg * R;
+    int rows = b < a.batch ? min(R, a.group - row0) : 0;
+    ChunkSeq seq = {0, 0, 0};
+    if constexpr (kChunk) {
+        if (b < a.batch) seq = chunk_seq(a.starts, a.own_lens, b, a.tokens, a.max_new, a.max_own, threadIdx.x == 0);
+        const int64_t all = (int64_t)seq.rows * a.group;
+        rows = a.few > 0 && all > a.few ? 0 : (int)min((int64_t)R, max(all - row0, (int64_t)0));
+    }
+    const auto token_of_row = [&](int row) { return a.group == 1 ? row0 + row : (row0 + row) / a.group; };
+    const auto place_of_row = [&](int row, int64_t token_stride, int64_t head_stride) {          // of q or out
+        if (!kChunk) return b * token_stride + (int64_t)(kvh * a.group + row0 + row) * head_stride;
+        const int token = token_of_row(row);
+        return (int64_t)(seq.start + token) * token_stride + (int64_t)(kvh * a.group + row0 + row - token * a.group) * head_stride;
+    };
     // Chunks of 16 tokens: those of the prefix that are taken here, then the sequence's own.  A lane looks a chunk's two halves of 8 tokens up (a page holds a
     // multiple of 8), for 32 chunks at a time; the first of them before the sequence's length is known, whatever it is: entries up to max_own may be read.
     const int chunks_ahead = (a.ahead + 15) / 16;
@@ -599,19 +629,25 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         return __ldcg((chunk < chunks_ahead ? a.prefix_pages : a.block_table + b * a.table_stride) + token / a.page);
     };
     int page_lo = 0, page_hi = 0;
-    if (PHASE != 2 && a.ranks == 1) {
+    if (PHASE != 2 && a.ranks == 1 && !(kChunk && a.window)) {
         page_lo = page_of(warp + 4 * lane, 0);
         page_hi = page_of(warp + 4 * lane, 1);
     }
     int own = 0;
-    if (PHASE != 2 && b < a.batch && a.max_own > 0) {
+    int low = 0;                                                                 // the first token that any row sees
+    if (kChunk) {
+        own = rows > 0 ? max(seq.first + seq.rows, 0) : 0;
+        if (a.window) low = max(seq.first + 1 - a.window, 0);
+    }
+    if (PHASE != 2 && !kChunk && b < a.batch && a.max_own > 0) {
         own = __ldcg(a.own_lens + b);
         if (own < 0 || own > a.max_own) {
             if (threadIdx.x == 0) atomicExch(&g_attn_flag, kFlagLmLength);
             own = own < 0 ? 0 : a.max_own;
         }
     }
-    const int chunks = PHASE != 2 && b < a.batch ? chunks_ahead + (own + 15) / 16 : 0, first = (int)((int64_t)chunks * rank / a.ranks) + warp, last = (int)((int64_t)chunks * (rank + 1) / a.ranks);
+    const int skipped = kChunk ? min(low, own) / 16 : 0;                         // chunks in front of what any row sees
+    const int chunks = PHASE != 2 && b < a.batch ? chunks_ahead + (own + 15) / 16 - skipped : 0, first = skipped + (int)((int64_t)chunks * rank / a.ranks) + warp, last = skipped + (int)((int64_t)chunks * (rank + 1) / a.ranks);
     const auto token_of = [&](int chunk) { return 16 * (chunk < chunks_ahead ? chunk : chunk - chunks_ahead); };
     const auto limit_of = [&](int chunk) { return chunk < chunks_ahead ? a.ahead : own; };
     float o[VB][4][NT][4] = {};
@@ -626,8 +662,14 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             for (int i = 0; i < KB; ++i) {
                 q[t][i] = make_uint4(0, 0, 0, 0);
                 if (t * 8 + g < rows && 32 * i + 8 * c < a.D)
-                    q[t][i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)(kvh * a.group + row0 + t * 8 + g) * a.q_head + 32 * i + 8 * c));
+                    q[t][i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + place_of_row(t * 8 + g, a.q_stride, a.q_head) + 32 * i + 8 * c));
             }
+        int end[NT][2];                                                          // of what this lane's rows see
+        if constexpr (kChunk)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) end[t][j] = seq.first + token_of_row(min(8 * t + 2 * c + j, max(rows - 1, 0))) + 1;
         int64_t at_lo = -1, at_hi = -1;                                        // where a half lies, or -1: zeros
         const auto place = [&](int chunk, int half, int page) -> int64_t {
             const int token = token_of(chunk) + 8 * half;
@@ -641,7 +683,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         const auto where = [&](int turn, int64_t& lo, int64_t& hi) {           // of chunk first + 4 turn, turns in order
             if ((turn & 31) == 0) {
                 const int chunk = first + 4 * (turn + lane);
-                if (turn > 0 || a.ranks > 1) {
+                if (turn > 0 || a.ranks > 1 || (kChunk && a.window)) {
                     page_lo = chunk < last ? page_of(chunk, 0) : 0;
                     page_hi = chunk < last ? page_of(chunk, 1) : 0;
                 }
@@ -661,13 +703,13 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                 int64_t lo, hi;
                 where(turn, lo, hi);
                 const uint32_t to = ring + (turn % kStages) * (2 * kHalf);
-                const int left = limit_of(chunk) - token_of(chunk);
+                const int left = limit_of(chunk) - token_of(chunk), gone = kChunk ? low - token_of(chunk) : 0;
                 const bool col = 8 * piece < a.D;
 #pragma unroll
                 for (int i = 0; i < 16 / kRows; ++i) {
                     const int row = i * kRows + row0;
                     const int64_t base = row < 8 ? lo : hi;
-                    const bool there = col && base >= 0 && row < left;
+                    const bool there = col && base >= 0 && row < left && (!kChunk || row >= gone);
                     const int64_t at = there ? base + (row & 7) * a.token_stride + 8 * piece : 0;
                     const uint32_t bytes = there ? 16 : 0, dst = to + row * (DP * 2);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + ((piece ^ ((row & 1) << 2)) << 4)), "l"(static_cast<const T*>(a.k) + at), "r"(bytes) : "memory");
@@ -699,12 +741,27 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             const bool in0 = g < left, in1 = g + 8 < left;
             float up[NT][2];
             bool grown = false;
+            uint32_t hidden = 0;                                                 // scores that are masked
+            bool edge = false;                                                   // not all of these tokens are seen by all rows
+            if constexpr (kChunk) {
+                const int token = token_of(chunk), all = seq.first + 1;
+                edge = token + 16 > all || (a.window && token < all + seq.rows - 1 - a.window);
+                if (edge) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int at = token + g + 8 * (j >> 1);
+                            hidden |= (uint32_t)(at >= end[t][j & 1] || (a.window && at < end[t][j & 1] - a.window)) << (4 * t + j);
+                        }
+                }
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    s[t][j] = in0 ? s[t][j] * scale : -INFINITY;
-                    s[t][2 + j] = in1 ? s[t][2 + j] * scale : -INFINITY;
+                    s[t][j] = in0 && !(hidden >> (4 * t + j) & 1) ? s[t][j] * scale : -INFINITY;
+                    s[t][2 + j] = in1 && !(hidden >> (4 * t + 2 + j) & 1) ? s[t][2 + j] * scale : -INFINITY;
                     float x = fmaxf(s[t][j], s[t][2 + j]);
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
@@ -735,6 +792,43 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
                 l[t][1] += x1 + y1;
                 p0[t] = transpose_8x8(lm_pack2<T>(x0, x1));
                 p1[t] = transpose_8x8(lm_pack2<T>(y0, y1));
+            }
+            if constexpr (kChunk) {
+                if (edge) {
+                    const int token = token_of(chunk);
+                    // values that are not finite meet only the rows that see them; the products get zeros
+                    constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+                    bool odd = false;
+                    for (int i = lane; i < 16 * kPer; i += 32) {
+                        const uint4 v = ld_shared_v4(values + 16 * i);
+                        odd |= (__vcmpeq2(v.x & kExp, kExp) | __vcmpeq2(v.y & kExp, kExp) | __vcmpeq2(v.z & kExp, kExp) | __vcmpeq2(v.w & kExp, kExp)) != 0;
+                    }
+                    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                        for (int k = 0; k < 16; ++k)
+#pragma unroll
+                            for (int i = 0; i < VB; ++i) {
+                                const uint4 v = ld_shared_v4(values + k * (DP * 2) + (((8 * i + g) ^ (k & 6)) << 4));
+                                const T* x = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float y = lm_to_f<T>(x[e]);
+                                    if (fabsf(y) < INFINITY) continue;
+#pragma unroll
+                                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                        for (int j = 0; j < 2; ++j)
+                                            if (token + k < end[t][j] && !(a.window && token + k < end[t][j] - a.window)) o[i][e >> 1][t][2 * (e & 1) + j] += y;
+                                }
+                            }
+                        __syncwarp();
+                        for (int i = lane; i < 16 * kPer; i += 32) {
+                            const uint4 v = ld_shared_v4(values + 16 * i);
+                            st_shared_v4(values + 16 * i, v.x & ~__vcmpeq2(v.x & kExp, kExp), v.y & ~__vcmpeq2(v.y & kExp, kExp), v.z & ~__vcmpeq2(v.z & kExp, kExp), v.w & ~__vcmpeq2(v.w & kExp, kExp));
+                        }
+                        __syncwarp();
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < VB; ++i) {
@@ -835,7 +929,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = 1.f / sum;
+        const float inv = kChunk && sum == 0.f ? 0.f : 1.f / sum;             // (0: a row that sees no token)
 #pragma unroll
         for (int k = 0; k < kMaxParts / 32; ++k)
             if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;
@@ -873,13 +967,14 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
             acc.z += __shfl_xor_sync(0xffffffffu, acc.z, k); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, k);
         }
         if (!real || sub != 0) continue;
-        T* dst = static_cast<T*>(a.out) + b * a.out_stride + (int64_t)(kvh * a.group + row0 + row) * a.out_head + 4 * i4;
+        T* dst = static_cast<T*>(a.out) + place_of_row(row, a.out_stride, a.out_head) + 4 * i4;
         if (a.out_vec) {
             *reinterpret_cast<uint2*>(dst) = make_uint2(lm_pack2<T>(acc.x, acc.y), lm_pack2<T>(acc.z, acc.w));
         } else {
             dst[0] = lm_from_f<T>(acc.x); dst[1] = lm_from_f<T>(acc.y); dst[2] = lm_from_f<T>(acc.z); dst[3] = lm_from_f<T>(acc.w);
         }
     }
+    if (kChunk && a.beside && blockIdx.x == gridDim.x - 1) griddep_wait();       // so that this launch ends behind the one that it runs beside
     // The others have read this block's part.  (Whatever a lane has loaded of theirs has gone into a shuffle or a store in front of its arrival: nothing is left to order.)
     if (a.ranks > 1) { cluster_arrive_relaxed(); cluster_wait(); }
     if (nf) nf->end(job_id);
@@ -985,6 +1080,41 @@ int plan_attn(const pb_prefix_attn_params* p, AttnPlan& pl) {
     return PB_OK;
 }
 
+// What a launch of several kernels declares.  The last kernel reports, so its blocks are declared; the scheduler takes what they declare from the launch on, so together they
+// declare the most that any of the launch's kernels holds.
+struct LaunchHolds {
+    uint64_t threads = 0, smem = 0, regs = 0, columns = 0;
+    void add(const void* fn, int64_t blocks, uint64_t block_threads, uint64_t dynamic, uint64_t block_columns) {
+        cudaFuncAttributes fa = {};
+        if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) cudaGetLastError();       // (without a GPU: what the host knows)
+        threads = std::max<uint64_t>(threads, blocks * block_threads);
+        smem = std::max<uint64_t>(smem, blocks * (fa.sharedSizeBytes + dynamic));
+        regs = std::max<uint64_t>(regs, blocks * block_threads * fa.numRegs);
+        columns = std::max<uint64_t>(columns, blocks * block_columns);
+    }
+    void declare(int64_t blocks, pb_launch_info* out) const {
+        out->num_blocks = (uint32_t)blocks;
+        out->threads_per_block = (uint32_t)ceil_div<uint64_t>(threads, blocks);
+        out->smem_per_block = (uint32_t)ceil_div<uint64_t>(smem, blocks);
+        out->regs_per_thread = (uint32_t)ceil_div<uint64_t>(regs, (uint64_t)blocks * out->threads_per_block);
+        out->tmem_cols_per_block = (uint32_t)ceil_div<uint64_t>(columns, blocks);
+    }
+};
+
+// The tensor map of a cache: [page][head][token][value] whatever the order in memory; a dimension of one needs no stride of its own.
+struct CacheShape {
+    bool half;
+    int head_dim, page_size, kv_heads;
+    int64_t n_pages, token_stride, head_stride, page_stride;
+    uint32_t box_rows;
+};
+int encode_cache(const CacheShape& c, const void* cache, CUtensorMap* map) {
+    const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_size, (uint64_t)c.kv_heads, (uint64_t)c.n_pages};
+    const uint64_t strides[3] = {(uint64_t)c.token_stride * 2, c.kv_heads > 1 ? (uint64_t)c.head_stride * 2 : 16, c.n_pages > 1 ? (uint64_t)c.page_stride * 2 : 16};
+    const uint32_t box[4] = {64, c.box_rows, 1, 1};
+    return encode_tiled_sw128(c.half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cache, 4, dims, strides, box, map);
+}
+
 const void* prefix_fn(const AttnPlan& pl) {
     if (pl.DP == 64) return pl.half ? (const void*)prefix_kernel<__half, 64> : (const void*)prefix_kernel<__nv_bfloat16, 64>;
     return pl.half ? (const void*)prefix_kernel<__half, 128> : (const void*)prefix_kernel<__nv_bfloat16, 128>;
@@ -1021,25 +1151,11 @@ int pb_prefix_attn_info(const pb_prefix_attn_params* p, pb_launch_info* out) {
     if (rc != PB_OK) return rc;
     PB_REQUIRE(out != nullptr, "pb_prefix_attn_info: NULL out");
     memset(out, 0, sizeof(*out));
-    // The last kernel reports, so its blocks are declared; the scheduler takes what they declare from the launch on, so together they declare the most that any of the launch's
-    // kernels holds.
-    out->num_blocks = (uint32_t)pl.own_blocks;
-    uint64_t threads = 0, smem = 0, regs = 0, columns = 0;
-    const auto holds = [&](const void* fn, int64_t blocks, uint64_t block_threads, uint64_t dynamic, uint64_t block_columns) {
-        cudaFuncAttributes fa = {};
-        if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) cudaGetLastError();       // (without a GPU: what the host knows)
-        threads = std::max<uint64_t>(threads, blocks * block_threads);
-        smem = std::max<uint64_t>(smem, blocks * (fa.sharedSizeBytes + dynamic));
-        regs = std::max<uint64_t>(regs, blocks * block_threads * fa.numRegs);
-        columns = std::max<uint64_t>(columns, blocks * block_columns);
-    };
-    if (pl.prefix_blocks > 0) holds(prefix_fn(pl), pl.prefix_blocks, 384, pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem, 512);
-    holds((const void*)pl.own, pl.own_blocks, 128, pl.own_smem, 0);
-    if (pl.join) holds((const void*)pl.join, pl.own_blocks, 128, 0, 0);
-    out->threads_per_block = (uint32_t)ceil_div<uint64_t>(threads, pl.own_blocks);
-    out->smem_per_block = (uint32_t)ceil_div<uint64_t>(smem, pl.own_blocks);
-    out->regs_per_thread = (uint32_t)ceil_div<uint64_t>(regs, (uint64_t)pl.own_blocks * out->threads_per_block);
-    out->tmem_cols_per_block = (uint32_t)ceil_div<uint64_t>(columns, pl.own_blocks);
+    LaunchHolds holds;
+    if (pl.prefix_blocks > 0) holds.add(prefix_fn(pl), pl.prefix_blocks, 384, pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem, 512);
+    holds.add((const void*)pl.own, pl.own_blocks, 128, pl.own_smem, 0);
+    if (pl.join) holds.add((const void*)pl.join, pl.own_blocks, 128, 0, 0);
+    holds.declare(pl.own_blocks, out);
     const uint64_t seen = (uint64_t)p->prefix_len + (uint64_t)p->batch * p->max_own_len;
     out->flops = 4ull * p->head_dim * p->q_heads * p->batch * ((uint64_t)p->prefix_len + p->max_own_len);
     out->bytes = p->batch ? 4ull * p->head_dim * (p->kv_heads * seen + (uint64_t)p->batch * p->q_heads) : 0;
@@ -1055,14 +1171,10 @@ int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t
     if (pl.prefix_blocks > 0) {
         PB_REQUIRE(p->scratch != nullptr && p->scratch_bytes >= pl.scratch && aligned(p->scratch, 16), "pb_prefix_attn: %llu bytes of scratch memory are needed, 16-byte aligned (%llu given)",
                    (unsigned long long)pl.scratch, (unsigned long long)(p->scratch ? p->scratch_bytes : 0));
-        // [page][head][token][value] whatever the order in memory; a dimension of one needs no stride of its own
-        const uint64_t dims[4] = {(uint64_t)p->head_dim, (uint64_t)p->page_size, (uint64_t)p->kv_heads, (uint64_t)p->n_pages};
-        const uint64_t strides[3] = {(uint64_t)p->token_stride * 2, p->kv_heads > 1 ? (uint64_t)p->head_stride * 2 : 16, p->n_pages > 1 ? (uint64_t)p->page_stride * 2 : 16};
-        const uint32_t box[4] = {64, (uint32_t)pl.a.box_rows, 1, 1};
-        const CUtensorMapDataType type = pl.half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const CacheShape shape = {pl.half, p->head_dim, p->page_size, p->kv_heads, p->n_pages, p->token_stride, p->head_stride, p->page_stride, (uint32_t)pl.a.box_rows};
         CUtensorMap km, vm;
-        int e = encode_tiled_sw128(type, p->k_cache, 4, dims, strides, box, &km);
-        if (e == PB_OK) e = encode_tiled_sw128(type, p->v_cache, 4, dims, strides, box, &vm);
+        int e = encode_cache(shape, p->k_cache, &km);
+        if (e == PB_OK) e = encode_cache(shape, p->v_cache, &vm);
         if (e == PB_OK) {
             if (pl.half) e = pl.DP == 64 ? launch_prefix<__half, 64>(pl, km, vm, st) : launch_prefix<__half, 128>(pl, km, vm, st);
             else e = pl.DP == 64 ? launch_prefix<__nv_bfloat16, 64>(pl, km, vm, st) : launch_prefix<__nv_bfloat16, 128>(pl, km, vm, st);
@@ -1079,22 +1191,52 @@ int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, uint32_t
 }
 
 int pb_chunk_attn_info(const pb_chunk_attn_params* p, pb_launch_info* out) {
-    ChunkArgs a;
-    const int rc = check_chunk(p, a);
+    ChunkPlan pl;
+    const int rc = plan_chunk(p, pl);
     if (rc != PB_OK) return rc;
     PB_REQUIRE(out != nullptr, "pb_chunk_attn_info: NULL out");
     memset(out, 0, sizeof(*out));
-    out->num_blocks = (uint32_t)std::max<int64_t>(1, ceil_div<int64_t>((int64_t)a.batch * a.max_new * a.q_heads, 4));
-    out->threads_per_block = 128;
+    const int64_t reporting = pl.many ? pl.join_blocks : pl.few_blocks;
+    LaunchHolds holds;
+    if (pl.many) {
+        holds.add((const void*)pl.chunk, kChunkBlocks, 384, pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem, 512);
+        holds.add((const void*)pl.join, std::min<int64_t>(pl.join_blocks, 148 * 16), 128, 0, 0);
+    }
+    if (pl.has_few) holds.add((const void*)pl.own, pl.few_blocks, 128, pl.own_smem, 0);
+    holds.declare(reporting, out);
+    const uint64_t rows = std::min<uint64_t>(p->tokens, (uint64_t)pl.a.batch * pl.a.max_new), len = pl.a.window ? std::min(p->max_len, p->window) : p->max_len;
+    out->flops = 4ull * p->head_dim * p->q_heads * rows * len;
+    out->bytes = pl.a.batch ? 4ull * p->head_dim * ((uint64_t)p->batch * p->kv_heads * (pl.a.window ? std::min<uint64_t>(p->max_len, (uint64_t)p->window + pl.a.max_new) : p->max_len) + rows * p->q_heads) : 0;
+    out->scratch_bytes = pl.scratch;
     return PB_OK;
 }
 
 int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t job_id, void* notifier) {
-    ChunkArgs a;
-    const int rc = check_chunk(p, a);
+    ChunkPlan pl;
+    const int rc = plan_chunk(p, pl);
     if (rc != PB_OK) return rc;
-    const int64_t blocks = std::max<int64_t>(1, ceil_div<int64_t>((int64_t)a.batch * a.max_new * a.q_heads, 4));
-    return lm_launch("pb_chunk_attn", p->dtype == PB_F16 ? chunk_simple_kernel<__half> : chunk_simple_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, 1, a, job_id, (FinishedBlockNotifier*)notifier);
+    const cudaStream_t st = (cudaStream_t)stream;
+    FinishedBlockNotifier* nf = (FinishedBlockNotifier*)notifier;
+    if (pl.many) {
+        PB_REQUIRE(p->scratch != nullptr && p->scratch_bytes >= pl.scratch && aligned(p->scratch, 16), "pb_chunk_attn: %llu bytes of scratch memory are needed, 16-byte aligned (%llu given)",
+                   (unsigned long long)pl.scratch, (unsigned long long)(p->scratch ? p->scratch_bytes : 0));
+        const CacheShape shape = {pl.half, p->head_dim, p->page_size, p->kv_heads, p->n_pages, p->token_stride, p->head_stride, p->page_stride, (uint32_t)pl.a.box_rows};
+        CUtensorMap km, vm;
+        int e = encode_cache(shape, p->k_cache, &km);
+        if (e == PB_OK) e = encode_cache(shape, p->v_cache, &vm);
+        if (e == PB_OK) e = lm_launch("pb_chunk_attn (plan)", plan_kernel, dim3(1), dim3(1024), 0, st, 1, pl.a);
+        if (e != PB_OK) return e;
+        const uint32_t smem = pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem;
+        PB_CUDA(cudaFuncSetAttribute(pl.chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        e = lm_launch("pb_chunk_attn", pl.chunk, dim3(kChunkBlocks), dim3(384), smem, st, 1, pl.a, km, vm);
+        if (e != PB_OK) return e;
+    }
+    if (pl.has_few) {
+        PB_CUDA(cudaFuncSetAttribute(pl.own, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.own_smem));
+        const int e = lm_launch("pb_chunk_attn (few rows)", pl.own, dim3((unsigned)pl.few_blocks), dim3(128), pl.own_smem, st, pl.few.ranks, pl.few, job_id, pl.many ? (FinishedBlockNotifier*)nullptr : nf);
+        if (e != PB_OK || !pl.many) return e;
+    }
+    return lm_launch("pb_chunk_attn (parts)", pl.join, dim3((unsigned)pl.join_blocks), dim3(128), 0, st, 1, pl.a, job_id, nf);
 }
 
 }  // extern "C"

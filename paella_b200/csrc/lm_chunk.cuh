@@ -1,80 +1,721 @@
-// Attention of chunks of new tokens over a paged cache (pb_chunk_attn): part of lm_attn.cu, whose exponentials and products it uses.
+// Attention of chunks of new tokens over a paged cache (pb_chunk_attn): part of lm_attn.cu, whose kernel for few rows, exponentials and products it uses.
 //
 //   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j   over the tokens that row r sees: up to its own position, with a window the last of them
+//
+// Sequences of up to 16 rows (new tokens x heads of a key head; of one new token any) go to own_kernel, which is bound by reading the cache.  For more the rows of a
+// sequence's query heads that share a key head are cut into pairs of tiles of 128, which meet the keys and values in tiles of 128 on the tensor cores (chunk_kernel): the arithmetic of
+// prefix_kernel, with a mask where a tile holds keys that not all rows see.
+//
+// Pairs differ in the keys that they see, and sequences in everything, all of which only the device knows.  So a block lays out the work first (plan_kernel): every pair's cost is known, all pairs for
+// all key heads stand in a row, and the row is cut into equal ranges, wherever that cuts a pair's keys.  A pair that is cut leaves a part of its sums with
+// each range, and join_kernel puts them together; the others are written at once.
 #pragma once
 
 namespace pb {
 namespace {
+
+constexpr int kFewRows = 16, kChunkBlocks = 148, kMaxRounds = 4, kJoinSlices = 4;
+
+// 256 rows of a sequence (fewer at its end), for every key head.
+struct alignas(16) ChunkUnit {
+    int32_t b, start, rows, first;       // the sequence, its first row of q, its rows, the position of its first token
+    int32_t row0, tile0, tiles, end;     // its row here; the tiles of 128 keys from the first that any of these rows sees; the end of what they see
+};
+static_assert(sizeof(ChunkUnit) == 32, "eight words, one a lane");
+struct alignas(16) ChunkCut {            // where a range begins
+    int32_t unit, head, step, pad;
+};
 
 struct ChunkArgs {
     const void *q, *k, *v;
     void* out;
     const int32_t *block_table, *starts, *lens;
     int64_t q_stride, q_head, out_stride, out_head, page_stride, token_stride, head_stride, table_stride;
-    int batch, tokens, q_heads, kv_heads, group, D, page, n_pages, max_new, max_len, window;
+    int batch, tokens, q_heads, kv_heads, group, D, page, n_pages, max_new, max_len, window, box_rows;
+    int few;                             // rows of a sequence that another kernel takes
     float scale;
+    int max_units, max_ranges;
+    ChunkUnit* units;
+    int64_t* before;                     // [max_units + 1]: costs of the units in front
+    ChunkCut* cuts;                      // [max_ranges + 1]
+    int32_t* counts;                     // units, ranges
+    float4* part_o;                      // [2 max_ranges][2][DP / 4][128]
+    float2* part_ml;                     // [2 max_ranges][2][128]: (m, l)
 };
 
-// A sequence's rows and length, as they count.
-struct ChunkSeq {
-    int start, rows, first, len;       // its first row, its rows, the first one's position, its tokens in the cache
-};
-__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int b, bool tell) {
-    const int s0 = a.starts[b], s1 = a.starts[b + 1], l = a.lens[b];
-    const int start = min(max(s0, 0), a.tokens), end = min(max(s1, start), a.tokens), len = min(max(l, 0), a.max_len);
-    const int n = end - start;
-    if (tell && (start != s0 || end != s1 || len != l || n > a.max_new)) atomicExch(&g_attn_flag, kFlagLmLength);
-    return {start, min(n, a.max_new), len - n, len};
+// Costs: a step of two row tiles, of one, and what a pair costs beside its steps.
+constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 6;
+
+__device__ __forceinline__ int ceil_pos(int x, int d) { return x > 0 ? (x + d - 1) / d : 0; }
+
+// The work: units, their costs, and the ranges.  One block; a sequence a warp, its pairs a lane each.
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ ChunkArgs a) {
+    __shared__ int64_t s_scan[32];
+    __shared__ int s_base[1024];
+    griddep_wait();
+    griddep_launch();
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    // inclusive sums over the block
+    const auto scan = [&](int64_t x) {
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = x;
+        __syncthreads();
+        if (warp == 0) {
+            int64_t w = s_scan[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= o) w += y;
+            }
+            s_scan[lane] = w;
+        }
+        __syncthreads();
+        return x + (warp ? s_scan[warp - 1] : 0);
+    };
+    int64_t units = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 1024) {
+        int mine = 0;
+        if (b0 + t < a.batch) {
+            const ChunkSeq s = chunk_seq(a.starts, a.lens, b0 + t, a.tokens, a.max_new, a.max_len, true);
+            const int64_t rows = (int64_t)s.rows * a.group;
+            mine = rows > a.few ? (int)((rows + 255) / 256) : 0;
+        }
+        const int64_t upto = scan(mine);
+        s_base[t] = (int)min(units + upto - mine, (int64_t)a.max_units);
+        __syncthreads();
+        const int n = min(1024, a.batch - b0);
+        for (int i = warp; i < n; i += 32) {
+            const ChunkSeq s = chunk_seq(a.starts, a.lens, b0 + i, a.tokens, a.max_new, a.max_len, false);
+            const int rows = s.rows * a.group, base = s_base[i];
+            if (rows <= a.few) continue;
+            // (starts that fall can make more units than rows have room for: those behind the last place are left out)
+            for (int p = lane; p < (rows + 255) / 256 && base + p < a.max_units; p += 32) {
+                ChunkUnit u;
+                u.b = b0 + i; u.start = s.start; u.rows = rows; u.first = s.first; u.row0 = 256 * p;
+                const int pos0 = s.first + u.row0 / a.group, pos1 = s.first + (min(u.row0 + 256, rows) - 1) / a.group;
+                u.end = max(pos1 + 1, 0);
+                u.tile0 = a.window ? max(pos0 - a.window + 1, 0) / 128 : 0;
+                u.tiles = max((u.end + 127) / 128 - u.tile0, 0);
+                a.units[base + p] = u;
+            }
+        }
+        const int64_t all = s_scan[31];
+        __syncthreads();
+        units += all;
+    }
+    const int U = (int)min(units, (int64_t)a.max_units);
+    if (units > a.max_units && t == 0) atomicExch(&g_attn_flag, kFlagLmLength);
+    __syncthreads();                     // (units are this block's own stores)
+    int64_t sum = 0;
+    for (int u0 = 0; u0 < U; u0 += 1024) {
+        int64_t mine = 0;
+        if (u0 + t < U) {
+            const ChunkUnit u = a.units[u0 + t];
+            mine = kCostPair + (int64_t)u.tiles * (u.row0 + 128 < u.rows ? kCostTwo : kCostOne);
+        }
+        const int64_t upto = scan(mine);
+        if (u0 + t < U) a.before[u0 + t] = sum + upto - mine;
+        sum += s_scan[31];
+        __syncthreads();
+    }
+    if (t == 0) a.before[U] = sum;
+    __syncthreads();
+    const int64_t total = sum * a.kv_heads;
+    // Ranges: one for each block, several where they are long (so that the blocks are at the same keys at the same time, and those come from the L2 cache), fewer where there is little to do.
+    const long long rounds = min(max((long long)total / (kChunkBlocks * 400), 1LL), (long long)(a.max_ranges / kChunkBlocks));
+    int N = (int)min(kChunkBlocks * rounds, max((long long)total / (kCostPair + 3 * kCostTwo), 1LL));
+    if (U == 0) N = 0;
+    for (int r = t; r <= N; r += 1024) {
+        ChunkCut c = {0, a.kv_heads, 0, 0};
+        if (r < N) {
+            const int64_t w = total / N * r + total % N * r / N;
+            c.head = (int)(w / sum);
+            const int64_t rest = w - c.head * sum;
+            int lo = 0, hi = U - 1;      // the last unit that begins at or in front of it
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (a.before[mid] <= rest) lo = mid;
+                else hi = mid - 1;
+            }
+            const ChunkUnit u = a.units[lo];
+            const int each = u.row0 + 128 < u.rows ? kCostTwo : kCostOne, near = (int)min((long long)total / N / (8 * each), 1000LL);
+            const int step = (int)(max((long long)(rest - a.before[lo] - kCostPair), 0LL) / each);
+            c.unit = lo;
+            if (step > near && step < u.tiles - near) c.step = step;
+            else if (step > near || 2 * step > u.tiles) {                // a cut near a pair's end is none
+                if (++c.unit == U) { c.unit = 0; ++c.head; }
+            }
+        }
+        a.cuts[r] = c;
+    }
+    if (t == 0) { a.counts[0] = U; a.counts[1] = N; }
 }
 
-// A warp a row and head.
-template <typename T>
-__global__ void __launch_bounds__(128) chunk_simple_kernel(const __grid_constant__ ChunkArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+// The parts of a block's ranges, one after the other.
+struct ChunkItem {
+    int b, start, rows, first, row0, tile0, tiles, end, head, from, to, slot;      // slot: of the part that it leaves, -1 if it is whole
+};
+struct ChunkWalk {
+    const ChunkArgs& a;
+    int range, units, ranges, unit, head, step, to_unit, to_head, to_step, word;
+    __device__ __forceinline__ ChunkWalk(const ChunkArgs& args) : a(args) {
+        units = __ldcg(a.counts);
+        ranges = __ldcg(a.counts + 1);
+        range = (int)blockIdx.x;
+        begin();
+    }
+    __device__ __forceinline__ void fetch() { word = __ldcg(reinterpret_cast<const int32_t*>(a.units + unit) + (threadIdx.x & 7)); }
+    __device__ __forceinline__ void begin() {
+        if (range >= ranges) return;
+        const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + range)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + range + 1));
+        unit = c.x; head = c.y; step = c.z; to_unit = d.x; to_head = d.y; to_step = d.z;
+        if (unit < units) fetch();
+    }
+    __device__ __forceinline__ bool next(ChunkItem& x) {                 // a whole warp
+        while (true) {
+            if (range >= ranges) return false;
+            const bool in_last = head == to_head && unit == to_unit;
+            if (head > to_head || (head == to_head && unit > to_unit) || (in_last && step >= to_step)) {
+                range += (int)gridDim.x;
+                begin();
+                continue;
+            }
+            int32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __shfl_sync(0xffffffffu, word, i);
+            x.b = w[0]; x.start = w[1]; x.rows = w[2]; x.first = w[3]; x.row0 = w[4]; x.tile0 = w[5]; x.tiles = w[6]; x.end = w[7];
+            x.head = head; x.from = step; x.to = in_last ? to_step : x.tiles;
+            x.slot = x.from > 0 ? 2 * range : x.to < x.tiles ? 2 * range + 1 : -1;
+            step = 0;
+            if (++unit == units) { unit = 0; ++head; }
+            fetch();                     // the next one's, in time
+            return true;
+        }
+    }
+};
+
+// Warps 0-3 and 4-7: softmax of one row tile each, a row a thread; warps 8 and 11 copy keys and values; warps 9 and 10 issue the products of one row tile each, 64 keys at a time.  As in
+// prefix_kernel: S = Q K^T into 64 columns of tensor memory, P takes its place as the A operand of O += P V.  Rings and barriers run on from one pair to the next; the next pair's queries come while the last
+// values of the one before are worked on.
+template <typename T, int DP>
+__global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages;
+    constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
+    static_assert(kStages >= 4, "a wait for an entry of the ring has seen the one before in its place");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_free[2], s_q[2], s_edge;
+    __shared__ int s_pages[2][4][32];
+    __shared__ uint32_t s_odd[8];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile uint32_t s_abort;
+    const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + 2 * kTile;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+    if (warp == 9) {
+        tcgen05_alloc(smem_u32(&s_tmem), 512);
+        tcgen05_relinquish();
+    }
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_empty[i]), 2);                         // groups that use a tile
+        }
+        for (int i = 0; i < 2; ++i) {
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(smem_u32(&s_scores[i][h]), 1);
+                mbar_init(smem_u32(&s_probs[i][h]), 4);
+            }
+            mbar_init(smem_u32(&s_half[i]), 1);
+            mbar_init(smem_u32(&s_turn[i]), 1);
+            mbar_init(smem_u32(&s_done[i]), 1);
+            mbar_init(smem_u32(&s_free[i]), 4);
+            mbar_init(smem_u32(&s_q[i]), 128);
+        }
+        mbar_init(smem_u32(&s_edge), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mbar_arrive(smem_u32(&s_turn[0]));                               // the first group begins
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = uniform(s_tmem);
+    griddep_wait();
+    griddep_launch();
+
+    const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &s_abort, &g_attn_flag, kFlagLmWait)); };
+    struct Place {                       // in the ring: keys of a block's tile t at 2 t, its values at 2 t + 1, over all its items
+        uint32_t st, parity;
+        __device__ __forceinline__ void on() {
+            st += 2;
+            if (st >= kStages) { st -= kStages; parity ^= 1; }
+        }
+    };
+    if (warp == 8 || warp == 11) {
+        // One warp copies keys, one values.  A lane copies a box: `box_rows` tokens of a page, 64 values of each, whose page it looked up two copies ahead.
+        const bool values = warp == 11;
+        const int box = lane / kBlocks, blk = lane % kBlocks;
+        const uint32_t words = smem_u32(&s_pages[values][0][lane]);
+        struct Tiles {                   // the block's tiles in order
+            ChunkWalk walk;
+            ChunkItem x;
+            int step;
+            bool more;
+            __device__ __forceinline__ Tiles(const ChunkArgs& a) : walk(a) { item(); }
+            __device__ __forceinline__ void item() {
+                do more = walk.next(x);
+                while (more && x.from >= x.to);
+                step = x.from;
+            }
+            __device__ __forceinline__ void on() {
+                if (++step >= x.to) item();
+            }
+        };
+        Tiles ahead(a), now(a);
+        int i = 0, i_ahead = 0;
+        const auto look_up = [&]() {
+            const int token = (ahead.x.tile0 + ahead.step) * 128 + box * a.box_rows;
+            if (ahead.more && box * a.box_rows < 128 && token < ahead.x.end)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + (i_ahead & 3) * 128), "l"(a.block_table + ahead.x.b * a.table_stride + token / a.page) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ++i_ahead;
+            if (ahead.more) ahead.on();
+        };
+        look_up();
+        look_up();
+        Place at = {values ? 1u : 0u, 1};
+        uint32_t edges = 0, item = 0;
+        bool ok = true, fresh = true;
+        while (ok && now.more) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            const int first = (now.x.tile0 + now.step) * 128, there = min(128, now.x.end - first), boxes = (there + a.box_rows - 1) / a.box_rows;
+            ok = wait(&s_empty[at.st], at.parity);
+            if (!ok) break;
+            // Values of a tile whose keys not all rows see: what lies behind the last one is zeros, and so is what is not finite (zero times which would be NaN for
+            // the rows that do not see it; s_odd tells the softmax groups to add it where it is seen).
+            bool edge = false;
+            if (values) {
+                const int pos0 = now.x.first + now.x.row0 / a.group, pos1 = now.x.end - 1;
+                edge = first + 128 > pos0 + 1 || (a.window && first < pos1 - a.window + 1);
+                if (fresh && lane == 0) s_odd[item & 7] = 0;
+                fresh = false;
+            }
+            const uint32_t to = ring + at.st * kTile, bar = smem_u32(edge ? &s_edge : &s_full[at.st]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * kBlocks * a.box_rows * 128));
+            __syncwarp();
+            if (box < boxes) {
+                int page;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(page) : "r"(words + (i & 3) * 128) : "memory");
+                if ((uint32_t)page >= (uint32_t)a.n_pages) {
+                    atomicExch(&g_attn_flag, kFlagLmPage);
+                    page = a.n_pages;                                    // outside of the map: zeros
+                }
+                tma_load_4d(to + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, (first + box * a.box_rows) % a.page, now.x.head, page, bar);
+            }
+            __syncwarp();
+            if (edge) {
+                ok = wait(&s_edge, edges & 1);
+                ++edges;
+                if (!ok) break;
+                constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+                bool odd = false;
+                for (int c = lane; c < 128 * 8 * kBlocks; c += 32) {
+                    const uint32_t from = to + c * 16;
+                    if ((c >> 3) % 128 >= there) {
+                        st_shared_v4(from, 0, 0, 0, 0);
+                        continue;
+                    }
+                    uint4 v = ld_shared_v4(from);
+                    const uint32_t x = __vcmpeq2(v.x & kExp, kExp), y = __vcmpeq2(v.y & kExp, kExp), z = __vcmpeq2(v.z & kExp, kExp), w = __vcmpeq2(v.w & kExp, kExp);
+                    if (x | y | z | w) {
+                        odd = true;
+                        st_shared_v4(from, v.x & ~x, v.y & ~y, v.z & ~z, v.w & ~w);
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[item & 7] = 1;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_full[at.st]));
+            }
+            at.on();
+            ++i;
+            const bool last = now.step + 1 >= now.x.to;
+            now.on();
+            if (last) { ++item; fresh = true; }
+            look_up();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else if (warp == 9 || warp == 10) {
+        constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t idesc_s = (1u << 4) | kType | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+        const int g = warp - 9;
+        const uint32_t d_s = tmem + g * 128, d_o = tmem + 256 + g * DP;
+        const uint64_t desc_q = umma_desc_sw128(q_smem + g * kTile), desc_k = umma_desc_sw128(ring), desc_v = umma_desc_sw128_mn(ring, kBlock);
+        const uint32_t high_k = (uint32_t)(desc_k >> 32), high_v = (uint32_t)(desc_v >> 32), low_q = (uint32_t)desc_q;
+        Place keys = {0, 0}, vals = {1, 0};
+        uint32_t turn = 0, tiles = 0, items = 0;       // phases: of the turns, of this group's tiles and items
+        ChunkWalk walk(a);
+        ChunkItem x;
+        bool ok = true;
+        while (ok && walk.next(x)) {
+            const int n = x.to - x.from;
+            if (n <= 0) continue;
+            const bool two = x.row0 + 128 < x.rows;
+            if (g == 1 && !two) {                      // nothing to do here but to let the ring go on
+                for (int u = 0; ok && u < n; ++u) {
+                    ok = wait(&s_full[keys.st], keys.parity);
+                    if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty[keys.st]));
+                    keys.on();
+                    ok = ok && wait(&s_full[vals.st], vals.parity);
+                    if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty[vals.st]));
+                    vals.on();
+                }
+                continue;
+            }
+            // Two groups take turns at the tensor cores, as in prefix_kernel.
+            const auto take_turn = [&]() {
+                if (!two) return true;
+                const bool now = wait(&s_turn[g], turn);
+                turn ^= 1;
+                return now;
+            };
+            const auto scores = [&](uint32_t h) {
+                if (h == 0 && !wait(&s_full[keys.st], keys.parity)) return false;
+                tcgen05_fence_after();
+                const uint32_t low = (uint32_t)desc_k + keys.st * (kTile >> 4) + h * (8192 >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        if (two && k == DP / 32) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
+                        tcgen05_mma_bf16(d_s + h * 64, pack_f32x2(low_q + (k >> 2) * (kBlock >> 4) + (k & 3) * 2, high_k), pack_f32x2(low + (k >> 2) * (kBlock >> 4) + (k & 3) * 2, high_k), idesc_s, k > 0);
+                    }
+                    tcgen05_commit(smem_u32(&s_scores[g][h]));
+                    if (h == 1) tcgen05_commit(smem_u32(&s_empty[keys.st]));
+                }
+                __syncwarp();
+                if (h == 1) keys.on();
+                return true;
+            };
+            ok = wait(&s_q[g], items & 1) && take_turn() && scores(0) && take_turn() && scores(1);
+            for (int u = 0; ok && u < n; ++u, ++tiles) {
+                const bool last = u == n - 1;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    if (h == 0) {
+                        ok = wait(&s_full[vals.st], vals.parity);
+                        if (ok && u == 0 && items > 0) ok = wait(&s_free[g], (items - 1) & 1);          // the sums of the item before have been read
+                        if (!ok) break;
+                    }
+                    ok = wait(&s_probs[g][h], tiles & 1) && take_turn();
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint32_t low = (uint32_t)desc_v + vals.st * (kTile >> 4) + h * (8192 >> 4), more = u > 0;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tcgen05_mma_f16_ts(d_o, d_s + h * 64 + k * 8, pack_f32x2(low + k * (2048 >> 4), high_v), idesc_o, more | (uint32_t)(h > 0 || k > 0));
+                        if (h == 1) tcgen05_commit(smem_u32(&s_empty[vals.st]));
+                        if (last) tcgen05_commit(smem_u32(h == 0 ? &s_half[g] : &s_done[g]));
+                    }
+                    __syncwarp();
+                    if (!last) ok = scores(h);
+                    else if (two && elect_one()) mbar_arrive(smem_u32(&s_turn[g ^ 1]));
+                    __syncwarp();
+                    if (!ok) break;
+                }
+                vals.on();
+            }
+            ++items;
+        }
+    } else {
+        const int g = warp >> 2, in_tile = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;                       // this warp's lanes of tensor memory
+        const float c = fmaxf(fabsf(a.scale) * kLog2e, 1e-38f);                  // (a scale of 0 must not meet the infinities of masked keys)
+        const auto place = [&](const ChunkItem& x, int row, int64_t token_stride, int64_t head_stride) {       // of q or out
+            const int token = row / a.group;
+            return (int64_t)(x.start + token) * token_stride + (int64_t)(x.head * a.group + row - token * a.group) * head_stride;
+        };
+        const auto write = [&](const ChunkItem& x, int row, int col, const uint32_t (&o)[32], float f) {       // 32 values of a row
+            T* dst = static_cast<T*>(a.out) + place(x, row, a.out_stride, a.out_head) + col;
+            const bool vec = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * 2) | (uintptr_t)(a.out_head * 2)) & 15) == 0;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+                if (col + e >= a.D) break;
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * f;
+                if (vec) {
+                    *reinterpret_cast<uint4*>(dst + e) = make_uint4(lm_pack2<T>(v[0], v[1]), lm_pack2<T>(v[2], v[3]), lm_pack2<T>(v[4], v[5]), lm_pack2<T>(v[6], v[7]));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) dst[e + k] = lm_from_f<T>(v[k]);
+                }
+            }
+        };
+        ChunkWalk walk(a);
+        ChunkItem x, nx;
+        uint32_t live_items = 0, all_items = 0, tiles = 0, item = 0, next_item = 0;      // item: its number among those with tiles
+        // The next item with something to do here; rows that see nothing are written on the way.
+        const auto advance = [&]() {
+            while (walk.next(nx)) {
+                const int row = nx.row0 + g * 128 + in_tile;
+                if (nx.from >= nx.to) {
+                    if (row < nx.rows && nx.tiles == 0) {
+                        const uint32_t zeros[32] = {};
+#pragma unroll 1
+                        for (int j = 0; j < a.D; j += 32) write(nx, row, j, zeros, 0.f);
+                    }
+                    continue;
+                }
+                next_item = all_items++;
+                if (g == 0 || nx.row0 + 128 < nx.rows) return true;
+            }
+            return false;
+        };
+        // neighbouring lanes on neighbouring bytes of a row
+        constexpr int kPerRow = DP / 8, kStep = 128 / kPerRow;                   // 16-byte pieces of a row; rows from one of a thread's pieces to the next
+        const int thread = threadIdx.x & 127, piece = thread % kPerRow, r0 = thread / kPerRow;
+        const uint32_t mine = q_smem + g * kTile + (piece >> 3) * kBlock + r0 * 128 + (((piece & 7) ^ (r0 & 7)) << 4);
+        const auto load_q = [&](const ChunkItem& y) {
+            const int b_step = kStep / a.group, h_step = kStep - b_step * a.group;
+            int r = y.row0 + g * 128 + r0, h = r % a.group;
+            const int64_t step = b_step * a.q_stride + h_step * a.q_head, wrap = a.q_stride - a.group * a.q_head;
+            const T* src = static_cast<const T*>(a.q) + (int64_t)(y.start + r / a.group) * a.q_stride + ((int64_t)y.head * a.group + h) * a.q_head + 8 * piece;
+#pragma unroll 2
+            for (int i = 0; i < kPerRow; ++i) {
+                const bool there = r < y.rows && 8 * piece < a.D;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine + i * (kStep * 128)), "l"(there ? src : static_cast<const T*>(a.q)), "r"(there ? 16 : 0) : "memory");
+                r += kStep;
+                h += h_step;
+                src += step;
+                if (h >= a.group) { h -= a.group; src += wrap; }
+            }
+        };
+        const auto have_q = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (a.scale < 0.f) {                                                 // |scale| from here on
+#pragma unroll 1
+                for (int i = 0; i < kPerRow; ++i) {
+                    const uint4 v = ld_shared_v4(mine + i * (kStep * 128));
+                    st_shared_v4(mine + i * (kStep * 128), v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                }
+            }
+            fence_proxy_async();
+            mbar_arrive(smem_u32(&s_q[g]));
+        };
+        bool ok = true, more = advance();
+        if (more) {
+            load_q(nx);
+            have_q();
+        }
+        while (ok && more) {
+            x = nx;
+            item = next_item;
+            const int row = x.row0 + g * 128 + in_tile, n = x.to - x.from;
+            const bool live_warp = row - lane < x.rows;
+            const int limit = x.first + min(row, x.rows - 1) / a.group + 1, low = a.window ? limit - a.window : 0;     // the row sees tokens low to limit - 1
+            float m = -INFINITY, l = 0.f;
+            for (int i = 0; i < 2 * n; ++i) {
+                const int h = i & 1;
+                ok = wait(&s_scores[g][h], (tiles + (uint32_t)(i >> 1)) & 1);
+                if (!ok) break;
+                if (i == 2 * n - 1) {                  // the queries have been used: the next ones come
+                    more = advance();
+                    if (more) load_q(nx);
+                }
+                if (live_warp) {
+                    tcgen05_fence_after();
+                    const uint32_t ts = tmem + lanes + g * 128 + h * 64;
+                    uint32_t s[64], p[32];
+                    tcgen05_ld32(ts, s);
+                    tcgen05_ld32(ts + 32, s + 32);
+                    tcgen05_wait_ld();
+                    const int key = (x.tile0 + x.from + (i >> 1)) * 128 + h * 64, hi = limit - key, lo = low - key;
+                    if (__any_sync(0xffffffffu, hi < 64 || lo > 0)) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            if (j >= hi || j < lo) s[j] = 0xff800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                    const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                    if (i == 0) {
+                        m = next;
+                    } else if (__any_sync(0xffffffffu, (next - m) * c > kSlack)) {   // (a NaN difference, -inf to -inf, is no growth)
+                        // The products of the half before may still be adding to O: the scores behind them tell of their end, or, for the last half, a barrier.
+                        ok = i + 1 < 2 * n ? wait(&s_scores[g][h ^ 1], (tiles + (uint32_t)((i + 1) >> 1)) & 1) : wait(&s_half[g], live_items & 1);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+                        const float keep = next == m ? 1.f : ex2((m - next) * c);
+                        const uint32_t to = tmem + lanes + 256 + g * DP;
+#pragma unroll 1
+                        for (int j = 0; j < DP; j += 32) {
+                            uint32_t o[32];
+                            tcgen05_ld32(to + j, o);
+                            tcgen05_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tcgen05_st32(to + j, o);
+                        }
+                        l *= keep;
+                        m = next;
+                    }
+                    l += values_of<T>(s, c, m == -INFINITY ? 0.f : p_shift<T>() - m * c, p);
+                    tcgen05_st32(ts, p);
+                    tcgen05_wait_st();
+                    tcgen05_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_probs[g][h]));
+            }
+            if (!ok) break;
+            if (more) have_q();
+            ok = wait(&s_done[g], live_items & 1);
+            if (!ok) break;
+            tiles += (uint32_t)n;
+            ++live_items;
+            if (live_warp) {
+                tcgen05_fence_after();
+                const uint32_t from = tmem + lanes + 256 + g * DP;
+                const bool odd = *(volatile uint32_t*)&s_odd[item & 7] != 0;
+                const int64_t part = (int64_t)x.slot * 2 + g;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                if (x.slot >= 0) a.part_ml[part * 128 + in_tile] = make_float2(m == -INFINITY ? m : m * c, l);
+#pragma unroll 1
+                for (int j = 0; j < DP; j += 32) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tcgen05_ld32(from + j, o);
+                    tcgen05_wait_ld();
+                    if (odd) {
+                        // values that are not finite: their tiles held zeros in their places
+#pragma unroll 1
+                        for (int s = x.from; s < x.to; ++s) {
+                            const int key = (x.tile0 + s) * 128, pos0 = x.first + x.row0 / a.group;
+                            if (key + 128 <= pos0 + 1 && !(a.window && key < x.end - a.window)) continue;
+#pragma unroll 1
+                            for (int at = max(key, low); at < min(key + 128, limit); ++at) {
+                                const int page = __ldcg(a.block_table + x.b * a.table_stride + at / a.page);
+                                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                                const T* v = static_cast<const T*>(a.v) + page * a.page_stride + (at % a.page) * a.token_stride + x.head * a.head_stride + j;
+#pragma unroll
+                                for (int e = 0; e < 32; e += 8) {
+                                    if (j + e >= a.D) break;
+                                    const uint4 w = __ldcg(reinterpret_cast<const uint4*>(v + e));
+                                    const T* y = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) {
+                                        const float z = lm_to_f<T>(y[k]);
+                                        if (!(fabsf(z) < INFINITY)) o[e + k] = __float_as_uint(__uint_as_float(o[e + k]) + z);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    if (x.slot >= 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            a.part_o[(part * (DP / 4) + j / 4 + e) * 128 + in_tile] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                    } else if (row < x.rows) {
+                        write(x, row, j, o, inv);
+                    }
+                }
+                __syncwarp();
+                tcgen05_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_free[g]));
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (s_abort) {             // copies in flight end before their shared memory does
+        const unsigned long long t0 = globaltimer_ns();
+        for (int i = 0; i < 100000 && globaltimer_ns() - t0 < 50000; ++i) __nanosleep(500);
+    }
+    if (warp == 9) {
+        tcgen05_fence_after();
+        tcgen05_dealloc(tmem, 512);
+    }
+}
+
+// The parts of pairs that were cut: sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  kJoinSlices blocks for each cut, which a pair's first cut works for; a row a lane.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ ChunkArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (item < (int64_t)a.batch * a.max_new * a.q_heads) {          // (none of 0: no quotient by it either)
-        const int b = (int)(item / ((int64_t)a.max_new * a.q_heads));
-        const int i = (int)(item / a.q_heads % a.max_new), h = (int)(item % a.q_heads);
-        const ChunkSeq s = chunk_seq(a, b, lane == 0 && i == 0 && h == 0);
-        if (i < s.rows) {
-            const T* q = static_cast<const T*>(a.q) + (s.start + i) * a.q_stride + h * a.q_head;
-            float x[4], o[4] = {}, m = -INFINITY, l = 0.f;
-            for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < a.D ? lm_to_f<T>(q[lane + 32 * e]) * a.scale * kLog2e : 0.f;
-            const int p = s.first + i;
-            for (int j = a.window ? max(0, p - a.window + 1) : 0; j <= p; ++j) {
-                const int page = a.block_table[b * a.table_stride + j / a.page];
-                const bool there = page >= 0 && page < a.n_pages;
-                if (!there && lane == 0) atomicExch(&g_attn_flag, kFlagLmPage);
-                const int64_t at = page * a.page_stride + (j % a.page) * a.token_stride + h / a.group * a.head_stride;
-                float z = 0.f, v[4] = {};
-                for (int e = 0; e < 4; ++e)
-                    if (there && lane + 32 * e < a.D) {
-                        z = fmaf(x[e], lm_to_f<T>(static_cast<const T*>(a.k)[at + lane + 32 * e]), z);
-                        v[e] = lm_to_f<T>(static_cast<const T*>(a.v)[at + lane + 32 * e]);
-                    }
-                for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
-                if (z > m) {
-                    const float keep = ex2(m - z);
-                    l *= keep;
-                    for (int e = 0; e < 4; ++e) o[e] *= keep;
-                    m = z;
-                }
-                const float w = ex2(z - m);
-                l += w;
-                for (int e = 0; e < 4; ++e) o[e] = fmaf(lm_to_f<T>(lm_from_f<T>(w)), v[e], o[e]);
+    constexpr int kRows = 256 / kJoinSlices;
+    const int r = (int)blockIdx.x / kJoinSlices + 1, slice = (int)blockIdx.x % kJoinSlices, ranges = __ldcg(a.counts + 1);
+    if (r < ranges) {
+        const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + r)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + r - 1));
+        const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
+        if (c.z > 0 && !(same(d) && d.z > 0)) {
+            const ChunkUnit u = a.units[c.x];
+            int last = r;                              // the pair's last range
+            while (last + 1 < ranges) {
+                const int4 e = __ldcg(reinterpret_cast<const int4*>(a.cuts + last + 1));
+                if (!same(e) || e.z == 0) break;
+                ++last;
             }
-            T* out = static_cast<T*>(a.out) + (s.start + i) * a.out_stride + h * a.out_head;
-            for (int e = 0; e < 4; ++e)
-                if (lane + 32 * e < a.D) out[lane + 32 * e] = lm_from_f<T>(p < 0 ? 0.f : o[e] / l);
+            const int parts = last - r + 2;
+            const int in_pair = slice * kRows + (int)(threadIdx.x & (kRows - 1)), sub = (int)threadIdx.x / kRows, row = u.row0 + in_pair, g = in_pair >> 7, in_tile = in_pair & 127;
+            const auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (r - 1) + 1 : 2 * (r + i - 1)) * 2 + g; };
+            if (row < u.rows) {
+                float top = -INFINITY, sum = 0.f;
+                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(a.part_ml + slot(i) * 128 + in_tile).x);
+                for (int i = 0; i < parts; ++i) {
+                    const float2 ml = __ldcg(a.part_ml + slot(i) * 128 + in_tile);
+                    sum = fmaf(ml.x == -INFINITY ? 0.f : ex2(ml.x - top), ml.y, sum);
+                }
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const int token = row / a.group;
+                T* dst = static_cast<T*>(a.out) + (int64_t)(u.start + token) * a.out_stride + (int64_t)(c.y * a.group + row - token * a.group) * a.out_head;
+                for (int i4 = sub; i4 < a.D / 4; i4 += 128 / kRows) {
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int i = 0; i < parts; ++i) {
+                        const float m = __ldcg(a.part_ml + slot(i) * 128 + in_tile).x, w = m == -INFINITY ? 0.f : ex2(m - top);
+                        const float4 o = __ldcg(a.part_o + (slot(i) * (DP / 4) + i4) * 128 + in_tile);
+                        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+                    }
+                    dst[4 * i4] = lm_from_f<T>(acc.x * inv); dst[4 * i4 + 1] = lm_from_f<T>(acc.y * inv); dst[4 * i4 + 2] = lm_from_f<T>(acc.z * inv); dst[4 * i4 + 3] = lm_from_f<T>(acc.w * inv);
+                }
+            }
         }
     }
     if (nf) nf->end(job_id);
 }
 
-int check_chunk(const pb_chunk_attn_params* p, ChunkArgs& a) {
+typedef void (*JoinFn)(ChunkArgs, uint32_t, FinishedBlockNotifier*);
+typedef void (*ChunkFn)(ChunkArgs, CUtensorMap, CUtensorMap);
+
+struct ChunkPlan {
+    ChunkArgs a;
+    AttnArgs few;              // own_kernel's, where it takes part
+    int DP, NT;
+    bool half, many, has_few;  // many: plan, chunk and join kernels
+    int64_t few_blocks, join_blocks;
+    uint64_t scratch;
+    OwnFn own;
+    uint32_t own_smem;
+    ChunkFn chunk;
+    JoinFn join;
+};
+
+template <typename T> void pick_chunk(ChunkPlan& pl) {
+    pl.own = own_fn<T, 3>(pl.DP, pl.NT);
+    pl.chunk = pl.DP == 64 ? chunk_kernel<T, 64> : chunk_kernel<T, 128>;
+    pl.join = pl.DP == 64 ? join_kernel<T, 64> : join_kernel<T, 128>;
+}
+
+int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     const char* who = "pb_chunk_attn";
     PB_REQUIRE(p != nullptr, "%s: NULL params", who);
     PB_REQUIRE(p->dtype == PB_BF16 || p->dtype == PB_F16, "%s: dtype %d (PB_BF16 or PB_F16)", who, p->dtype);
@@ -89,18 +730,76 @@ int check_chunk(const pb_chunk_attn_params* p, ChunkArgs& a) {
     PB_REQUIRE(p->page_stride % 8 == 0 && p->token_stride % 8 == 0 && p->head_stride % 8 == 0 && p->page_stride > 0 && p->token_stride > 0 && p->head_stride > 0, "%s: strides of the cache are positive multiples of 8", who);
     PB_REQUIRE(p->q_stride % 8 == 0 && p->q_head_stride % 8 == 0, "%s: rows of q start on 16 bytes", who);
     PB_REQUIRE(rows_apart(p->tokens, p->out_stride, p->head_dim) && rows_apart(p->q_heads, p->out_head_stride, p->head_dim), "%s: rows of out overlap (strides %lld, %lld)", who, (long long)p->out_stride, (long long)p->out_head_stride);
-    if (p->batch > 0 && p->tokens > 0 && p->max_new > 0) {
+    memset(&pl, 0, sizeof(pl));
+    ChunkArgs& a = pl.a;
+    a.max_new = std::min(p->max_new, p->tokens);
+    a.batch = a.max_new > 0 ? p->batch : 0;
+    a.group = p->q_heads / p->kv_heads;
+    PB_REQUIRE((int64_t)a.max_new * a.group <= 1 << 30, "%s: %d new tokens of %d heads for a key head are too many rows", who, a.max_new, a.group);
+    if (a.batch > 0) {
         PB_REQUIRE(p->q && p->out && p->starts && p->lens, "%s: NULL buffer", who);
         PB_REQUIRE(p->max_len == 0 || (p->k_cache && p->v_cache && p->block_table && p->n_pages > 0), "%s: a NULL cache or block_table, or a cache without pages", who);
         PB_REQUIRE(aligned(p->q, 16) && aligned(p->k_cache, 16) && aligned(p->v_cache, 16) && aligned(p->out, 2), "%s: q and the cache must be 16-byte aligned", who);
         PB_REQUIRE(aligned(p->block_table, 4) && aligned(p->starts, 4) && aligned(p->lens, 4), "%s: a table is not aligned to its elements", who);
     }
-    memset(&a, 0, sizeof(a));
     a.q = p->q; a.k = p->k_cache; a.v = p->v_cache; a.out = p->out; a.block_table = p->block_table; a.starts = p->starts; a.lens = p->lens;
     a.q_stride = p->q_stride; a.q_head = p->q_head_stride; a.out_stride = p->out_stride; a.out_head = p->out_head_stride;
     a.page_stride = p->page_stride; a.token_stride = p->token_stride; a.head_stride = p->head_stride; a.table_stride = p->table_stride;
-    a.batch = p->tokens > 0 && p->max_new > 0 ? p->batch : 0; a.tokens = p->tokens; a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.group = p->q_heads / p->kv_heads; a.D = p->head_dim;
-    a.page = p->page_size; a.n_pages = (int)p->n_pages; a.max_new = p->max_new < p->tokens ? p->max_new : p->tokens; a.max_len = p->max_len; a.window = p->window; a.scale = p->scale;
+    a.tokens = p->tokens; a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.D = p->head_dim;
+    a.page = p->page_size; a.n_pages = (int)p->n_pages; a.max_len = p->max_len; a.window = p->window < p->max_len ? p->window : 0; a.scale = p->scale;
+    a.box_rows = 8;
+    while (a.box_rows < 64 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
+    pl.DP = p->head_dim <= 64 ? 64 : 128;
+    pl.half = p->dtype == PB_F16;
+    const int64_t most_rows = (int64_t)a.max_new * a.group;
+    pl.many = a.max_new > 1 && most_rows > kFewRows && a.batch > 0 && a.max_len > 0;
+    pl.has_few = !pl.many || a.batch > 1;
+    if (pl.has_few) {
+        const int few_rows = (int)(pl.many ? std::min<int64_t>(most_rows, kFewRows) : std::max<int64_t>(most_rows, 1));
+        pl.NT = few_rows <= 8 ? 1 : 2;
+        AttnArgs& f = pl.few;
+        f.q = a.q; f.k = a.k; f.v = a.v; f.out = a.out; f.block_table = a.block_table; f.own_lens = a.lens; f.starts = a.starts;
+        f.q_stride = a.q_stride; f.q_head = a.q_head; f.out_stride = a.out_stride; f.out_head = a.out_head;
+        f.page_stride = a.page_stride; f.token_stride = a.token_stride; f.head_stride = a.head_stride; f.table_stride = a.table_stride;
+        f.batch = a.batch; f.group = a.group; f.D = a.D; f.page = a.page; f.n_pages = a.n_pages; f.max_own = a.max_len; f.scale = a.scale; f.kv_heads = a.kv_heads;
+        f.tokens = a.tokens; f.max_new = a.max_new; f.window = a.window; f.few = pl.many ? kFewRows : 0; f.beside = pl.many;
+        f.per_piece = (uint32_t)ceil_div(1 << 16, a.D / 4);
+        f.out_vec = aligned(a.out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
+        f.splits = f.row_parts = 1;
+        f.row_groups = (int)ceil_div<int64_t>(few_rows, 8 * pl.NT);
+        // as for pb_prefix_attn: clusters of blocks on a sequence and key head while they fit the GPU, 128 tokens each at least
+        const int64_t units = (int64_t)a.batch * a.kv_heads * f.row_groups, tokens = a.window ? std::min<int64_t>(a.window + a.max_new, a.max_len) : a.max_len;
+        f.ranks = 1;
+        while (f.ranks < kMaxRanks && units > 0 && units * f.ranks * 2 <= 3 * 148 && tokens / (2 * f.ranks) >= 128) f.ranks *= 2;
+        pl.few_blocks = std::max<int64_t>(units * f.ranks, 1);
+        PB_REQUIRE(pl.few_blocks <= 0x7fffffff, "%s: too many blocks for one launch", who);
+    }
+    pl.own_smem = pl.DP == 64 ? OwnShape<64>::smem : OwnShape<128>::smem;
+    if (pl.half) pick_chunk<__half>(pl);
+    else pick_chunk<__nv_bfloat16>(pl);
+    if (pl.many) {
+        a.few = pl.has_few ? kFewRows : 0;
+        const int64_t units = std::min((int64_t)a.tokens * a.group / 256 + a.batch, a.batch * ceil_div<int64_t>(most_rows, 256));
+        PB_REQUIRE(units * a.kv_heads <= 1 << 30, "%s: %lld pairs of row tiles are too many", who, (long long)units);
+        a.max_units = (int)units;
+        const int64_t cache = (int64_t)a.batch * a.max_len * a.kv_heads * a.D * 4;
+        const int rounds = (int)std::min<int64_t>(std::max<int64_t>(cache >> 26, 1), kMaxRounds);
+        a.max_ranges = kChunkBlocks * rounds;
+        uint64_t at = 0;
+        const auto take = [&](uint64_t bytes) {
+            const uint64_t from = at;
+            at += round_up<uint64_t>(bytes, 128);
+            return (char*)p->scratch + from;
+        };
+        a.counts = (int32_t*)take(8);
+        a.cuts = (ChunkCut*)take((a.max_ranges + 1) * sizeof(ChunkCut));
+        a.units = (ChunkUnit*)take(a.max_units * sizeof(ChunkUnit));
+        a.before = (int64_t*)take((a.max_units + 1) * sizeof(int64_t));
+        a.part_ml = (float2*)take(2ull * a.max_ranges * 256 * sizeof(float2));
+        a.part_o = (float4*)take(2ull * a.max_ranges * 256 * pl.DP * sizeof(float));
+        pl.scratch = at;
+        pl.join_blocks = (int64_t)(a.max_ranges - 1) * kJoinSlices;
+    }
     return PB_OK;
 }
 
