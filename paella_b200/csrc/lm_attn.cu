@@ -99,15 +99,15 @@ constexpr float kSlack = 8.f;
 // fp16 has few exponents below 1: its values are scaled up by 2^5 (2^13 with the slack; the sums with them).
 template <typename T> __device__ __forceinline__ constexpr float p_shift() { return sizeof(T) == 2 && std::is_same<T, __half>::value ? 5.f : 0.f; }
 
-// 64 keys: 2^(s c + base) from their scores, rounded to pairs, and the sum of what they were.  One pair in four on the multipliers (none, one in eight, three, two:
+// 2 N keys (64, as all figures): 2^(s c + base) from their scores, rounded to pairs, and the sum of what they were.  One pair in four on the multipliers (none, one in eight, three, two:
 // 156, 168, 144, 158 us against 139 behind 16384 tokens).
-template <typename T>
-__device__ __forceinline__ float values_of(const uint32_t* s, float c, float base, uint32_t (&p)[32]) {
+template <typename T, int N>
+__device__ __forceinline__ float values_of(const uint32_t* s, float c, float base, uint32_t (&p)[N]) {
     const uint64_t c2 = pack_f32x2(__float_as_uint(c), __float_as_uint(c)), base2 = pack_f32x2(__float_as_uint(base), __float_as_uint(base));
     uint64_t sum[2] = {0, 0};
     float x, y;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < N; ++j) {
         uint64_t e = fma_f32x2(pack_f32x2(s[2 * j], s[2 * j + 1]), c2, base2);
         if (j % 4 == 3) {
             e = ex2_pair(e);
@@ -1200,7 +1200,7 @@ int pb_chunk_attn_info(const pb_chunk_attn_params* p, pb_launch_info* out) {
     LaunchHolds holds;
     if (pl.many) {
         holds.add((const void*)pl.chunk, kChunkBlocks, 384, pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem, 512);
-        holds.add((const void*)pl.join, std::min<int64_t>(pl.join_blocks, 148 * 16), 128, 0, 0);
+        holds.add((const void*)pl.join, std::min<int64_t>(pl.join_blocks, 148 * 8), 256, 0, 0);
     }
     if (pl.has_few) holds.add((const void*)pl.own, pl.few_blocks, 128, pl.own_smem, 0);
     holds.declare(reporting, out);
@@ -1236,7 +1236,7 @@ int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t j
         const int e = lm_launch("pb_chunk_attn (few rows)", pl.own, dim3((unsigned)pl.few_blocks), dim3(128), pl.own_smem, st, pl.few.ranks, pl.few, job_id, pl.many ? (FinishedBlockNotifier*)nullptr : nf);
         if (e != PB_OK || !pl.many) return e;
     }
-    return lm_launch("pb_chunk_attn (parts)", pl.join, dim3((unsigned)pl.join_blocks), dim3(128), 0, st, 1, pl.a, job_id, nf);
+    return lm_launch("pb_chunk_attn (parts)", pl.join, dim3((unsigned)pl.join_blocks), dim3(256), 0, st, 1, pl.a, job_id, nf);
 }
 
 }  // extern "C"

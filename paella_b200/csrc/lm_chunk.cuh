@@ -14,7 +14,7 @@
 namespace pb {
 namespace {
 
-constexpr int kFewRows = 16, kChunkBlocks = 148, kMaxRounds = 4, kJoinSlices = 4;
+constexpr int kFewRows = 16, kChunkBlocks = 148, kMaxRounds = 4, kJoinSlices = 8;
 
 // 256 rows of a sequence (fewer at its end), for every key head.
 struct alignas(16) ChunkUnit {
@@ -24,6 +24,7 @@ struct alignas(16) ChunkUnit {
 static_assert(sizeof(ChunkUnit) == 32, "eight words, one a lane");
 struct alignas(16) ChunkCut {            // where a range begins
     int32_t unit, head, step, pad;
+    ChunkUnit begins;                    // a copy of that unit, so that a block has it in one access
 };
 
 struct ChunkArgs {
@@ -48,112 +49,122 @@ constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 6;
 
 __device__ __forceinline__ int ceil_pos(int x, int d) { return x > 0 ? (x + d - 1) / d : 0; }
 
-// The work: units, their costs, and the ranges.  One block; a sequence a warp, its pairs a lane each.
+// The work: units, their costs, and the ranges.  One block, which the others wait for: a thread a sequence, a unit, a range, with all that is looked up in shared memory as long as there are no more than
+// kPlanUnits units.
+constexpr int kPlanUnits = 2048;
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ ChunkArgs a) {
-    __shared__ int64_t s_scan[32];
-    __shared__ int s_base[1024];
+    __shared__ int64_t s_scan[2][32], s_before[kPlanUnits + 1];
+    __shared__ int s_base[1025];
+    __shared__ ChunkSeq s_seq[1024];
+    __shared__ int s_tiles[kPlanUnits];            // tiles, twice, and whether there are two row tiles
     griddep_wait();
     griddep_launch();
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    // inclusive sums over the block
-    const auto scan = [&](int64_t x) {
+    const bool in_shared = a.max_units <= kPlanUnits;
+    int turn = 0;
+    const auto scan_warp = [&](int64_t x) {
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
             const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        __syncthreads();
-        if (lane == 31) s_scan[warp] = x;
-        __syncthreads();
-        if (warp == 0) {
-            int64_t w = s_scan[lane];
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-                if (lane >= o) w += y;
-            }
-            s_scan[lane] = w;
-        }
-        __syncthreads();
-        return x + (warp ? s_scan[warp - 1] : 0);
+        return x;
     };
-    int64_t units = 0;
+    // Sums of the threads up to this one, and of all.
+    const auto scan = [&](int64_t x, int64_t& all) {
+        x = scan_warp(x);
+        if (lane == 31) s_scan[turn][warp] = x;
+        __syncthreads();
+        const int64_t warps = scan_warp(s_scan[turn][lane]);
+        turn ^= 1;                                 // (who writes there again has passed the next barrier, and with it everyone has read)
+        all = __shfl_sync(0xffffffffu, warps, 31);
+        const int64_t ahead = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
+        return x + (warp ? ahead : 0);
+    };
+    int units = 0;
+    int64_t sum = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 1024) {
         int mine = 0;
         if (b0 + t < a.batch) {
             const ChunkSeq s = chunk_seq(a.starts, a.lens, b0 + t, a.tokens, a.max_new, a.max_len, true);
-            const int64_t rows = (int64_t)s.rows * a.group;
-            mine = rows > a.few ? (int)((rows + 255) / 256) : 0;
+            const int rows = s.rows * a.group;
+            mine = rows > a.few ? (rows + 255) / 256 : 0;
+            s_seq[t] = s;
         }
-        const int64_t upto = scan(mine);
-        s_base[t] = (int)min(units + upto - mine, (int64_t)a.max_units);
+        int64_t all;
+        const int64_t upto = scan(mine, all);
+        s_base[t] = (int)min((long long)(upto - mine), 0x7fffffffLL);
+        // (starts that fall can make more units than rows have room for: those behind the last place are left out)
+        const int here = (int)min((long long)all, (long long)(a.max_units - units)), n = min(1024, a.batch - b0);
+        if (all > here && t == 0) atomicExch(&g_attn_flag, kFlagLmLength);
         __syncthreads();
-        const int n = min(1024, a.batch - b0);
-        for (int i = warp; i < n; i += 32) {
-            const ChunkSeq s = chunk_seq(a.starts, a.lens, b0 + i, a.tokens, a.max_new, a.max_len, false);
-            const int rows = s.rows * a.group, base = s_base[i];
-            if (rows <= a.few) continue;
-            // (starts that fall can make more units than rows have room for: those behind the last place are left out)
-            for (int p = lane; p < (rows + 255) / 256 && base + p < a.max_units; p += 32) {
+        for (int i0 = 0; i0 < here; i0 += 1024) {
+            const int i = i0 + t;
+            int64_t cost = 0;
+            int tiles = 0;
+            if (i < here) {
+                int lo = 0, hi = n - 1;            // the last sequence whose units begin at or in front of this one (sequences without units share their beginning with the next)
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) / 2;
+                    if (s_base[mid] <= i) lo = mid;
+                    else hi = mid - 1;
+                }
+                const ChunkSeq s = s_seq[lo];
                 ChunkUnit u;
-                u.b = b0 + i; u.start = s.start; u.rows = rows; u.first = s.first; u.row0 = 256 * p;
-                const int pos0 = s.first + u.row0 / a.group, pos1 = s.first + (min(u.row0 + 256, rows) - 1) / a.group;
+                u.b = b0 + lo; u.start = s.start; u.rows = s.rows * a.group; u.first = s.first; u.row0 = 256 * (i - s_base[lo]);
+                const int pos0 = s.first + u.row0 / a.group, pos1 = s.first + (min(u.row0 + 256, u.rows) - 1) / a.group;
                 u.end = max(pos1 + 1, 0);
                 u.tile0 = a.window ? max(pos0 - a.window + 1, 0) / 128 : 0;
                 u.tiles = max((u.end + 127) / 128 - u.tile0, 0);
-                a.units[base + p] = u;
+                a.units[units + i] = u;
+                const bool two = u.row0 + 128 < u.rows;
+                cost = kCostPair + (int64_t)u.tiles * (two ? kCostTwo : kCostOne);
+                tiles = 2 * u.tiles + two;
             }
+            int64_t chunk;
+            const int64_t before = sum + scan(cost, chunk) - cost;
+            if (i < here) {
+                if (in_shared) { s_before[units + i] = before; s_tiles[units + i] = tiles; }
+                else a.before[units + i] = before;
+            }
+            sum += chunk;
         }
-        const int64_t all = s_scan[31];
-        __syncthreads();
-        units += all;
-    }
-    const int U = (int)min(units, (int64_t)a.max_units);
-    if (units > a.max_units && t == 0) atomicExch(&g_attn_flag, kFlagLmLength);
-    __syncthreads();                     // (units are this block's own stores)
-    int64_t sum = 0;
-    for (int u0 = 0; u0 < U; u0 += 1024) {
-        int64_t mine = 0;
-        if (u0 + t < U) {
-            const ChunkUnit u = a.units[u0 + t];
-            mine = kCostPair + (int64_t)u.tiles * (u.row0 + 128 < u.rows ? kCostTwo : kCostOne);
-        }
-        const int64_t upto = scan(mine);
-        if (u0 + t < U) a.before[u0 + t] = sum + upto - mine;
-        sum += s_scan[31];
+        units += here;
         __syncthreads();
     }
-    if (t == 0) a.before[U] = sum;
-    __syncthreads();
     const int64_t total = sum * a.kv_heads;
     // Ranges: one for each block, several where they are long (so that the blocks are at the same keys at the same time, and those come from the L2 cache), fewer where there is little to do.
     const long long rounds = min(max((long long)total / (kChunkBlocks * 400), 1LL), (long long)(a.max_ranges / kChunkBlocks));
     int N = (int)min(kChunkBlocks * rounds, max((long long)total / (kCostPair + 3 * kCostTwo), 1LL));
-    if (U == 0) N = 0;
+    if (units == 0) N = 0;
     for (int r = t; r <= N; r += 1024) {
-        ChunkCut c = {0, a.kv_heads, 0, 0};
+        ChunkCut c = {0, a.kv_heads, 0, 0, {}};
         if (r < N) {
             const int64_t w = total / N * r + total % N * r / N;
             c.head = (int)(w / sum);
             const int64_t rest = w - c.head * sum;
-            int lo = 0, hi = U - 1;      // the last unit that begins at or in front of it
+            const int64_t* table = in_shared ? s_before : a.before;
+            int lo = 0, hi = units - 1;            // the last unit that begins at or in front of it
             while (lo < hi) {
                 const int mid = (lo + hi + 1) / 2;
-                if (a.before[mid] <= rest) lo = mid;
+                if (table[mid] <= rest) lo = mid;
                 else hi = mid - 1;
             }
-            const ChunkUnit u = a.units[lo];
-            const int each = u.row0 + 128 < u.rows ? kCostTwo : kCostOne, near = (int)min((long long)total / N / (8 * each), 1000LL);
-            const int step = (int)(max((long long)(rest - a.before[lo] - kCostPair), 0LL) / each);
             c.unit = lo;
-            if (step > near && step < u.tiles - near) c.step = step;
-            else if (step > near || 2 * step > u.tiles) {                // a cut near a pair's end is none
-                if (++c.unit == U) { c.unit = 0; ++c.head; }
+            c.begins = a.units[lo];
+            const int tiles = in_shared ? s_tiles[lo] >> 1 : c.begins.tiles;
+            const int each = (in_shared ? s_tiles[lo] & 1 : c.begins.row0 + 128 < c.begins.rows) ? kCostTwo : kCostOne, near = (int)min((long long)total / N / (8 * each), 1000LL);
+            const int step = (int)(max((long long)(rest - table[lo] - kCostPair), 0LL) / each);
+            if (step > near && step < tiles - near) {
+                c.step = step;
+            } else if (step > near || 2 * step > tiles) {                // a cut near a pair's end is none
+                if (++c.unit == units) { c.unit = 0; ++c.head; }
+                c.begins = a.units[c.unit];
             }
         }
         a.cuts[r] = c;
     }
-    if (t == 0) { a.counts[0] = U; a.counts[1] = N; }
+    if (t == 0) { a.counts[0] = units; a.counts[1] = N; }
 }
 
 // The parts of a block's ranges, one after the other.
@@ -164,17 +175,15 @@ struct ChunkWalk {
     const ChunkArgs& a;
     int range, units, ranges, unit, head, step, to_unit, to_head, to_step, word;
     __device__ __forceinline__ ChunkWalk(const ChunkArgs& args) : a(args) {
+        range = (int)blockIdx.x;
+        begin();                         // (what lies there if there are fewer ranges is not used)
         units = __ldcg(a.counts);
         ranges = __ldcg(a.counts + 1);
-        range = (int)blockIdx.x;
-        begin();
     }
-    __device__ __forceinline__ void fetch() { word = __ldcg(reinterpret_cast<const int32_t*>(a.units + unit) + (threadIdx.x & 7)); }
     __device__ __forceinline__ void begin() {
-        if (range >= ranges) return;
         const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + range)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + range + 1));
+        word = __ldcg(reinterpret_cast<const int32_t*>(&a.cuts[range].begins) + (threadIdx.x & 7));
         unit = c.x; head = c.y; step = c.z; to_unit = d.x; to_head = d.y; to_step = d.z;
-        if (unit < units) fetch();
     }
     __device__ __forceinline__ bool next(ChunkItem& x) {                 // a whole warp
         while (true) {
@@ -182,7 +191,7 @@ struct ChunkWalk {
             const bool in_last = head == to_head && unit == to_unit;
             if (head > to_head || (head == to_head && unit > to_unit) || (in_last && step >= to_step)) {
                 range += (int)gridDim.x;
-                begin();
+                if (range < ranges) begin();
                 continue;
             }
             int32_t w[8];
@@ -193,23 +202,29 @@ struct ChunkWalk {
             x.slot = x.from > 0 ? 2 * range : x.to < x.tiles ? 2 * range + 1 : -1;
             step = 0;
             if (++unit == units) { unit = 0; ++head; }
-            fetch();                     // the next one's, in time
+            word = __ldcg(reinterpret_cast<const int32_t*>(a.units + unit) + (threadIdx.x & 7));       // the next one's, in time
             return true;
         }
     }
 };
 
-// Warps 0-3 and 4-7: softmax of one row tile each, a row a thread; warps 8 and 11 copy keys and values; warps 9 and 10 issue the products of one row tile each, 64 keys at a time.  As in
-// prefix_kernel: S = Q K^T into 64 columns of tensor memory, P takes its place as the A operand of O += P V.  Rings and barriers run on from one pair to the next; the next pair's queries come while the last
-// values of the one before are worked on.
+// Warps 0-3 and 4-7: softmax of one row tile each, a row a thread; warps 8 and 11 copy keys and values; warps 9 and 10 issue the products of one row tile each.  As in prefix_kernel: S = Q K^T into 64
+// memory, P takes its place, 64 keys at a time, as the A operand of O += P V.  Rings and barriers run on from one pair to the next;
+// the next pair's queries come while the results of the one before are written.
+// Registers that a load from tensor memory wrote, behind its wait: what uses them stays behind it, too.
+__device__ __forceinline__ void pin(uint32_t (&r)[32]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+    asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages;
     constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
     static_assert(kStages >= 4, "a wait for an entry of the ring has seen the one before in its place");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_free[2], s_q[2], s_edge;
-    __shared__ int s_pages[2][4][32];
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_free[2], s_edge;
+    __shared__ int s_pages[2][4][16];
     __shared__ uint32_t s_odd[8];
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
@@ -235,7 +250,6 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             mbar_init(smem_u32(&s_turn[i]), 1);
             mbar_init(smem_u32(&s_done[i]), 1);
             mbar_init(smem_u32(&s_free[i]), 4);
-            mbar_init(smem_u32(&s_q[i]), 128);
         }
         mbar_init(smem_u32(&s_edge), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -260,7 +274,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         // One warp copies keys, one values.  A lane copies a box: `box_rows` tokens of a page, 64 values of each, whose page it looked up two copies ahead.
         const bool values = warp == 11;
         const int box = lane / kBlocks, blk = lane % kBlocks;
-        const uint32_t words = smem_u32(&s_pages[values][0][lane]);
+        const uint32_t words = smem_u32(&s_pages[values][0][box & 15]);
         struct Tiles {                   // the block's tiles in order
             ChunkWalk walk;
             ChunkItem x;
@@ -280,8 +294,8 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         int i = 0, i_ahead = 0;
         const auto look_up = [&]() {
             const int token = (ahead.x.tile0 + ahead.step) * 128 + box * a.box_rows;
-            if (ahead.more && box * a.box_rows < 128 && token < ahead.x.end)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + (i_ahead & 3) * 128), "l"(a.block_table + ahead.x.b * a.table_stride + token / a.page) : "memory");
+            if (ahead.more && blk == 0 && box * a.box_rows < 128 && token < ahead.x.end)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + (i_ahead & 3) * 64), "l"(a.block_table + ahead.x.b * a.table_stride + token / a.page) : "memory");
             asm volatile("cp.async.commit_group;" ::: "memory");
             ++i_ahead;
             if (ahead.more) ahead.on();
@@ -299,8 +313,8 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             // Values of a tile whose keys not all rows see: what lies behind the last one is zeros, and so is what is not finite (zero times which would be NaN for
             // the rows that do not see it; s_odd tells the softmax groups to add it where it is seen).
             bool edge = false;
+            const int pos0 = now.x.first + now.x.row0 / a.group, pos1 = now.x.end - 1;
             if (values) {
-                const int pos0 = now.x.first + now.x.row0 / a.group, pos1 = now.x.end - 1;
                 edge = first + 128 > pos0 + 1 || (a.window && first < pos1 - a.window + 1);
                 if (fresh && lane == 0) s_odd[item & 7] = 0;
                 fresh = false;
@@ -310,7 +324,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             __syncwarp();
             if (box < boxes) {
                 int page;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(page) : "r"(words + (i & 3) * 128) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(page) : "r"(words + (i & 3) * 64) : "memory");
                 if ((uint32_t)page >= (uint32_t)a.n_pages) {
                     atomicExch(&g_attn_flag, kFlagLmPage);
                     page = a.n_pages;                                    // outside of the map: zeros
@@ -324,17 +338,30 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 if (!ok) break;
                 constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
                 bool odd = false;
-                for (int c = lane; c < 128 * 8 * kBlocks; c += 32) {
-                    const uint32_t from = to + c * 16;
-                    if ((c >> 3) % 128 >= there) {
-                        st_shared_v4(from, 0, 0, 0, 0);
-                        continue;
+                for (int c = there * 8 + lane; c < 1024; c += 32)
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i) st_shared_v4(to + i * kBlock + c * 16, 0, 0, 0, 0);
+                // rows that not all see: those behind the first row's position, or, under a window, all
+                const int rows0 = a.window ? 0 : max(pos0 + 1 - first, 0);
+#pragma unroll 1
+                for (int c0 = rows0 * 8; c0 < there * 8; c0 += 128) {
+                    uint4 v[4 * kBlocks];
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < 4 * kBlocks; ++i) {
+                        const int c = c0 + 32 * (i / kBlocks) + lane;
+                        v[i] = c < there * 8 ? ld_shared_v4(to + (i % kBlocks) * kBlock + c * 16) : make_uint4(0, 0, 0, 0);
                     }
-                    uint4 v = ld_shared_v4(from);
-                    const uint32_t x = __vcmpeq2(v.x & kExp, kExp), y = __vcmpeq2(v.y & kExp, kExp), z = __vcmpeq2(v.z & kExp, kExp), w = __vcmpeq2(v.w & kExp, kExp);
-                    if (x | y | z | w) {
-                        odd = true;
-                        st_shared_v4(from, v.x & ~x, v.y & ~y, v.z & ~z, v.w & ~w);
+#pragma unroll
+                    for (int i = 0; i < 4 * kBlocks; ++i) any |= __vcmpeq2(v[i].x & kExp, kExp) | __vcmpeq2(v[i].y & kExp, kExp) | __vcmpeq2(v[i].z & kExp, kExp) | __vcmpeq2(v[i].w & kExp, kExp);
+                    if (!any) continue;
+                    odd = true;
+#pragma unroll
+                    for (int i = 0; i < 4 * kBlocks; ++i) {
+                        const int c = c0 + 32 * (i / kBlocks) + lane;
+                        if (c < there * 8)
+                            st_shared_v4(to + (i % kBlocks) * kBlock + c * 16, v[i].x & ~__vcmpeq2(v[i].x & kExp, kExp), v[i].y & ~__vcmpeq2(v[i].y & kExp, kExp), v[i].z & ~__vcmpeq2(v[i].z & kExp, kExp),
+                                         v[i].w & ~__vcmpeq2(v[i].w & kExp, kExp));
                     }
                 }
                 if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[item & 7] = 1;
@@ -363,6 +390,37 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         ChunkWalk walk(a);
         ChunkItem x;
         bool ok = true;
+        // This group's queries, neighbouring lanes on neighbouring bytes of a row: when the scores of the item before have become values, while its results are written.
+        constexpr int kPerRow = DP / 8, kStep = 32 / kPerRow;                    // 16-byte pieces of a row; rows from one of a lane's pieces to the next
+        const int piece = lane % kPerRow, r0 = lane / kPerRow, b_step = kStep / a.group, h_step = kStep - b_step * a.group;
+        const int64_t q_step = b_step * a.q_stride + h_step * a.q_head, q_wrap = a.q_stride - a.group * a.q_head;
+        const uint32_t q_block = q_smem + g * kTile + (piece >> 3) * kBlock;
+        const auto load_q = [&](const ChunkItem& y) {
+            int r = y.row0 + g * 128 + r0;
+            const int token = r / a.group;
+            int h = r - token * a.group;
+            const T* src = static_cast<const T*>(a.q) + (int64_t)(y.start + token) * a.q_stride + ((int64_t)y.head * a.group + h) * a.q_head + 8 * piece;
+#pragma unroll 8
+            for (int i = r0; i < 128; i += kStep) {
+                const bool there = r < y.rows && 8 * piece < a.D;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_block + i * 128 + (((piece & 7) ^ (i & 7)) << 4)), "l"(there ? src : static_cast<const T*>(a.q)), "r"(there ? 16 : 0) : "memory");
+                r += kStep;
+                h += h_step;
+                src += q_step;
+                if (h >= a.group) { h -= a.group; src += q_wrap; }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (a.scale < 0.f) {                                                 // |scale| from here on
+#pragma unroll 1
+                for (int i = r0; i < 128; i += kStep) {
+                    const uint32_t at = q_block + i * 128 + (((piece & 7) ^ (i & 7)) << 4);
+                    const uint4 v = ld_shared_v4(at);
+                    st_shared_v4(at, v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+        };
         while (ok && walk.next(x)) {
             const int n = x.to - x.from;
             if (n <= 0) continue;
@@ -378,6 +436,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 }
                 continue;
             }
+            load_q(x);
             // Two groups take turns at the tensor cores, as in prefix_kernel.
             const auto take_turn = [&]() {
                 if (!two) return true;
@@ -402,7 +461,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 if (h == 1) keys.on();
                 return true;
             };
-            ok = wait(&s_q[g], items & 1) && take_turn() && scores(0) && take_turn() && scores(1);
+            ok = take_turn() && scores(0) && take_turn() && scores(1);
             for (int u = 0; ok && u < n; ++u, ++tiles) {
                 const bool last = u == n - 1;
 #pragma unroll
@@ -441,133 +500,122 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             const int token = row / a.group;
             return (int64_t)(x.start + token) * token_stride + (int64_t)(x.head * a.group + row - token * a.group) * head_stride;
         };
-        const auto write = [&](const ChunkItem& x, int row, int col, const uint32_t (&o)[32], float f) {       // 32 values of a row
-            T* dst = static_cast<T*>(a.out) + place(x, row, a.out_stride, a.out_head) + col;
-            const bool vec = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * 2) | (uintptr_t)(a.out_head * 2)) & 15) == 0;
+        const bool out_vec = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * 2) | (uintptr_t)(a.out_head * 2)) & 15) == 0;
+        // 32 values of each lane's row, from column `col` on.  Four lanes exchange their 16-byte pieces first, so that they write 64 bytes of one row at a time (each 16 of its own row: 7000
+        // clocks for two row tiles instead of 2000).  The whole warp.
+        const auto write = [&](const ChunkItem& x, T* base, int row, int col, const uint32_t (&o)[32], float f) {
+            uint4 v[4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-                if (col + e >= a.D) break;
-                float v[8];
+            for (int e = 0; e < 4; ++e)
+                v[e] = make_uint4(lm_pack2<T>(__uint_as_float(o[8 * e]) * f, __uint_as_float(o[8 * e + 1]) * f), lm_pack2<T>(__uint_as_float(o[8 * e + 2]) * f, __uint_as_float(o[8 * e + 3]) * f),
+                                  lm_pack2<T>(__uint_as_float(o[8 * e + 4]) * f, __uint_as_float(o[8 * e + 5]) * f), lm_pack2<T>(__uint_as_float(o[8 * e + 6]) * f, __uint_as_float(o[8 * e + 7]) * f));
+            if (!out_vec) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * f;
-                if (vec) {
-                    *reinterpret_cast<uint4*>(dst + e) = make_uint4(lm_pack2<T>(v[0], v[1]), lm_pack2<T>(v[2], v[3]), lm_pack2<T>(v[4], v[5]), lm_pack2<T>(v[6], v[7]));
-                } else {
+                for (int e = 0; e < 4; ++e) {
+                    if (col + 8 * e >= a.D || row >= x.rows) break;
+                    const T* y = reinterpret_cast<const T*>(&v[e]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) dst[e + k] = lm_from_f<T>(v[k]);
+                    for (int k = 0; k < 8; ++k) base[col + 8 * e + k] = y[k];
                 }
+                return;
+            }
+            const auto swap = [&](uint4& lo, uint4& hi, int with) {              // my `hi` for the other lane's `lo`, or the other way round
+                const bool up = lane & with;
+                uint4 give = up ? lo : hi;
+                give.x = __shfl_xor_sync(0xffffffffu, give.x, with);
+                give.y = __shfl_xor_sync(0xffffffffu, give.y, with);
+                give.z = __shfl_xor_sync(0xffffffffu, give.z, with);
+                give.w = __shfl_xor_sync(0xffffffffu, give.w, with);
+                (up ? lo : hi) = give;
+            };
+            swap(v[0], v[1], 1);
+            swap(v[2], v[3], 1);
+            swap(v[0], v[2], 2);
+            swap(v[1], v[3], 2);
+            // v[k]: piece lane % 4 of the row of the quad's lane k
+            const int first = row - (lane & 3), piece = col + 8 * (lane & 3);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, (unsigned long long)base, (lane & ~3) + k));
+                if (piece < a.D && first + k < x.rows) *reinterpret_cast<uint4*>(to + piece) = v[k];
             }
         };
         ChunkWalk walk(a);
-        ChunkItem x, nx;
-        uint32_t live_items = 0, all_items = 0, tiles = 0, item = 0, next_item = 0;      // item: its number among those with tiles
-        // The next item with something to do here; rows that see nothing are written on the way.
-        const auto advance = [&]() {
-            while (walk.next(nx)) {
-                const int row = nx.row0 + g * 128 + in_tile;
-                if (nx.from >= nx.to) {
-                    if (row < nx.rows && nx.tiles == 0) {
-                        const uint32_t zeros[32] = {};
-#pragma unroll 1
-                        for (int j = 0; j < a.D; j += 32) write(nx, row, j, zeros, 0.f);
-                    }
-                    continue;
-                }
-                next_item = all_items++;
-                if (g == 0 || nx.row0 + 128 < nx.rows) return true;
-            }
-            return false;
-        };
-        // neighbouring lanes on neighbouring bytes of a row
-        constexpr int kPerRow = DP / 8, kStep = 128 / kPerRow;                   // 16-byte pieces of a row; rows from one of a thread's pieces to the next
-        const int thread = threadIdx.x & 127, piece = thread % kPerRow, r0 = thread / kPerRow;
-        const uint32_t mine = q_smem + g * kTile + (piece >> 3) * kBlock + r0 * 128 + (((piece & 7) ^ (r0 & 7)) << 4);
-        const auto load_q = [&](const ChunkItem& y) {
-            const int b_step = kStep / a.group, h_step = kStep - b_step * a.group;
-            int r = y.row0 + g * 128 + r0, h = r % a.group;
-            const int64_t step = b_step * a.q_stride + h_step * a.q_head, wrap = a.q_stride - a.group * a.q_head;
-            const T* src = static_cast<const T*>(a.q) + (int64_t)(y.start + r / a.group) * a.q_stride + ((int64_t)y.head * a.group + h) * a.q_head + 8 * piece;
-#pragma unroll 2
-            for (int i = 0; i < kPerRow; ++i) {
-                const bool there = r < y.rows && 8 * piece < a.D;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine + i * (kStep * 128)), "l"(there ? src : static_cast<const T*>(a.q)), "r"(there ? 16 : 0) : "memory");
-                r += kStep;
-                h += h_step;
-                src += step;
-                if (h >= a.group) { h -= a.group; src += wrap; }
-            }
-        };
-        const auto have_q = [&]() {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            if (a.scale < 0.f) {                                                 // |scale| from here on
-#pragma unroll 1
-                for (int i = 0; i < kPerRow; ++i) {
-                    const uint4 v = ld_shared_v4(mine + i * (kStep * 128));
-                    st_shared_v4(mine + i * (kStep * 128), v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
-                }
-            }
-            fence_proxy_async();
-            mbar_arrive(smem_u32(&s_q[g]));
-        };
-        bool ok = true, more = advance();
-        if (more) {
-            load_q(nx);
-            have_q();
-        }
-        while (ok && more) {
-            x = nx;
-            item = next_item;
+        ChunkItem x;
+        uint32_t items = 0, all_items = 0, tiles = 0;                            // this group's, all of those with tiles, this group's tiles
+        bool ok = true;
+        while (ok && walk.next(x)) {
             const int row = x.row0 + g * 128 + in_tile, n = x.to - x.from;
             const bool live_warp = row - lane < x.rows;
+            if (n <= 0) {                              // rows that see nothing
+                if (live_warp && x.tiles == 0) {
+                    const uint32_t zeros[32] = {};
+                    T* const base = static_cast<T*>(a.out) + place(x, min(row, x.rows - 1), a.out_stride, a.out_head);
+#pragma unroll 1
+                    for (int j = 0; j < a.D; j += 32) write(x, base, row, j, zeros, 0.f);
+                }
+                continue;
+            }
+            const uint32_t item = all_items++;
+            if (g == 1 && x.row0 + 128 >= x.rows) continue;
             const int limit = x.first + min(row, x.rows - 1) / a.group + 1, low = a.window ? limit - a.window : 0;     // the row sees tokens low to limit - 1
             float m = -INFINITY, l = 0.f;
             for (int i = 0; i < 2 * n; ++i) {
                 const int h = i & 1;
                 ok = wait(&s_scores[g][h], (tiles + (uint32_t)(i >> 1)) & 1);
                 if (!ok) break;
-                if (i == 2 * n - 1) {                  // the queries have been used: the next ones come
-                    more = advance();
-                    if (more) load_q(nx);
-                }
                 if (live_warp) {
                     tcgen05_fence_after();
                     const uint32_t ts = tmem + lanes + g * 128 + h * 64;
-                    uint32_t s[64], p[32];
-                    tcgen05_ld32(ts, s);
-                    tcgen05_ld32(ts + 32, s + 32);
-                    tcgen05_wait_ld();
                     const int key = (x.tile0 + x.from + (i >> 1)) * 128 + h * 64, hi = limit - key, lo = low - key;
-                    if (__any_sync(0xffffffffu, hi < 64 || lo > 0)) {
+                    const bool edge = __any_sync(0xffffffffu, hi < 64 || lo > 0);
+                    uint32_t p[32];
+                    float sum;
+                    // The exponentials are of the maximum so far, so that they need not wait for this half's; where that is too low they are done again.
+                    while (true) {
+                        uint32_t s[2][32];             // the second scores come while the first ones are worked on
+                        float top[2] = {-INFINITY, -INFINITY};
+                        const float base = m == -INFINITY ? 0.f : p_shift<T>() - m * c;
+                        tcgen05_ld32(ts, s[0]);
+                        sum = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 64; ++j)
-                            if (j >= hi || j < lo) s[j] = 0xff800000u;
-                    }
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < 64; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-                    const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-                    if (i == 0) {
-                        m = next;
-                    } else if (__any_sync(0xffffffffu, (next - m) * c > kSlack)) {   // (a NaN difference, -inf to -inf, is no growth)
-                        // The products of the half before may still be adding to O: the scores behind them tell of their end, or, for the last half, a barrier.
-                        ok = i + 1 < 2 * n ? wait(&s_scores[g][h ^ 1], (tiles + (uint32_t)((i + 1) >> 1)) & 1) : wait(&s_half[g], live_items & 1);
-                        if (!ok) break;
-                        tcgen05_fence_after();
-                        const float keep = next == m ? 1.f : ex2((m - next) * c);
-                        const uint32_t to = tmem + lanes + 256 + g * DP;
-#pragma unroll 1
-                        for (int j = 0; j < DP; j += 32) {
-                            uint32_t o[32];
-                            tcgen05_ld32(to + j, o);
+                        for (int k = 0; k < 2; ++k) {
                             tcgen05_wait_ld();
+                            pin(s[k]);
+                            if (k == 0) tcgen05_ld32(ts + 32, s[1]);
+                            if (edge) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tcgen05_st32(to + j, o);
+                                for (int j = 0; j < 32; ++j)
+                                    if (32 * k + j >= hi || 32 * k + j < lo) s[k][j] = 0xff800000u;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) top[(j >> 1) & 1] = max3(top[(j >> 1) & 1], __uint_as_float(s[k][j]), __uint_as_float(s[k][j + 1]));
+                            sum += values_of<T>(s[k], c, base, *reinterpret_cast<uint32_t (*)[16]>(p + 16 * k));
                         }
-                        l *= keep;
+                        const float next = fmaxf(m, fmaxf(top[0], top[1]));
+                        if (!__any_sync(0xffffffffu, (next - m) * c > kSlack)) break;          // (a NaN difference, -inf to -inf, is no growth)
+                        if (i > 0) {
+                            // The products of the half before may still be adding to O: the scores behind them tell of their end, or, for the last half, a barrier.
+                            ok = i + 1 < 2 * n ? wait(&s_scores[g][h ^ 1], (tiles + (uint32_t)((i + 1) >> 1)) & 1) : wait(&s_half[g], items & 1);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                            const float keep = next == m ? 1.f : ex2((m - next) * c);
+                            const uint32_t to = tmem + lanes + 256 + g * DP;
+#pragma unroll 1
+                            for (int j = 0; j < DP; j += 32) {
+                                uint32_t o[32];
+                                tcgen05_ld32(to + j, o);
+                                tcgen05_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                                tcgen05_st32(to + j, o);
+                            }
+                            l *= keep;
+                        }
                         m = next;
                     }
-                    l += values_of<T>(s, c, m == -INFINITY ? 0.f : p_shift<T>() - m * c, p);
+                    if (!ok) break;
+                    l += sum;
                     tcgen05_st32(ts, p);
                     tcgen05_wait_st();
                     tcgen05_fence_before();
@@ -576,17 +624,17 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 if (lane == 0) mbar_arrive(smem_u32(&s_probs[g][h]));
             }
             if (!ok) break;
-            if (more) have_q();
-            ok = wait(&s_done[g], live_items & 1);
+            ok = wait(&s_done[g], items & 1);
             if (!ok) break;
             tiles += (uint32_t)n;
-            ++live_items;
+            ++items;
             if (live_warp) {
                 tcgen05_fence_after();
                 const uint32_t from = tmem + lanes + 256 + g * DP;
                 const bool odd = *(volatile uint32_t*)&s_odd[item & 7] != 0;
                 const int64_t part = (int64_t)x.slot * 2 + g;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
+                T* const base = static_cast<T*>(a.out) + place(x, min(row, x.rows - 1), a.out_stride, a.out_head);
                 if (x.slot >= 0) a.part_ml[part * 128 + in_tile] = make_float2(m == -INFINITY ? m : m * c, l);
 #pragma unroll 1
                 for (int j = 0; j < DP; j += 32) {
@@ -623,8 +671,9 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             a.part_o[(part * (DP / 4) + j / 4 + e) * 128 + in_tile] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-                    } else if (row < x.rows) {
-                        write(x, row, j, o, inv);
+                    } else {
+                        __syncwarp();
+                        write(x, base, row, j, o, inv);
                     }
                 }
                 __syncwarp();
@@ -646,46 +695,58 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
     }
 }
 
-// The parts of pairs that were cut: sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  kJoinSlices blocks for each cut, which a pair's first cut works for; a row a lane.
+// The parts of pairs that were cut: sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  kJoinSlices blocks for each cut, which a pair's first cut works for; a row a lane, a piece of its values a warp.
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ ChunkArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ ChunkArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
-    constexpr int kRows = 256 / kJoinSlices;
+    static_assert(256 / kJoinSlices == 32, "a row a lane");
+    constexpr int kEach = DP / 4 / 8;                  // 16-byte pieces of a thread
     const int r = (int)blockIdx.x / kJoinSlices + 1, slice = (int)blockIdx.x % kJoinSlices, ranges = __ldcg(a.counts + 1);
-    if (r < ranges) {
-        const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + r)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + r - 1));
-        const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
-        if (c.z > 0 && !(same(d) && d.z > 0)) {
-            const ChunkUnit u = a.units[c.x];
-            int last = r;                              // the pair's last range
-            while (last + 1 < ranges) {
-                const int4 e = __ldcg(reinterpret_cast<const int4*>(a.cuts + last + 1));
-                if (!same(e) || e.z == 0) break;
-                ++last;
-            }
-            const int parts = last - r + 2;
-            const int in_pair = slice * kRows + (int)(threadIdx.x & (kRows - 1)), sub = (int)threadIdx.x / kRows, row = u.row0 + in_pair, g = in_pair >> 7, in_tile = in_pair & 127;
-            const auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (r - 1) + 1 : 2 * (r + i - 1)) * 2 + g; };
-            if (row < u.rows) {
-                float top = -INFINITY, sum = 0.f;
-                for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(a.part_ml + slot(i) * 128 + in_tile).x);
-                for (int i = 0; i < parts; ++i) {
-                    const float2 ml = __ldcg(a.part_ml + slot(i) * 128 + in_tile);
-                    sum = fmaf(ml.x == -INFINITY ? 0.f : ex2(ml.x - top), ml.y, sum);
+    const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + r)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + r - 1));       // (used if there are so many)
+    const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
+    if (r < ranges && c.z > 0 && !(same(d) && d.z > 0)) {
+        const ChunkUnit u = a.cuts[r].begins;
+        int last = r;                                  // the pair's last range
+        while (last + 1 < ranges) {
+            const int4 e = __ldcg(reinterpret_cast<const int4*>(a.cuts + last + 1));
+            if (!same(e) || e.z == 0) break;
+            ++last;
+        }
+        const int parts = last - r + 2, in_pair = slice * 32 + (int)(threadIdx.x & 31), warp = (int)threadIdx.x >> 5, row = u.row0 + in_pair, g = in_pair >> 7, in_tile = in_pair & 127;
+        const auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (r - 1) + 1 : 2 * (r + i - 1)) * 2 + g; };
+        if (row < u.rows) {
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(a.part_ml + slot(i) * 128 + in_tile).x);
+            float4 acc[kEach] = {};
+#pragma unroll 2
+            for (int i = 0; i < parts; ++i) {
+                const float2 ml = __ldcg(a.part_ml + slot(i) * 128 + in_tile);
+                float4 o[kEach];
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) o[k] = __ldcg(a.part_o + (slot(i) * (DP / 4) + warp * kEach + k) * 128 + in_tile);
+                const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                sum = fmaf(w, ml.y, sum);
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    acc[k].x = fmaf(w, o[k].x, acc[k].x); acc[k].y = fmaf(w, o[k].y, acc[k].y); acc[k].z = fmaf(w, o[k].z, acc[k].z); acc[k].w = fmaf(w, o[k].w, acc[k].w);
                 }
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int token = row / a.group;
-                T* dst = static_cast<T*>(a.out) + (int64_t)(u.start + token) * a.out_stride + (int64_t)(c.y * a.group + row - token * a.group) * a.out_head;
-                for (int i4 = sub; i4 < a.D / 4; i4 += 128 / kRows) {
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int i = 0; i < parts; ++i) {
-                        const float m = __ldcg(a.part_ml + slot(i) * 128 + in_tile).x, w = m == -INFINITY ? 0.f : ex2(m - top);
-                        const float4 o = __ldcg(a.part_o + (slot(i) * (DP / 4) + i4) * 128 + in_tile);
-                        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
-                    }
-                    dst[4 * i4] = lm_from_f<T>(acc.x * inv); dst[4 * i4 + 1] = lm_from_f<T>(acc.y * inv); dst[4 * i4 + 2] = lm_from_f<T>(acc.z * inv); dst[4 * i4 + 3] = lm_from_f<T>(acc.w * inv);
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int token = row / a.group;
+            T* dst = static_cast<T*>(a.out) + (int64_t)(u.start + token) * a.out_stride + (int64_t)(c.y * a.group + row - token * a.group) * a.out_head;
+            const bool vec = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * 2) | (uintptr_t)(a.out_head * 2)) & 7) == 0;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int col = 4 * (warp * kEach + k);
+                if (col >= a.D) break;
+                const float x = acc[k].x * inv, y = acc[k].y * inv, z = acc[k].z * inv, w = acc[k].w * inv;
+                if (vec) {
+                    *reinterpret_cast<uint2*>(dst + col) = make_uint2(lm_pack2<T>(x, y), lm_pack2<T>(z, w));
+                } else {
+                    dst[col] = lm_from_f<T>(x); dst[col + 1] = lm_from_f<T>(y); dst[col + 2] = lm_from_f<T>(z); dst[col + 3] = lm_from_f<T>(w);
                 }
             }
         }
@@ -792,7 +853,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
             return (char*)p->scratch + from;
         };
         a.counts = (int32_t*)take(8);
-        a.cuts = (ChunkCut*)take((a.max_ranges + 1) * sizeof(ChunkCut));
+        a.cuts = (ChunkCut*)take((a.max_ranges + 2) * sizeof(ChunkCut));
         a.units = (ChunkUnit*)take(a.max_units * sizeof(ChunkUnit));
         a.before = (int64_t*)take((a.max_units + 1) * sizeof(int64_t));
         a.part_ml = (float2*)take(2ull * a.max_ranges * 256 * sizeof(float2));
