@@ -1221,14 +1221,24 @@ int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t j
         PB_REQUIRE(p->scratch != nullptr && p->scratch_bytes >= pl.scratch && aligned(p->scratch, 16), "pb_chunk_attn: %llu bytes of scratch memory are needed, 16-byte aligned (%llu given)",
                    (unsigned long long)pl.scratch, (unsigned long long)(p->scratch ? p->scratch_bytes : 0));
         const CacheShape shape = {pl.half, p->head_dim, p->page_size, p->kv_heads, p->n_pages, p->token_stride, p->head_stride, p->page_stride, (uint32_t)pl.a.box_rows};
-        CUtensorMap km, vm;
+        CUtensorMap qm, km, vm;
         int e = encode_cache(shape, p->k_cache, &km);
         if (e == PB_OK) e = encode_cache(shape, p->v_cache, &vm);
+        if (e == PB_OK && pl.a.q_boxes) {
+            // [token][key head][head of it][value]: a row tile is 128 / group tokens
+            const int64_t group = pl.a.group;
+            const uint64_t dims[4] = {(uint64_t)p->head_dim, (uint64_t)group, (uint64_t)p->kv_heads, (uint64_t)p->tokens};
+            const uint64_t strides[3] = {(uint64_t)p->q_head_stride * 2, (uint64_t)(group * p->q_head_stride) * 2, (uint64_t)p->q_stride * 2};
+            const uint32_t box[4] = {64, (uint32_t)group, 1, (uint32_t)(128 / group)};
+            e = encode_tiled_sw128(pl.half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p->q, 4, dims, strides, box, &qm);
+        } else {
+            qm = km;                                       // (not used)
+        }
         if (e == PB_OK) e = lm_launch("pb_chunk_attn (plan)", plan_kernel, dim3(1), dim3(1024), 0, st, 1, pl.a);
         if (e != PB_OK) return e;
         const uint32_t smem = pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem;
         PB_CUDA(cudaFuncSetAttribute(pl.chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        e = lm_launch("pb_chunk_attn", pl.chunk, dim3(kChunkBlocks), dim3(384), smem, st, 1, pl.a, km, vm);
+        e = lm_launch("pb_chunk_attn", pl.chunk, dim3(kChunkBlocks), dim3(384), smem, st, 1, pl.a, qm, km, vm);
         if (e != PB_OK) return e;
     }
     if (pl.has_few) {

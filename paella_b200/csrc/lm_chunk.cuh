@@ -34,6 +34,7 @@ struct ChunkArgs {
     int64_t q_stride, q_head, out_stride, out_head, page_stride, token_stride, head_stride, table_stride;
     int batch, tokens, q_heads, kv_heads, group, D, page, n_pages, max_new, max_len, window, box_rows;
     int few;                             // rows of a sequence that another kernel takes
+    int q_boxes;                         // a row tile's queries are boxes of a tensor map (whole tokens to a tile, positive strides and scale)
     float scale;
     int max_units, max_ranges;
     ChunkUnit* units;
@@ -140,8 +141,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
     for (int r = t; r <= N; r += 1024) {
         ChunkCut c = {0, a.kv_heads, 0, 0, {}};
         if (r < N) {
-            const int64_t w = total / N * r + total % N * r / N;
-            c.head = (int)(w / sum);
+            // (quotients of 64 bits take some hundred instructions each)
+            const bool small = total < (1LL << 32) / (kChunkBlocks * kMaxRounds);
+            const int64_t w = small ? (uint32_t)total * (uint32_t)r / (uint32_t)N : total * r / N;
+            c.head = small ? (uint32_t)w / (uint32_t)sum : (int)(w / sum);
             const int64_t rest = w - c.head * sum;
             const int64_t* table = in_shared ? s_before : a.before;
             int lo = 0, hi = units - 1;            // the last unit that begins at or in front of it
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
             c.unit = lo;
             c.begins = a.units[lo];
             const int tiles = in_shared ? s_tiles[lo] >> 1 : c.begins.tiles;
-            const int each = (in_shared ? s_tiles[lo] & 1 : c.begins.row0 + 128 < c.begins.rows) ? kCostTwo : kCostOne, near = (int)min((long long)total / N / (8 * each), 1000LL);
+            const int each = (in_shared ? s_tiles[lo] & 1 : c.begins.row0 + 128 < c.begins.rows) ? kCostTwo : kCostOne, near = (int)min((long long)total / N / (8 * each), 2LL);
             const int step = (int)(max((long long)(rest - table[lo] - kCostPair), 0LL) / each);
             if (step > near && step < tiles - near) {
                 c.step = step;
@@ -208,22 +211,22 @@ struct ChunkWalk {
     }
 };
 
-// Warps 0-3 and 4-7: softmax of one row tile each, a row a thread; warps 8 and 11 copy keys and values; warps 9 and 10 issue the products of one row tile each.  As in prefix_kernel: S = Q K^T into 64
-// memory, P takes its place, 64 keys at a time, as the A operand of O += P V.  Rings and barriers run on from one pair to the next;
-// the next pair's queries come while the results of the one before are written.
 // Registers that a load from tensor memory wrote, behind its wait: what uses them stays behind it, too.
 __device__ __forceinline__ void pin(uint32_t (&r)[32]) {
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
     asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 
+// Warps 0-3 and 4-7: softmax of one row tile each, a row a thread; warps 8 and 11 copy keys and values; warps 9 and 10 issue the products of one row tile each.  As in prefix_kernel: S = Q K^T
+// into 64 columns of tensor memory, P takes its place as the A operand of O += P V.  Rings and barriers run on from one pair to the next; the next pair's queries come while the results of the one before
+// are written.
 template <typename T, int DP>
-__global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int kBlocks = DP / 64, kStages = PrefixShape<DP>::stages;
     constexpr uint32_t kTile = PrefixShape<DP>::tile, kBlock = 128 * 128;
     static_assert(kStages >= 4, "a wait for an entry of the ring has seen the one before in its place");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_free[2], s_edge;
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_scores[2][2], s_probs[2][2], s_half[2], s_turn[2], s_done[2], s_free[2], s_q[2], s_edge;
     __shared__ int s_pages[2][4][16];
     __shared__ uint32_t s_odd[8];
     __shared__ uint32_t s_tmem;
@@ -250,6 +253,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             mbar_init(smem_u32(&s_turn[i]), 1);
             mbar_init(smem_u32(&s_done[i]), 1);
             mbar_init(smem_u32(&s_free[i]), 4);
+            mbar_init(smem_u32(&s_q[i]), 1);
         }
         mbar_init(smem_u32(&s_edge), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -317,6 +321,12 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             if (values) {
                 edge = first + 128 > pos0 + 1 || (a.window && first < pos1 - a.window + 1);
                 if (fresh && lane == 0) s_odd[item & 7] = 0;
+                fresh = false;
+            }
+            if (!values && fresh && a.q_boxes) {
+                // the item's queries, which the issuing warps will fetch
+                const int tile = lane / kBlocks, row0 = now.x.row0 + tile * 128;
+                if (tile < 2 && row0 < now.x.rows) tma_prefetch_4d(&qmap, (lane % kBlocks) * 64, 0, now.x.head, now.x.start + row0 / a.group);
                 fresh = false;
             }
             const uint32_t to = ring + at.st * kTile, bar = smem_u32(edge ? &s_edge : &s_full[at.st]);
@@ -395,7 +405,16 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         const int piece = lane % kPerRow, r0 = lane / kPerRow, b_step = kStep / a.group, h_step = kStep - b_step * a.group;
         const int64_t q_step = b_step * a.q_stride + h_step * a.q_head, q_wrap = a.q_stride - a.group * a.q_head;
         const uint32_t q_block = q_smem + g * kTile + (piece >> 3) * kBlock;
-        const auto load_q = [&](const ChunkItem& y) {
+        const auto load_q = [&](const ChunkItem& y) -> bool {
+            if (a.q_boxes) {
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(smem_u32(&s_q[g]), kTile);
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i) tma_load_4d(q_smem + g * kTile + i * kBlock, &qmap, i * 64, 0, y.head, y.start + (y.row0 + g * 128) / a.group, smem_u32(&s_q[g]));
+                }
+                __syncwarp();
+                return wait(&s_q[g], items & 1);
+            }
             int r = y.row0 + g * 128 + r0;
             const int token = r / a.group;
             int h = r - token * a.group;
@@ -420,6 +439,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             }
             fence_proxy_async();
             __syncwarp();
+            return true;
         };
         while (ok && walk.next(x)) {
             const int n = x.to - x.from;
@@ -436,7 +456,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 }
                 continue;
             }
-            load_q(x);
+            ok = load_q(x);
             // Two groups take turns at the tensor cores, as in prefix_kernel.
             const auto take_turn = [&]() {
                 if (!two) return true;
@@ -461,7 +481,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 if (h == 1) keys.on();
                 return true;
             };
-            ok = take_turn() && scores(0) && take_turn() && scores(1);
+            ok = ok && take_turn() && scores(0) && take_turn() && scores(1);
             for (int u = 0; ok && u < n; ++u, ++tiles) {
                 const bool last = u == n - 1;
 #pragma unroll
@@ -538,6 +558,36 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             for (int k = 0; k < 4; ++k) {
                 T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, (unsigned long long)base, (lane & ~3) + k));
                 if (piece < a.D && first + k < x.rows) *reinterpret_cast<uint4*>(to + piece) = v[k];
+            }
+        };
+        // Values of V that are not finite, whose tiles held zeros in their places, into the sums of the rows that see them.
+        const auto add_odd = [&](const ChunkItem& x, uint32_t from, int limit, int low) {
+#pragma unroll 1
+            for (int j = 0; j < a.D; j += 8) {
+                uint32_t o[8];
+                __syncwarp();
+                tcgen05_ld8(from + j, o);
+                tcgen05_wait_ld();
+#pragma unroll 1
+                for (int s = x.from; s < x.to; ++s) {
+                    const int key = (x.tile0 + s) * 128, pos0 = x.first + x.row0 / a.group;
+                    if (key + 128 <= pos0 + 1 && !(a.window && key < x.end - a.window)) continue;
+#pragma unroll 1
+                    for (int at = max(key, low); at < min(key + 128, limit); ++at) {
+                        const int page = __ldcg(a.block_table + x.b * a.table_stride + at / a.page);
+                        if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                        const uint4 w = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + page * a.page_stride + (at % a.page) * a.token_stride + x.head * a.head_stride + j));
+                        const T* y = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float z = lm_to_f<T>(y[k]);
+                            if (!(fabsf(z) < INFINITY)) o[k] = __float_as_uint(__uint_as_float(o[k]) + z);
+                        }
+                    }
+                }
+                __syncwarp();
+                tcgen05_st8(from + j, o);
+                tcgen05_wait_st();
             }
         };
         ChunkWalk walk(a);
@@ -631,49 +681,25 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             if (live_warp) {
                 tcgen05_fence_after();
                 const uint32_t from = tmem + lanes + 256 + g * DP;
-                const bool odd = *(volatile uint32_t*)&s_odd[item & 7] != 0;
+                if (*(volatile uint32_t*)&s_odd[item & 7] != 0) add_odd(x, from, limit, low);
                 const int64_t part = (int64_t)x.slot * 2 + g;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 T* const base = static_cast<T*>(a.out) + place(x, min(row, x.rows - 1), a.out_stride, a.out_head);
                 if (x.slot >= 0) a.part_ml[part * 128 + in_tile] = make_float2(m == -INFINITY ? m : m * c, l);
+                // (Rolled up: code that runs once for an item comes from memory.)
 #pragma unroll 1
-                for (int j = 0; j < DP; j += 32) {
-                    uint32_t o[32];
+                for (int k = 0; k < DP / 32; ++k) {
+                    uint32_t v[32];
                     __syncwarp();
-                    tcgen05_ld32(from + j, o);
+                    tcgen05_ld32(from + 32 * k, v);
                     tcgen05_wait_ld();
-                    if (odd) {
-                        // values that are not finite: their tiles held zeros in their places
-#pragma unroll 1
-                        for (int s = x.from; s < x.to; ++s) {
-                            const int key = (x.tile0 + s) * 128, pos0 = x.first + x.row0 / a.group;
-                            if (key + 128 <= pos0 + 1 && !(a.window && key < x.end - a.window)) continue;
-#pragma unroll 1
-                            for (int at = max(key, low); at < min(key + 128, limit); ++at) {
-                                const int page = __ldcg(a.block_table + x.b * a.table_stride + at / a.page);
-                                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                                const T* v = static_cast<const T*>(a.v) + page * a.page_stride + (at % a.page) * a.token_stride + x.head * a.head_stride + j;
-#pragma unroll
-                                for (int e = 0; e < 32; e += 8) {
-                                    if (j + e >= a.D) break;
-                                    const uint4 w = __ldcg(reinterpret_cast<const uint4*>(v + e));
-                                    const T* y = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                                    for (int k = 0; k < 8; ++k) {
-                                        const float z = lm_to_f<T>(y[k]);
-                                        if (!(fabsf(z) < INFINITY)) o[e + k] = __float_as_uint(__uint_as_float(o[e + k]) + z);
-                                    }
-                                }
-                            }
-                        }
-                    }
+                    pin(v);
                     if (x.slot >= 0) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            a.part_o[(part * (DP / 4) + j / 4 + e) * 128 + in_tile] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                            a.part_o[(part * (DP / 4) + 8 * k + e) * 128 + in_tile] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
                     } else {
-                        __syncwarp();
-                        write(x, base, row, j, o, inv);
+                        write(x, base, row, 32 * k, v, inv);
                     }
                 }
                 __syncwarp();
@@ -755,7 +781,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chunk
 }
 
 typedef void (*JoinFn)(ChunkArgs, uint32_t, FinishedBlockNotifier*);
-typedef void (*ChunkFn)(ChunkArgs, CUtensorMap, CUtensorMap);
+typedef void (*ChunkFn)(ChunkArgs, CUtensorMap, CUtensorMap, CUtensorMap);
 
 struct ChunkPlan {
     ChunkArgs a;
@@ -808,6 +834,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     a.page_stride = p->page_stride; a.token_stride = p->token_stride; a.head_stride = p->head_stride; a.table_stride = p->table_stride;
     a.tokens = p->tokens; a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.D = p->head_dim;
     a.page = p->page_size; a.n_pages = (int)p->n_pages; a.max_len = p->max_len; a.window = p->window < p->max_len ? p->window : 0; a.scale = p->scale;
+    a.q_boxes = 128 % a.group == 0 && a.scale >= 0.f && a.q_stride > 0 && a.q_head > 0 && a.q_stride < 1 << 30 && a.q_head < 1 << 30 && (int64_t)a.group * a.q_head < 1 << 30;
     a.box_rows = 8;
     while (a.box_rows < 64 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
     pl.DP = p->head_dim <= 64 ? 64 : 128;

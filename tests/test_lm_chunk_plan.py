@@ -43,12 +43,12 @@ def plan(units, heads, max_ranges):
     n = min(BLOCKS * rounds, max(total // (PAIR + 3 * TWO), 1))
     cuts = []
     for r in range(n):
-        w = total // n * r + total % n * r // n
+        w = total * r // n
         head = w // before[-1]
         rest = w - head * before[-1]
         at = max(i for i in range(len(units)) if before[i] <= rest)
         each, tiles = each_of(units[at]), units[at]["tiles"]
-        near, step = min(total // n // (8 * each), 1000), max(rest - before[at] - PAIR, 0) // each
+        near, step = min(total // n // (8 * each), 2), max(rest - before[at] - PAIR, 0) // each
         if near < step < tiles - near:
             cuts.append((head, at, step))
         elif step > near or 2 * step > tiles:
