@@ -7,8 +7,9 @@
 // rescaled a few times a row; all of a row's threads join at its end.
 //
 // The likeliest tokens come out of the same pass: a thread remembers the first of its vectors with its largest logit.  Tokens are ordered by keys of
-// 64 bits, the logit's order above the index's, so that no two are equal; the k-th largest of the threads' largest keys is a bound that k tokens
-// reach, and exactly k threads have any.  Only their vectors are read again (from the caches), each by a warp that keeps the 32 largest keys of what it saw in order, one a lane.
+// 64 bits, the logit's order above the index's, so that no two are equal.  The k-th largest of the threads' largest logits (the largest of four threads each) is a bound that k tokens reach; the few threads
+// that have any have their vectors read again, from the caches, and what reaches the bound is put in order by counting, for each, those in front of it.  Where that is more than there is room for
+// (rows whose large logits lie with few threads), those that came give a higher bound.
 #include <cmath>
 
 #include "lm.cuh"
@@ -19,7 +20,7 @@ namespace {
 
 __device__ uint32_t g_logprobs_flag;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxTop = 32, kMaxRanks = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxTop = 32, kMaxRanks = 8, kList = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogprobsArgs {
@@ -29,7 +30,7 @@ struct LogprobsArgs {
     int32_t *ranks, *top_ids;
     int64_t stride, top_stride;
     int tokens, vocab, top, ranks_of_row;      // ranks_of_row: blocks of a cluster that share a row out
-    float scale, c, slack, far;                // c: scale * log2(e); 16 and 256 in powers of two as differences of logits
+    float scale, c, inv_c, slack, far;         // c: scale * log2(e); 16 and 256 in powers of two as differences of logits
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -55,21 +56,25 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 __device__ __forceinline__ uint64_t key_of(uint32_t order, int index) { return (uint64_t)order << 32 | (0x7fffffffu - (uint32_t)index); }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)(0x7fffffffu - (uint32_t)key); }
 
-// 16 bytes of logits.
+// 32 bytes of logits, 16-byte aligned.
 template <typename T> struct Logits {
-    static constexpr int V = 16 / (int)sizeof(T);
-    uint4 w;
-    __device__ __forceinline__ void load(const T* p) { w = __ldcg(reinterpret_cast<const uint4*>(p)); }
+    static constexpr int V = 32 / (int)sizeof(T);
+    uint4 w[2];
+    __device__ __forceinline__ void load(const T* p) {
+        w[0] = __ldcg(reinterpret_cast<const uint4*>(p));
+        w[1] = __ldcg(reinterpret_cast<const uint4*>(p) + 1);
+    }
+    __device__ __forceinline__ uint32_t word(int i) const { return (&w[i >> 2].x)[i & 3]; }
     // value pairs as they are multiplied
     __device__ __forceinline__ uint64_t pair(int i) const {
-        const uint32_t* q = &w.x;
         if constexpr (sizeof(T) == 4) {
-            return pack_f32x2(q[2 * i], q[2 * i + 1]);
+            return pack_f32x2(word(2 * i), word(2 * i + 1));
         } else if constexpr (std::is_same<T, __half>::value) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(q + i));
+            const uint32_t q = word(i);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q));
             return pack_f32x2(__float_as_uint(f.x), __float_as_uint(f.y));
         } else {
-            return pack_f32x2(q[i] << 16, q[i] & 0xffff0000u);
+            return pack_f32x2(word(i) << 16, word(i) & 0xffff0000u);
         }
     }
     __device__ __forceinline__ float operator[](int i) const {
@@ -80,32 +85,54 @@ template <typename T> struct Logits {
     // the largest, or NaN if there is one
     __device__ __forceinline__ float top() const {
         if constexpr (sizeof(T) == 4) {
-            return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
-        } else if constexpr (std::is_same<T, __half>::value) {
-            const __half2* q = reinterpret_cast<const __half2*>(&w);
-            const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(q[0], q[1]), __hmax2_nan(q[2], q[3])));
-            return max_nan(f.x, f.y);
+            float t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = max_nan(__uint_as_float(word(i)), __uint_as_float(word(i + 4)));
+            return max_nan(max_nan(t[0], t[1]), max_nan(t[2], t[3]));
         } else {
-            const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(&w);
-            const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(q[0], q[1]), __hmax2_nan(q[2], q[3])));
-            return max_nan(f.x, f.y);
+            Two t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = __hmax2_nan(two(i), two(i + 4));
+            const Two m = __hmax2_nan(__hmax2_nan(t[0], t[1]), __hmax2_nan(t[2], t[3]));
+            return max_nan(__low2float(m), __high2float(m));
         }
     }
     // none below `low` (no NaN among them)
     __device__ __forceinline__ void raise(T low) {
-        if constexpr (sizeof(T) == 4) {
-            w = make_uint4(__float_as_uint(fmaxf(__uint_as_float(w.x), low)), __float_as_uint(fmaxf(__uint_as_float(w.y), low)), __float_as_uint(fmaxf(__uint_as_float(w.z), low)),
-                           __float_as_uint(fmaxf(__uint_as_float(w.w), low)));
-        } else if constexpr (std::is_same<T, __half>::value) {
-            __half2* q = reinterpret_cast<__half2*>(&w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = __hmax2(q[i], __half2half2(low));
-        } else {
-            __nv_bfloat162* q = reinterpret_cast<__nv_bfloat162*>(&w);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = __hmax2(q[i], __bfloat162bfloat162(low));
+        for (int i = 0; i < 8; ++i) {
+            uint32_t& x = (&w[i >> 2].x)[i & 3];
+            if constexpr (sizeof(T) == 4) {
+                x = __float_as_uint(fmaxf(__uint_as_float(x), low));
+            } else {
+                const Two m = __hmax2(two(i), both(low));
+                x = *reinterpret_cast<const uint32_t*>(&m);
+            }
         }
     }
+    // how many are above `x`, or not below it (no NaN among them)
+    template <bool OR_SAME> __device__ __forceinline__ int above(T x) const {
+        if constexpr (sizeof(T) == 4) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n += OR_SAME ? __uint_as_float(word(i)) >= x : __uint_as_float(word(i)) > x;
+            return n;
+        } else {
+            Two n = OR_SAME ? __hge2(two(0), both(x)) : __hgt2(two(0), both(x));      // ones: whole numbers up to 256 are exact
+#pragma unroll
+            for (int i = 1; i < 8; ++i) n = __hadd2(n, OR_SAME ? __hge2(two(i), both(x)) : __hgt2(two(i), both(x)));
+            return (int)(__low2float(n) + __high2float(n));
+        }
+    }
+
+   private:
+    using Two = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    __device__ __forceinline__ Two two(int i) const {
+        const uint32_t x = word(i);
+        return *reinterpret_cast<const Two*>(&x);
+    }
+    static __device__ __forceinline__ __half2 both(__half x) { return __half2half2(x); }
+    static __device__ __forceinline__ __nv_bfloat162 both(__nv_bfloat16 x) { return __bfloat162bfloat162(x); }
 };
 
 template <typename T> __device__ __forceinline__ float lowest();
@@ -142,36 +169,14 @@ struct Sums {
     }
 };
 
-// 32 keys, one a lane, brought into falling order; or, of a rising-then-falling sequence, its last steps.
-__device__ __forceinline__ uint64_t exchange(uint64_t k, int with, bool keep_larger) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, k, with);
-    return (k > o) == keep_larger ? k : o;
-}
-__device__ __forceinline__ uint64_t merge_32(uint64_t k, int lane) {
-#pragma unroll
-    for (int j = 16; j > 0; j >>= 1) k = exchange(k, j, (lane & j) == 0);
-    return k;
-}
-__device__ __forceinline__ uint64_t sort_32(uint64_t k, int lane) {
-#pragma unroll
-    for (int n = 2; n <= 32; n *= 2)
-#pragma unroll
-        for (int j = n / 2; j > 0; j >>= 1) k = exchange(k, j, ((lane & j) == 0) == ((lane & n) == 0));
-    return k;
-}
-// The 32 largest of two falling sequences.
-__device__ __forceinline__ uint64_t largest_32(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-    return merge_32(a > r ? a : r, lane);
-}
-
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ LogprobsArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_constant__ LogprobsArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr int V = Logits<T>::V;
     __shared__ Sums s_sums[kWarps];
     __shared__ int s_before[kWarps];
-    __shared__ uint64_t s_keys[TOP ? kWarps : 1][32];
-    __shared__ int s_segment[kMaxTop], s_segments;
+    __shared__ uint64_t s_quads[TOP ? kThreads / 4 : 1], s_bound, s_top[TOP ? kMaxTop : 1], s_list[TOP ? kList : 1];
+    __shared__ uint16_t s_who[TOP ? kThreads : 1];
+    __shared__ int s_found, s_many;
     griddep_wait();
     if (nf) nf->start(job_id);
     griddep_launch();
@@ -179,16 +184,24 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     const int rank = blockIdx.x % a.ranks_of_row, row = blockIdx.x / a.ranks_of_row;
     const bool live = row < a.tokens;
     const T* x = static_cast<const T*>(a.logits) + (live ? row : 0) * a.stride;
-    // the row: up to V - 1 logits until 16 bytes are aligned, n vectors, up to V - 1 more.  This block's share of the vectors; the first block has the others, too.
+    // the row: logits until 16 bytes are aligned, n vectors, and those that are left.  This block's share of the vectors; the first block has the others, too.
     const int head = live ? min((int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T), a.vocab) : 0, n = live ? (a.vocab - head) / V : 0;
     const int first = (int)((int64_t)n * rank / a.ranks_of_row), last = (int)((int64_t)n * (rank + 1) / a.ranks_of_row);
     const int loose = live && rank == 0 ? a.vocab - n * V : 0;           // logits outside of the vectors: the first `head`, and those behind
-    const auto loose_index = [&](int i) { return i < head ? i : n * V + i; };
+    const T* body = x + head;
+    // two vectors come while a third is worked on, the first ones while the target is looked up
+    Logits<T> v[3];
+    const auto load = [&](Logits<T>& to, int i) {
+        if (i < last) to.load(body + (int64_t)i * V);
+    };
+    load(v[0], first + t);
+    load(v[1], first + t + kThreads);
     int target = -1;
     if (live && a.targets) target = a.targets[row];
     if (target >= a.vocab && t == 0) atomicExch(&g_logprobs_flag, kFlagLmToken);
     const bool ranked = target >= 0 && target < a.vocab;
-    const float wanted = ranked ? lm_to_f<T>(x[target]) : 0.f;
+    const T wanted_as = ranked ? x[target] : lm_from_f<T>(0.f);
+    const float wanted = lm_to_f<T>(wanted_as);
     const uint64_t wanted_key = ranked ? key_of(order_of(wanted), target) : ~0ull;
 
     Sums sums = {-INFINITY, 0.f, 0.f};
@@ -196,26 +209,32 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     uint32_t best = 0;
     float best_logit = -INFINITY, limit = __uint_as_float(0x7fffffffu);     // limit: vectors whose largest logit is not above it are the common ones
     T low = lm_from_f<T>(0.f);
-    uint64_t S2 = 0, E2 = 0;
-    const T* body = x + head;
+    uint64_t S2[2] = {0, 0}, E2[2] = {0, 0};
     const uint64_t c2 = pack_f32x2(__float_as_uint(a.c), __float_as_uint(a.c));
-    uint64_t minus_m = 0;
+    uint64_t minus_mc = 0;
     const int with_target = ranked && target >= head && target < head + n * V ? (target - head) / V : -1;
-    // The sums of the common vectors, as pairs, into the others.
+    float mc = 0.f;                           // m c, rounded: the common vectors' exponents are x c - mc, one operation
+    // The sums of the common vectors, as pairs, into the others.  Their exponents are r = mc - m c too small, which mc's rounding left.
     const auto fold = [&]() {
         float lo, hi, elo, ehi;
-        unpack_f32x2(S2, lo, hi);
-        unpack_f32x2(E2, elo, ehi);
-        sums.S += lo + hi;
-        sums.E += elo + ehi;
-        S2 = E2 = 0;
+        unpack_f32x2(add_f32x2(S2[0], S2[1]), lo, hi);
+        unpack_f32x2(add_f32x2(E2[0], E2[1]), elo, ehi);
+        if (lo + hi > 0.f) {
+            const float r = fmaf(-sums.m, a.c, mc), f = ex2(r);
+            sums.E = fmaf(fmaf(r, lo + hi, elo + ehi) * f, a.inv_c, sums.E);
+            sums.S = fmaf(lo + hi, f, sums.S);
+        }
+        S2[0] = S2[1] = E2[0] = E2[1] = 0;
     };
-    const auto take = [&](Logits<T> v, int i) {
+    const auto take = [&](Logits<T>& v, int i) {
         const float top = v.top();
-        if (TOP && top > best_logit) { best_logit = top; best = order_of(top); at = i; }
+        if (TOP && top > best_logit) { best_logit = top; at = i; }
         if (!(top <= limit)) {
             // a first vector, one that is far above what came so far, or one with a NaN or infinity
-            if (TOP && (top != top || top == -INFINITY) && best < order_of(top)) { best = order_of(top); at = i; best_logit = top == top ? top : INFINITY; }
+            if (TOP) {
+                if (top != top && best == 0) { best = 0xffffffffu; at = i; best_logit = INFINITY; }          // the first NaN: nothing comes in front of it
+                else if (at < 0) at = i;
+            }
             fold();
             if (top > sums.m && top < INFINITY) sums.rescale(top, a.c);
             // Logits far below the maximum are raised to `low`, where their exponentials are zeros: masks of -infinity need no case of their own.  Not where
@@ -223,11 +242,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
             low = lm_from_f<T>(fmaxf(sums.m - a.far, lowest<T>()));
             const bool common = sums.m > -INFINITY && (sums.m - lm_to_f<T>(low)) * a.c >= 200.f;
             limit = common ? sums.m + a.slack : __uint_as_float(0x7fffffffu);
-            minus_m = pack_f32x2(__float_as_uint(-sums.m), __float_as_uint(-sums.m));
+            mc = sums.m * a.c;
+            minus_mc = pack_f32x2(__float_as_uint(-mc), __float_as_uint(-mc));
             if (!(top <= limit)) {
+                if (top == -INFINITY) {
+                    if (ranked && wanted == -INFINITY) before += max(min(target - (head + i * V), V), 0);
+                    return;
+                }
 #pragma unroll 1
                 for (int j = 0; j < V; ++j) {
-                    const float logit = v[j];
+                    const float logit = lm_to_f<T>(body[(int64_t)i * V + j]);
                     sums.add_logit(logit, a.c);
                     if (ranked) before += key_of(order_of(logit), head + i * V + j) > wanted_key;
                 }
@@ -237,46 +261,38 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
         if (ranked && top >= wanted) {
             if (i == with_target) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) before += key_of(order_of(v[j]), head + i * V + j) > wanted_key;
-            } else if (head + i * V < target) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) before += v[j] >= wanted;
+                for (int j = 0; j < V; ++j) before += v[j] > wanted || (v[j] == wanted && head + i * V + j < target);
             } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) before += v[j] > wanted;
+                before += head + i * V < target ? v.template above<true>(wanted_as) : v.template above<false>(wanted_as);
             }
         }
         v.raise(low);
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
-            const uint64_t d = add_f32x2(v.pair(j), minus_m);
+            const uint64_t d = fma_f32x2(v.pair(j), c2, minus_mc);
             float lo, hi;
-            unpack_f32x2(mul_f32x2(d, c2), lo, hi);
+            unpack_f32x2(d, lo, hi);
             const uint64_t e = pack_f32x2(__float_as_uint(ex2(lo)), __float_as_uint(ex2(hi)));
-            S2 = add_f32x2(S2, e);
-            E2 = fma_f32x2(e, d, E2);
+            S2[j & 1] = add_f32x2(S2[j & 1], e);
+            E2[j & 1] = fma_f32x2(e, d, E2[j & 1]);
         }
     };
     {
-        constexpr int U = 4;                                              // vectors in flight
         int i = first + t;
-        for (; i + (U - 1) * kThreads < last; i += U * kThreads) {
-            Logits<T> v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u].load(body + (int64_t)(i + u * kThreads) * V);
-#pragma unroll
-            for (int u = 0; u < U; ++u) take(v[u], i + u * kThreads);
-        }
-        for (; i < last; i += kThreads) {
-            Logits<T> v;
-            v.load(body + (int64_t)i * V);
-            take(v, i);
+        for (; i < last; i += 3 * kThreads) {
+            load(v[2], i + 2 * kThreads);
+            take(v[0], i);
+            load(v[0], i + 3 * kThreads);
+            if (i + kThreads < last) take(v[1], i + kThreads);
+            load(v[1], i + 4 * kThreads);
+            if (i + 2 * kThreads < last) take(v[2], i + 2 * kThreads);
         }
         fold();
     }
+    if (at >= 0 && best == 0) best = order_of(best_logit);
     uint64_t loose_key = 0;
     if (t < loose) {
-        const int index = loose_index(t);
+        const int index = t < head ? t : n * V + t;
         const float v = lm_to_f<T>(x[index]);
         sums.add_logit(v, a.c);
         loose_key = key_of(order_of(v), index);
@@ -295,90 +311,124 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     if (lane == 0) { s_sums[warp] = sums; s_before[warp] = before; }
-    if (threadIdx.x == 0) s_segments = 0;
 
     if constexpr (TOP) {
-        // this thread's largest key, and the k-th largest of the block's
-        uint64_t mine = 0;
-        if (at >= 0) {
-            Logits<T> v;
-            v.load(body + (int64_t)at * V);
-            int j = V - 1;
+        // A bound that `top` tokens reach: the top-th largest of the quads' largest logits, each as if it were the last of its vector.
+        uint64_t quad = at >= 0 ? key_of(best, head + at * V + V - 1) : 0;
 #pragma unroll
-            for (int e = V - 1; e >= 0; --e) j = order_of(v[e]) == best ? e : j;
-            mine = key_of(best, head + at * V + j);
+        for (int o = 1; o < 4; o *= 2) {
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, quad, o);
+            quad = other > quad ? other : quad;
         }
-        const auto largest_of_block = [&](uint64_t falling) {             // of the warps' falling sequences; in warp 0
-            s_keys[warp][lane] = falling;
-            __syncthreads();
-            for (int half = kWarps / 2; half > 0; half /= 2) {
-                if (warp < half) {
-                    falling = largest_32(falling, s_keys[warp + half][lane], lane);
-                    s_keys[warp][lane] = falling;
-                }
-                __syncthreads();
-            }
-            return s_keys[0][lane];
-        };
-        largest_of_block(sort_32(mine, lane));
-        const uint64_t bound = s_keys[0][a.top - 1];                      // (0 where fewer threads have vectors)
-        if (mine > 0 && mine >= bound) s_segment[atomicAdd(&s_segments, 1)] = t;
+        if ((lane & 3) == 0) s_quads[t >> 2] = quad;
+        if (t == 0) { s_bound = 0; s_found = s_many = 0; }
         __syncthreads();
-        // the loose logits are in any case looked at: warp 0's first
-        uint64_t list = 0;
-        if (warp == 0) list = sort_32(loose_key, lane);
-        for (int s = warp; s < s_segments; s += kWarps) {
-            const int from = first + s_segment[s];
-            for (int base = from; base < last; base += 32 * kThreads) {
-                const int i = base + lane * kThreads;
-                Logits<T> v;
-                if (i < last) v.load(body + (int64_t)i * V);
-#pragma unroll 1
-                for (int j = 0; j < V; ++j) {
-                    const uint64_t key = i < last ? key_of(order_of(v[j]), head + i * V + j) : 0;
-                    const uint64_t least = __shfl_sync(0xffffffffu, list, 31);
-                    if (__any_sync(0xffffffffu, key >= bound && key > least)) list = largest_32(list, sort_32(key >= bound ? key : 0, lane), lane);
+        // the number of keys in front of mine
+        const auto place = [&](const uint64_t* keys, int count, uint64_t mine) {
+            int in_front = 0;
+#pragma unroll 8
+            for (int i = 0; i < count; ++i) in_front += keys[i] > mine;
+            return in_front;
+        };
+        if (t < kThreads / 4 && s_quads[t] > 0 && place(s_quads, kThreads / 4, s_quads[t]) == a.top - 1) s_bound = s_quads[t];
+        __syncthreads();
+        while (true) {
+            const uint64_t bound = s_bound;
+            const auto found = [&](uint64_t key) {
+                if (key < bound) return;
+                const int i = atomicAdd(&s_found, 1);
+                if (i < kList) s_list[i] = key;
+            };
+            if (loose_key) found(loose_key);
+            // threads with a logit that may reach the bound: the warps look through their vectors in turn
+            if (at >= 0 && key_of(best, head + at * V) >= bound) s_who[atomicAdd(&s_many, 1)] = (uint16_t)t;
+            __syncthreads();
+            const float reach = logit_of((uint32_t)(bound >> 32));
+            for (int w = warp; w < s_many; w += kWarps)
+                for (int i = first + s_who[w] + lane * kThreads; i < last; i += 32 * kThreads) {
+                    Logits<T> v;
+                    v.load(body + (int64_t)i * V);
+                    uint32_t there = 0;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) there |= (uint32_t)!(v[j] < reach) << j;
+                    while (there) {
+                        const int j = __ffs(there) - 1;
+                        there &= there - 1;
+                        found(key_of(order_of(lm_to_f<T>(body[(int64_t)i * V + j])), head + i * V + j));
+                    }
                 }
-            }
+            __syncthreads();
+            const int count = s_found;
+            if (count <= kList) break;
+            // More than there is room for: those that came are a bound again, a higher one.
+            uint64_t mine[kList / kThreads];
+            for (int k = 0; k < kList / kThreads; ++k) mine[k] = s_list[t + k * kThreads];
+            for (int k = 0; k < kList / kThreads; ++k)
+                if (place(s_list, kList, mine[k]) == a.top - 1) s_bound = mine[k];
+            __syncthreads();
+            if (t == 0) s_found = s_many = 0;
+            __syncthreads();
         }
-        largest_of_block(list);
-    } else {
+        const int count = s_found;
+        for (int i = t; i < count; i += kThreads) {
+            const int p = place(s_list, count, s_list[i]);
+            if (p < a.top) s_top[p] = s_list[i];
+        }
+        for (int i = count + t; i < a.top; i += kThreads) s_top[i] = 0;   // (a block of a cluster whose share is that small)
+    }
+    __syncthreads();
+    if (a.ranks_of_row > 1) { cluster_arrive(); cluster_wait(); }
+    if (TOP && a.ranks_of_row > 1 && rank == 0) {
+        // all blocks' first tokens
+        uint64_t mine = 0;
+        if (lane < a.top && warp < a.ranks_of_row) asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(mine) : "r"(cluster_addr(smem_u32(&s_top[lane]), (uint32_t)warp)) : "memory");
+        __syncthreads();
+        static_assert(kMaxRanks <= kWarps && kThreads <= kList, "a warp for each block's list");
+        s_list[t] = mine;
+        __syncthreads();
+        int p = 0;
+        for (int r = 0; r < a.ranks_of_row; ++r)
+            for (int i = 0; i < a.top; ++i) p += s_list[32 * r + i] > mine;
+        if (mine > 0 && p < a.top) s_top[p] = mine;
         __syncthreads();
     }
-    if (a.ranks_of_row > 1) { cluster_arrive(); cluster_wait(); }
     if (rank == 0 && warp == 0 && live) {
         // all warps' sums of all blocks: a warp a lane, block after block
         Sums all = {-INFINITY, 0.f, 0.f};
         int count = 0;
-        uint64_t list = TOP ? s_keys[0][lane] : 0;
-        for (int r = 0; r < a.ranks_of_row; ++r) {
-            if (lane < kWarps) {
-                Sums o;
+        Sums o[kMaxRanks];
+        int b[kMaxRanks];
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; ++r) {
+            o[r] = {-INFINITY, 0.f, 0.f};
+            b[r] = 0;
+            if (r < a.ranks_of_row && lane < kWarps) {
                 const uint32_t from = cluster_addr(smem_u32(&s_sums[lane]), (uint32_t)r);
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(from) : "memory");
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.S) : "r"(from + 4) : "memory");
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.E) : "r"(from + 8) : "memory");
-                int b;
-                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(b) : "r"(cluster_addr(smem_u32(&s_before[lane]), (uint32_t)r)) : "memory");
-                all.add(o, a.c);
-                count += b;
-            }
-            if (TOP && r > 0) {
-                uint64_t other;
-                asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(other) : "r"(cluster_addr(smem_u32(&s_keys[0][lane]), (uint32_t)r)) : "memory");
-                list = largest_32(list, other, lane);
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[r].m) : "r"(from) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[r].S) : "r"(from + 4) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[r].E) : "r"(from + 8) : "memory");
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(b[r]) : "r"(cluster_addr(smem_u32(&s_before[lane]), (uint32_t)r)) : "memory");
             }
         }
+#pragma unroll 1
+        for (int r = 0; r < kMaxRanks; ++r) {
+            if (r < a.ranks_of_row) {
+                all.add(o[0], a.c);
+                count += b[0];
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+            for (int k = 0; k + 1 < kMaxRanks; ++k) { o[k] = o[k + 1]; b[k] = b[k + 1]; }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
             Sums other;
-            other.m = __shfl_xor_sync(0xffffffffu, all.m, o);
-            other.S = __shfl_xor_sync(0xffffffffu, all.S, o);
-            other.E = __shfl_xor_sync(0xffffffffu, all.E, o);
-            Sums lower = lane & o ? other : all;
-            lower.add(lane & o ? all : other, a.c);
+            other.m = __shfl_xor_sync(0xffffffffu, all.m, d);
+            other.S = __shfl_xor_sync(0xffffffffu, all.S, d);
+            other.E = __shfl_xor_sync(0xffffffffu, all.E, d);
+            Sums lower = lane & d ? other : all;
+            lower.add(lane & d ? all : other, a.c);
             all = lower;
-            count += __shfl_xor_sync(0xffffffffu, count, o);
+            count += __shfl_xor_sync(0xffffffffu, count, d);
         }
         const float logs = logf(all.S);
         const bool nothing = all.m == -INFINITY && all.S == 0.f;
@@ -389,8 +439,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
             if (a.entropy) a.entropy[row] = nothing ? 0.f : fmaf(-all.E / all.S, a.scale, logs);
         }
         if (TOP && lane < a.top) {
-            if (a.top_ids) a.top_ids[row * a.top_stride + lane] = index_of(list);
-            if (a.top_logprobs) a.top_logprobs[row * a.top_stride + lane] = logprob(logit_of((uint32_t)(list >> 32)));
+            const uint64_t key = s_top[lane];
+            if (a.top_ids) a.top_ids[row * a.top_stride + lane] = index_of(key);
+            if (a.top_logprobs) a.top_logprobs[row * a.top_stride + lane] = logprob(logit_of((uint32_t)(key >> 32)));
         }
     }
     if (a.ranks_of_row > 1) { cluster_arrive_relaxed(); cluster_wait(); }      // the first block has read what the others hold
@@ -423,7 +474,8 @@ int plan_logprobs(const pb_logprobs_params* p, LogprobsPlan& pl) {
     }
     const bool top = p->top_ids || p->top_logprobs;
     LogprobsArgs& a = pl.a;
-    a = {p->logits, p->targets, p->logprobs, p->entropy, p->top_logprobs, p->ranks, p->top_ids, p->logits_stride, p->top_stride, p->tokens, p->vocab, p->top, 1, p->scale, p->scale * kLog2e, 0.f, 0.f};
+    a = {p->logits, p->targets, p->logprobs, p->entropy, p->top_logprobs, p->ranks, p->top_ids, p->logits_stride, p->top_stride, p->tokens, p->vocab, p->top, 1, p->scale, p->scale * kLog2e, 0.f, 0.f, 0.f};
+    a.inv_c = 1.f / a.c;
     a.slack = 16.f / a.c;
     a.far = 256.f / a.c;
     // Few rows: a cluster on each, as long as that gives SMs something to do and a block some vectors for each thread.
