@@ -126,6 +126,7 @@ uint32_t* lm_rope_error_flag_ptr();
 uint32_t* lm_int8_error_flag_ptr();
 uint32_t* lm_attn_error_flag_ptr();
 uint32_t* lm_logprobs_error_flag_ptr();
+uint32_t* lm_norm_error_flag_ptr();
 uint32_t* noalloc_error_flag_ptr(int device);   // NULL until the no-allocation path ran on the device
 
 }  // namespace pb
