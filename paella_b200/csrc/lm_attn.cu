@@ -45,7 +45,8 @@ struct AttnArgs {
     int ahead;                 // tokens of the prefix that own_kernel takes as if they were each sequence's own: all of them, or none
     // chunks of new tokens (phase 3 of own_kernel): own_lens are whole lengths
     const int32_t* starts;
-    int tokens, max_new, window, few, beside;      // few: the most rows of a sequence that is taken here; beside: starts beside a kernel of the same launch
+    const int32_t* few_from;   // the most rows of a sequence that is taken here, or NULL: all
+    int tokens, max_new, window, beside;           // beside: starts beside a kernel of the same launch
 };
 
 // A sequence of a batch of chunks, as its lengths count.
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     if constexpr (kChunk) {
         if (b < a.batch) seq = chunk_seq(a.starts, a.own_lens, b, a.tokens, a.max_new, a.max_own, threadIdx.x == 0);
         const int64_t all = (int64_t)seq.rows * a.group;
-        rows = a.few > 0 && all > a.few ? 0 : (int)min((int64_t)R, max(all - row0, (int64_t)0));
+        rows = a.few_from && all > __ldcg(a.few_from) ? 0 : (int)min((int64_t)R, max(all - row0, (int64_t)0));
     }
     const auto token_of_row = [&](int row) { return a.group == 1 ? row0 + row : (row0 + row) / a.group; };
     const auto place_of_row = [&](int row, int64_t token_stride, int64_t head_stride) {          // of q or out

@@ -33,20 +33,20 @@ struct ChunkArgs {
     const int32_t *block_table, *starts, *lens;
     int64_t q_stride, q_head, out_stride, out_head, page_stride, token_stride, head_stride, table_stride;
     int batch, tokens, q_heads, kv_heads, group, D, page, n_pages, max_new, max_len, window, box_rows;
-    int few;                             // rows of a sequence that another kernel takes
+    int few, few_ranks;                  // rows of a sequence that own_kernel may take (0: none), the blocks that it would have for one and a key head
     int q_boxes;                         // a row tile's queries are boxes of a tensor map (whole tokens to a tile, positive strides and scale)
     float scale;
     int max_units, max_ranges;
     ChunkUnit* units;
     int64_t* before;                     // [max_units + 1]: costs of the units in front
     ChunkCut* cuts;                      // [max_ranges + 1]
-    int32_t* counts;                     // units, ranges
+    int32_t* counts;                     // units, ranges, rows of a sequence that own_kernel takes
     float4* part_o;                      // [2 max_ranges][2][DP / 4][128]
     float2* part_ml;                     // [2 max_ranges][2][128]: (m, l)
 };
 
 // Costs: a step of two row tiles, of one, and what a pair costs beside its steps.
-constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 6;
+constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 9;
 
 __device__ __forceinline__ int ceil_pos(int x, int d) { return x > 0 ? (x + d - 1) / d : 0; }
 
@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
     __shared__ int s_base[1025];
     __shared__ ChunkSeq s_seq[1024];
     __shared__ int s_tiles[kPlanUnits];            // tiles, twice, and whether there are two row tiles
+    __shared__ int s_most[3];                      // sequences of few rows, the most tokens that one's rows see; the highest cost of a unit
     griddep_wait();
     griddep_launch();
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -82,14 +83,40 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
         const int64_t ahead = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
         return x + (warp ? ahead : 0);
     };
+    // Sequences of few rows: own_kernel goes through the cache faster for all of them together, but has a sequence's tokens for a few blocks only.  In nanoseconds: some 40 bytes each for a block, 6000 for all
+    // of them, 5000 to begin with; here 1600 for a tile of keys and 5000 for an item, on all SMs.  (24 sequences of up to 17 new tokens behind 4000, six of which have few rows: 98 us with own_kernel, 70 without.)
+    ChunkSeq own = {0, 0, 0};                      // of the thread's first sequence
+    if (t < a.batch) own = chunk_seq(a.starts, a.lens, t, a.tokens, a.max_new, a.max_len, true);
+    if (t < 3) s_most[t] = 0;
+    __syncthreads();
+    int few = 0;
+    if (a.few) {
+        int many = 0, most = 0;
+        for (int b = t; b < a.batch; b += 1024) {
+            const ChunkSeq s = b == t ? own : chunk_seq(a.starts, a.lens, b, a.tokens, a.max_new, a.max_len, false);
+            if (s.rows == 0 || s.rows * a.group > a.few) continue;
+            ++many;
+            most = max(most, max(s.first + s.rows, 0) - (a.window ? max(s.first + 1 - a.window, 0) : 0));
+        }
+        many = __reduce_add_sync(0xffffffffu, many);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && many) {
+            atomicAdd(&s_most[0], many);
+            atomicMax(&s_most[1], most);
+        }
+        __syncthreads();
+        // (all as long as the longest)
+        const float each = 4.f * a.D * s_most[1], all = (float)s_most[0] * a.kv_heads, there = fmaxf(all * each / 6000.f, each / (40.f * a.few_ranks)) + 5000.f;
+        if (there < all * (s_most[1] * (1600.f / 128.f) + 5000.f) / kChunkBlocks) few = a.few;
+    }
     int units = 0;
     int64_t sum = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 1024) {
         int mine = 0;
         if (b0 + t < a.batch) {
-            const ChunkSeq s = chunk_seq(a.starts, a.lens, b0 + t, a.tokens, a.max_new, a.max_len, true);
+            const ChunkSeq s = b0 == 0 ? own : chunk_seq(a.starts, a.lens, b0 + t, a.tokens, a.max_new, a.max_len, true);
             const int rows = s.rows * a.group;
-            mine = rows > a.few ? (rows + 255) / 256 : 0;
+            mine = rows > few ? (rows + 255) / 256 : 0;
             s_seq[t] = s;
         }
         int64_t all;
@@ -122,6 +149,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
                 cost = kCostPair + (int64_t)u.tiles * (two ? kCostTwo : kCostOne);
                 tiles = 2 * u.tiles + two;
             }
+            const int highest = __reduce_max_sync(0xffffffffu, (int)min((long long)cost, 1LL << 30));
+            if (lane == 0) atomicMax(&s_most[2], highest);
             int64_t chunk;
             const int64_t before = sum + scan(cost, chunk) - cost;
             if (i < here) {
@@ -137,10 +166,16 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
     // Ranges: one for each block, several where they are long (so that the blocks are at the same keys at the same time, and those come from the L2 cache), fewer where there is little to do.
     const long long rounds = min(max((long long)total / (kChunkBlocks * 400), 1LL), (long long)(a.max_ranges / kChunkBlocks));
     int N = (int)min(kChunkBlocks * rounds, max((long long)total / (kCostPair + 3 * kCostTwo), 1LL));
-    if (units == 0) N = 0;
+    // A pair for each block where they are few and short: cuts would cost more than they even out.  (512 tokens of 8 x 4 heads 23 us, cut 31.)
+    const bool whole = (int64_t)units * a.kv_heads <= kChunkBlocks && s_most[2] <= kCostPair + 8 * kCostTwo;
+    if (whole) N = units * a.kv_heads;
     for (int r = t; r <= N; r += 1024) {
         ChunkCut c = {0, a.kv_heads, 0, 0, {}};
-        if (r < N) {
+        if (r < N && whole) {
+            c.head = r / units;
+            c.unit = r - c.head * units;
+            c.begins = a.units[c.unit];
+        } else if (r < N) {
             // (quotients of 64 bits take some hundred instructions each)
             const bool small = total < (1LL << 32) / (kChunkBlocks * kMaxRounds);
             const int64_t w = small ? (uint32_t)total * (uint32_t)r / (uint32_t)N : total * r / N;
@@ -167,7 +202,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
         }
         a.cuts[r] = c;
     }
-    if (t == 0) { a.counts[0] = units; a.counts[1] = N; }
+    if (t == 0) { a.counts[0] = units; a.counts[1] = N; a.counts[2] = few; }
 }
 
 // The parts of a block's ranges, one after the other.
@@ -850,7 +885,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         f.q_stride = a.q_stride; f.q_head = a.q_head; f.out_stride = a.out_stride; f.out_head = a.out_head;
         f.page_stride = a.page_stride; f.token_stride = a.token_stride; f.head_stride = a.head_stride; f.table_stride = a.table_stride;
         f.batch = a.batch; f.group = a.group; f.D = a.D; f.page = a.page; f.n_pages = a.n_pages; f.max_own = a.max_len; f.scale = a.scale; f.kv_heads = a.kv_heads;
-        f.tokens = a.tokens; f.max_new = a.max_new; f.window = a.window; f.few = pl.many ? kFewRows : 0; f.beside = pl.many;
+        f.tokens = a.tokens; f.max_new = a.max_new; f.window = a.window; f.beside = pl.many;
         f.per_piece = (uint32_t)ceil_div(1 << 16, a.D / 4);
         f.out_vec = aligned(a.out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
         f.splits = f.row_parts = 1;
@@ -867,6 +902,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     else pick_chunk<__nv_bfloat16>(pl);
     if (pl.many) {
         a.few = pl.has_few ? kFewRows : 0;
+        a.few_ranks = pl.few.ranks;
         const int64_t units = std::min((int64_t)a.tokens * a.group / 256 + a.batch, a.batch * ceil_div<int64_t>(most_rows, 256));
         PB_REQUIRE(units * a.kv_heads <= 1 << 30, "%s: %lld pairs of row tiles are too many", who, (long long)units);
         a.max_units = (int)units;
@@ -879,7 +915,8 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
             at += round_up<uint64_t>(bytes, 128);
             return (char*)p->scratch + from;
         };
-        a.counts = (int32_t*)take(8);
+        a.counts = (int32_t*)take(12);
+        pl.few.few_from = a.counts + 2;
         a.cuts = (ChunkCut*)take((a.max_ranges + 2) * sizeof(ChunkCut));
         a.units = (ChunkUnit*)take(a.max_units * sizeof(ChunkUnit));
         a.before = (int64_t*)take((a.max_units + 1) * sizeof(int64_t));

@@ -41,6 +41,8 @@ def plan(units, heads, max_ranges):
     total = before[-1] * heads
     rounds = min(max(total // (BLOCKS * 400), 1), max_ranges // BLOCKS)
     n = min(BLOCKS * rounds, max(total // (PAIR + 3 * TWO), 1))
+    if len(units) * heads <= BLOCKS and max(b - a for a, b in zip(before, before[1:])) <= PAIR + 8 * TWO:
+        return [(r // len(units), r % len(units), 0) for r in range(len(units) * heads)] + [(heads, 0, 0)]
     cuts = []
     for r in range(n):
         w = total * r // n
