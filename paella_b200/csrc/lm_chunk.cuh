@@ -425,6 +425,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
     } else if (warp == 9 || warp == 10) {
         constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
         constexpr uint32_t idesc_s = (1u << 4) | kType | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+        // (All DP values of a head, zeros behind its own: with a bound on the loop below instead heads of 96 gained nothing, and heads of 128 lost 2 %.)
         constexpr uint32_t idesc_o = (1u << 4) | kType | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
         const int g = warp - 9;
         const uint32_t d_s = tmem + g * 128, d_o = tmem + 256 + g * DP;
@@ -764,10 +765,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chunk
     griddep_launch();
     static_assert(256 / kJoinSlices == 32, "a row a lane");
     constexpr int kEach = DP / 4 / 8;                  // 16-byte pieces of a thread
-    const int r = (int)blockIdx.x / kJoinSlices + 1, slice = (int)blockIdx.x % kJoinSlices, ranges = __ldcg(a.counts + 1);
-    const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + r)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + r - 1));       // (used if there are so many)
-    const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
-    if (r < ranges && c.z > 0 && !(same(d) && d.z > 0)) {
+    const int slice = (int)blockIdx.x % kJoinSlices, ranges = __ldcg(a.counts + 1);
+    for (int r = (int)blockIdx.x / kJoinSlices + 1; r < max(ranges, 2); r += kChunkBlocks) {
+        const int4 c = __ldcg(reinterpret_cast<const int4*>(a.cuts + r)), d = __ldcg(reinterpret_cast<const int4*>(a.cuts + r - 1));   // (used if there are so many)
+        const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
+        if (r >= ranges || c.z == 0 || (same(d) && d.z > 0)) continue;
         const ChunkUnit u = a.cuts[r].begins;
         int last = r;                                  // the pair's last range
         while (last + 1 < ranges) {
@@ -878,7 +880,8 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     pl.many = a.max_new > 1 && most_rows > kFewRows && a.batch > 0 && a.max_len > 0;
     pl.has_few = !pl.many || a.batch > 1;
     if (pl.has_few) {
-        const int few_rows = (int)(pl.many ? std::min<int64_t>(most_rows, kFewRows) : std::max<int64_t>(most_rows, 1));
+        // beside chunks: 8 rows where a token's fit (three blocks an SM), 16 otherwise (two)
+        const int limit = a.group <= kFewRows / 2 ? kFewRows / 2 : kFewRows, few_rows = (int)(pl.many ? std::min<int64_t>(most_rows, limit) : std::max<int64_t>(most_rows, 1));
         pl.NT = few_rows <= 8 ? 1 : 2;
         AttnArgs& f = pl.few;
         f.q = a.q; f.k = a.k; f.v = a.v; f.out = a.out; f.block_table = a.block_table; f.own_lens = a.lens; f.starts = a.starts;
@@ -901,7 +904,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     if (pl.half) pick_chunk<__half>(pl);
     else pick_chunk<__nv_bfloat16>(pl);
     if (pl.many) {
-        a.few = pl.has_few ? kFewRows : 0;
+        a.few = !pl.has_few ? 0 : a.group <= kFewRows / 2 ? kFewRows / 2 : kFewRows;
         a.few_ranks = pl.few.ranks;
         const int64_t units = std::min((int64_t)a.tokens * a.group / 256 + a.batch, a.batch * ceil_div<int64_t>(most_rows, 256));
         PB_REQUIRE(units * a.kv_heads <= 1 << 30, "%s: %lld pairs of row tiles are too many", who, (long long)units);
@@ -923,7 +926,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         a.part_ml = (float2*)take(2ull * a.max_ranges * 256 * sizeof(float2));
         a.part_o = (float4*)take(2ull * a.max_ranges * 256 * pl.DP * sizeof(float));
         pl.scratch = at;
-        pl.join_blocks = (int64_t)(a.max_ranges - 1) * kJoinSlices;
+        pl.join_blocks = kChunkBlocks * kJoinSlices;
     }
     return PB_OK;
 }

@@ -153,7 +153,7 @@ __device__ __forceinline__ float group_sum(float v, int group, float* s_part) {
 
 // A row for `group` threads.
 template <typename T, typename H, int V, int CH>
-__global__ void __launch_bounds__(V > 1 && CH <= 2 ? 256 : 1024, V > 1 && CH <= 2 ? 6 / CH : 1) norm_kernel(const __grid_constant__ NormArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+__global__ void __launch_bounds__(V > 1 && CH <= 2 ? 256 : V == 1 && CH <= 16 ? 640 : 1024, V > 1 && CH <= 2 ? 6 / CH : V == 1 && CH <= 8 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     __shared__ float s_part[2][32];
     griddep_wait();
     if (nf) nf->start(job_id);
@@ -290,7 +290,7 @@ int plan_norm(const pb_residual_norm_params* p, NormPlan& pl) {
                       aligned(p->post_weight, 16) && aligned(p->weight, 16);
     const int vectors = wide ? p->channels / VN : p->channels;
     int pieces = wide ? 1 : 4;
-    while (vectors > (wide && pieces <= 2 ? 256 : 1024) * pieces) pieces *= 2;
+    while (vectors > (wide ? (pieces <= 2 ? 256 : 1024) : pieces <= 16 ? 640 : 1024) * pieces) pieces *= 2;
     a.group = round_up(ceil_div(vectors, pieces), 32);
     const int rows = a.group >= 256 ? 1 : 256 / a.group;
     pl.threads = (unsigned)(a.group * rows);
