@@ -210,11 +210,11 @@ PB_API int pb_conv2d_umma_noalloc(const pb_op_params* p, void* stream, uint32_t 
 PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
 
 /* ------------------------------------------------------------------------ *
- * Operators of language models: what one attention layer does to serve the next tokens.  No counterpart in the
+ * Operators of language models: what a layer does to serve a prompt and the next tokens, and what a request asks of the logits.  No counterpart in the
  * reference, whose adapters serve image models.  In the manner of the operators above: a params structure filled by the
  * caller, `_info` for the geometry a job stage declares, `_launch` to enqueue on `stream` (a cudaStream_t of the current
  * device, where all buffers live).
- *  - Each launcher enqueues one kernel, pb_prefix_attn_launch up to three.  Every block of the only, or last, kernel reports
+ *  - Each launcher enqueues one kernel, pb_prefix_attn_launch up to three, pb_chunk_attn_launch up to four.  Every block of the only, or last, kernel reports
  *    start/end on `notifier` (may be NULL) for `job_id`.  `_info` declares that kernel's blocks; where an earlier kernel of the
  *    launch holds more threads, registers, shared or tensor memory, a block is declared with so much more that num_blocks
  *    times it is what that kernel holds.
@@ -224,7 +224,7 @@ PB_API int pb_device_error_flag(int device, uint32_t* flag_out, int reset);
  *  - Launches allocate nothing and may be captured into a CUDA graph, the first one included.  The pointers and sizes of the
  *    params are read at the launch, what they point to when the kernels run.
  *  - What the host can see to be wrong is refused with PB_ERR_INVALID before anything is enqueued.  What only the device can
- *    see (a page, position, slot or length out of range) raises the flag that pb_device_error_flag reads; what such a value
+ *    see (a page, position, slot, length or token out of range) raises the flag that pb_device_error_flag reads; what such a value
  *    says below is done, and nothing outside the buffers is touched.
  * ------------------------------------------------------------------------ */
 typedef enum pb_dtype {

@@ -2,13 +2,14 @@
 //
 //   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j   over the tokens that row r sees: up to its own position, with a window the last of them
 //
-// Sequences of up to 16 rows (new tokens x heads of a key head; of one new token any) go to own_kernel, which is bound by reading the cache.  For more the rows of a
-// sequence's query heads that share a key head are cut into pairs of tiles of 128, which meet the keys and values in tiles of 128 on the tensor cores (chunk_kernel): the arithmetic of
-// prefix_kernel, with a mask where a tile holds keys that not all rows see.
+// A launch whose sequences have few rows (new tokens x heads of a key head: up to 16, or one new token) is own_kernel's, which is bound by reading the cache (64 sequences of one token behind up to 8000: 176 us,
+// 6 TB/s).  Otherwise the rows of a sequence's query heads that share a key head are cut into pairs of tiles of 128, which meet the keys and values in tiles of 128 on the tensor cores (chunk_kernel): the
+// arithmetic of prefix_kernel, with a mask where a tile holds keys that not all rows see.  Bound by the products and the softmax beside them, which share shared memory and issue slots: 3950 clocks for a pair and 128 keys,
+// of which the products alone take 2048 (a prompt of 8192 tokens of 8 x 4 heads of 128: 530 us, 1.04 PFLOP/s; 2048 tokens behind 65000: 1970 to 2020 us, 1.1 PFLOP/s at the power limit).
 //
 // Pairs differ in the keys that they see, and sequences in everything, all of which only the device knows.  So a block lays out the work first (plan_kernel): every pair's cost is known, all pairs for
 // all key heads stand in a row, and the row is cut into equal ranges, wherever that cuts a pair's keys.  A pair that is cut leaves a part of its sums with
-// each range, and join_kernel puts them together; the others are written at once.
+// each range, and join_kernel puts them together; the others are written at once.  (Plan and join take some 4 and 5 us.)
 #pragma once
 
 namespace pb {
@@ -45,7 +46,7 @@ struct ChunkArgs {
     float2* part_ml;                     // [2 max_ranges][2][128]: (m, l)
 };
 
-// Costs: a step of two row tiles, of one, and what a pair costs beside its steps.
+// Costs: a step of two row tiles, of one, and what a pair costs beside its steps: queries, first scores, results, some 9000 clocks.  (A prompt of 8192 tokens with 6, 9, 12 for that: 537, 522, 527 us.)
 constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 9;
 
 __device__ __forceinline__ int ceil_pos(int x, int d) { return x > 0 ? (x + d - 1) / d : 0; }
@@ -893,7 +894,8 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         f.out_vec = aligned(a.out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
         f.splits = f.row_parts = 1;
         f.row_groups = (int)ceil_div<int64_t>(few_rows, 8 * pl.NT);
-        // as for pb_prefix_attn: clusters of blocks on a sequence and key head while they fit the GPU, 128 tokens each at least
+        // As for pb_prefix_attn: clusters of blocks on a sequence and key head while they fit the GPU, 128 tokens each at least.  (24 sequences of 4 tokens x 4 heads, 8 key heads, up to 4096 tokens: twice as many
+        // blocks 64 us instead of 55; 32 of one token behind up to 2000 30 instead of 33.)
         const int64_t units = (int64_t)a.batch * a.kv_heads * f.row_groups, tokens = a.window ? std::min<int64_t>(a.window + a.max_new, a.max_len) : a.max_len;
         f.ranks = 1;
         while (f.ranks < kMaxRanks && units > 0 && units * f.ranks * 2 <= 3 * 148 && tokens / (2 * f.ranks) >= 128) f.ranks *= 2;

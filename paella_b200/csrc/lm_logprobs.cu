@@ -2,7 +2,8 @@
 //
 //   log p_t = s x_t - log sum_j exp(s x_j);   H = log S - sum_j e_j d_j / S   with d_j = s (x_j - m), e_j = exp(d_j), S = sum_j e_j
 //
-// Bound by memory: the logits are read once (their exponentials take three quarters of the special-function units' time at that rate in 16 bits).  Each
+// Bound by issue slots and the exponentials beside the reading: nine instructions a logit, one of them on the special-function units, which take 59 us for what memory delivers in 82 (2048 rows of 131072 in bf16:
+// 117 us, 4.6 TB/s, and 133 with the five likeliest tokens; 4096 rows of 32000 in fp16 72 us; 4 rows of 131072 in fp32 with twenty tokens 15 us).  Each
 // thread runs along its own vectors of a row with a maximum m of its own, which it follows only once it has grown by 2^16, so that sums are
 // rescaled a few times a row; all of a row's threads join at its end.
 //
