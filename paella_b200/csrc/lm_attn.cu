@@ -590,13 +590,14 @@ template <int DP> struct OwnShape {
 // what it sees, and with a window a beginning.
 template <typename T, int DP, int NT, int PHASE>
 __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    constexpr int kParts = PHASE == 3 ? 4 * kMaxRanks : kMaxParts;        // of a row, at most
     constexpr int R = 8 * NT, KB = DP / 32, VB = DP / 64, kStages = OwnShape<DP>::stages;
     constexpr uint32_t kHalf = OwnShape<DP>::half;
     static_assert(4 * R * DP * 4 <= OwnShape<DP>::smem, "the warps' parts fit where their rings were");
     extern __shared__ __align__(128) uint8_t smem_raw[];
     float (*s_o)[R][DP] = reinterpret_cast<float (*)[R][DP]>(smem_raw);
     __shared__ __align__(8) float2 s_ml[4][R];
-    __shared__ float s_w[R][kMaxParts];
+    __shared__ float s_w[R][kParts];
     constexpr bool kChunk = PHASE == 3;
     if (kChunk ? !a.beside : PHASE == 2 || !a.early) griddep_wait();
     if (PHASE == 1 || (kChunk && a.beside)) griddep_launch();
@@ -910,21 +911,21 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     const int ahead = a.early ? a.row_parts : 0, parts = ahead + (chunks > 0 ? 4 * a.ranks : 0);
     for (int row = warp; row < rows; row += 4) {
         const float2* ml = a.part_ml + first_part(row);
-        float2 x[kMaxParts / 32];
+        float2 x[kParts / 32];
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kMaxParts / 32; ++k) {
+        for (int k = 0; k < kParts / 32; ++k) {
             const int i = lane + 32 * k, w = i - ahead;
             x[k] = make_float2(-INFINITY, 0.f);
             if (i < ahead) x[k] = __ldcg(ml + (int64_t)i * 128);
             else if (i < parts) x[k] = ld_cluster_f2(cluster_addr(smem_u32(&s_ml[w & 3][row]), (uint32_t)w >> 2));
         }
 #pragma unroll
-        for (int k = 0; k < kMaxParts / 32; ++k) top = fmaxf(top, x[k].x);
+        for (int k = 0; k < kParts / 32; ++k) top = fmaxf(top, x[k].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-        for (int k = 0; k < kMaxParts / 32; ++k) {
+        for (int k = 0; k < kParts / 32; ++k) {
             x[k].x = x[k].x == -INFINITY ? 0.f : ex2(x[k].x - top);
             sum = fmaf(x[k].x, x[k].y, sum);
         }
@@ -932,7 +933,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float inv = kChunk && sum == 0.f ? 0.f : 1.f / sum;             // (0: a row that sees no token)
 #pragma unroll
-        for (int k = 0; k < kMaxParts / 32; ++k)
+        for (int k = 0; k < kParts / 32; ++k)
             if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;
     }
     __syncthreads();

@@ -772,20 +772,26 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chunk
         const auto same = [&](const int4& x) { return x.x == c.x && x.y == c.y; };
         if (r >= ranges || c.z == 0 || (same(d) && d.z > 0)) continue;
         const ChunkUnit u = a.cuts[r].begins;
-        int last = r;                                  // the pair's last range
-        while (last + 1 < ranges) {
-            const int4 e = __ldcg(reinterpret_cast<const int4*>(a.cuts + last + 1));
-            if (!same(e) || e.z == 0) break;
-            ++last;
+        int last = r;                                  // the pair's last range: a warp looks at 32 cuts at a time
+        while (true) {
+            const int at = last + 1 + (int)(threadIdx.x & 31);
+            bool on = at < ranges;
+            if (on) {
+                const int4 e = __ldcg(reinterpret_cast<const int4*>(a.cuts + at));
+                on = same(e) && e.z > 0;
+            }
+            const uint32_t run = __ballot_sync(0xffffffffu, on);
+            last += run == 0xffffffffu ? 32 : __ffs(~run) - 1;
+            if (run != 0xffffffffu) break;
         }
         const int parts = last - r + 2, in_pair = slice * 32 + (int)(threadIdx.x & 31), warp = (int)threadIdx.x >> 5, row = u.row0 + in_pair, g = in_pair >> 7, in_tile = in_pair & 127;
         const auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (r - 1) + 1 : 2 * (r + i - 1)) * 2 + g; };
         if (row < u.rows) {
             float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(a.part_ml + slot(i) * 128 + in_tile).x);
             float4 acc[kEach] = {};
-#pragma unroll 2
+#pragma unroll 4
             for (int i = 0; i < parts; ++i) {
                 const float2 ml = __ldcg(a.part_ml + slot(i) * 128 + in_tile);
                 float4 o[kEach];
@@ -877,8 +883,24 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     while (a.box_rows < 64 && p->page_size % (2 * a.box_rows) == 0) a.box_rows *= 2;
     pl.DP = p->head_dim <= 64 ? 64 : 128;
     pl.half = p->dtype == PB_F16;
-    const int64_t most_rows = (int64_t)a.max_new * a.group;
-    pl.many = a.max_new > 1 && most_rows > kFewRows && a.batch > 0 && a.max_len > 0;
+    const int64_t most_rows = (int64_t)a.max_new * a.group, tokens = a.window ? std::min<int64_t>(a.window + a.max_new, a.max_len) : a.max_len;
+    // own_kernel: as for pb_prefix_attn, clusters of blocks on a sequence and key head while they fit the GPU, 128 tokens each at least.  (24 sequences of 4 tokens x 4 heads, 8 key heads, up to 4096 tokens: twice as many
+    // blocks 64 us instead of 55; 32 of one token behind up to 2000 30 instead of 33.)
+    const auto ranks_of = [&](int64_t units) {
+        int ranks = 1;
+        while (ranks < kMaxRanks && units > 0 && units * ranks * 2 <= 3 * 148 && tokens / (2 * ranks) >= 128) ranks *= 2;
+        return ranks;
+    };
+    pl.many = a.max_new > 1 && most_rows > kFewRows;
+    if (!pl.many && a.batch > 0) {
+        // Few rows of long sequences that are too few for own_kernel's blocks, as if all were as long as max_len says: the times that plan_kernel compares, and 30 us for plan, beginning, parts and join.  (One new
+        // token behind 30000, 8 key heads of 128: 49 us with own_kernel, 48 here; behind 60000 91 and 67, behind 130000 188 and 111.)
+        const int64_t groups = ceil_div<int64_t>(most_rows, most_rows <= 8 ? 8 : 16);
+        const double each = 4.0 * a.D * tokens, units = (double)a.batch * a.kv_heads;
+        const double there = std::max(each * units / 6000.0, each / (40.0 * ranks_of(a.batch * a.kv_heads * groups))) + 5000.0, here = units * (tokens * 1600.0 / 128 + 5000.0) / kChunkBlocks + 30000.0;
+        pl.many = here < there;
+    }
+    pl.many = pl.many && a.batch > 0 && a.max_len > 0;
     pl.has_few = !pl.many || a.batch > 1;
     if (pl.has_few) {
         // beside chunks: 8 rows where a token's fit (three blocks an SM), 16 otherwise (two)
@@ -894,11 +916,8 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         f.out_vec = aligned(a.out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
         f.splits = f.row_parts = 1;
         f.row_groups = (int)ceil_div<int64_t>(few_rows, 8 * pl.NT);
-        // As for pb_prefix_attn: clusters of blocks on a sequence and key head while they fit the GPU, 128 tokens each at least.  (24 sequences of 4 tokens x 4 heads, 8 key heads, up to 4096 tokens: twice as many
-        // blocks 64 us instead of 55; 32 of one token behind up to 2000 30 instead of 33.)
-        const int64_t units = (int64_t)a.batch * a.kv_heads * f.row_groups, tokens = a.window ? std::min<int64_t>(a.window + a.max_new, a.max_len) : a.max_len;
-        f.ranks = 1;
-        while (f.ranks < kMaxRanks && units > 0 && units * f.ranks * 2 <= 3 * 148 && tokens / (2 * f.ranks) >= 128) f.ranks *= 2;
+        const int64_t units = (int64_t)a.batch * a.kv_heads * f.row_groups;
+        f.ranks = ranks_of(units);
         pl.few_blocks = std::max<int64_t>(units * f.ranks, 1);
         PB_REQUIRE(pl.few_blocks <= 0x7fffffff, "%s: too many blocks for one launch", who);
     }

@@ -27,6 +27,15 @@ def test_long_caches_in_several_rounds():
     assert gu.error_flag() == 0
 
 
+# one sequence's next tokens behind a long cache: few rows that all blocks share out
+@pytest.mark.parametrize("window", [0, 90000])
+@pytest.mark.parametrize("seqs,hkv,group", [([(1, 100001)], 2, 4), ([(3, 90000)], 1, 5), ([(1, 110000), (1, 50), (0, 7)], 1, 8), ([(1, 70000), (1, 0), (2, 60001)], 2, 3)])
+def test_few_rows_of_long_caches(seqs, hkv, group, window):
+    p = Problem(seqs, hkv, group, 128, 64, window=window)
+    p.check(p.run())
+    assert gu.error_flag() == 0
+
+
 def test_one_scratch_for_launches_that_follow_one_another():
     a, b = Problem([(300, 1500), (40, 900)], 2, 4, 128, 32), Problem([(20, 5000), (700, 900)], 2, 4, 128, 32, seed=3)
     pa, pb = a.params(), b.params()
