@@ -4,8 +4,8 @@
 //   a = x * w' / sqrt(mean(x^2) + eps);   h = residual + scale * gate * a;   y = h * w / sqrt(mean(h^2) + eps)
 //
 // Bound by memory: a row is read once and written once (some 4 operations a byte), so a row stays in registers from its first load to its
-// last store, in fp32.  (16384 rows of 4096: in bf16 with both norms and a gate 119 us, 4.5 TB/s, where two sums a row one after the other hold it back; with residuals in fp32 129 us, 6.2 TB/s; all in fp32
-// 171 us, 6.3 TB/s.  777 rows of 5001 in fp16, value by value, 25 us.  One row 2.4 us.)
+// last store, in fp32.  (16384 rows of 4096: in bf16 with both norms and a gate 101 us, 5.3 TB/s; with a gate for each token and one norm 101 us, 6.6 TB/s; with residuals in fp32 125 us, 6.4 TB/s.  777 rows of 5001 in
+// fp16, value by value, 25 us.  One row 2.4 us.)
 #include <algorithm>
 #include <cmath>
 
@@ -17,7 +17,9 @@ namespace {
 
 __device__ uint32_t g_norm_flag;
 
-constexpr int kMaxChannels = 32768, kMaxStages = 6;
+// Two rows of a block are on their way, the next one asked for when a row's results have been stored: more at a time, or sooner, come slower, where memory is what counts.  (16384 rows of 4096, all in fp32 / in
+// bf16 with a gate for each token / with residuals in fp32: 171, 101, 125 us; as soon as a row has been read 162, 109, 134; six rows, as soon as that 192, 119, 125.)
+constexpr int kMaxChannels = 32768, kMaxStages = 2;
 constexpr uint64_t kRingBytes = 208 * 1024;      // of an SM's shared memory
 
 struct NormArgs {
@@ -172,16 +174,18 @@ __global__ void __launch_bounds__(V > 1 && CH <= 2 ? 256 : V == 1 && CH <= 16 ? 
     if (nf) nf->end(job_id);
 }
 
-// The same for many rows, which come through a ring of bulk copies in shared memory: a block takes every gridDim.x-th.  With up to two pieces a thread, the weights and a gate of all tokens stay in its registers
-// (the ring leaves no room for them in the first-level cache: 133 us instead of 118 for 16384 rows of 4096 in bf16 with both norms and such a gate).
+// The same for many rows, which come through a ring of bulk copies in shared memory: a block takes every gridDim.x-th.  Up to two pieces a thread, the weights and a gate of all tokens stay in its registers,
+// since the ring leaves no room for them in the first-level cache.  (16384 rows of 4096 in bf16 with both norms and such a gate: 101 us, read again for each row 133; with a piece a thread and twice the
+// threads 149, with four pieces 152.)
 template <typename T, typename H, int CH>
 __global__ void __launch_bounds__(CH == 1 ? 256 : 512, CH == 1 ? 3 : 1) norm_ring_kernel(const __grid_constant__ NormArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
     constexpr bool kKeep = CH <= 2;
     constexpr int V = 16 / (int)sizeof(T);
     extern __shared__ __align__(128) uint8_t s_rows[];
-    __shared__ float s_part[2][2][32];
+    __shared__ __align__(16) float s_part[2][2][16];                     // (of warps that the block does not have: zeros)
     __shared__ uint64_t s_full[kMaxStages];
     __shared__ volatile uint32_t s_abort;
+    if (threadIdx.x < 64) reinterpret_cast<float*>(s_part)[threadIdx.x] = 0.f;
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&s_full[i]), 1);
@@ -203,6 +207,14 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : 512, CH == 1 ? 3 : 1) norm_rin
     if (t == 0)
         for (int i = 0; i < a.stages; ++i)
             if ((int64_t)blockIdx.x + (int64_t)i * gridDim.x < a.tokens) fetch((int64_t)blockIdx.x + (int64_t)i * gridDim.x, i);
+    const auto all_parts = [&](const float* part) {
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = reinterpret_cast<const float4*>(part)[i];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) { x[0].x += x[i].x; x[0].y += x[i].y; x[0].z += x[i].z; x[0].w += x[i].w; }
+        return (x[0].x + x[0].y) + (x[0].z + x[0].w);
+    };
     Raw<float, V> post[CH], weight[CH];
     Raw<T, V> gate[CH];
     if (kKeep) {
@@ -232,15 +244,15 @@ __global__ void __launch_bounds__(CH == 1 ? 256 : 512, CH == 1 ? 3 : 1) norm_rin
         float sum = warp_sum(p.squares_of_x());
         if ((t & 31) == 0) s_part[turn][0][t >> 5] = sum;
         if (!__syncthreads_and(ok)) break;                               // all have read the stage
-        if (t == 0 && row + (int64_t)a.stages * gridDim.x < a.tokens) fetch(row + (int64_t)a.stages * gridDim.x, stage);
-        float factor = 1.f;
-        if (a.post_weight) {
-            sum = 0.f;
-            for (int i = 0; i < a.group >> 5; ++i) sum += s_part[turn][0][i];
-            factor = rsqrtf(sum * a.inv_channels + a.eps);
-        }
+        const float factor = a.post_weight ? rsqrtf(all_parts(s_part[turn][0]) * a.inv_channels + a.eps) : 1.f;
         sum = p.into_residual(a, factor, row, t, true, kKeep ? post : nullptr);
-        if (a.y) p.normed(a, rsqrtf(group_sum(sum, a.group, s_part[turn][1]) * a.inv_channels + a.eps), row, t, true, kKeep ? weight : nullptr);
+        if (a.y) {
+            sum = warp_sum(sum);
+            if ((t & 31) == 0) s_part[turn][1][t >> 5] = sum;
+            __syncthreads();
+            p.normed(a, rsqrtf(all_parts(s_part[turn][1]) * a.inv_channels + a.eps), row, t, true, kKeep ? weight : nullptr);
+        }
+        if (t == 0 && row + (int64_t)a.stages * gridDim.x < a.tokens) fetch(row + (int64_t)a.stages * gridDim.x, stage);
         turn ^= 1;
         if (++stage == a.stages) { stage = 0; parity ^= 1; }
     }
