@@ -174,12 +174,12 @@ __global__ void __launch_bounds__(V > 1 && CH <= 2 ? 256 : V == 1 && CH <= 16 ? 
     if (nf) nf->end(job_id);
 }
 
-// The same for many rows, which come through a ring of bulk copies in shared memory: a block takes every gridDim.x-th.  Up to two pieces a thread, the weights and a gate of all tokens stay in its registers,
+// The same for many rows, which come through a ring of bulk copies in shared memory: a block takes every gridDim.x-th.  With two pieces a thread, the weights and a gate of all tokens stay in its registers,
 // since the ring leaves no room for them in the first-level cache.  (16384 rows of 4096 in bf16 with both norms and such a gate: 101 us, read again for each row 133; with a piece a thread and twice the
 // threads 149, with four pieces 152.)
 template <typename T, typename H, int CH>
-__global__ void __launch_bounds__(CH == 1 ? 256 : 512, CH == 1 ? 3 : 1) norm_ring_kernel(const __grid_constant__ NormArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
-    constexpr bool kKeep = CH <= 2;
+__global__ void __launch_bounds__(512, 1) norm_ring_kernel(const __grid_constant__ NormArgs a, uint32_t job_id, FinishedBlockNotifier* nf) {
+    constexpr bool kKeep = CH == 2;
     constexpr int V = 16 / (int)sizeof(T);
     extern __shared__ __align__(128) uint8_t s_rows[];
     __shared__ __align__(16) float s_part[2][2][16];                     // (of warps that the block does not have: zeros)
@@ -271,11 +271,11 @@ struct NormPlan {
     unsigned blocks, threads, smem;
 };
 
-// wide: 16-byte accesses of T, up to 8 pieces a thread; otherwise single values, up to 32.  ring: rows through shared memory, up to 4 pieces.
+// wide: 16-byte accesses of T, up to 8 pieces a thread; otherwise single values, up to 32.  ring: rows through shared memory, 2 or 4 pieces.
 template <typename T, typename H>
 NormFn pick(bool wide, bool ring, int pieces) {
     constexpr int VN = 16 / (int)sizeof(T);
-    if (ring) return pieces == 1 ? norm_ring_kernel<T, H, 1> : pieces == 2 ? norm_ring_kernel<T, H, 2> : norm_ring_kernel<T, H, 4>;
+    if (ring) return pieces == 2 ? norm_ring_kernel<T, H, 2> : norm_ring_kernel<T, H, 4>;
     if (wide) return pieces == 1 ? norm_kernel<T, H, VN, 1> : pieces == 2 ? norm_kernel<T, H, VN, 2> : pieces == 4 ? norm_kernel<T, H, VN, 4> : norm_kernel<T, H, VN, 8>;
     return pieces == 4 ? norm_kernel<T, H, 1, 4> : pieces == 8 ? norm_kernel<T, H, 1, 8> : pieces == 16 ? norm_kernel<T, H, 1, 16> : norm_kernel<T, H, 1, 32>;
 }
@@ -309,13 +309,13 @@ int plan_norm(const pb_residual_norm_params* p, NormPlan& pl) {
     pl.threads = (unsigned)(a.group * rows);
     int64_t blocks = ceil_div<int64_t>(p->tokens, rows);
     pl.smem = 0;
-    // Many rows come through rings, as many blocks an SM as have room for two rows each.
+    // Many rows come through rings, 512 threads an SM as far as there is room for two rows of each block.  (65536 rows of 1024 in bf16 90 us, from registers alone 102; 4096 of them 7.9 and 7.5.)
     bool ring = false;
     const uint64_t row_bytes = (uint64_t)p->channels * (es + (p->residual ? hs : 0) + (p->gate && p->gate_stride ? es : 0));
-    if (wide && vectors >= 256 && vectors <= 2048) {
-        const int each = vectors <= 256 ? 1 : vectors <= 1024 ? 2 : 4;
+    if (wide && vectors >= 64 && vectors <= 2048) {
+        const int each = vectors <= 1024 ? 2 : 4;
         const unsigned threads = (unsigned)round_up(ceil_div(vectors, each), 32);
-        const int resident = (int)std::min<uint64_t>(each == 1 ? 3 : std::max(1u, 512 / threads), kRingBytes / (2 * row_bytes));
+        const int resident = (int)std::min<uint64_t>(std::max(1u, 512 / threads), kRingBytes / (2 * row_bytes));
         if (resident >= 1 && p->tokens >= 2 * 148 * resident) {
             ring = true;
             pieces = each;
