@@ -271,12 +271,14 @@ struct NormPlan {
     unsigned blocks, threads, smem;
 };
 
-// wide: 16-byte accesses of T, up to 8 pieces a thread; otherwise single values, up to 32.  ring: rows through shared memory, 2 or 4 pieces.
+// wide: 16-byte accesses of T, up to 4 pieces a thread (8 of fp32); otherwise single values, up to 32.  ring: rows through shared memory, 2 or 4 pieces.
 template <typename T, typename H>
 NormFn pick(bool wide, bool ring, int pieces) {
     constexpr int VN = 16 / (int)sizeof(T);
     if (ring) return pieces == 2 ? norm_ring_kernel<T, H, 2> : norm_ring_kernel<T, H, 4>;
-    if (wide) return pieces == 1 ? norm_kernel<T, H, VN, 1> : pieces == 2 ? norm_kernel<T, H, VN, 2> : pieces == 4 ? norm_kernel<T, H, VN, 4> : norm_kernel<T, H, VN, 8>;
+    if constexpr (sizeof(T) == 4)
+        if (wide && pieces == 8) return norm_kernel<T, H, VN, 8>;
+    if (wide) return pieces == 1 ? norm_kernel<T, H, VN, 1> : pieces == 2 ? norm_kernel<T, H, VN, 2> : norm_kernel<T, H, VN, 4>;
     return pieces == 4 ? norm_kernel<T, H, 1, 4> : pieces == 8 ? norm_kernel<T, H, 1, 8> : pieces == 16 ? norm_kernel<T, H, 1, 16> : norm_kernel<T, H, 1, 32>;
 }
 
