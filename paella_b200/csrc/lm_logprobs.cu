@@ -242,9 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
             // Logits far below the maximum are raised to `low`, where their exponentials are zeros: masks of -infinity need no case of their own.  Not where
             // logits are so large that `low` and the maximum are too near each other in their type: those go one by one.
             low = lm_from_f<T>(fmaxf(sums.m - a.far, lowest<T>()));
-            const bool common = sums.m > -INFINITY && (sums.m - lm_to_f<T>(low)) * a.c >= 200.f;
-            limit = common ? sums.m + a.slack : __uint_as_float(0x7fffffffu);
+            // Nor where mc's rounding is so large that the exponents x c - mc leave fp32's range before `fold` can take it back, as from some 2^31 on (up to 16, an exponential is off by 2^-20 of itself).
             mc = sums.m * a.c;
+            const bool common = sums.m > -INFINITY && (sums.m - lm_to_f<T>(low)) * a.c >= 200.f && fabsf(fmaf(-sums.m, a.c, mc)) <= 16.f;
+            limit = common ? sums.m + a.slack : __uint_as_float(0x7fffffffu);
             minus_mc = pack_f32x2(__float_as_uint(-mc), __float_as_uint(-mc));
             if (!(top <= limit)) {
                 if (top == -INFINITY) {
