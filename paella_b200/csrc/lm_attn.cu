@@ -47,16 +47,24 @@ struct AttnArgs {
     const int32_t* starts;
     const int32_t* few_from;   // the most rows of a sequence that is taken here, or NULL: all
     int tokens, max_new, window, beside;           // beside: starts beside a kernel of the same launch
+    int given;                 // starts are the caller's, of up to kGivenStarts sequences; otherwise they are counted already
 };
 
-// A sequence of a batch of chunks, as its lengths count.
+// Up to so many sequences each block looks through the starts in front of its own, which takes 0.2 us of the launch; beyond that, where it would take all blocks together the square of the batch, a kernel of one
+// block does it once.  (In 256 sequences of one token behind up to 100 and 500 the former is 34.1 and 56.8 us, the latter 34.4 and 57.7.)
+constexpr int kGivenStarts = 256;
+
+// A sequence of a batch of chunks: what is given of it, and as that counts.  Its start counts as no less than `ahead`, the starts in front of it.
+struct ChunkGiven {
+    int start, end, len;
+    __device__ __forceinline__ ChunkGiven(const int32_t* starts, const int32_t* lens, int b) : start(__ldcg(starts + b)), end(__ldcg(starts + b + 1)), len(__ldcg(lens + b)) {}
+};
 struct ChunkSeq {
     int start, rows, first;    // its first row of q, its new tokens, the position of the first of them
 };
-__device__ __forceinline__ ChunkSeq chunk_seq(const int32_t* starts, const int32_t* lens, int b, int tokens, int max_new, int max_len, bool tell) {
-    const int s0 = __ldcg(starts + b), s1 = __ldcg(starts + b + 1), l = __ldcg(lens + b);
-    const int start = min(max(s0, 0), tokens), end = min(max(s1, start), tokens), len = min(max(l, 0), max_len), n = end - start;
-    if (tell && (start != s0 || end != s1 || len != l || n > max_new)) atomicExch(&g_attn_flag, kFlagLmLength);
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkGiven& g, int ahead, int tokens, int max_new, int max_len, bool tell) {
+    const int start = min(max(g.start, ahead), tokens), end = min(max(g.end, start), tokens), len = min(max(g.len, 0), max_len), n = end - start;
+    if (tell && (start != g.start || end != g.end || len != g.len || n > max_new)) atomicExch(&g_attn_flag, kFlagLmLength);
     return {start, min(n, max_new), len - n};
 }
 
@@ -612,7 +620,19 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
     int rows = b < a.batch ? min(R, a.group - row0) : 0;
     ChunkSeq seq = {0, 0, 0};
     if constexpr (kChunk) {
-        if (b < a.batch) seq = chunk_seq(a.starts, a.own_lens, b, a.tokens, a.max_new, a.max_own, threadIdx.x == 0);
+        if (b < a.batch) {
+            const ChunkGiven given(a.starts, a.own_lens, b);
+            int ahead = 0;
+            if (a.given) {                                                       // (these come together with the sequence's own)
+                int more[kGivenStarts / 32];
+#pragma unroll
+                for (int i = 0; i < kGivenStarts / 32; ++i) more[i] = 32 * i + lane < b ? __ldcg(a.starts + 32 * i + lane) : 0;
+#pragma unroll
+                for (int i = 0; i < kGivenStarts / 32; ++i) ahead = max(ahead, more[i]);
+                ahead = __reduce_max_sync(0xffffffffu, ahead);
+            }
+            seq = chunk_seq(given, ahead, a.tokens, a.max_new, a.max_own, threadIdx.x == 0);
+        }
         const int64_t all = (int64_t)seq.rows * a.group;
         rows = a.few_from && all > __ldcg(a.few_from) ? 0 : (int)min((int64_t)R, max(all - row0, (int64_t)0));
     }
@@ -1219,9 +1239,9 @@ int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t j
     if (rc != PB_OK) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
     FinishedBlockNotifier* nf = (FinishedBlockNotifier*)notifier;
+    PB_REQUIRE(pl.scratch == 0 || (p->scratch != nullptr && p->scratch_bytes >= pl.scratch && aligned(p->scratch, 16)), "pb_chunk_attn: %llu bytes of scratch memory are needed, 16-byte aligned (%llu given)",
+               (unsigned long long)pl.scratch, (unsigned long long)(p->scratch ? p->scratch_bytes : 0));
     if (pl.many) {
-        PB_REQUIRE(p->scratch != nullptr && p->scratch_bytes >= pl.scratch && aligned(p->scratch, 16), "pb_chunk_attn: %llu bytes of scratch memory are needed, 16-byte aligned (%llu given)",
-                   (unsigned long long)pl.scratch, (unsigned long long)(p->scratch ? p->scratch_bytes : 0));
         const CacheShape shape = {pl.half, p->head_dim, p->page_size, p->kv_heads, p->n_pages, p->token_stride, p->head_stride, p->page_stride, (uint32_t)pl.a.box_rows};
         CUtensorMap qm, km, vm;
         int e = encode_cache(shape, p->k_cache, &km);
@@ -1241,6 +1261,9 @@ int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uint32_t j
         const uint32_t smem = pl.DP == 64 ? PrefixShape<64>::smem : PrefixShape<128>::smem;
         PB_CUDA(cudaFuncSetAttribute(pl.chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         e = lm_launch("pb_chunk_attn", pl.chunk, dim3(kChunkBlocks), dim3(384), smem, st, 1, pl.a, qm, km, vm);
+        if (e != PB_OK) return e;
+    } else if (!pl.few.given) {
+        const int e = lm_launch("pb_chunk_attn (starts)", starts_kernel, dim3(1), dim3(1024), 0, st, 1, pl.a);
         if (e != PB_OK) return e;
     }
     if (pl.has_few) {

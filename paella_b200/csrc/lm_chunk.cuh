@@ -42,6 +42,7 @@ struct ChunkArgs {
     int64_t* before;                     // [max_units + 1]: costs of the units in front
     ChunkCut* cuts;                      // [max_ranges + 1]
     int32_t* counts;                     // units, ranges, rows of a sequence that own_kernel takes
+    int32_t* counted;                    // [batch + 1]: the starts as they count
     float4* part_o;                      // [2 max_ranges][2][DP / 4][128]
     float2* part_ml;                     // [2 max_ranges][2][128]: (m, l)
 };
@@ -50,6 +51,48 @@ struct ChunkArgs {
 constexpr int kCostTwo = 4, kCostOne = 3, kCostPair = 9;
 
 __device__ __forceinline__ int ceil_pos(int x, int d) { return x > 0 ? (x + d - 1) / d : 0; }
+
+// The starts as they count: not below 0, above `tokens` or below one in front of them, so that no two sequences have a row in common and the units fit.  A block of 1024 threads; whether a start fell.
+__device__ __forceinline__ bool count_starts(const ChunkArgs& a) {
+    __shared__ int s_high[32];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    bool fell = false, other = false;
+    for (int b = t; b <= a.batch; b += 1024) {
+        const int s = __ldcg(a.starts + b), before = __ldcg(a.starts + max(b - 1, 0)), counts = min(max(s, 0), a.tokens);
+        a.counted[b] = counts;
+        fell |= s < before;
+        other |= s != counts;
+    }
+    if (fell || other) atomicExch(&g_attn_flag, kFlagLmLength);
+    if (!__syncthreads_or(fell)) return false;
+    const auto highest = [&](int x) {                                    // of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x = max(x, y);
+        }
+        return x;
+    };
+    int ahead = 0;
+    for (int b0 = 0; b0 <= a.batch; b0 += 1024) {
+        const bool there = b0 + t <= a.batch;
+        const int s = highest(there ? a.counted[b0 + t] : 0);            // (which this thread wrote)
+        if (lane == 31) s_high[warp] = s;
+        __syncthreads();
+        const int warps = highest(s_high[lane]), in_front = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
+        if (there) a.counted[b0 + t] = max(max(s, ahead), warp ? in_front : 0);
+        ahead = max(ahead, __shfl_sync(0xffffffffu, warps, 31));
+        __syncthreads();
+    }
+    return true;
+}
+
+// In front of own_kernel alone, where a warp of it does not look through all starts (kGivenStarts).
+__global__ void __launch_bounds__(1024) starts_kernel(const __grid_constant__ ChunkArgs a) {
+    griddep_wait();
+    griddep_launch();
+    count_starts(a);
+}
 
 // The work: units, their costs, and the ranges.  One block, which the others wait for: a thread a sequence, a unit, a range, with all that is looked up in shared memory as long as there are no more than
 // kPlanUnits units.
@@ -87,14 +130,14 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
     // Sequences of few rows: own_kernel goes through the cache faster for all of them together, but has a sequence's tokens for a few blocks only.  In nanoseconds: some 40 bytes each for a block, 6000 for all
     // of them, 5000 to begin with; here 1600 for a tile of keys and 5000 for an item, on all SMs.  (24 sequences of up to 17 new tokens behind 4000, six of which have few rows: 98 us with own_kernel, 70 without.)
     ChunkSeq own = {0, 0, 0};                      // of the thread's first sequence
-    if (t < a.batch) own = chunk_seq(a.starts, a.lens, t, a.tokens, a.max_new, a.max_len, true);
+    if (t < a.batch) own = chunk_seq(ChunkGiven(a.starts, a.lens, t), 0, a.tokens, a.max_new, a.max_len, true);
     if (t < 3) s_most[t] = 0;
-    __syncthreads();
+    if (count_starts(a) && t < a.batch) own = chunk_seq(ChunkGiven(a.counted, a.lens, t), 0, a.tokens, a.max_new, a.max_len, true);
     int few = 0;
     if (a.few) {
         int many = 0, most = 0;
         for (int b = t; b < a.batch; b += 1024) {
-            const ChunkSeq s = b == t ? own : chunk_seq(a.starts, a.lens, b, a.tokens, a.max_new, a.max_len, false);
+            const ChunkSeq s = b == t ? own : chunk_seq(ChunkGiven(a.counted, a.lens, b), 0, a.tokens, a.max_new, a.max_len, false);
             if (s.rows == 0 || s.rows * a.group > a.few) continue;
             ++many;
             most = max(most, max(s.first + s.rows, 0) - (a.window ? max(s.first + 1 - a.window, 0) : 0));
@@ -115,7 +158,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
     for (int b0 = 0; b0 < a.batch; b0 += 1024) {
         int mine = 0;
         if (b0 + t < a.batch) {
-            const ChunkSeq s = b0 == 0 ? own : chunk_seq(a.starts, a.lens, b0 + t, a.tokens, a.max_new, a.max_len, true);
+            const ChunkSeq s = b0 == 0 ? own : chunk_seq(ChunkGiven(a.counted, a.lens, b0 + t), 0, a.tokens, a.max_new, a.max_len, true);
             const int rows = s.rows * a.group;
             mine = rows > few ? (rows + 255) / 256 : 0;
             s_seq[t] = s;
@@ -123,9 +166,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
         int64_t all;
         const int64_t upto = scan(mine, all);
         s_base[t] = (int)min((long long)(upto - mine), 0x7fffffffLL);
-        // (starts that fall can make more units than rows have room for: those behind the last place are left out)
-        const int here = (int)min((long long)all, (long long)(a.max_units - units)), n = min(1024, a.batch - b0);
-        if (all > here && t == 0) atomicExch(&g_attn_flag, kFlagLmLength);
+        const int here = (int)min((long long)all, (long long)(a.max_units - units)), n = min(1024, a.batch - b0);      // (all of them fit, as long as starts and lens do not change meanwhile)
         __syncthreads();
         for (int i0 = 0; i0 < here; i0 += 1024) {
             const int i = i0 + t;
@@ -911,6 +952,7 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         f.q_stride = a.q_stride; f.q_head = a.q_head; f.out_stride = a.out_stride; f.out_head = a.out_head;
         f.page_stride = a.page_stride; f.token_stride = a.token_stride; f.head_stride = a.head_stride; f.table_stride = a.table_stride;
         f.batch = a.batch; f.group = a.group; f.D = a.D; f.page = a.page; f.n_pages = a.n_pages; f.max_own = a.max_len; f.scale = a.scale; f.kv_heads = a.kv_heads;
+        f.given = !pl.many && a.batch <= kGivenStarts;
         f.tokens = a.tokens; f.max_new = a.max_new; f.window = a.window; f.beside = pl.many;
         f.per_piece = (uint32_t)ceil_div(1 << 16, a.D / 4);
         f.out_vec = aligned(a.out, 8) && a.out_stride % 4 == 0 && a.out_head % 4 == 0;
@@ -924,6 +966,16 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     pl.own_smem = pl.DP == 64 ? OwnShape<64>::smem : OwnShape<128>::smem;
     if (pl.half) pick_chunk<__half>(pl);
     else pick_chunk<__nv_bfloat16>(pl);
+    uint64_t at = 0;
+    const auto take = [&](uint64_t bytes) {
+        const uint64_t from = at;
+        at += round_up<uint64_t>(bytes, 128);
+        return (char*)p->scratch + from;
+    };
+    if (pl.many || !pl.few.given) {
+        a.counted = (int32_t*)take((a.batch + 1ull) * sizeof(int32_t));
+        pl.few.starts = a.counted;
+    }
     if (pl.many) {
         a.few = !pl.has_few ? 0 : a.group <= kFewRows / 2 ? kFewRows / 2 : kFewRows;
         a.few_ranks = pl.few.ranks;
@@ -933,12 +985,6 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         const int64_t cache = (int64_t)a.batch * a.max_len * a.kv_heads * a.D * 4;
         const int rounds = (int)std::min<int64_t>(std::max<int64_t>(cache >> 26, 1), kMaxRounds);
         a.max_ranges = kChunkBlocks * rounds;
-        uint64_t at = 0;
-        const auto take = [&](uint64_t bytes) {
-            const uint64_t from = at;
-            at += round_up<uint64_t>(bytes, 128);
-            return (char*)p->scratch + from;
-        };
         a.counts = (int32_t*)take(12);
         pl.few.few_from = a.counts + 2;
         a.cuts = (ChunkCut*)take((a.max_ranges + 2) * sizeof(ChunkCut));
@@ -946,9 +992,9 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
         a.before = (int64_t*)take((a.max_units + 1) * sizeof(int64_t));
         a.part_ml = (float2*)take(2ull * a.max_ranges * 256 * sizeof(float2));
         a.part_o = (float4*)take(2ull * a.max_ranges * 256 * pl.DP * sizeof(float));
-        pl.scratch = at;
         pl.join_blocks = kChunkBlocks * kJoinSlices;
     }
+    pl.scratch = at;
     return PB_OK;
 }
 

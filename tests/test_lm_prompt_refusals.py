@@ -95,3 +95,13 @@ def test_chunk_struct_size_and_null_params():
     assert C.sizeof(capi.ChunkAttnParams) == 12 * 4 + 9 * 8 + 9 * 8
     L, li = capi.load(), capi.LaunchInfo()
     assert L.pb_chunk_attn_info(None, C.byref(li)) == -2 and L.pb_chunk_attn_launch(None, None, 0, None) == -2
+
+
+def test_chunk_starts_of_many_sequences_need_scratch():
+    few, many = chunk(batch=256, max_new=1), chunk(batch=257, max_new=1)
+    assert lu.info("chunk_attn", few).scratch_bytes == 0
+    need = lu.info("chunk_attn", many).scratch_bytes
+    assert need >= 4 * 258
+    L = capi.load()
+    for over in (dict(scratch=None, scratch_bytes=need), dict(scratch=A, scratch_bytes=need - 1), dict(scratch=A + 8, scratch_bytes=need)):
+        assert L.pb_chunk_attn_launch(C.byref(chunk(batch=257, max_new=1, **over)), None, 0, None) == -2 and b"scratch" in L.pb_last_error()
