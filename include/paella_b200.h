@@ -366,7 +366,8 @@ PB_API int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, u
  * zeros.  What a row does not see has no part in it, whatever it holds; a value of V that is not finite leaves the rows that see it with
  * one that is not.  Rows that belong to no sequence are left as they are.
  * A length outside of [0, max_len] counts as the nearer end, as does a start outside of [0, tokens]; a start below one in front of it counts as the
- * highest of those, so that no row belongs to two sequences.  Of more than max_new new tokens the first max_new rows are computed, at the positions that they have.  A page number outside of [0, n_pages) counts as a page of zeros. */
+ * highest of those, so that no row belongs to two sequences.  Of more than max_new new tokens the first max_new rows are computed, at the positions that they have.  A page number outside of [0, n_pages) counts as a page of zeros.
+ * Pages that hold no token that any row of the sequence sees, behind its end or in front of its window, are not used, and what block_table says of them does not matter. */
 typedef struct pb_chunk_attn_params {
     int32_t dtype;               /* PB_BF16 or PB_F16 */
     int32_t batch;               /* sequences, 0 = nothing to do */

@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         int64_t at_lo = -1, at_hi = -1;                                        // where a half lies, or -1: zeros
         const auto place = [&](int chunk, int half, int page) -> int64_t {
             const int token = token_of(chunk) + 8 * half;
-            if (chunk >= last || token >= limit_of(chunk)) return -1;
+            if (chunk >= last || token >= limit_of(chunk) || (kChunk && token + 8 <= low)) return -1;      // (in front of the window: a page that may be gone)
             if (page < 0 || page >= a.n_pages) {
                 atomicExch(&g_attn_flag, kFlagLmPage);
                 return -1;

@@ -359,13 +359,14 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         struct Tiles {                   // the block's tiles in order
             ChunkWalk walk;
             ChunkItem x;
-            int step;
+            int step, seen;              // seen: the first token that any row of the item sees
             bool more;
             __device__ __forceinline__ Tiles(const ChunkArgs& a) : walk(a) { item(); }
             __device__ __forceinline__ void item() {
                 do more = walk.next(x);
                 while (more && x.from >= x.to);
                 step = x.from;
+                seen = walk.a.window ? x.first + x.row0 / walk.a.group + 1 - walk.a.window : 0;
             }
             __device__ __forceinline__ void on() {
                 if (++step >= x.to) item();
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
         int i = 0, i_ahead = 0;
         const auto look_up = [&]() {
             const int token = (ahead.x.tile0 + ahead.step) * 128 + box * a.box_rows;
-            if (ahead.more && blk == 0 && box * a.box_rows < 128 && token < ahead.x.end)
+            if (ahead.more && blk == 0 && box * a.box_rows < 128 && token < ahead.x.end && token + a.box_rows > ahead.seen)
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(words + (i_ahead & 3) * 64), "l"(a.block_table + ahead.x.b * a.table_stride + token / a.page) : "memory");
             asm volatile("cp.async.commit_group;" ::: "memory");
             ++i_ahead;
@@ -412,8 +413,9 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
             if (box < boxes) {
                 int page;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(page) : "r"(words + (i & 3) * 64) : "memory");
-                if ((uint32_t)page >= (uint32_t)a.n_pages) {
-                    atomicExch(&g_attn_flag, kFlagLmPage);
+                const bool seen = first + (box + 1) * a.box_rows > now.seen;     // in front of the window the page may be gone, and was not looked up
+                if (!seen || (uint32_t)page >= (uint32_t)a.n_pages) {
+                    if (seen) atomicExch(&g_attn_flag, kFlagLmPage);
                     page = a.n_pages;                                    // outside of the map: zeros
                 }
                 tma_load_4d(to + blk * kBlock + box * a.box_rows * 128, values ? &vmap : &kmap, blk * 64, (first + box * a.box_rows) % a.page, now.x.head, page, bar);
