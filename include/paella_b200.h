@@ -363,7 +363,7 @@ PB_API int pb_prefix_attn_launch(const pb_prefix_attn_params* p, void* stream, u
  * starts[b + 1] - 1 of q and out.  The i-th of them stands at position p = lens[b] - n + i and sees the tokens 0 to p, with a window those from
  * p - window + 1 on: out = softmax(scale * q K^T) V, query head h over key head h / (q_heads / kv_heads).  Products of bf16 / fp16 operands in
  * fp32; softmax in fp32, its values rounded to the cache's type before they meet V.  A row that sees no token (p < 0) gets
- * zeros.  What a row does not see has no part in it, whatever it holds; a value of V that is not finite leaves the rows that see it with
+ * zeros, one whose scores are all -infinity NaNs.  What a row does not see has no part in it, whatever it holds; a value of V that is not finite leaves the rows that see it with
  * one that is not.  Rows that belong to no sequence are left as they are.
  * A length outside of [0, max_len] counts as the nearer end, as does a start outside of [0, tokens]; a start below one in front of it counts as the
  * highest of those, so that no row belongs to two sequences.  Of more than max_new new tokens the first max_new rows are computed, at the positions that they have.  A page number outside of [0, n_pages) counts as a page of zeros.

@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ AttnAr
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = kChunk && sum == 0.f ? 0.f : 1.f / sum;             // (0: a row that sees no token)
+        const float inv = kChunk && seq.first + token_of_row(row) < 0 ? 0.f : 1.f / sum;             // (0: a row that sees no token)
 #pragma unroll
         for (int k = 0; k < kParts / 32; ++k)
             if (lane + 32 * k < parts) s_w[row][lane + 32 * k] = x[k].x * inv;

@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(384, 1) chunk_kernel(const __grid_constant__ C
                 const uint32_t from = tmem + lanes + 256 + g * DP;
                 if (*(volatile uint32_t*)&s_odd[item & 7] != 0) add_odd(x, from, limit, low);
                 const int64_t part = (int64_t)x.slot * 2 + g;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = limit <= 0 ? 0.f : 1.f / l;                    // (0: a row that sees no token)
                 T* const base = static_cast<T*>(a.out) + place(x, min(row, x.rows - 1), a.out_stride, a.out_head);
                 if (x.slot >= 0) a.part_ml[part * 128 + in_tile] = make_float2(m == -INFINITY ? m : m * c, l);
                 // (Rolled up: code that runs once for an item comes from memory.)
@@ -847,8 +847,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Chunk
                     acc[k].x = fmaf(w, o[k].x, acc[k].x); acc[k].y = fmaf(w, o[k].y, acc[k].y); acc[k].z = fmaf(w, o[k].z, acc[k].z); acc[k].w = fmaf(w, o[k].w, acc[k].w);
                 }
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int token = row / a.group;
+            const float inv = u.first + token < 0 ? 0.f : 1.f / sum;             // (as in chunk_kernel)
             T* dst = static_cast<T*>(a.out) + (int64_t)(u.start + token) * a.out_stride + (int64_t)(c.y * a.group + row - token * a.group) * a.out_head;
             const bool vec = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * 2) | (uintptr_t)(a.out_head * 2)) & 7) == 0;
 #pragma unroll
