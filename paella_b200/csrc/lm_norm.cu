@@ -359,8 +359,10 @@ int pb_residual_norm_info(const pb_residual_norm_params* p, pb_launch_info* out)
     const uint64_t t = (uint64_t)p->tokens, c = (uint64_t)p->channels, es = dtype_bytes(p->dtype), hs = dtype_bytes(p->h_dtype);
     out->num_blocks = pl.blocks;
     out->threads_per_block = pl.threads;
-    out->smem_per_block = pl.smem;
-    out->regs_per_thread = lm_regs(pl.fn);
+    cudaFuncAttributes fa = {};
+    if (cudaFuncGetAttributes(&fa, (const void*)pl.fn) != cudaSuccess) cudaGetLastError();        // (without a GPU: what the host knows)
+    out->smem_per_block = pl.smem + (uint32_t)fa.sharedSizeBytes;
+    out->regs_per_thread = (uint32_t)fa.numRegs;
     out->flops = t * c * (2 + (p->post_weight ? 4 : 0) + (p->gate ? 1 : 0) + (p->y ? 4 : 0));
     if (t)
         out->bytes = t * c * (es * (1 + (p->y ? 1 : 0)) + hs * ((p->residual ? 1 : 0) + (p->h ? 1 : 0))) + (p->gate ? (p->gate_stride ? t : 1) * c * es : 0) +
