@@ -377,7 +377,8 @@ typedef struct pb_chunk_attn_params {
     int32_t page_size;           /* a multiple of 8 */
     int32_t max_blocks;          /* entries of a row of block_table */
     int32_t max_new;             /* the most new tokens that a sequence has */
-    int32_t max_len;             /* the most that lens holds; <= max_blocks * page_size */
+    int32_t max_len;             /* the most that lens holds; <= max_blocks * page_size.  What `_info` declares, and for few new tokens which
+                                    kernels run, goes by it: the nearer to the lengths the better */
     int32_t window;              /* tokens that a row sees, itself the last of them; 0 = all */
     float scale;
     int64_t n_pages;
@@ -401,7 +402,7 @@ PB_API int pb_chunk_attn_launch(const pb_chunk_attn_params* p, void* stream, uin
  *     h = residual + scale * (gate * a)               gate NULL: ones; residual NULL: zeros
  *     y = h * weight / sqrt(mean(h^2) + eps)          the norm in front of the next block (weight NULL: ones)
  * Means are over a row's `channels` values.  In fp32; h and y are rounded once each, y from the h in front of its rounding.
- * A row whose sum of squares passes fp32's range (3.4e38) becomes zeros behind that norm. */
+ * A row whose sum of squares passes fp32's range (3.4e38) becomes zeros behind that norm; where the mean of the squares and eps are both below 1e-38, they lose bits. */
 typedef struct pb_residual_norm_params {
     int32_t tokens;              /* 0 = nothing to do */
     int32_t channels;            /* 1 to 32768 */

@@ -2,14 +2,16 @@
 //
 //   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j   over the tokens that row r sees: up to its own position, with a window the last of them
 //
-// A launch whose sequences have few rows (new tokens x heads of a key head: up to 16, or one new token) is own_kernel's, which is bound by reading the cache (64 sequences of one token behind up to 8000: 176 us,
-// 6 TB/s).  Otherwise the rows of a sequence's query heads that share a key head are cut into pairs of tiles of 128, which meet the keys and values in tiles of 128 on the tensor cores (chunk_kernel): the
+// A launch whose sequences have few rows (new tokens x heads of a key head: up to 16, or one new token) is own_kernel's, which is bound by reading the cache (64 sequences of one token behind up to 8000: 180 us,
+// 5.8 TB/s), unless they are so few and max_len is so large that its blocks could not read as fast as all SMs.  Otherwise the rows of a sequence's query heads that share a key head are cut into pairs of tiles of 128, which meet the keys and values in tiles of 128 on the tensor cores (chunk_kernel): the
 // arithmetic of prefix_kernel, with a mask where a tile holds keys that not all rows see.  Bound by the products and the softmax beside them, which share shared memory and issue slots: 3950 clocks for a pair and 128 keys,
-// of which the products alone take 2048 (a prompt of 8192 tokens of 8 x 4 heads of 128: 530 us, 1.04 PFLOP/s; 2048 tokens behind 65000: 1970 to 2020 us, 1.1 PFLOP/s at the power limit).
+// of which the products alone take 2048 (a prompt of 8192 tokens of 8 x 4 heads of 128: 530 us, 1.04 PFLOP/s; 2048 tokens behind 65000: 2000 us, 1.1 PFLOP/s, both for a few milliseconds; launches that go on
+// for a second run at 1.68 and 1.62 GHz under the power limit: 602 us, 913 TFLOP/s, and 2280 us, 972 TFLOP/s).
 //
 // Pairs differ in the keys that they see, and sequences in everything, all of which only the device knows.  So a block lays out the work first (plan_kernel): every pair's cost is known, all pairs for
 // all key heads stand in a row, and the row is cut into equal ranges, wherever that cuts a pair's keys.  A pair that is cut leaves a part of its sums with
-// each range, and join_kernel puts them together; the others are written at once.  (Plan and join take some 4 and 5 us.)
+// each range, and join_kernel puts them together; the others are written at once.  (Under the counters, which start from cold and wait for each kernel, plan takes
+// 9 us and join 11 to 17, 40 where it reads the 110 MB of parts that 2048 tokens behind 65000 leave.)
 #pragma once
 
 namespace pb {
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Chun
         return x + (warp ? ahead : 0);
     };
     // Sequences of few rows: own_kernel goes through the cache faster for all of them together, but has a sequence's tokens for a few blocks only.  In nanoseconds: some 40 bytes each for a block, 6000 for all
-    // of them, 5000 to begin with; here 1600 for a tile of keys and 5000 for an item, on all SMs.  (24 sequences of up to 17 new tokens behind 4000, six of which have few rows: 98 us with own_kernel, 70 without.)
+    // of them, 5000 to begin with; here 1600 for a tile of keys and 5000 for an item, on all SMs.  (24 sequences of up to 17 new tokens behind 4000, six of which have few rows: 98 us with own_kernel, 65 without.)
     ChunkSeq own = {0, 0, 0};                      // of the thread's first sequence
     if (t < a.batch) own = chunk_seq(ChunkGiven(a.starts, a.lens, t), 0, a.tokens, a.max_new, a.max_len, true);
     if (t < 3) s_most[t] = 0;
@@ -937,7 +939,8 @@ int plan_chunk(const pb_chunk_attn_params* p, ChunkPlan& pl) {
     pl.many = a.max_new > 1 && most_rows > kFewRows;
     if (!pl.many && a.batch > 0) {
         // Few rows of long sequences that are too few for own_kernel's blocks, as if all were as long as max_len says: the times that plan_kernel compares, and 30 us for plan, beginning, parts and join.  (One new
-        // token behind 30000, 8 key heads of 128: 49 us with own_kernel, 48 here; behind 60000 91 and 67, behind 130000 188 and 111.)
+        // token behind 30000, 8 key heads of 128: 49 us with own_kernel, 48 here; behind 60000 91 and 67, behind 130000 188 and 111.  The host knows no lengths: behind 500 tokens a lone sequence takes 9.0 us where max_len
+        // is 501 and 19.4 where it is 32768 or more, 64 sequences 34.8 and, from 131072 on, 44.0.)
         const int64_t groups = ceil_div<int64_t>(most_rows, most_rows <= 8 ? 8 : 16);
         const double each = 4.0 * a.D * tokens, units = (double)a.batch * a.kv_heads;
         const double there = std::max(each * units / 6000.0, each / (40.0 * ranks_of(a.batch * a.kv_heads * groups))) + 5000.0, here = units * (tokens * 1600.0 / 128 + 5000.0) / kChunkBlocks + 30000.0;

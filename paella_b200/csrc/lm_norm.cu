@@ -311,7 +311,8 @@ int plan_norm(const pb_residual_norm_params* p, NormPlan& pl) {
     pl.threads = (unsigned)(a.group * rows);
     int64_t blocks = ceil_div<int64_t>(p->tokens, rows);
     pl.smem = 0;
-    // Many rows come through rings, 512 threads an SM as far as there is room for two rows of each block.  (65536 rows of 1024 in bf16 90 us, from registers alone 102; 4096 of them 7.9 and 7.5.)
+    // Many rows come through rings, 512 threads an SM as far as there is room for two rows of each block.  (Rows of 1024 in bf16, and from registers alone: 65536 of them 90 and 102 us, 16384 25.3 and 27.3, 8192
+    // 12.7 and 13.5, 4096 7.9 and 7.5, 2400 5.3 both.  Rows of 4096: 16384 of them 92 and 124, 2048 12.5 and 12.8, 700 6.1 both.)
     bool ring = false;
     const uint64_t row_bytes = (uint64_t)p->channels * (es + (p->residual ? hs : 0) + (p->gate && p->gate_stride ? es : 0));
     if (wide && vectors >= 64 && vectors <= 2048) {
